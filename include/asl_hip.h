@@ -462,6 +462,72 @@ typedef struct asl_attn_params {
 int asl_attention_fwd(const asl_attn_params* p, const void* qkv, void* out, asl_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Training the classifier end
+ * ----------------------------------------------------------------------------------
+ * These entry points take fp32 or bf16 tensors (ASL_F32 / ASL_BF16 per argument), any sizes, row strides in elements, and
+ * need no more than the element type's own alignment except where a workspace is named.  Everything they add up is held in
+ * fp32 or wider and added in a fixed order, so a call's results do not vary from run to run. */
+enum { ASL_F32 = 0, ASL_BF16 = 1 };
+
+/* nn.LayerNorm(d) with saved statistics, and its backward.
+ *   y = (x - mean) * rstd * gamma + beta;   gamma == NULL stands for ones, beta == NULL for noughts
+ *   dx = rstd * (g - mean_d(g) - h * mean_d(g h)),  g = dy * gamma,  h = (x - mean) * rstd
+ *   dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy      (NULL: not wanted; written as w_type)
+ * x [rows][ld_x] and dx [rows][ld_dx] are of x_type, y and dy [rows][ld_y] of y_type, gamma and beta of w_type.  mean and
+ * rstd are fp32 [rows]; forward takes NULL for either.  The places between d and a row's stride are left alone.  rows == 0
+ * is a call like any other (dgamma and dbeta are nought).  Backward needs `workspace`, 16-byte aligned, of
+ * asl_layernorm_bwd_workspace(p) bytes (a negative return is an ASL_E* code). */
+typedef struct asl_layernorm_params {
+    int32_t rows, d;
+    int64_t ld_x, ld_y, ld_dx;
+    int32_t x_type, w_type, y_type;
+    float eps;
+} asl_layernorm_params;
+
+int asl_layernorm_fwd(const asl_layernorm_params* p, const void* x, const void* gamma, const void* beta, void* y,
+                      float* mean, float* rstd, asl_stream_t stream);
+int64_t asl_layernorm_bwd_workspace(const asl_layernorm_params* p);
+int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void* x, const void* gamma, const float* mean,
+                      const float* rstd, void* dx, void* dgamma, void* dbeta, float* workspace, asl_stream_t stream);
+
+/* F.cross_entropy(F.linear(x, w, bias), target, ignore_index, reduction, label_smoothing), and its gradients, without
+ * holding the logits: x [n][ld_x] and w [classes][ld_w] are of `type`, bias (NULL: none) of bias_type, target int64 [n].
+ *   loss: fp32, one value, or [n] for ASL_REDUCE_NONE.  ASL_REDUCE_MEAN divides by the rows whose target is not
+ *         ignore_index (none of them: NaN, as 0 / 0); ignored rows have loss 0 and gradient 0.
+ *   lse:  fp32 [n], log sum exp of each row's logits (NULL: not wanted).
+ *   asl_linear_xent_grad also writes dx [n][d], dw [classes][d] (dense, of `type`) and dbias [classes] (of bias_type), each
+ *   NULL if not wanted.  upstream is the gradient of the loss: fp32, one value, or [n] for ASL_REDUCE_NONE; NULL stands for 1.
+ * A bias of -inf masks a class.  A target outside [0, classes) that is not ignore_index makes the loss, the row's dx and
+ * every dw NaN rather than being read.  workspace: 256-byte aligned, asl_linear_xent_workspace(p, grad) bytes -- at most
+ * about 1 GiB of exponentials at a time plus what sums need (a negative return is an ASL_E* code; classes above 2^21, d
+ * above 2^20 or n above 2^28 return ASL_ETOOBIG). */
+enum { ASL_REDUCE_NONE = 0, ASL_REDUCE_SUM = 1, ASL_REDUCE_MEAN = 2 };
+typedef struct asl_xent_params {
+    int32_t n, classes, d;
+    int32_t type, bias_type, reduction;
+    int64_t ld_x, ld_w, ignore_index;
+    float label_smoothing;
+    int32_t reserved;
+} asl_xent_params;
+
+int64_t asl_linear_xent_workspace(const asl_xent_params* p, int grad);
+int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, const void* w, const void* bias, const int64_t* target,
+                        float* loss, float* lse, void* workspace, asl_stream_t stream);
+int asl_linear_xent_grad(const asl_xent_params* p, const void* x, const void* w, const void* bias, const int64_t* target,
+                         const float* upstream, float* loss, float* lse, void* dx, void* dw, void* dbias, void* workspace,
+                         asl_stream_t stream);
+
+/* The norm over all elements of `count` dense tensors, and the tensors clipped by it (torch.nn.utils.clip_grad_norm_):
+ *   norm = sqrt(sum g^2), or max |g| with inf_norm != 0;   out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))
+ * grads, numel, in_type (ASL_F32 / ASL_BF16 each), out and out_type are HOST arrays, read during the call; grads[i] and
+ * out[i] are device pointers.  out == NULL computes the norm alone; out[i] == grads[i] clips in place (same type); any other
+ * overlap of an output with another tensor returns ASL_EINVAL.  norm: fp32, one value, on the device; nothing is waited for.
+ * A NaN among the gradients makes norm and every output NaN.  workspace: 8-byte aligned, asl_grad_clip_workspace bytes. */
+int64_t asl_grad_clip_workspace(int count, const int64_t* numel);
+int asl_grad_clip(int count, const void* const* grads, const int64_t* numel, const int32_t* in_type, void* const* out,
+                  const int32_t* out_type, float max_norm, int inf_norm, float* norm, double* workspace, asl_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Batched issue
  * ---------------------------------------------------------------------------------- */
 

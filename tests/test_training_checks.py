@@ -1,0 +1,161 @@
+"""CPU: the training operators refuse what they cannot compute -- at the C boundary before anything is launched, and in
+Python with the reason -- and their workspace sizes are what the sizes ask for."""
+import ctypes as C
+
+import pytest
+import torch
+
+FAKE = C.c_void_p(0x1000)        # aligned, never dereferenced: validation comes first
+OFF = C.c_void_p(0x1001)
+
+
+def _norm(L, **kw):
+    a = dict(rows=4, d=16, ld_x=16, ld_y=16, ld_dx=16, x_type=L.F32, w_type=L.F32, y_type=L.F32, eps=1e-5)
+    a.update(kw)
+    return L.LayerNormParams(**a)
+
+
+def _xent(L, **kw):
+    a = dict(n=4, classes=10, d=16, type=L.F32, bias_type=L.F32, reduction=L.REDUCE_MEAN, ld_x=16, ld_w=16, ignore_index=-100,
+             label_smoothing=0.0)
+    a.update(kw)
+    return L.XentParams(**a)
+
+
+def test_struct_sizes():
+    from video_asl_recognition_amd import _lib as L
+    assert C.sizeof(L.LayerNormParams) == 2 * 4 + 3 * 8 + 4 * 4
+    assert C.sizeof(L.XentParams) == 6 * 4 + 3 * 8 + 2 * 4
+
+
+@pytest.mark.parametrize("kw", [dict(d=0), dict(rows=-1), dict(ld_x=15), dict(ld_y=15), dict(ld_dx=8), dict(x_type=2),
+                                dict(w_type=-1), dict(y_type=7)])
+def test_layernorm_refuses(kw):
+    from video_asl_recognition_amd import _lib as L
+    p = _norm(L, **kw)
+    assert L.lib.asl_layernorm_fwd(C.byref(p), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == L.ASL_EINVAL
+    assert L.lib.asl_layernorm_bwd(C.byref(p), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == L.ASL_EINVAL
+    assert L.lib.asl_layernorm_bwd_workspace(C.byref(p)) == L.ASL_EINVAL
+
+
+def test_layernorm_refuses_pointers():
+    from video_asl_recognition_amd import _lib as L
+    p = _norm(L)
+    assert L.lib.asl_layernorm_fwd(None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == L.ASL_EINVAL
+    for i in (0, 3):             # x, y
+        args = [FAKE] * 6
+        args[i] = None
+        assert L.lib.asl_layernorm_fwd(C.byref(p), *args, None) == L.ASL_EINVAL
+    for i in range(6):
+        args = [FAKE] * 6
+        args[i] = OFF
+        assert L.lib.asl_layernorm_fwd(C.byref(p), *args, None) == L.ASL_EINVAL
+    for i in (0, 1, 3, 4, 5, 8):
+        args = [FAKE] * 9
+        args[i] = None
+        assert L.lib.asl_layernorm_bwd(C.byref(p), *args, None) == L.ASL_EINVAL
+    for i in range(9):
+        args = [FAKE] * 9
+        args[i] = OFF
+        assert L.lib.asl_layernorm_bwd(C.byref(p), *args, None) == L.ASL_EINVAL
+    p = _norm(L, rows=0)         # nothing to do, nothing launched
+    assert L.lib.asl_layernorm_fwd(C.byref(p), None, None, None, None, None, None, None) == L.ASL_OK
+
+
+@pytest.mark.parametrize("kw", [dict(n=-1), dict(classes=0), dict(d=0), dict(type=2), dict(bias_type=3), dict(reduction=3),
+                                dict(reduction=-1), dict(ld_x=15), dict(ld_w=15), dict(label_smoothing=-0.1),
+                                dict(label_smoothing=1.5), dict(label_smoothing=float("nan"))])
+def test_xent_refuses(kw):
+    from video_asl_recognition_amd import _lib as L
+    p = _xent(L, **kw)
+    assert L.lib.asl_linear_xent_fwd(C.byref(p), *[FAKE] * 7, None) == L.ASL_EINVAL
+    assert L.lib.asl_linear_xent_grad(C.byref(p), *[FAKE] * 11, None) == L.ASL_EINVAL
+    assert L.lib.asl_linear_xent_workspace(C.byref(p), 1) == L.ASL_EINVAL
+
+
+def test_xent_refuses_pointers_and_sizes():
+    from video_asl_recognition_amd import _lib as L
+    p = _xent(L)
+    for i in (0, 1, 3, 4, 6):    # x, w, target, loss, workspace
+        args = [FAKE] * 7
+        args[i] = None
+        assert L.lib.asl_linear_xent_fwd(C.byref(p), *args, None) == L.ASL_EINVAL
+    for i in range(7):
+        args = [FAKE] * 7
+        args[i] = OFF
+        assert L.lib.asl_linear_xent_fwd(C.byref(p), *args, None) == L.ASL_EINVAL
+    for i in range(11):
+        args = [FAKE] * 11
+        args[i] = OFF
+        assert L.lib.asl_linear_xent_grad(C.byref(p), *args, None) == L.ASL_EINVAL
+    for kw in (dict(classes=(1 << 21) + 1), dict(n=(1 << 28) + 1), dict(d=(1 << 20) + 1, ld_x=1 << 21, ld_w=1 << 21)):
+        p = _xent(L, **kw)
+        assert L.lib.asl_linear_xent_workspace(C.byref(p), 0) == L.ASL_ETOOBIG
+
+
+def test_xent_workspace_of_no_rows():
+    from video_asl_recognition_amd import _lib as L
+    for grad in (0, 1):
+        assert L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=0)), grad) >= 0
+
+
+def test_xent_workspace_is_bounded():
+    """a hundred times the rows do not take a hundred times the exponentials"""
+    from video_asl_recognition_amd import _lib as L
+    one = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=16384, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), 1)
+    many = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=1638400, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), 1)
+    assert 1 << 30 <= one <= 3 << 30 and many < 2 * one
+    small = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=16384, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), 0)
+    assert small < 1 << 28
+
+
+def _clip(L, n=2, numel=(8, 8), ptrs=(0x1000, 0x2000), types=(0, 0), out=(0x3000, 0x4000), otypes=(0, 0), max_norm=1.0, norm=FAKE,
+          ws=FAKE):
+    arr = lambda t, v: (t * len(v))(*v) if v is not None else None
+    return L.lib.asl_grad_clip(n, arr(C.c_void_p, ptrs), arr(C.c_int64, numel), arr(C.c_int32, types), arr(C.c_void_p, out),
+                               arr(C.c_int32, otypes), max_norm, 0, norm, ws, None)
+
+
+@pytest.mark.parametrize("kw", [dict(n=-1), dict(ptrs=None), dict(numel=None), dict(types=None), dict(otypes=None),
+                                dict(numel=(8, -1)), dict(types=(0, 2)), dict(otypes=(5, 0)), dict(ptrs=(0, 0x2000)),
+                                dict(out=(0x3000, 0)), dict(ptrs=(0x1002, 0x2000)), dict(out=(0x3001, 0x4000)),
+                                dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(norm=None), dict(norm=OFF), dict(ws=None),
+                                dict(ws=C.c_void_p(0x1004)),
+                                dict(out=(0x3000, 0x3010)),                      # outputs overlap each other
+                                dict(out=(0x2000, 0x4000)),                      # an output is another gradient
+                                dict(out=(0x1ff0, 0x4000)),                      # or reaches into one
+                                dict(ptrs=(0x1000, 0x1000), out=(0x1000, 0x1000)),   # the same tensor twice, in place
+                                dict(out=(0x1000, 0x4000), otypes=(1, 0))])      # in place, of another type
+def test_grad_clip_refuses(kw):
+    from video_asl_recognition_amd import _lib as L
+    assert _clip(L, **kw) == L.ASL_EINVAL
+
+
+def test_grad_clip_workspace():
+    from video_asl_recognition_amd import _lib as L
+    arr = lambda v: (C.c_int64 * len(v))(*v)
+    assert L.lib.asl_grad_clip_workspace(0, None) == 0
+    assert L.lib.asl_grad_clip_workspace(2, arr((0, 1))) == 8
+    assert L.lib.asl_grad_clip_workspace(2, arr((1 << 40, 1))) == 2048 * 8
+    assert L.lib.asl_grad_clip_workspace(2, arr((5, -1))) == L.ASL_EINVAL
+
+
+def test_python_refuses():
+    from video_asl_recognition_amd import training as T
+    x, w, b = torch.zeros(3, 8), torch.ones(8), torch.zeros(8)
+    t = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="GPU"):
+        T.layer_norm(x, w, b)
+    with pytest.raises(ValueError, match="GPU"):
+        T.linear_cross_entropy(x, torch.zeros(5, 8), t)
+    with pytest.raises(ValueError, match="GPU"):
+        T.clip_grads([x], 1.0)
+    with pytest.raises(ValueError, match="no gradients"):
+        T.grad_norm([])
+    with pytest.raises(ValueError, match="norm_type"):
+        T.clip_grads([x], 1.0, norm_type=3)
+    with pytest.raises(ValueError, match="max_norm"):
+        T.clip_grads([x], -1.0)
+    with pytest.raises(ValueError, match="weight"):
+        T.linear_cross_entropy(x, torch.zeros(5, 7), t)
+    assert not T._dense(torch.zeros(4, 4)[:, :2]) and T._dense(torch.zeros(4, 3).t()) and not T._dense(torch.zeros(1).expand(4))

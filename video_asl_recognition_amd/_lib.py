@@ -104,6 +104,20 @@ class AttnParams(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("batch", "t", "heads", "head_dim", "ld_qkv", "ld_out")]
 
 
+F32, BF16 = 0, 1
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+
+
+class LayerNormParams(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("d", C.c_int32), ("ld_x", C.c_int64), ("ld_y", C.c_int64), ("ld_dx", C.c_int64),
+                ("x_type", C.c_int32), ("w_type", C.c_int32), ("y_type", C.c_int32), ("eps", C.c_float)]
+
+
+class XentParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "classes", "d", "type", "bias_type", "reduction")] + [
+        (n, C.c_int64) for n in ("ld_x", "ld_w", "ignore_index")] + [("label_smoothing", C.c_float), ("reserved", C.c_int32)]
+
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(
         f"{LIB_PATH} is missing: build it with `make -C {os.path.join(_HERE, 'csrc')}` "
@@ -150,6 +164,14 @@ _PROTOS = {
     "asl_add_rows_f32": ([_P, _I, _I, _P, _I, _P, _P, _I, _P], C.c_int),
     "asl_cast_pad_bf16": ([_P, _I, _I, _P, _I, _P], C.c_int),
     "asl_attention_fwd": ([C.POINTER(AttnParams), _P, _P, _P], C.c_int),
+    "asl_layernorm_fwd": ([C.POINTER(LayerNormParams)] + [_P] * 7, C.c_int),
+    "asl_layernorm_bwd_workspace": ([C.POINTER(LayerNormParams)], C.c_int64),
+    "asl_layernorm_bwd": ([C.POINTER(LayerNormParams)] + [_P] * 10, C.c_int),
+    "asl_linear_xent_workspace": ([C.POINTER(XentParams), _I], C.c_int64),
+    "asl_linear_xent_fwd": ([C.POINTER(XentParams)] + [_P] * 8, C.c_int),
+    "asl_linear_xent_grad": ([C.POINTER(XentParams)] + [_P] * 12, C.c_int),
+    "asl_grad_clip_workspace": ([_I, _P], C.c_int64),
+    "asl_grad_clip": ([_I, _P, _P, _P, _P, _P, C.c_float, _I, _P, _P, _P], C.c_int),
     "asl_run_ops": ([C.POINTER(Op), _I, C.POINTER(C.c_void_p), _I, C.POINTER(C.c_int)], C.c_int),
 }
 

@@ -1,0 +1,249 @@
+// Global norm of many gradient tensors, and clipping by it, for gfx950.
+//
+//   n = sqrt(sum over all elements g^2)   or   n = max |g|;    c = min(1, max_norm / (n + 1e-6));    out = g c
+//
+// Two launches for up to kTensors tensors (two more for every kTensors further): the first leaves one partial a workgroup, the
+// second adds the partials up in every workgroup -- in the same order, so all see the same c -- and writes g c.  Tensors are
+// cut into chunks; a chunk's tensor is found by a binary search over the chunk counts, which travel with the pointers in the
+// kernel's arguments: nothing is copied to the device and nothing outlives the call.  The sum is held in 64 bits: the vector
+// pipe has room for it under the loads, the largest fp32 gradients do not overflow it, and its order does not show in the
+// result.  The second pass walks the chunks from the last to the first, because the end of what the first pass read is what
+// the 256 MB cache still holds.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
+#include "asl_hip.h"
+#include "train_common.h"
+
+namespace asl_detail {
+
+constexpr int kTensors = 96;              // per launch: 96 * 36 bytes of arguments and a little, under the 4 KiB they may take
+constexpr int kChunk = 8192;              // elements: 256 threads x 8 x 4
+constexpr int kClipBlocks = 2048;         // at most, per launch: 8 workgroups of 256 a CU
+
+struct ClipArgs {
+    const void* in[kTensors];
+    void* out[kTensors];
+    long long n[kTensors];
+    long long first[kTensors + 1];        // first chunk of each tensor in this launch; the last entry is the chunk count
+    unsigned char in_bf16[kTensors], out_bf16[kTensors];
+    double* part;
+    float* norm;
+    float max_norm;
+    int tensors, part0, parts, inf_norm, write_norm;
+};
+static_assert(sizeof(ClipArgs) <= 4096, "kernel arguments");
+
+// the larger of two magnitudes, a NaN before any number
+__device__ __forceinline__ double max_nan(double a, double b) { return (a > b || a != a) ? a : b; }
+
+__device__ __forceinline__ double combine(double a, double b, int inf_norm) { return inf_norm ? max_nan(a, b) : a + b; }
+
+// over the 256 threads of a workgroup, the same in every thread
+__device__ __forceinline__ double block_combine(double v, int inf_norm, double* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = combine(v, __shfl_xor(v, o, 64), inf_norm);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return combine(combine(lds[0], lds[1], inf_norm), combine(lds[2], lds[3], inf_norm), inf_norm);
+}
+
+__device__ __forceinline__ int tensor_of(const ClipArgs& a, long long chunk) {
+    int lo = 0, hi = a.tensors;           // first[lo] <= chunk < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.first[mid] <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void accumulate(const T* p, long long left, int inf_norm, double& v) {
+    F8 g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long k = (i * 256 + threadIdx.x) * 8LL;
+        g[i] = load8(p + (k < left ? k : 0), left - k > 8 ? 8 : (int)(left - k < 0 ? 0 : left - k));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double x = (double)g[i].v[e];
+            v = inf_norm ? max_nan(fabs(x), v) : v + x * x;
+        }
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(const ClipArgs a) {
+    __shared__ double lds[4];
+    double v = 0.0;
+    for (long long c = blockIdx.x; c < a.first[a.tensors]; c += gridDim.x) {
+        const int t = tensor_of(a, c);
+        const long long at = (c - a.first[t]) * kChunk;
+        if (a.in_bf16[t]) accumulate((const short*)a.in[t] + at, a.n[t] - at, a.inf_norm, v);
+        else accumulate((const float*)a.in[t] + at, a.n[t] - at, a.inf_norm, v);
+    }
+    v = block_combine(v, a.inf_norm, lds);
+    if (threadIdx.x == 0) a.part[a.part0 + blockIdx.x] = v;
+}
+
+template <typename T, typename U>
+__device__ __forceinline__ void scale_chunk(const T* p, U* q, long long left, float c) {
+    F8 g[4];
+    int n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long k = (i * 256 + threadIdx.x) * 8LL;
+        n[i] = left - k > 8 ? 8 : (int)(left - k < 0 ? 0 : left - k);
+        g[i] = load8(p + (k < left ? k : 0), n[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (n[i] > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[i].v[e] *= c;
+            store8(q + (i * 256 + threadIdx.x) * 8LL, n[i], g[i]);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void grad_scale_kernel(const ClipArgs a) {
+    __shared__ double lds[4];
+    double v = 0.0;
+    for (int i = threadIdx.x; i < a.parts; i += 256) v = combine(v, a.part[i], a.inf_norm);
+    v = block_combine(v, a.inf_norm, lds);
+    const float norm = (float)(a.inf_norm ? v : sqrt(v));
+    if (a.write_norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+    // a norm that is not a number makes every gradient one, an infinite norm makes them nought (and NaN where infinite)
+    const float r = a.max_norm / (norm + 1e-6f);
+    const float c = r > 1.0f ? 1.0f : r;
+    const long long chunks = a.first[a.tensors];
+    for (long long i = blockIdx.x; i < chunks; i += gridDim.x) {
+        const long long k = chunks - 1 - i;
+        const int t = tensor_of(a, k);
+        if (c == 1.0f && a.in[t] == a.out[t]) continue;        // in place and nothing to clip: as it is
+        const long long at = (k - a.first[t]) * kChunk, left = a.n[t] - at;
+        if (a.in_bf16[t]) {
+            if (a.out_bf16[t]) scale_chunk((const short*)a.in[t] + at, (short*)a.out[t] + at, left, c);
+            else scale_chunk((const short*)a.in[t] + at, (float*)a.out[t] + at, left, c);
+        } else {
+            if (a.out_bf16[t]) scale_chunk((const float*)a.in[t] + at, (short*)a.out[t] + at, left, c);
+            else scale_chunk((const float*)a.in[t] + at, (float*)a.out[t] + at, left, c);
+        }
+    }
+}
+
+// the norm alone: one workgroup over the partials
+__global__ __launch_bounds__(256) void grad_norm_finish_kernel(const double* part, int parts, int inf_norm, float* norm) {
+    __shared__ double lds[4];
+    double v = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) v = combine(v, part[i], inf_norm);
+    v = block_combine(v, inf_norm, lds);
+    if (threadIdx.x == 0) *norm = (float)(inf_norm ? v : sqrt(v));
+}
+
+inline int launch_parts(long long chunks) { return (int)(chunks < kClipBlocks ? chunks : kClipBlocks); }
+
+// an output may be its own input, in place and of the same type; any other overlap of an output would race
+bool overlaps(int count, const void* const* in, void* const* out, const int64_t* numel, const int32_t* in_type,
+              const int32_t* out_type) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> outs, ins;
+    for (int i = 0; i < count; ++i) {
+        if (!numel[i]) continue;
+        const uintptr_t o = (uintptr_t)out[i], p = (uintptr_t)in[i];
+        outs.push_back({o, o + numel[i] * (out_type[i] ? 2 : 4)});
+        if (p != o) ins.push_back({p, p + numel[i] * (in_type[i] ? 2 : 4)});
+        else if (in_type[i] != out_type[i]) return true;
+    }
+    std::sort(outs.begin(), outs.end());
+    for (size_t i = 1; i < outs.size(); ++i)
+        if (outs[i].first < outs[i - 1].second) return true;
+    for (const auto& q : ins) {          // outs are disjoint and sorted: only the last that begins before q's end can reach it
+        auto it = std::lower_bound(outs.begin(), outs.end(), std::make_pair(q.second, (uintptr_t)0));
+        if (it != outs.begin() && (it - 1)->second > q.first) return true;
+    }
+    return false;
+}
+
+}  // namespace asl_detail
+using namespace asl_detail;
+
+extern "C" int64_t asl_grad_clip_workspace(int count, const int64_t* numel) {
+    if (count < 0 || (count && !numel)) return ASL_EINVAL;
+    long long parts = 0, chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        if (numel[i] < 0) return ASL_EINVAL;
+        chunks += (numel[i] + kChunk - 1) / kChunk;
+        if (i % kTensors == kTensors - 1 || i == count - 1) {
+            parts += launch_parts(chunks);
+            chunks = 0;
+        }
+    }
+    return parts * (int64_t)sizeof(double);
+}
+
+extern "C" int asl_grad_clip(int count, const void* const* grads, const int64_t* numel, const int32_t* in_type,
+                             void* const* out, const int32_t* out_type, float max_norm, int inf_norm, float* norm,
+                             double* workspace, asl_stream_t stream) {
+    if (count < 0 || !norm || ((uintptr_t)norm & 3) || ((uintptr_t)workspace & 7)) return ASL_EINVAL;
+    if (count && (!grads || !numel || !in_type)) return ASL_EINVAL;
+    if (out && (!out_type || !(max_norm >= 0.f))) return ASL_EINVAL;
+    const int64_t need = asl_grad_clip_workspace(count, numel);
+    if (need < 0 || (need && !workspace)) return ASL_EINVAL;
+    for (int i = 0; i < count; ++i) {
+        if (in_type[i] < 0 || in_type[i] > 1 || (out && (out_type[i] < 0 || out_type[i] > 1))) return ASL_EINVAL;
+        if (!numel[i]) continue;
+        if (!grads[i] || ((uintptr_t)grads[i] & (in_type[i] ? 1 : 3))) return ASL_EINVAL;
+        if (out && (!out[i] || ((uintptr_t)out[i] & (out_type[i] ? 1 : 3)))) return ASL_EINVAL;
+    }
+    if (out && count) {
+        try {
+            if (overlaps(count, grads, out, numel, in_type, out_type)) return ASL_EINVAL;
+        } catch (const std::bad_alloc&) {
+            return ASL_ETOOBIG;
+        }
+    }
+    hipStream_t s = (hipStream_t)stream;
+    const int parts = (int)(need / (int64_t)sizeof(double));
+    const auto fill = [&](ClipArgs& a, int t0) {
+        a.tensors = count - t0 < kTensors ? count - t0 : kTensors;
+        a.first[0] = 0;
+        for (int i = 0; i < a.tensors; ++i) {
+            a.in[i] = grads[t0 + i];
+            a.out[i] = out ? out[t0 + i] : nullptr;
+            a.n[i] = numel[t0 + i];
+            a.in_bf16[i] = (unsigned char)in_type[t0 + i];
+            a.out_bf16[i] = out ? (unsigned char)out_type[t0 + i] : 0;
+            a.first[i + 1] = a.first[i] + (a.n[i] + kChunk - 1) / kChunk;
+        }
+        return launch_parts(a.first[a.tensors]);
+    };
+    ClipArgs a;
+    a.part = workspace; a.norm = norm; a.max_norm = max_norm; a.parts = parts; a.inf_norm = inf_norm ? 1 : 0;
+    a.part0 = 0;
+    for (int t0 = 0; t0 < count; t0 += kTensors) {
+        const int blocks = fill(a, t0);
+        if (!blocks) continue;
+        hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        a.part0 += blocks;
+    }
+    if (!out || !parts) {
+        hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(256), 0, s, workspace, parts, inf_norm ? 1 : 0, norm);
+        return (int)hipGetLastError();
+    }
+    a.write_norm = 1;
+    // the last launch's tensors first: they are what the cache still holds
+    for (int t0 = (count - 1) / kTensors * kTensors; t0 >= 0; t0 -= kTensors) {
+        const int blocks = fill(a, t0);
+        if (!blocks) continue;
+        hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        a.write_norm = 0;
+    }
+    return (int)hipGetLastError();
+}

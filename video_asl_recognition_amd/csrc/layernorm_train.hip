@@ -1,0 +1,513 @@
+// LayerNorm for training on gfx950: forward with saved statistics, and backward with the reduction of the weight's and
+// bias's gradients.
+//
+//   mu = mean x,  r = 1 / sqrt(mean (x - mu)^2 + eps),  h = (x - mu) r,  y = h w + b
+//   g = dy w,  dx = r (g - mean g - h mean(g h)),  dw = sum over rows of dy h,  db = sum over rows of dy
+//
+// Both directions move bytes and little else, so a row is read once: a group of G lanes (a quarter wave up to a workgroup of
+// 1024) holds it in registers, J vectors of eight elements a lane, and all sums are taken there, in fp32, the variance about
+// the mean that was just found.  Backward keeps each lane's columns fixed while its group walks over rows, so the column
+// sums dw and db also stay in registers; a workgroup leaves one partial row of each in the workspace and a second launch
+// adds those up in a fixed order (no atomics: results do not vary from run to run).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "asl_hip.h"
+#include "train_common.h"
+
+namespace asl_detail {
+
+// eight of a weight or bias, or of the constant that stands for a missing one
+__device__ __forceinline__ F8 load8_or(const void* base, int bf16, long long at, int n, float missing) {
+    if (base) return load8_any(base, bf16, at, n);
+    return {{missing, missing, missing, missing, missing, missing, missing, missing}};
+}
+
+struct LnArgs {
+    const void* x;
+    const void* dy;
+    const void* w;
+    const void* b;
+    void* y;                 // forward: y; backward: dx
+    float* mean;
+    float* rstd;
+    float* part;             // backward: [blocks][2][d] column sums
+    long long ld_x, ld_y, ld_dy;
+    int rows, d, w_bf16;
+    float eps;
+};
+
+// a variance that rounding took below nought is nought; a NaN stays one (fmaxf would hide it)
+__device__ __forceinline__ float not_below_nought(float v) { return v < 0.f ? 0.f : v; }
+
+// Sum over the G lanes of a group, the same in every lane.  Groups wider than a wave meet in LDS: `slot` alternates from
+// call to call, so one barrier a call is enough (a slot is written again only behind the next call's barrier).
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float* lds, int& slot) {
+    constexpr int W = G < 64 ? G : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], o, 64);
+    if constexpr (G > 64) {
+        constexpr int NW = G / 64;
+        float* s = lds + slot * (NW * N);
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < N; ++k) s[(threadIdx.x >> 6) * N + k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) t += s[i * N + k];
+            v[k] = t;
+        }
+        slot ^= 1;
+    }
+}
+
+template <typename XT, typename YT, int G, int J>
+__global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs a) {
+    constexpr int BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
+    __shared__ float lds[2 * 2 * (G > 64 ? G / 64 : 1)];
+    int slot = 0;
+    const int t = threadIdx.x % G;
+    const float inv_d = 1.0f / (float)a.d;
+    // w and b stay in registers from row to row; a workgroup of 1024 has 128 registers a lane and reads them again instead
+    constexpr bool HOLD = G < 1024;
+    F8 w[HOLD ? J : 1], b[HOLD ? J : 1];
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            w[j] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, a.d - k, 1.f);
+            b[j] = load8_or(a.b, a.w_bf16, k < a.d ? k : 0, a.d - k, 0.f);
+        }
+    }
+    for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB) {
+        const long long row = row0 + threadIdx.x / G;
+        if (G <= 64 && row >= a.rows) return;        // groups within a wave share no barrier
+        const XT* xr = (const XT*)a.x + row * a.ld_x;
+        F8 x[J];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            x[j] = load8(xr + (k < a.d ? k : 0), a.d - k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[0] += x[j].v[e];
+        }
+        group_sum<G>(s, lds, slot);
+        const float mean = s[0] * inv_d;
+        // about the rounded mean; the rest of the mean that its rounding left comes out of the same pass, so a row of
+        // equal large values has variance nought and not the square of its last bit
+        float q[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int n = a.d - (t + j * G) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[j].v[e] = e < n ? x[j].v[e] - mean : 0.f;
+                q[0] += x[j].v[e];
+                q[1] += x[j].v[e] * x[j].v[e];
+            }
+        }
+        group_sum<G>(q, lds, slot);
+        const float rest = q[0] * inv_d;
+        const float rstd = 1.0f / sqrtf(not_below_nought(q[1] * inv_d - rest * rest) + a.eps);
+        YT* yr = (YT*)a.y + row * a.ld_y;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            if (k < a.d) {
+                if constexpr (!HOLD) {
+                    w[0] = load8_or(a.w, a.w_bf16, k, a.d - k, 1.f);
+                    b[0] = load8_or(a.b, a.w_bf16, k, a.d - k, 0.f);
+                }
+                const F8 &wj = w[HOLD ? j : 0], &bj = b[HOLD ? j : 0];
+                F8 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[e] = (x[j].v[e] - rest) * rstd * wj.v[e] + bj.v[e];
+                store8(yr + k, a.d - k, o);
+            }
+        }
+        if (t == 0) {
+            if (a.mean) a.mean[row] = mean + rest;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+// rows longer than the registers of a workgroup: the same sums in three passes over the row, the later two from L2
+template <typename XT, typename YT>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
+    constexpr int G = 1024;
+    __shared__ float lds[2 * 2 * (G / 64)];
+    int slot = 0;
+    const int t = threadIdx.x;
+    const float inv_d = 1.0f / (float)a.d;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const XT* xr = (const XT*)a.x + row * a.ld_x;
+        float s[1] = {0.f};
+        for (int k = t * 8; k < a.d; k += G * 8) {
+            const F8 x = load8(xr + k, a.d - k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[0] += x.v[e];
+        }
+        group_sum<G>(s, lds, slot);
+        const float mean = s[0] * inv_d;
+        float q[2] = {0.f, 0.f};
+        for (int k = t * 8; k < a.d; k += G * 8) {
+            const F8 x = load8(xr + k, a.d - k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float c = k + e < a.d ? x.v[e] - mean : 0.f;
+                q[0] += c;
+                q[1] += c * c;
+            }
+        }
+        group_sum<G>(q, lds, slot);
+        const float rest = q[0] * inv_d;
+        const float rstd = 1.0f / sqrtf(not_below_nought(q[1] * inv_d - rest * rest) + a.eps);
+        YT* yr = (YT*)a.y + row * a.ld_y;
+        for (int k = t * 8; k < a.d; k += G * 8) {
+            const F8 x = load8(xr + k, a.d - k);
+            const F8 w = load8_or(a.w, a.w_bf16, k, a.d - k, 1.f), b = load8_or(a.b, a.w_bf16, k, a.d - k, 0.f);
+            F8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o.v[e] = (x.v[e] - mean - rest) * rstd * w.v[e] + b.v[e];
+            store8(yr + k, a.d - k, o);
+        }
+        if (t == 0) {
+            if (a.mean) a.mean[row] = mean + rest;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+template <typename XT, typename YT, int G, int J>
+__global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs a) {
+    constexpr int BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
+    __shared__ float lds[2 * 2 * (G > 64 ? G / 64 : 1)];
+    __shared__ __attribute__((aligned(16))) float cols[RPB > 1 ? (BLOCK / 64) * 2 * (G < 64 ? G : 64) * J * 8 : 1];
+    int slot = 0;
+    const int t = threadIdx.x % G;
+    const float inv_d = 1.0f / (float)a.d;
+    constexpr bool HOLD = G * J < 2048;
+    F8 w[HOLD ? J : 1], dw[J], db[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int k = (t + j * G) * 8;
+        if constexpr (HOLD) w[j] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, a.d - k, 1.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[j].v[e] = db[j].v[e] = 0.f;
+    }
+    for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB) {
+        const long long row = row0 + threadIdx.x / G;
+        if (G <= 64 && row >= a.rows) break;         // groups within a wave share no barrier inside the loop
+        const XT* xr = (const XT*)a.x + row * a.ld_x;
+        const YT* dyr = (const YT*)a.dy + row * a.ld_dy;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        F8 h[J], g[J];
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8, n = a.d - k;
+            h[j] = load8(xr + (k < a.d ? k : 0), n);
+            g[j] = load8(dyr + (k < a.d ? k : 0), n);
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8, n = a.d - k;
+            if constexpr (!HOLD) w[0] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, n, 1.f);
+            const F8& wj = w[HOLD ? j : 0];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[j].v[e] = e < n ? (h[j].v[e] - mean) * rstd : 0.f;
+                dw[j].v[e] += g[j].v[e] * h[j].v[e];
+                db[j].v[e] += g[j].v[e];
+                g[j].v[e] *= wj.v[e];
+                s[0] += g[j].v[e];
+                s[1] += g[j].v[e] * h[j].v[e];
+            }
+        }
+        group_sum<G>(s, lds, slot);
+        const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
+        XT* dxr = (XT*)a.y + row * a.ld_y;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            if (k < a.d) {
+                F8 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[e] = (g[j].v[e] - m0 - h[j].v[e] * m1) * rstd;
+                store8(dxr + k, a.d - k, o);
+            }
+        }
+    }
+    float* part = a.part + (long long)blockIdx.x * 2 * a.d;
+    if constexpr (RPB == 1) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            if (k < a.d) {
+                store8(part + k, a.d - k, dw[j]);
+                store8(part + a.d + k, a.d - k, db[j]);
+            }
+        }
+    } else {
+        // several groups a workgroup: within the wave by lane exchange, then the waves' sums through LDS
+        constexpr int COLS = (G < 64 ? G : 64) * J * 8, NW = BLOCK / 64;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int o = 32; o >= G; o >>= 1) {
+                    dw[j].v[e] += __shfl_xor(dw[j].v[e], o, 64);
+                    db[j].v[e] += __shfl_xor(db[j].v[e], o, 64);
+                }
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        if (lane < G) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int k = (t + j * G) * 8;
+                store8_full(cols + (wave * 2 + 0) * COLS + k, dw[j]);
+                store8_full(cols + (wave * 2 + 1) * COLS + k, db[j]);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * COLS; i += BLOCK) {
+            const int which = i / COLS, k = i % COLS;
+            float v = 0.f;
+#pragma unroll
+            for (int q = 0; q < NW; ++q) v += cols[(q * 2 + which) * COLS + k];
+            if (k < a.d) part[which * a.d + k] = v;
+        }
+    }
+}
+
+// rows longer than the registers of a workgroup: sums, then dx, from re-read rows; the column sums live in the workgroup's
+// partial row in memory, each element read and written by the one thread that owns it
+template <typename XT, typename YT>
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
+    constexpr int G = 1024;
+    __shared__ float lds[2 * 2 * (G / 64)];
+    int slot = 0;
+    const int t = threadIdx.x;
+    const float inv_d = 1.0f / (float)a.d;
+    float* part = a.part + (long long)blockIdx.x * 2 * a.d;
+    const F8 zero = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+    for (int k = t * 8; k < a.d; k += G * 8) {
+        store8(part + k, a.d - k, zero);
+        store8(part + a.d + k, a.d - k, zero);
+    }
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const XT* xr = (const XT*)a.x + row * a.ld_x;
+        const YT* dyr = (const YT*)a.dy + row * a.ld_dy;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s[2] = {0.f, 0.f};
+        for (int k = t * 8; k < a.d; k += G * 8) {
+            const int n = a.d - k;
+            const F8 x = load8(xr + k, n), dy = load8(dyr + k, n), w = load8_or(a.w, a.w_bf16, k, n, 1.f);
+            F8 pw = load8(part + k, n), pb = load8(part + a.d + k, n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float h = (x.v[e] - mean) * rstd, g = dy.v[e] * w.v[e];     // dy is nought behind the row's end
+                pw.v[e] += dy.v[e] * h;
+                pb.v[e] += dy.v[e];
+                s[0] += g;
+                s[1] += g * h;
+            }
+            store8(part + k, n, pw);
+            store8(part + a.d + k, n, pb);
+        }
+        group_sum<G>(s, lds, slot);
+        const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
+        XT* dxr = (XT*)a.y + row * a.ld_y;
+        for (int k = t * 8; k < a.d; k += G * 8) {
+            const int n = a.d - k;
+            const F8 x = load8(xr + k, n), dy = load8(dyr + k, n), w = load8_or(a.w, a.w_bf16, k, n, 1.f);
+            F8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o.v[e] = (dy.v[e] * w.v[e] - m0 - (x.v[e] - mean) * rstd * m1) * rstd;
+            store8(dxr + k, n, o);
+        }
+    }
+}
+
+// dw and db: the workgroups' partial rows [parts][2][d] added up, 16 columns-of-four by 16 row strides a workgroup
+__global__ __launch_bounds__(256) void ln_cols_kernel(const float* __restrict__ part, int parts, int d, void* dw, void* db,
+                                                      int bf16) {
+    __shared__ float s[16][64 + 1];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const long long cols = 2LL * d, c0 = (long long)blockIdx.x * 64 + c * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c0 < cols) {
+        const int n = cols - c0 < 4 ? (int)(cols - c0) : 4;
+#pragma unroll 4
+        for (int p = r; p < parts; p += 16) {
+            const float* src = part + p * cols + c0;
+            if (n == 4) {
+                const f32x4u q = *(const f32x4u*)src;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += q[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < n) v[e] += src[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[r][c * 4 + e] = v[e];
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const long long col = (long long)blockIdx.x * 64 + threadIdx.x;
+        if (col < cols) {
+            float o = 0.f;
+#pragma unroll
+            for (int p = 0; p < 16; ++p) o += s[p][threadIdx.x];
+            void* out = col < d ? dw : db;
+            const long long at = col < d ? col : col - d;
+            if (out) {
+                if (bf16) store1((short*)out + at, o);
+                else store1((float*)out + at, o);
+            }
+        }
+    }
+}
+
+// Lanes a row and vectors a lane, by the row's length.  Forward holds one row (8 J registers), so a wave takes up to 2048
+// elements; backward holds x, dy, w and two column sums (40 J registers), so a wave takes up to 1024.
+struct LnShape {
+    int g, j;
+};
+inline LnShape fwd_shape(int d) {
+    if (d <= 128) return {16, 1};
+    if (d <= 512) return {64, 1};
+    if (d <= 1024) return {64, 2};
+    if (d <= 2048) return {64, 4};
+    if (d <= 4096) return {256, 2};
+    if (d <= 8192) return {256, 4};
+    if (d <= 32768) return {1024, 4};
+    return {0, 0};
+}
+inline LnShape bwd_shape(int d) {
+    if (d <= 128) return {16, 1};
+    if (d <= 512) return {64, 1};
+    if (d <= 1024) return {64, 2};
+    if (d <= 2048) return {256, 1};
+    if (d <= 4096) return {256, 2};
+    if (d <= 8192) return {1024, 1};
+    if (d <= 16384) return {1024, 2};
+    return {0, 0};
+}
+inline int rows_per_block(int g) { return g == 0 || g > 256 ? 1 : 256 / g; }
+
+// workgroups of a backward call = partial rows of its column sums: a few a CU, so that the partial rows stay small
+// against the tensors
+inline int bwd_blocks(int rows, int d) {
+    const int rpb = rows_per_block(bwd_shape(d).g);
+    const long long need = ((long long)rows + rpb - 1) / rpb;
+    return (int)(need < 512 ? need : 512);
+}
+
+template <typename XT, typename YT>
+int launch_fwd(const LnArgs& a, hipStream_t s) {
+    const LnShape sh = fwd_shape(a.d);
+    const int rpb = rows_per_block(sh.g);
+    const long long need = ((long long)a.rows + rpb - 1) / rpb;
+    const dim3 grid((unsigned)(need < 4096 ? need : 4096)), b256(256), b1024(1024);
+    switch (sh.g * 8 + sh.j) {
+        case 16 * 8 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 16, 1>), grid, b256, 0, s, a); break;
+        case 64 * 8 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
+        case 64 * 8 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
+        case 64 * 8 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 4>), grid, b256, 0, s, a); break;
+        case 256 * 8 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
+        case 256 * 8 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 4>), grid, b256, 0, s, a); break;
+        case 1024 * 8 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 1024, 4>), grid, b1024, 0, s, a); break;
+        default: hipLaunchKernelGGL((ln_fwd_long_kernel<XT, YT>), grid, b1024, 0, s, a); break;
+    }
+    return (int)hipGetLastError();
+}
+
+template <typename XT, typename YT>
+int launch_bwd(const LnArgs& a, int blocks, hipStream_t s) {
+    const LnShape sh = bwd_shape(a.d);
+    const dim3 grid((unsigned)blocks), b256(256), b1024(1024);
+    switch (sh.g * 8 + sh.j) {
+        case 16 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 16, 1>), grid, b256, 0, s, a); break;
+        case 64 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
+        case 64 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
+        case 256 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 1>), grid, b256, 0, s, a); break;
+        case 256 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
+        case 1024 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 1>), grid, b1024, 0, s, a); break;
+        case 1024 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 2>), grid, b1024, 0, s, a); break;
+        default: hipLaunchKernelGGL((ln_bwd_long_kernel<XT, YT>), grid, b1024, 0, s, a); break;
+    }
+    return (int)hipGetLastError();
+}
+
+int ln_check(const asl_layernorm_params* p) {
+    if (!p || p->rows < 0 || p->d <= 0 || p->d > (1 << 30)) return ASL_EINVAL;
+    if (p->x_type < 0 || p->x_type > 1 || p->w_type < 0 || p->w_type > 1 || p->y_type < 0 || p->y_type > 1) return ASL_EINVAL;
+    if (p->ld_x < p->d || p->ld_y < p->d || p->ld_dx < p->d) return ASL_EINVAL;
+    return ASL_OK;
+}
+inline bool misaligned(const void* p, int type) { return ((uintptr_t)p & (type ? 1 : 3)) != 0; }
+
+}  // namespace asl_detail
+using namespace asl_detail;
+
+extern "C" int asl_layernorm_fwd(const asl_layernorm_params* p, const void* x, const void* gamma, const void* beta, void* y,
+                                 float* mean, float* rstd, asl_stream_t stream) {
+    const int rc = ln_check(p);
+    if (rc != ASL_OK) return rc;
+    if (p->rows == 0) return ASL_OK;
+    if (!x || !y) return ASL_EINVAL;
+    if (misaligned(x, p->x_type) || misaligned(y, p->y_type) || misaligned(gamma, p->w_type) || misaligned(beta, p->w_type) ||
+        misaligned(mean, 0) || misaligned(rstd, 0))
+        return ASL_EINVAL;
+    LnArgs a = {};
+    a.x = x; a.w = gamma; a.b = beta; a.y = y; a.mean = mean; a.rstd = rstd;
+    a.ld_x = p->ld_x; a.ld_y = p->ld_y; a.rows = p->rows; a.d = p->d; a.w_bf16 = p->w_type; a.eps = p->eps;
+    hipStream_t s = (hipStream_t)stream;
+    if (p->x_type) return p->y_type ? launch_fwd<short, short>(a, s) : launch_fwd<short, float>(a, s);
+    return p->y_type ? launch_fwd<float, short>(a, s) : launch_fwd<float, float>(a, s);
+}
+
+extern "C" int64_t asl_layernorm_bwd_workspace(const asl_layernorm_params* p) {
+    if (ln_check(p) != ASL_OK) return ASL_EINVAL;
+    return (int64_t)bwd_blocks(p->rows, p->d) * 2 * p->d * (int64_t)sizeof(float);
+}
+
+extern "C" int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void* x, const void* gamma,
+                                 const float* mean, const float* rstd, void* dx, void* dgamma, void* dbeta, float* workspace,
+                                 asl_stream_t stream) {
+    const int rc = ln_check(p);
+    if (rc != ASL_OK) return rc;
+    if (!dgamma && !dbeta && p->rows == 0) return ASL_OK;
+    if (p->rows && (!dy || !x || !mean || !rstd || !dx || !workspace)) return ASL_EINVAL;
+    if (misaligned(dy, p->y_type) || misaligned(x, p->x_type) || misaligned(gamma, p->w_type) || misaligned(dx, p->x_type) ||
+        misaligned(dgamma, p->w_type) || misaligned(dbeta, p->w_type) || misaligned(mean, 0) || misaligned(rstd, 0) ||
+        ((uintptr_t)workspace & 15))
+        return ASL_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    const int blocks = bwd_blocks(p->rows, p->d);
+    if (blocks) {
+        LnArgs a = {};
+        a.x = x; a.dy = dy; a.w = gamma; a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.part = workspace;
+        a.ld_x = p->ld_x; a.ld_y = p->ld_dx; a.ld_dy = p->ld_y; a.rows = p->rows; a.d = p->d; a.w_bf16 = p->w_type;
+        int e;
+        if (p->x_type) e = p->y_type ? launch_bwd<short, short>(a, blocks, s) : launch_bwd<short, float>(a, blocks, s);
+        else e = p->y_type ? launch_bwd<float, short>(a, blocks, s) : launch_bwd<float, float>(a, blocks, s);
+        if (e) return e;
+    }
+    if (dgamma || dbeta) {
+        const unsigned nb = (unsigned)((2LL * p->d + 63) / 64);
+        hipLaunchKernelGGL(ln_cols_kernel, dim3(nb), dim3(256), 0, s, workspace, blocks, p->d, dgamma, dbeta, p->w_type);
+    }
+    return (int)hipGetLastError();
+}

@@ -1,0 +1,644 @@
+// Linear + softmax cross entropy over a class vocabulary, with gradients, for gfx950.
+//
+//   l = x W^T + b,  lse = log sum_j exp l_j,  loss = lse - (1 - e) l_t - (e / V) sum_j l_j          (e: label smoothing)
+//   G = g (softmax(l) - (1 - e) [j = t] - e / V),  dx = G W,  dW = G^T x,  db = sum over rows of G   (g: the row's weight)
+//
+// The logits are never held.  Rows are taken in pieces; the product x W^T leaves, for every row and every tile of classes, the
+// tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself in the operands' type
+// (between 0 and 1, so 16 bits keep it to 2^-8 of its value).  One pass over the per-tile numbers gives lse, the loss and
+// the factors g exp(m - lse); one pass over the exponentials turns them into G in place, the target's entry from its own
+// 32-bit logit (g expm1(l_t - lse), where p - 1 of a rounded p would cancel), and adds up db in 32 bits.  Then two products.
+//
+// Both gradient products have operands whose contraction index is not the contiguous one; see the tile kernels.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "asl_hip.h"
+#include "train_common.h"
+
+namespace asl_detail {
+
+// D[j][i] = sum over k of P(i, k) Q(j, k).  P is the MFMA's row operand, so a lane ends up with four consecutive i of one j
+// and D is stored along i.  Each operand is contiguous along k ("KC") or along its own index.
+struct XentGemm {
+    const void* p;
+    const void* q;
+    long long ld_p, ld_q;    // elements from one row of the stored matrix to the next
+    int I, Jn, K;
+    // plain products
+    void* out;               // of the operands' type, or fp32 slabs [gridDim.z][Jn][I] when slabs != 0
+    long long ld_out;
+    int slabs, add, k_per_split;
+    // logits
+    const void* bias;
+    int bias_bf16, smooth, store_e;
+    const long long* target; // of row j
+    float* tile_max;         // [Jn][tiles]
+    float* tile_sum;         // [Jn][tiles]
+    float* tile_lin;         // [Jn][tiles]: sum of the logits (label smoothing)
+    float* target_logit;     // [Jn]
+    int tiles;
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<short> {
+    static constexpr int BK = 64, PAD = 8, KSTEP = 32;
+    using Frag = bf16x8;
+    static __device__ __forceinline__ Frag frag(const short* row, int k0, int q) { return *(const bf16x8*)(row + k0 + q * 8); }
+    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#else
+        return c;
+#endif
+    }
+    static __device__ __forceinline__ float exp_(float v) { return __expf(v); }
+};
+template <>
+struct Mma<float> {
+    static constexpr int BK = 32, PAD = 4, KSTEP = 4;
+    using Frag = float;
+    static __device__ __forceinline__ Frag frag(const float* row, int k0, int q) { return row[k0 + q]; }
+    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+#else
+        return c;
+#endif
+    }
+    static __device__ __forceinline__ float exp_(float v) { return expf(v); }
+};
+
+constexpr int kTile = 64;                 // of either index in the general kernel
+
+// one thread's share of a 64 x BK operand tile: held in registers while the previous tile is multiplied
+template <typename T, bool KC>
+struct Stage {
+    static constexpr int BK = Mma<T>::BK, LD = BK + Mma<T>::PAD, N = kTile * BK / 8 / 256;
+    F8 r[N];
+    __device__ __forceinline__ void load(const T* base, long long ld, int row0, int rows, int k0, int k1) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int v = u * 256 + threadIdx.x;
+            const int a = KC ? v / (BK / 8) : v / (kTile / 8), c = (KC ? v % (BK / 8) : v % (kTile / 8)) * 8;
+            // KC: stored row = operand index; else stored row = contraction index
+            const int srow = (KC ? row0 : k0) + a, scol = (KC ? k0 : row0) + c;
+            const bool ok = srow < (KC ? rows : k1);
+            const int n = ok ? (KC ? k1 : rows) - scol : 0;
+            r[u] = load8(base + (n > 0 ? srow * ld + scol : 0), n);
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int v = u * 256 + threadIdx.x;
+            if constexpr (KC) {
+                store8_full(lds + (v / (BK / 8)) * LD + (v % (BK / 8)) * 8, r[u]);
+            } else {
+                const int k = v / (kTile / 8), i = (v % (kTile / 8)) * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) store1(lds + (i + e) * LD + k, r[u].v[e]);
+            }
+        }
+    }
+};
+
+// Any sizes, strides and alignment.  Four waves, 32 x 32 of the tile each.
+template <typename T, bool PKC, bool QKC, bool LOGITS>
+__global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
+    constexpr int BK = Mma<T>::BK, LD = BK + Mma<T>::PAD, KSTEP = Mma<T>::KSTEP;
+    __shared__ __attribute__((aligned(16))) T lp[kTile * LD];
+    __shared__ __attribute__((aligned(16))) T lq[kTile * LD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+    const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+    const int i0 = blockIdx.x * kTile, j0 = blockIdx.y * kTile;
+    const int kb = blockIdx.z * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Stage<T, PKC> sp;
+    Stage<T, QKC> sq;
+    sp.load((const T*)a.p, a.ld_p, i0, a.I, kb, ke);
+    sq.load((const T*)a.q, a.ld_q, j0, a.Jn, kb, ke);
+    for (int k = kb; k < ke; k += BK) {
+        sp.store(lp);
+        sq.store(lq);
+        __syncthreads();
+        if (k + BK < ke) {
+            sp.load((const T*)a.p, a.ld_p, i0, a.I, k + BK, ke);
+            sq.load((const T*)a.q, a.ld_q, j0, a.Jn, k + BK, ke);
+        }
+#pragma unroll
+        for (int ks = 0; ks < BK; ks += KSTEP) {
+            typename Mma<T>::Frag fp[2], fqv[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                fp[u] = Mma<T>::frag(lp + (wi + u * 16 + fr) * LD, ks, fq);
+                fqv[u] = Mma<T>::frag(lq + (wj + u * 16 + fr) * LD, ks, fq);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = Mma<T>::mma(fp[i], fqv[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+    // lane: i = i0 + wi + u*16 + fq*4 + e, j = j0 + wj + v*16 + fr
+    if constexpr (!LOGITS) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            const int j = j0 + wj + v * 16 + fr;
+            if (j >= a.Jn) continue;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = i0 + wi + u * 16 + fq * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i + e >= a.I) continue;
+                    if (a.slabs) {
+                        float* o = (float*)a.out + ((long long)blockIdx.z * a.Jn + j) * a.I + i + e;
+                        *o = a.add ? *o + acc[u][v][e] : acc[u][v][e];
+                    } else {
+                        store1((T*)a.out + j * a.ld_out + i + e, acc[u][v][e]);
+                    }
+                }
+            }
+        }
+    } else {
+        __shared__ float red[2][kTile][3];
+        const int tile = blockIdx.x;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            const int j = j0 + wj + v * 16 + fr;
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = i0 + wi + u * 16 + fq * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float l = -INFINITY;
+                    if (i + e < a.I) {
+                        l = acc[u][v][e];
+                        if (a.bias) l += a.bias_bf16 ? load1((const short*)a.bias + i + e) : load1((const float*)a.bias + i + e);
+                    }
+                    acc[u][v][e] = l;
+                    m = fmaxf(m, l);
+                }
+            }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            if (fq == 0) red[wave >> 1][wj + v * 16 + fr][0] = m;
+            if (j < a.Jn) {
+                const long long t = a.target[j];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = i0 + wi + u * 16 + fq * 4 + e;
+                        if (i == t && i < a.I) a.target_logit[j] = acc[u][v][e];
+                    }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            const int jl = wj + v * 16 + fr, j = j0 + jl;
+            const float m = fmaxf(red[0][jl][0], red[1][jl][0]);
+            const float ref = m == -INFINITY ? 0.f : m;      // a tile whose classes are all masked: sum nought, not NaN
+            float s = 0.f, lin = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = i0 + wi + u * 16 + fq * 4;
+                F8 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float l = acc[u][v][e], x = Mma<T>::exp_(l - ref);
+                    if (a.smooth && i + e < a.I) lin += l;
+                    s += x;
+                    o.v[e] = x;
+                }
+                if (a.store_e && j < a.Jn) {                 // the exponentials' rows are padded to whole tiles
+                    T* er = (T*)a.out + j * a.ld_out + i;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) store1(er + e, o.v[e]);
+                }
+            }
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            lin += __shfl_xor(lin, 16, 64);
+            lin += __shfl_xor(lin, 32, 64);
+            if (fq == 0) {
+                red[wave >> 1][jl][1] = s;
+                red[wave >> 1][jl][2] = lin;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < kTile) {
+            const int j = j0 + threadIdx.x;
+            if (j < a.Jn) {
+                const long long at = (long long)j * a.tiles + tile;
+                a.tile_max[at] = fmaxf(red[0][threadIdx.x][0], red[1][threadIdx.x][0]);
+                a.tile_sum[at] = red[0][threadIdx.x][1] + red[1][threadIdx.x][1];
+                if (a.smooth) a.tile_lin[at] = red[0][threadIdx.x][2] + red[1][threadIdx.x][2];
+            }
+        }
+    }
+}
+
+// rows that carry a label, among all n of the call
+__device__ __forceinline__ int count_kept(const long long* target, int n, long long ignore, int* lds) {
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += 256) c += target[i] != ignore;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = c;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+constexpr int kCountInPlace = 1024;       // up to so many rows every workgroup counts for itself; above, one launch ahead
+
+__global__ __launch_bounds__(256) void xent_count_kernel(const long long* target, int n, long long ignore, int* count) {
+    __shared__ int lds[4];
+    const int c = count_kept(target, n, ignore, lds);
+    if (threadIdx.x == 0) *count = c;
+}
+
+struct XentRows {
+    const long long* target;              // of this piece's rows
+    const long long* all_target;
+    const int* count;                     // null: count here (mean)
+    const float* upstream;                // null: 1
+    float* tile_max;                      // in: maxima; out (factors != 0): g exp(m - lse)
+    const float* tile_sum;
+    const float* tile_lin;
+    const float* target_logit;
+    float* target_g;                      // G at the target
+    float* row_g;                         // g (label smoothing's even part)
+    float* loss;
+    float* lse;
+    long long ignore;
+    float smoothing, inv_classes;
+    int rows, n, classes, tiles, reduction, upstream_rows, factors;
+};
+
+// one wave a row: the tiles' maxima and sums to lse, the loss, and the factors that turn exp(l - m) into G
+__global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
+    __shared__ int lds[4];
+    float scale = 1.f;
+    if (a.factors && a.reduction == ASL_REDUCE_MEAN)
+        scale = 1.f / (float)(a.count ? *a.count : count_kept(a.all_target, a.n, a.ignore, lds));
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= a.rows) return;
+    float* mx = a.tile_max + (long long)row * a.tiles;
+    const float* sm = a.tile_sum + (long long)row * a.tiles;
+    float m = -INFINITY, lin = 0.f;
+    for (int t = lane; t < a.tiles; t += 64) m = fmaxf(m, mx[t]);
+    m = wave_max(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+    for (int t = lane; t < a.tiles; t += 64) s += sm[t] * expf(mx[t] - ref);
+    if (a.smoothing != 0.f) {
+        const float* ln = a.tile_lin + (long long)row * a.tiles;
+        for (int t = lane; t < a.tiles; t += 64) lin += ln[t];
+        lin = wave_sum(lin);
+    }
+    s = wave_sum(s);
+    const float lse = ref + logf(s);
+    const long long t = a.target[row];
+    const bool kept = t != a.ignore, valid = t >= 0 && t < a.classes;
+    float g = 0.f;
+    if (kept) g = scale * (a.upstream ? a.upstream[a.upstream_rows ? row : 0] : 1.f);
+    const float lt = valid ? a.target_logit[row] : NAN;       // a label outside the vocabulary makes loss and gradients NaN
+    if (lane == 0) {
+        float l = lse - lt;
+        if (a.smoothing != 0.f) l = lse - (1.f - a.smoothing) * lt - a.smoothing * a.inv_classes * lin;
+        a.loss[row] = kept ? l : 0.f;
+        if (a.lse) a.lse[row] = lse;
+        if (a.factors) {
+            a.target_g[row] = g * (expm1f(lt - lse) + a.smoothing - a.smoothing * a.inv_classes);
+            a.row_g[row] = g;
+        }
+    }
+    if (a.factors)
+        for (int t2 = lane; t2 < a.tiles; t2 += 64) mx[t2] = valid ? g * expf(mx[t2] - lse) : NAN;
+}
+
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// the call's loss from the rows' losses: sum, or mean over the rows that carry a label (none: 0 / 0)
+__device__ __forceinline__ void reduce_loss(const float* rows, const long long* target, int n, long long ignore, int mean,
+                                            float* out) {
+    __shared__ float lf[4];
+    __shared__ int li[4];
+    float v = 0.f;
+    for (int i = threadIdx.x; i < n; i += 256) v += rows[i];
+    v = block_sum(v, lf);
+    if (mean) v /= (float)count_kept(target, n, ignore, li);
+    if (threadIdx.x == 0) *out = v;
+}
+
+__global__ __launch_bounds__(256) void xent_loss_kernel(const float* rows, const long long* target, int n, long long ignore,
+                                                        int mean, float* out) {
+    reduce_loss(rows, target, n, ignore, mean, out);
+}
+
+constexpr int kGradRows = 32;             // rows a workgroup of the G pass takes; it leaves one partial row of db
+
+struct XentG {
+    void* e;                              // exp(l - m) in, G out
+    long long ld;
+    const float* factor;                  // [rows][tiles]
+    const float* target_g;
+    const float* row_g;
+    const long long* target;
+    const float* loss_rows;               // with loss: the whole call's rows
+    const long long* all_target;
+    float* loss;                          // null: not this launch's business
+    float* db_part;                       // [row groups][ld], null: no bias gradient
+    long long ignore;
+    float smoothing, inv_classes;
+    int rows, classes, tiles, tile_shift, n, mean, db_add;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
+    const long long col = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+    const int r0 = blockIdx.y * kGradRows, r1 = r0 + kGradRows < a.rows ? r0 + kGradRows : a.rows;
+    if (col < a.ld) {
+        F8 db;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) db.v[e] = 0.f;
+        for (int r = r0; r < r1; ++r) {
+            const long long t = a.target[r];
+            T* p = (T*)a.e + r * a.ld + col;
+            F8 g = load8_full(p);
+            const float f = a.factor[(long long)r * a.tiles + (col >> a.tile_shift)];
+            const float even = a.smoothing * a.inv_classes * a.row_g[r];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                g.v[e] = col + e < a.classes ? g.v[e] * f - even : 0.f;
+                if (col + e == t) g.v[e] = a.target_g[r];
+                if (t == a.ignore) g.v[e] = 0.f;             // whatever the row held
+                db.v[e] += g.v[e];
+            }
+            store8_full(p, g);
+        }
+        if (a.db_part) {
+            float* o = a.db_part + blockIdx.y * a.ld + col;
+            if (a.db_add) {                                  // on top of the earlier pieces' rows
+                const F8 q = load8_full(o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) db.v[e] += q.v[e];
+            }
+            store8_full(o, db);
+        }
+    }
+    if (a.loss && blockIdx.x == 0 && blockIdx.y == 0)
+        reduce_loss(a.loss_rows, a.all_target, a.n, a.ignore, a.mean, a.loss);
+}
+
+// out[r][c] = sum over s of slab s, in the order of s; a row of `cols` values, slabs `stride` apart
+template <typename U>
+__global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int slabs, long long stride, long long ld_in, int rows,
+                                                        int cols, U* out, long long ld_out) {
+    const long long c = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (c >= cols) return;
+    const int n = (int)(cols - c < 8 ? cols - c : 8);
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        F8 v = load8(in + r * ld_in + c, n);
+        for (int s = 1; s < slabs; ++s) {
+            const F8 q = load8(in + s * stride + r * ld_in + c, n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] += q.v[e];
+        }
+        store8(out + r * ld_out + c, n, v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side: how a call is cut up
+// ---------------------------------------------------------------------------------------------
+struct XentPlan {
+    int esize, rows, pieces, tiles, tile, tile_shift, dx_splits, dw_splits, row_groups;
+    long long ld_e;
+    bool dw_slabs;
+    // workspace offsets, bytes
+    long long count, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, total;
+};
+
+constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
+constexpr int kPieceRows = 1 << 17;               // and rows: what grids and per-tile numbers are sized by
+
+inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// slices of a contraction so that `tiles` workgroups become enough to fill the 256 CUs twice over, none shorter than four
+// steps, and few enough that the slabs stay small
+inline int splits_for(long long tiles, int k, int bk) {
+    const long long want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
+    const long long most = ((long long)k + 4 * bk - 1) / (4 * bk);
+    const long long s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
+}
+inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, splits), bk) * bk; }
+
+XentPlan xent_plan(const asl_xent_params& p, bool grad, bool want_dx, bool want_dw, bool want_db) {
+    XentPlan q = {};
+    q.esize = p.type ? 2 : 4;
+    q.tile = kTile;
+    q.tile_shift = 6;
+    q.tiles = ceil_div(p.classes, q.tile);
+    q.ld_e = (long long)q.tiles * q.tile;
+    long long rows = p.n < kPieceRows ? p.n : kPieceRows;
+    if (grad) {
+        const long long most = kPieceBytes / (q.ld_e * q.esize) / 256 * 256;
+        if (rows > most) rows = most < 256 ? 256 : most;
+    }
+    q.rows = (int)rows;
+    q.pieces = p.n ? ceil_div(p.n, rows) : 0;
+    q.row_groups = ceil_div(rows, kGradRows);
+    const int bk = p.type ? Mma<short>::BK : Mma<float>::BK;
+    q.dx_splits = splits_for((long long)ceil_div(rows, kTile) * ceil_div(p.d, kTile), p.classes, bk);
+    q.dw_splits = splits_for((long long)ceil_div(p.classes, kTile) * ceil_div(p.d, kTile), (int)rows, bk);
+    q.dx_splits = ceil_div(p.classes, k_per_split(p.classes, q.dx_splits, bk));
+    q.dw_splits = rows ? ceil_div(rows, k_per_split((int)rows, q.dw_splits, bk)) : 1;
+    q.dw_slabs = q.dw_splits > 1 || q.pieces > 1;
+    long long at = 0;
+    const auto take = [&](long long bytes) {
+        const long long r = at;
+        at += (bytes + 255) / 256 * 256;
+        return r;
+    };
+    q.count = take(4);
+    q.loss = take(4LL * p.n);
+    q.lse = take(4LL * p.n);
+    q.tmax = take(4LL * rows * q.tiles);
+    q.tsum = take(4LL * rows * q.tiles);
+    q.tlin = take(p.label_smoothing != 0.f ? 4LL * rows * q.tiles : 0);
+    q.tlogit = take(4LL * rows);
+    if (grad) {
+        q.tg = take(4LL * rows);
+        q.rg = take(4LL * rows);
+        q.e = take(q.esize * rows * q.ld_e);
+        q.dbp = take(want_db ? 4LL * q.row_groups * q.ld_e : 0);
+        q.dxs = take(want_dx && q.dx_splits > 1 ? 4LL * q.dx_splits * rows * p.d : 0);
+        q.dws = take(want_dw && q.dw_slabs ? 4LL * q.dw_splits * p.classes * p.d : 0);
+    }
+    q.total = at;
+    return q;
+}
+
+int xent_check(const asl_xent_params* p) {
+    if (!p || p->n < 0 || p->classes <= 0 || p->d <= 0) return ASL_EINVAL;
+    if (p->type < 0 || p->type > 1 || p->bias_type < 0 || p->bias_type > 1) return ASL_EINVAL;
+    if (p->reduction < ASL_REDUCE_NONE || p->reduction > ASL_REDUCE_MEAN) return ASL_EINVAL;
+    if (p->ld_x < p->d || p->ld_w < p->d) return ASL_EINVAL;
+    if (!(p->label_smoothing >= 0.f && p->label_smoothing <= 1.f)) return ASL_EINVAL;
+    // grids take one of their 65535 rows of workgroups per 64 classes
+    if (p->n > (1 << 28) || p->classes > (1 << 21) || p->d > (1 << 20)) return ASL_ETOOBIG;
+    return ASL_OK;
+}
+
+template <typename T>
+int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void* x, const void* w, const void* bias,
+             const long long* target, const float* upstream, float* loss, float* lse, void* dx, void* dw, void* db, char* ws,
+             hipStream_t s) {
+    constexpr int bk = Mma<T>::BK;
+    const bool none = p.reduction == ASL_REDUCE_NONE, mean = p.reduction == ASL_REDUCE_MEAN;
+    float* loss_rows = none ? loss : (float*)(ws + q.loss);
+    int* count = (int*)(ws + q.count);
+    if (grad && mean && p.n > kCountInPlace)
+        hipLaunchKernelGGL(xent_count_kernel, dim3(1), dim3(256), 0, s, target, p.n, (long long)p.ignore_index, count);
+    for (int piece = 0; piece < q.pieces; ++piece) {
+        const int r0 = piece * q.rows, rows = p.n - r0 < q.rows ? p.n - r0 : q.rows;
+        const T* xr = (const T*)x + r0 * p.ld_x;
+        XentGemm g = {};
+        g.p = w; g.ld_p = p.ld_w; g.q = xr; g.ld_q = p.ld_x; g.I = p.classes; g.Jn = rows; g.K = p.d; g.k_per_split = p.d;
+        g.out = ws + q.e; g.ld_out = q.ld_e; g.bias = bias; g.bias_bf16 = p.bias_type; g.smooth = p.label_smoothing != 0.f;
+        g.store_e = grad; g.target = target + r0; g.tile_max = (float*)(ws + q.tmax); g.tile_sum = (float*)(ws + q.tsum);
+        g.tile_lin = (float*)(ws + q.tlin); g.target_logit = (float*)(ws + q.tlogit); g.tiles = q.tiles;
+        hipLaunchKernelGGL((xent_gemm_kernel<T, true, true, true>), dim3(q.tiles, ceil_div(rows, kTile)), dim3(256), 0, s, g);
+        XentRows r = {};
+        r.target = target + r0; r.all_target = target; r.count = p.n > kCountInPlace ? count : nullptr;
+        r.upstream = upstream ? upstream + (none ? r0 : 0) : nullptr; r.upstream_rows = none;
+        r.tile_max = g.tile_max; r.tile_sum = g.tile_sum; r.tile_lin = g.tile_lin; r.target_logit = g.target_logit;
+        r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
+        r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr;
+        r.ignore = p.ignore_index; r.smoothing = p.label_smoothing; r.inv_classes = 1.f / (float)p.classes;
+        r.rows = rows; r.n = p.n; r.classes = p.classes; r.tiles = q.tiles; r.reduction = p.reduction; r.factors = grad;
+        hipLaunchKernelGGL(xent_rows_kernel, dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
+        if (!grad) continue;
+        const bool last = piece == q.pieces - 1;
+        XentG c = {};
+        c.e = ws + q.e; c.ld = q.ld_e; c.factor = g.tile_max; c.target_g = r.target_g; c.row_g = r.row_g; c.target = target + r0;
+        c.loss_rows = loss_rows; c.all_target = target; c.loss = !none && last && loss ? loss : nullptr;
+        c.db_part = db ? (float*)(ws + q.dbp) : nullptr; c.db_add = piece > 0;
+        c.ignore = p.ignore_index; c.smoothing = p.label_smoothing; c.inv_classes = r.inv_classes; c.rows = rows;
+        c.classes = p.classes; c.tiles = q.tiles; c.tile_shift = q.tile_shift; c.n = p.n; c.mean = mean;
+        const int groups = ceil_div(rows, kGradRows);
+        hipLaunchKernelGGL((xent_g_kernel<T>), dim3(ceil_div(q.ld_e, 2048), groups), dim3(256), 0, s, c);
+        if (dx) {                          // dx[row][k] = sum over classes G[row][v] W[v][k]
+            XentGemm h = {};
+            h.p = w; h.ld_p = p.ld_w; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
+            h.k_per_split = k_per_split(p.classes, q.dx_splits, bk);
+            h.slabs = q.dx_splits > 1;
+            T* dxr = (T*)dx + (long long)r0 * p.d;
+            h.out = h.slabs ? (void*)(ws + q.dxs) : (void*)dxr; h.ld_out = p.d;
+            hipLaunchKernelGGL((xent_gemm_kernel<T, false, true, false>), dim3(ceil_div(p.d, kTile), ceil_div(rows, kTile), q.dx_splits),
+                               dim3(256), 0, s, h);
+            if (h.slabs)
+                hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), rows < 4096 ? rows : 4096), dim3(256), 0, s,
+                                   (const float*)(ws + q.dxs), q.dx_splits, (long long)rows * p.d, (long long)p.d, rows, p.d, dxr,
+                                   (long long)p.d);
+        }
+        if (dw) {                          // dW[v][k] = sum over rows G[row][v] x[row][k]
+            XentGemm h = {};
+            h.p = xr; h.ld_p = p.ld_x; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
+            h.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
+            h.slabs = q.dw_slabs; h.add = piece > 0;
+            h.out = h.slabs ? (void*)(ws + q.dws) : dw; h.ld_out = p.d;
+            hipLaunchKernelGGL((xent_gemm_kernel<T, false, false, false>), dim3(ceil_div(p.d, kTile), ceil_div(p.classes, kTile), q.dw_splits),
+                               dim3(256), 0, s, h);
+            if (h.slabs && last)
+                hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), p.classes < 4096 ? p.classes : 4096), dim3(256), 0, s,
+                                   (const float*)(ws + q.dws), q.dw_splits, (long long)p.classes * p.d, (long long)p.d, p.classes,
+                                   p.d, (T*)dw, (long long)p.d);
+        }
+        if (db && last) {
+            const dim3 grid(ceil_div(p.classes, 2048), 1);
+            if (p.bias_type)
+                hipLaunchKernelGGL((xent_slab_kernel<short>), grid, dim3(256), 0, s, (const float*)(ws + q.dbp), q.row_groups, q.ld_e, 0LL, 1,
+                                   p.classes, (short*)db, 0LL);
+            else
+                hipLaunchKernelGGL((xent_slab_kernel<float>), grid, dim3(256), 0, s, (const float*)(ws + q.dbp), q.row_groups, q.ld_e, 0LL, 1,
+                                   p.classes, (float*)db, 0LL);
+        }
+    }
+    if (!none && loss && (!grad || !q.pieces))
+        hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, s, loss_rows, target, p.n, (long long)p.ignore_index, (int)mean, loss);
+    return (int)hipGetLastError();
+}
+
+// no rows: the weight's and bias's gradients are nought
+__global__ __launch_bounds__(256) void xent_zero_kernel(char* p, long long bytes) {
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < bytes; i += gridDim.x * 256LL) p[i] = 0;
+}
+
+inline bool off(const void* p, int type) { return ((uintptr_t)p & (type ? 1 : 3)) != 0; }
+
+}  // namespace asl_detail
+using namespace asl_detail;
+
+extern "C" int64_t asl_linear_xent_workspace(const asl_xent_params* p, int grad) {
+    const int rc = xent_check(p);
+    if (rc != ASL_OK) return rc;
+    return xent_plan(*p, grad != 0, true, true, true).total;
+}
+
+extern "C" int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, const void* w, const void* bias,
+                                   const int64_t* target, float* loss, float* lse, void* workspace, asl_stream_t stream) {
+    const int rc = xent_check(p);
+    if (rc != ASL_OK) return rc;
+    if (!w || !workspace || ((uintptr_t)workspace & 255) || !loss || ((uintptr_t)loss & 3) || ((uintptr_t)lse & 3)) return ASL_EINVAL;
+    if (p->n && (!x || !target)) return ASL_EINVAL;
+    if (off(x, p->type) || off(w, p->type) || off(bias, p->bias_type) || ((uintptr_t)target & 7)) return ASL_EINVAL;
+    const XentPlan q = xent_plan(*p, false, false, false, false);
+    const long long* t = (const long long*)target;
+    if (p->type) return xent_run<short>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
+    return xent_run<float>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
+}
+
+extern "C" int asl_linear_xent_grad(const asl_xent_params* p, const void* x, const void* w, const void* bias,
+                                    const int64_t* target, const float* upstream, float* loss, float* lse, void* dx, void* dw,
+                                    void* dbias, void* workspace, asl_stream_t stream) {
+    const int rc = xent_check(p);
+    if (rc != ASL_OK) return rc;
+    if (!w || !workspace || ((uintptr_t)workspace & 255) || ((uintptr_t)loss & 3) || ((uintptr_t)lse & 3) || ((uintptr_t)upstream & 3))
+        return ASL_EINVAL;
+    if (!loss) return ASL_EINVAL;
+    if (p->n && (!x || !target)) return ASL_EINVAL;
+    if (off(x, p->type) || off(w, p->type) || off(bias, p->bias_type) || off(dx, p->type) || off(dw, p->type) ||
+        off(dbias, p->bias_type) || ((uintptr_t)target & 7))
+        return ASL_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    if (p->n == 0) {
+        const auto zero = [&](void* out, long long bytes) {
+            if (out) hipLaunchKernelGGL(xent_zero_kernel, dim3(ceil_div(bytes, 4096) < 4096 ? ceil_div(bytes, 4096) : 4096), dim3(256), 0, s, (char*)out, bytes);
+        };
+        zero(dw, (long long)p->classes * p->d * (p->type ? 2 : 4));
+        zero(dbias, (long long)p->classes * (p->bias_type ? 2 : 4));
+    }
+    const XentPlan q = xent_plan(*p, true, dx != nullptr, dw != nullptr, dbias != nullptr);
+    const long long* t = (const long long*)target;
+    if (p->type) return xent_run<short>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
+    return xent_run<float>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
+}
