@@ -224,9 +224,10 @@ def xent_reference(x, w, b, t, up, ignore, smooth, reduction, bf16):
     hot = torch.zeros_like(p).scatter_(1, at, 1.0)
     G = gr * (p - (1 - smooth) * hot - smooth / v)
     G = torch.where(keep[:, None], G, 0.0)
-    # a logit's bound and lse's move p by as much of itself; what is rounded to bf16 on the way: the exponential, then G
+    # a logit's bound and lse's move p by as much of itself; rounded on the way for bf16: the exponential to fp16 of 2^15 its
+    # ratio to the tile's largest (2^-12 of it, or 2^-40 of the largest), then G to bf16
     tG = gr.abs() * p * (bound + trow[:, None] + rel + 4 * U32) + 4 * U32 * (gr.abs() * (p + hot + smooth / v))
-    tG32 = tG + (2.0 ** -8 * gr.abs() * p * (1 - hot) if bf16 else 0.0)
+    tG32 = tG + (gr.abs() * (1 - hot) * (2.0 ** -12 * p + 2.0 ** -40 * p.max(1, keepdim=True).values) if bf16 else 0.0)
     tG = tG32 + (2.0 ** -8 * G.abs() * (1 + 2.0 ** -8) if bf16 else 0.0)
     tG, tG32 = (torch.where(keep[:, None], q, 0.0) for q in (tG, tG32))
     dx, tdx = G @ w, tG @ w.abs() + (v + 40) * U32 * (G.abs() @ w.abs())
@@ -277,6 +278,18 @@ def test_linear_cross_entropy(gpu, n, v, d, dt):
     _xent_check(x, w, b, t, smooth=0.1, what="smoothed")
     _xent_check(x, w, b, t, reduction="sum", what="sum")
     _xent_check(x, w, b, t, reduction="none", what="none")
+
+
+@pytest.mark.parametrize("n,v,d", [(256, 32768, 64), (300, 33001, 72), (257, 32769, 8), (513, 22000, 520), (1000, 8200, 256),
+                                   (8200, 1100, 192), (4100, 2049, 1032)])
+def test_linear_cross_entropy_large_tiles(gpu, n, v, d):
+    """sizes that take the 256 x 256 tiles: whole ones, cut ones, k that ends inside a step"""
+    x, w, b, t = _xent_case(n, v, d, BF16, F32, 0.1)
+    b[v // 3: v // 2] = float("-inf")
+    t = torch.where((t >= v // 3) & (t < v // 2), 0, t)
+    _xent_check(x, w, b, t, what="large")
+    x, w, b, t = _xent_case(n, v, d, BF16, None, 0.1)
+    _xent_check(x, w, b, t, smooth=0.1, reduction="sum", what="large, smoothed")
 
 
 def test_linear_cross_entropy_bias_types_and_strides(gpu):

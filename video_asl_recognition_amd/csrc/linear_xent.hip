@@ -4,8 +4,8 @@
 //   G = g (softmax(l) - (1 - e) [j = t] - e / V),  dx = G W,  dW = G^T x,  db = sum over rows of G   (g: the row's weight)
 //
 // The logits are never held.  Rows are taken in pieces; the product x W^T leaves, for every row and every tile of classes, the
-// tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself in the operands' type
-// (between 0 and 1, so 16 bits keep it to 2^-8 of its value).  One pass over the per-tile numbers gives lse, the loss and
+// tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself (fp32, or for bf16 operands
+// fp16 of 2^15 times it: 11 bits of the value down to 2^-29 of the tile's largest, and 2^-40 of that below).  One pass over the per-tile numbers gives lse, the loss and
 // the factors g exp(m - lse); one pass over the exponentials turns them into G in place, the target's entry from its own
 // 32-bit logit (g expm1(l_t - lse), where p - 1 of a rounded p would cancel), and adds up db in 32 bits.  Then two products.
 //
@@ -14,31 +14,9 @@
 #include <stdint.h>
 
 #include "asl_hip.h"
-#include "train_common.h"
+#include "xent_args.h"
 
 namespace asl_detail {
-
-// D[j][i] = sum over k of P(i, k) Q(j, k).  P is the MFMA's row operand, so a lane ends up with four consecutive i of one j
-// and D is stored along i.  Each operand is contiguous along k ("KC") or along its own index.
-struct XentGemm {
-    const void* p;
-    const void* q;
-    long long ld_p, ld_q;    // elements from one row of the stored matrix to the next
-    int I, Jn, K;
-    // plain products
-    void* out;               // of the operands' type, or fp32 slabs [gridDim.z][Jn][I] when slabs != 0
-    long long ld_out;
-    int slabs, add, k_per_split;
-    // logits
-    const void* bias;
-    int bias_bf16, smooth, store_e;
-    const long long* target; // of row j
-    float* tile_max;         // [Jn][tiles]
-    float* tile_sum;         // [Jn][tiles]
-    float* tile_lin;         // [Jn][tiles]: sum of the logits (label smoothing)
-    float* target_logit;     // [Jn]
-    int tiles;
-};
 
 template <typename T>
 struct Mma;
@@ -55,6 +33,8 @@ struct Mma<short> {
 #endif
     }
     static __device__ __forceinline__ float exp_(float v) { return __expf(v); }
+    using Exp = _Float16;                 // how exp(l - m) is held, times SCALE
+    static constexpr float SCALE = kExpScale16;
 };
 template <>
 struct Mma<float> {
@@ -69,6 +49,8 @@ struct Mma<float> {
 #endif
     }
     static __device__ __forceinline__ float exp_(float v) { return expf(v); }
+    using Exp = float;
+    static constexpr float SCALE = 1.f;
 };
 
 constexpr int kTile = 64;                 // of either index in the general kernel
@@ -222,9 +204,9 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
                     o.v[e] = x;
                 }
                 if (a.store_e && j < a.Jn) {                 // the exponentials' rows are padded to whole tiles
-                    T* er = (T*)a.out + j * a.ld_out + i;
+                    typename Mma<T>::Exp* er = (typename Mma<T>::Exp*)a.out + j * a.ld_out + i;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) store1(er + e, o.v[e]);
+                    for (int e = 0; e < 4; ++e) er[e] = (typename Mma<T>::Exp)(o.v[e] * Mma<T>::SCALE);
                 }
             }
             s += __shfl_xor(s, 16, 64);
@@ -282,7 +264,7 @@ struct XentRows {
     float* loss;
     float* lse;
     long long ignore;
-    float smoothing, inv_classes;
+    float smoothing, inv_classes, exp_unit;         // exp_unit: one over the scale the exponentials are held at
     int rows, n, classes, tiles, reduction, upstream_rows, factors;
 };
 
@@ -325,7 +307,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
         }
     }
     if (a.factors)
-        for (int t2 = lane; t2 < a.tiles; t2 += 64) mx[t2] = valid ? g * expf(mx[t2] - lse) : NAN;
+        for (int t2 = lane; t2 < a.tiles; t2 += 64) mx[t2] = valid ? g * a.exp_unit * expf(mx[t2] - lse) : NAN;
 }
 
 __device__ __forceinline__ float block_sum(float v, float* lds) {
@@ -370,6 +352,16 @@ struct XentG {
     int rows, classes, tiles, tile_shift, n, mean, db_add;
 };
 
+__device__ __forceinline__ F8 load8_exp(const float* p) { return load8_full(p); }
+__device__ __forceinline__ F8 load8_exp(const _Float16* p) {
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+    const half8 a = *(const half8*)p;
+    F8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = (float)a[e];
+    return r;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
     const long long col = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
@@ -381,7 +373,7 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
         for (int r = r0; r < r1; ++r) {
             const long long t = a.target[r];
             T* p = (T*)a.e + r * a.ld + col;
-            F8 g = load8_full(p);
+            F8 g = load8_exp((const typename Mma<T>::Exp*)p);
             const float f = a.factor[(long long)r * a.tiles + (col >> a.tile_shift)];
             const float even = a.smoothing * a.inv_classes * a.row_g[r];
 #pragma unroll
@@ -430,6 +422,7 @@ __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int sla
 // ---------------------------------------------------------------------------------------------
 struct XentPlan {
     int esize, rows, pieces, tiles, tile, tile_shift, dx_splits, dw_splits, row_groups;
+    bool big;
     long long ld_e;
     bool dw_slabs;
     // workspace offsets, bytes
@@ -439,23 +432,23 @@ struct XentPlan {
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
 constexpr int kPieceRows = 1 << 17;               // and rows: what grids and per-tile numbers are sized by
 
-inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
-
-// slices of a contraction so that `tiles` workgroups become enough to fill the 256 CUs twice over, none shorter than four
-// steps, and few enough that the slabs stay small
-inline int splits_for(long long tiles, int k, int bk) {
-    const long long want = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
+// slices of a contraction so that `tiles` workgroups become `enough` to fill the CUs, none shorter than four steps, and few
+// enough that the slabs stay small
+inline int splits_for(long long tiles, int k, int bk, int enough) {
+    const long long want = tiles > 0 ? enough / tiles : 1;
     const long long most = ((long long)k + 4 * bk - 1) / (4 * bk);
     const long long s = want < most ? want : most;
     return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
 }
 inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, splits), bk) * bk; }
 
-XentPlan xent_plan(const asl_xent_params& p, bool grad, bool want_dx, bool want_dw, bool want_db) {
+XentPlan xent_plan(const asl_xent_params& p, bool aligned, bool grad, bool want_dx, bool want_dw, bool want_db) {
     XentPlan q = {};
     q.esize = p.type ? 2 : 4;
-    q.tile = kTile;
-    q.tile_shift = 6;
+    // the large tiles where the operands' rows lie on 16 bytes and there are tiles for half the CUs
+    q.big = p.type && aligned && (long long)ceil_div(p.n, kBigTile) * ceil_div(p.classes, kBigTile) >= 128;
+    q.tile = q.big ? kBigTile : kTile;
+    q.tile_shift = q.big ? 8 : 6;
     q.tiles = ceil_div(p.classes, q.tile);
     q.ld_e = (long long)q.tiles * q.tile;
     long long rows = p.n < kPieceRows ? p.n : kPieceRows;
@@ -467,8 +460,9 @@ XentPlan xent_plan(const asl_xent_params& p, bool grad, bool want_dx, bool want_
     q.pieces = p.n ? ceil_div(p.n, rows) : 0;
     q.row_groups = ceil_div(rows, kGradRows);
     const int bk = p.type ? Mma<short>::BK : Mma<float>::BK;
-    q.dx_splits = splits_for((long long)ceil_div(rows, kTile) * ceil_div(p.d, kTile), p.classes, bk);
-    q.dw_splits = splits_for((long long)ceil_div(p.classes, kTile) * ceil_div(p.d, kTile), (int)rows, bk);
+    const int want = q.big ? 256 : 512;   // workgroups: one a CU, or two
+    q.dx_splits = splits_for((long long)ceil_div(rows, q.tile) * ceil_div(p.d, q.tile), p.classes, bk, want);
+    q.dw_splits = splits_for((long long)ceil_div(p.classes, q.tile) * ceil_div(p.d, q.tile), (int)rows, bk, want);
     q.dx_splits = ceil_div(p.classes, k_per_split(p.classes, q.dx_splits, bk));
     q.dw_splits = rows ? ceil_div(rows, k_per_split((int)rows, q.dw_splits, bk)) : 1;
     q.dw_slabs = q.dw_splits > 1 || q.pieces > 1;
@@ -526,14 +520,20 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         g.out = ws + q.e; g.ld_out = q.ld_e; g.bias = bias; g.bias_bf16 = p.bias_type; g.smooth = p.label_smoothing != 0.f;
         g.store_e = grad; g.target = target + r0; g.tile_max = (float*)(ws + q.tmax); g.tile_sum = (float*)(ws + q.tsum);
         g.tile_lin = (float*)(ws + q.tlin); g.target_logit = (float*)(ws + q.tlogit); g.tiles = q.tiles;
-        hipLaunchKernelGGL((xent_gemm_kernel<T, true, true, true>), dim3(q.tiles, ceil_div(rows, kTile)), dim3(256), 0, s, g);
+        g.splits = 1;
+        if (q.big) {
+            const int rc = xent_big_logits(g, s);
+            if (rc) return rc;
+        } else {
+            hipLaunchKernelGGL((xent_gemm_kernel<T, true, true, true>), dim3(q.tiles, ceil_div(rows, kTile)), dim3(256), 0, s, g);
+        }
         XentRows r = {};
         r.target = target + r0; r.all_target = target; r.count = p.n > kCountInPlace ? count : nullptr;
         r.upstream = upstream ? upstream + (none ? r0 : 0) : nullptr; r.upstream_rows = none;
         r.tile_max = g.tile_max; r.tile_sum = g.tile_sum; r.tile_lin = g.tile_lin; r.target_logit = g.target_logit;
         r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
         r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr;
-        r.ignore = p.ignore_index; r.smoothing = p.label_smoothing; r.inv_classes = 1.f / (float)p.classes;
+        r.ignore = p.ignore_index; r.smoothing = p.label_smoothing; r.inv_classes = 1.f / (float)p.classes; r.exp_unit = 1.f / Mma<T>::SCALE;
         r.rows = rows; r.n = p.n; r.classes = p.classes; r.tiles = q.tiles; r.reduction = p.reduction; r.factors = grad;
         hipLaunchKernelGGL(xent_rows_kernel, dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
         if (!grad) continue;
@@ -553,8 +553,14 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             h.slabs = q.dx_splits > 1;
             T* dxr = (T*)dx + (long long)r0 * p.d;
             h.out = h.slabs ? (void*)(ws + q.dxs) : (void*)dxr; h.ld_out = p.d;
-            hipLaunchKernelGGL((xent_gemm_kernel<T, false, true, false>), dim3(ceil_div(p.d, kTile), ceil_div(rows, kTile), q.dx_splits),
-                               dim3(256), 0, s, h);
+            h.splits = q.dx_splits;
+            if (q.big) {
+                const int rc = xent_big_dx(h, s);
+                if (rc) return rc;
+            } else {
+                hipLaunchKernelGGL((xent_gemm_kernel<T, false, true, false>),
+                                   dim3(ceil_div(p.d, kTile), ceil_div(rows, kTile), q.dx_splits), dim3(256), 0, s, h);
+            }
             if (h.slabs)
                 hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), rows < 4096 ? rows : 4096), dim3(256), 0, s,
                                    (const float*)(ws + q.dxs), q.dx_splits, (long long)rows * p.d, (long long)p.d, rows, p.d, dxr,
@@ -566,8 +572,14 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             h.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
             h.slabs = q.dw_slabs; h.add = piece > 0;
             h.out = h.slabs ? (void*)(ws + q.dws) : dw; h.ld_out = p.d;
-            hipLaunchKernelGGL((xent_gemm_kernel<T, false, false, false>), dim3(ceil_div(p.d, kTile), ceil_div(p.classes, kTile), q.dw_splits),
-                               dim3(256), 0, s, h);
+            h.splits = q.dw_splits;
+            if (q.big) {
+                const int rc = xent_big_dw(h, s);
+                if (rc) return rc;
+            } else {
+                hipLaunchKernelGGL((xent_gemm_kernel<T, false, false, false>),
+                                   dim3(ceil_div(p.d, kTile), ceil_div(p.classes, kTile), q.dw_splits), dim3(256), 0, s, h);
+            }
             if (h.slabs && last)
                 hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), p.classes < 4096 ? p.classes : 4096), dim3(256), 0, s,
                                    (const float*)(ws + q.dws), q.dw_splits, (long long)p.classes * p.d, (long long)p.d, p.classes,
@@ -593,6 +605,12 @@ __global__ __launch_bounds__(256) void xent_zero_kernel(char* p, long long bytes
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < bytes; i += gridDim.x * 256LL) p[i] = 0;
 }
 
+// what the large tiles' 16-byte loads need (eight k lie on either side of d's end, never across it); a tile's rows are then
+// under 2 GiB
+inline bool aligned_rows(const asl_xent_params& p, const void* x, const void* w) {
+    return p.type && !(p.d & 7) && !(((uintptr_t)x | (uintptr_t)w) & 15) && !((p.ld_x | p.ld_w) & 7) && p.ld_x <= (1 << 20) && p.ld_w <= (1 << 20);
+}
+
 inline bool off(const void* p, int type) { return ((uintptr_t)p & (type ? 1 : 3)) != 0; }
 
 }  // namespace asl_detail
@@ -601,7 +619,9 @@ using namespace asl_detail;
 extern "C" int64_t asl_linear_xent_workspace(const asl_xent_params* p, int grad) {
     const int rc = xent_check(p);
     if (rc != ASL_OK) return rc;
-    return xent_plan(*p, grad != 0, true, true, true).total;
+    // whichever kernels the pointers' alignment will allow
+    const long long one = xent_plan(*p, false, grad != 0, true, true, true).total, two = xent_plan(*p, true, grad != 0, true, true, true).total;
+    return one > two ? one : two;
 }
 
 extern "C" int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, const void* w, const void* bias,
@@ -611,7 +631,7 @@ extern "C" int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, cons
     if (!w || !workspace || ((uintptr_t)workspace & 255) || !loss || ((uintptr_t)loss & 3) || ((uintptr_t)lse & 3)) return ASL_EINVAL;
     if (p->n && (!x || !target)) return ASL_EINVAL;
     if (off(x, p->type) || off(w, p->type) || off(bias, p->bias_type) || ((uintptr_t)target & 7)) return ASL_EINVAL;
-    const XentPlan q = xent_plan(*p, false, false, false, false);
+    const XentPlan q = xent_plan(*p, aligned_rows(*p, x, w), false, false, false, false);
     const long long* t = (const long long*)target;
     if (p->type) return xent_run<short>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
     return xent_run<float>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
@@ -637,7 +657,7 @@ extern "C" int asl_linear_xent_grad(const asl_xent_params* p, const void* x, con
         zero(dw, (long long)p->classes * p->d * (p->type ? 2 : 4));
         zero(dbias, (long long)p->classes * (p->bias_type ? 2 : 4));
     }
-    const XentPlan q = xent_plan(*p, true, dx != nullptr, dw != nullptr, dbias != nullptr);
+    const XentPlan q = xent_plan(*p, aligned_rows(*p, x, w), true, dx != nullptr, dw != nullptr, dbias != nullptr);
     const long long* t = (const long long*)target;
     if (p->type) return xent_run<short>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
     return xent_run<float>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);

@@ -7,6 +7,7 @@ namespace asl_detail {
 // Rows of a tensor need only their element's own alignment (odd widths, sliced tensors): the vector types below say so and
 // the compiler still issues 16-byte accesses, which gfx950 executes at any alignment.
 typedef short bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct F8 {

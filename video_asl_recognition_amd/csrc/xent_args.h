@@ -1,0 +1,40 @@
+// What the two product kernels of the cross entropy operator share (linear_xent.hip, xent_tile256.hip).
+#pragma once
+#include "train_common.h"
+
+namespace asl_detail {
+
+// D[j][i] = sum over k of P(i, k) Q(j, k).  P is the MFMA's row operand, so a lane ends up with four consecutive i of one j
+// and D is stored along i.  Each operand is contiguous along k ("KC") or along its own index.
+struct XentGemm {
+    const void* p;
+    const void* q;
+    long long ld_p, ld_q;    // elements from one row of the stored matrix to the next
+    int I, Jn, K;
+    // plain products
+    void* out;               // of the operands' type, or fp32 slabs [splits][Jn][I] when slabs != 0
+    long long ld_out;
+    int slabs, add, k_per_split, splits;
+    // logits
+    const void* bias;
+    int bias_bf16, smooth, store_e;
+    const long long* target; // of row j
+    float* tile_max;         // [Jn][tiles]
+    float* tile_sum;         // [Jn][tiles]
+    float* tile_lin;         // [Jn][tiles]: sum of the logits (label smoothing)
+    float* target_logit;     // [Jn]
+    int tiles;
+};
+
+inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+constexpr float kExpScale16 = 32768.f;    // exponentials in (0, 1] held as fp16: times this, so that fp16's range is used
+
+constexpr int kBigTile = 256;             // of either index in the large bf16 kernel
+
+// xent_tile256.hip: bf16, rows of both operands on 16 bytes
+int xent_big_logits(const XentGemm& a, hipStream_t s);
+int xent_big_dx(const XentGemm& a, hipStream_t s);     // P along its own index, Q along k
+int xent_big_dw(const XentGemm& a, hipStream_t s);     // both along their own index
+
+}  // namespace asl_detail
