@@ -1,7 +1,10 @@
 // Linear + softmax cross entropy over a class vocabulary, with gradients, for gfx950.
 //
 //   l = x W^T + b,  lse = log sum_j exp l_j,  loss = lse - (1 - e) l_t - (e / V) sum_j l_j          (e: label smoothing)
-//   G = g (softmax(l) - (1 - e) [j = t] - e / V),  dx = G W,  dW = G^T x,  db = sum over rows of G   (g: the row's weight)
+//   G = g (softmax(l) - (1 - e) [j = t] - e / V),  dx = c G W,  dW = c G^T x,  db = c sum over rows of G
+// with g the row's own weight (an upstream gradient a row, or 1) and c what all rows share (1 / rows, an upstream scalar).
+// c is applied to the 32-bit sums: within G it would move every target's entry, -1 for an unsure row, to the same value
+// between two bf16 numbers, and that one rounding would stand in all results.
 //
 // The logits are never held.  Rows are taken in pieces; the product x W^T leaves, for every row and every tile of classes, the
 // tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself (fp32, or for bf16 operands
@@ -131,6 +134,7 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
     }
     // lane: i = i0 + wi + u*16 + fq*4 + e, j = j0 + wj + v*16 + fr
     if constexpr (!LOGITS) {
+        const float c = a.slabs ? 1.f : *a.factor;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const int j = j0 + wj + v * 16 + fr;
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
                         float* o = (float*)a.out + ((long long)blockIdx.z * a.Jn + j) * a.I + i + e;
                         *o = a.add ? *o + acc[u][v][e] : acc[u][v][e];
                     } else {
-                        store1((T*)a.out + j * a.ld_out + i + e, acc[u][v][e]);
+                        store1((T*)a.out + j * a.ld_out + i + e, acc[u][v][e] * c);
                     }
                 }
             }
@@ -261,6 +265,7 @@ struct XentRows {
     const float* target_logit;
     float* target_g;                      // G at the target
     float* row_g;                         // g (label smoothing's even part)
+    float* shared;                        // c
     float* loss;
     float* lse;
     long long ignore;
@@ -271,9 +276,14 @@ struct XentRows {
 // one wave a row: the tiles' maxima and sums to lse, the loss, and the factors that turn exp(l - m) into G
 __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
     __shared__ int lds[4];
-    float scale = 1.f;
-    if (a.factors && a.reduction == ASL_REDUCE_MEAN)
-        scale = 1.f / (float)(a.count ? *a.count : count_kept(a.all_target, a.n, a.ignore, lds));
+    if (a.factors && blockIdx.x == 0) {
+        float c = a.upstream && !a.upstream_rows ? *a.upstream : 1.f;
+        if (a.reduction == ASL_REDUCE_MEAN) {
+            const int kept = a.count ? *a.count : count_kept(a.all_target, a.n, a.ignore, lds);
+            c = kept ? c / (float)kept : 0.f;                // no row with a label: gradients are nought, not 0 / 0
+        }
+        if (threadIdx.x == 0) *a.shared = c;
+    }
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (row >= a.rows) return;
     float* mx = a.tile_max + (long long)row * a.tiles;
@@ -294,7 +304,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
     const long long t = a.target[row];
     const bool kept = t != a.ignore, valid = t >= 0 && t < a.classes;
     float g = 0.f;
-    if (kept) g = scale * (a.upstream ? a.upstream[a.upstream_rows ? row : 0] : 1.f);
+    if (kept) g = a.upstream && a.upstream_rows ? a.upstream[row] : 1.f;
     const float lt = valid ? a.target_logit[row] : NAN;       // a label outside the vocabulary makes loss and gradients NaN
     if (lane == 0) {
         float l = lse - lt;
@@ -399,10 +409,11 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
         reduce_loss(a.loss_rows, a.all_target, a.n, a.ignore, a.mean, a.loss);
 }
 
-// out[r][c] = sum over s of slab s, in the order of s; a row of `cols` values, slabs `stride` apart
+// out[r][c] = *factor times the sum over s of slab s, in the order of s; a row of `cols` values, slabs `stride` apart
 template <typename U>
 __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int slabs, long long stride, long long ld_in, int rows,
-                                                        int cols, U* out, long long ld_out) {
+                                                        int cols, U* out, long long ld_out, const float* factor) {
+    const float f = *factor;
     const long long c = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
     if (c >= cols) return;
     const int n = (int)(cols - c < 8 ? cols - c : 8);
@@ -413,6 +424,8 @@ __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int sla
 #pragma unroll
             for (int e = 0; e < 8; ++e) v.v[e] += q.v[e];
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] *= f;
         store8(out + r * ld_out + c, n, v);
     }
 }
@@ -426,7 +439,7 @@ struct XentPlan {
     long long ld_e;
     bool dw_slabs;
     // workspace offsets, bytes
-    long long count, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, total;
+    long long count, shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, total;
 };
 
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
@@ -473,6 +486,7 @@ XentPlan xent_plan(const asl_xent_params& p, bool aligned, bool grad, bool want_
         return r;
     };
     q.count = take(4);
+    q.shared = take(4);
     q.loss = take(4LL * p.n);
     q.lse = take(4LL * p.n);
     q.tmax = take(4LL * rows * q.tiles);
@@ -510,6 +524,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
     const bool none = p.reduction == ASL_REDUCE_NONE, mean = p.reduction == ASL_REDUCE_MEAN;
     float* loss_rows = none ? loss : (float*)(ws + q.loss);
     int* count = (int*)(ws + q.count);
+    float* shared = (float*)(ws + q.shared);
     if (grad && mean && p.n > kCountInPlace)
         hipLaunchKernelGGL(xent_count_kernel, dim3(1), dim3(256), 0, s, target, p.n, (long long)p.ignore_index, count);
     for (int piece = 0; piece < q.pieces; ++piece) {
@@ -531,7 +546,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         r.target = target + r0; r.all_target = target; r.count = p.n > kCountInPlace ? count : nullptr;
         r.upstream = upstream ? upstream + (none ? r0 : 0) : nullptr; r.upstream_rows = none;
         r.tile_max = g.tile_max; r.tile_sum = g.tile_sum; r.tile_lin = g.tile_lin; r.target_logit = g.target_logit;
-        r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
+        r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg); r.shared = shared;
         r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr;
         r.ignore = p.ignore_index; r.smoothing = p.label_smoothing; r.inv_classes = 1.f / (float)p.classes; r.exp_unit = 1.f / Mma<T>::SCALE;
         r.rows = rows; r.n = p.n; r.classes = p.classes; r.tiles = q.tiles; r.reduction = p.reduction; r.factors = grad;
@@ -550,7 +565,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             XentGemm h = {};
             h.p = w; h.ld_p = p.ld_w; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
             h.k_per_split = k_per_split(p.classes, q.dx_splits, bk);
-            h.slabs = q.dx_splits > 1;
+            h.slabs = q.dx_splits > 1; h.factor = shared;
             T* dxr = (T*)dx + (long long)r0 * p.d;
             h.out = h.slabs ? (void*)(ws + q.dxs) : (void*)dxr; h.ld_out = p.d;
             h.splits = q.dx_splits;
@@ -564,13 +579,13 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             if (h.slabs)
                 hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), rows < 4096 ? rows : 4096), dim3(256), 0, s,
                                    (const float*)(ws + q.dxs), q.dx_splits, (long long)rows * p.d, (long long)p.d, rows, p.d, dxr,
-                                   (long long)p.d);
+                                   (long long)p.d, shared);
         }
         if (dw) {                          // dW[v][k] = sum over rows G[row][v] x[row][k]
             XentGemm h = {};
             h.p = xr; h.ld_p = p.ld_x; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
             h.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
-            h.slabs = q.dw_slabs; h.add = piece > 0;
+            h.slabs = q.dw_slabs; h.factor = shared; h.add = piece > 0;
             h.out = h.slabs ? (void*)(ws + q.dws) : dw; h.ld_out = p.d;
             h.splits = q.dw_splits;
             if (q.big) {
@@ -583,16 +598,16 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             if (h.slabs && last)
                 hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), p.classes < 4096 ? p.classes : 4096), dim3(256), 0, s,
                                    (const float*)(ws + q.dws), q.dw_splits, (long long)p.classes * p.d, (long long)p.d, p.classes,
-                                   p.d, (T*)dw, (long long)p.d);
+                                   p.d, (T*)dw, (long long)p.d, shared);
         }
         if (db && last) {
             const dim3 grid(ceil_div(p.classes, 2048), 1);
             if (p.bias_type)
                 hipLaunchKernelGGL((xent_slab_kernel<short>), grid, dim3(256), 0, s, (const float*)(ws + q.dbp), q.row_groups, q.ld_e, 0LL, 1,
-                                   p.classes, (short*)db, 0LL);
+                                   p.classes, (short*)db, 0LL, shared);
             else
                 hipLaunchKernelGGL((xent_slab_kernel<float>), grid, dim3(256), 0, s, (const float*)(ws + q.dbp), q.row_groups, q.ld_e, 0LL, 1,
-                                   p.classes, (float*)db, 0LL);
+                                   p.classes, (float*)db, 0LL, shared);
         }
     }
     if (!none && loss && (!grad || !q.pieces))

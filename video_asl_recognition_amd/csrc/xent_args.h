@@ -14,6 +14,7 @@ struct XentGemm {
     // plain products
     void* out;               // of the operands' type, or fp32 slabs [splits][Jn][I] when slabs != 0
     long long ld_out;
+    const float* factor;     // on the device; multiplies the sums on their way out (slabs: not yet)
     int slabs, add, k_per_split, splits;
     // logits
     const void* bias;

@@ -253,6 +253,7 @@ __global__ __launch_bounds__(256, 1) void xent_big_kernel(const XentGemm a, int 
             }
             return;
         }
+        const float c = *a.factor;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(256, 1) void xent_big_kernel(const XentGemm a, int 
                 for (int r = 0; r < 4; ++r) {
                     bf16x4 o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(acc[u][v][r * 4 + e]);
+                    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(acc[u][v][r * 4 + e] * c);
                     *(bf16x4*)(smem + (wj + v * 32 + (lane & 31)) * kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
                 }
     } else {
