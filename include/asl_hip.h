@@ -498,9 +498,10 @@ int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void*
  *   asl_linear_xent_grad also writes dx [n][d], dw [classes][d] (dense, of `type`) and dbias [classes] (of bias_type), each
  *   NULL if not wanted.  upstream is the gradient of the loss: fp32, one value, or [n] for ASL_REDUCE_NONE; NULL stands for 1.
  * A bias of -inf masks a class.  A target outside [0, classes) that is not ignore_index makes the loss, the row's dx and
- * every dw NaN rather than being read.  workspace: 256-byte aligned, asl_linear_xent_workspace(p, grad) bytes -- at most
- * about 1 GiB of exponentials at a time plus what sums need (a negative return is an ASL_E* code; classes above 2^21, d
- * above 2^20 or n above 2^28 return ASL_ETOOBIG). */
+ * every dw NaN rather than being read.  workspace: 256-byte aligned, asl_linear_xent_workspace(p, x, w, grad) bytes -- at
+ * most about 1 GiB of exponentials at a time plus what sums need; x and w are looked at for their alignment only (bf16
+ * operands off 16 bytes, or with d no multiple of 64, are copied there first).  A negative return is an ASL_E* code; classes
+ * above 2^21, d above 2^20 or n above 2^28 return ASL_ETOOBIG. */
 enum { ASL_REDUCE_NONE = 0, ASL_REDUCE_SUM = 1, ASL_REDUCE_MEAN = 2 };
 typedef struct asl_xent_params {
     int32_t n, classes, d;
@@ -510,7 +511,7 @@ typedef struct asl_xent_params {
     int32_t reserved;
 } asl_xent_params;
 
-int64_t asl_linear_xent_workspace(const asl_xent_params* p, int grad);
+int64_t asl_linear_xent_workspace(const asl_xent_params* p, const void* x, const void* w, int grad);
 int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, const void* w, const void* bias, const int64_t* target,
                         float* loss, float* lse, void* workspace, asl_stream_t stream);
 int asl_linear_xent_grad(const asl_xent_params* p, const void* x, const void* w, const void* bias, const int64_t* target,

@@ -70,7 +70,7 @@ def test_xent_refuses(kw):
     p = _xent(L, **kw)
     assert L.lib.asl_linear_xent_fwd(C.byref(p), *[FAKE] * 7, None) == L.ASL_EINVAL
     assert L.lib.asl_linear_xent_grad(C.byref(p), *[FAKE] * 11, None) == L.ASL_EINVAL
-    assert L.lib.asl_linear_xent_workspace(C.byref(p), 1) == L.ASL_EINVAL
+    assert L.lib.asl_linear_xent_workspace(C.byref(p), FAKE, FAKE, 1) == L.ASL_EINVAL
 
 
 def test_xent_refuses_pointers_and_sizes():
@@ -90,22 +90,22 @@ def test_xent_refuses_pointers_and_sizes():
         assert L.lib.asl_linear_xent_grad(C.byref(p), *args, None) == L.ASL_EINVAL
     for kw in (dict(classes=(1 << 21) + 1), dict(n=(1 << 28) + 1), dict(d=(1 << 20) + 1, ld_x=1 << 21, ld_w=1 << 21)):
         p = _xent(L, **kw)
-        assert L.lib.asl_linear_xent_workspace(C.byref(p), 0) == L.ASL_ETOOBIG
+        assert L.lib.asl_linear_xent_workspace(C.byref(p), FAKE, FAKE, 0) == L.ASL_ETOOBIG
 
 
 def test_xent_workspace_of_no_rows():
     from video_asl_recognition_amd import _lib as L
     for grad in (0, 1):
-        assert L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=0)), grad) >= 0
+        assert L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=0)), FAKE, FAKE, grad) >= 0
 
 
 def test_xent_workspace_is_bounded():
     """a hundred times the rows do not take a hundred times the exponentials"""
     from video_asl_recognition_amd import _lib as L
-    one = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=16384, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), 1)
-    many = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=1638400, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), 1)
+    one = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=16384, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), FAKE, FAKE, 1)
+    many = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=1638400, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), FAKE, FAKE, 1)
     assert 1 << 30 <= one <= 3 << 30 and many < 2 * one
-    small = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=16384, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), 0)
+    small = L.lib.asl_linear_xent_workspace(C.byref(_xent(L, n=16384, classes=32768, d=64, ld_x=64, ld_w=64, type=L.BF16)), FAKE, FAKE, 0)
     assert small < 1 << 28
 
 

@@ -167,7 +167,7 @@ _PROTOS = {
     "asl_layernorm_fwd": ([C.POINTER(LayerNormParams)] + [_P] * 7, C.c_int),
     "asl_layernorm_bwd_workspace": ([C.POINTER(LayerNormParams)], C.c_int64),
     "asl_layernorm_bwd": ([C.POINTER(LayerNormParams)] + [_P] * 10, C.c_int),
-    "asl_linear_xent_workspace": ([C.POINTER(XentParams), _I], C.c_int64),
+    "asl_linear_xent_workspace": ([C.POINTER(XentParams), _P, _P, _I], C.c_int64),
     "asl_linear_xent_fwd": ([C.POINTER(XentParams)] + [_P] * 8, C.c_int),
     "asl_linear_xent_grad": ([C.POINTER(XentParams)] + [_P] * 12, C.c_int),
     "asl_grad_clip_workspace": ([_I, _P], C.c_int64),

@@ -434,12 +434,11 @@ __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int sla
 // Host side: how a call is cut up
 // ---------------------------------------------------------------------------------------------
 struct XentPlan {
-    int esize, rows, pieces, tiles, tile, tile_shift, dx_splits, dw_splits, row_groups;
-    bool big;
-    long long ld_e;
-    bool dw_slabs;
+    int esize, rows, pieces, tiles, tile, tile_shift, dx_tile, dw_tile, dx_splits, dw_splits, row_groups;
+    long long ld_e, ld_pack;
+    bool dw_slabs, pack_x, pack_w;
     // workspace offsets, bytes
-    long long count, shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, total;
+    long long count, shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, total;
 };
 
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
@@ -455,13 +454,28 @@ inline int splits_for(long long tiles, int k, int bk, int enough) {
 }
 inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, splits), bk) * bk; }
 
-XentPlan xent_plan(const asl_xent_params& p, bool aligned, bool grad, bool want_dx, bool want_dw, bool want_db) {
+// rows on 16 bytes, whole steps of 64 k, a tile's rows within 32-bit offsets
+inline bool lies_well(const void* t, long long ld, int d) {
+    return !((uintptr_t)t & 15) && !(ld & 7) && !(d & 63) && ld <= (1 << 20);
+}
+
+// Tile of a product with `a` x `b` results.  256 x 256 takes the fewest bytes per FLOP but needs tiles for most of the 256
+// CUs (a long contraction makes `deep` of one); 128 x 128 fills them from a quarter of that; fp32, and results too narrow
+// for either, take 64 x 64.
+inline int tile_for(const asl_xent_params& p, long long a, long long b, int deep) {
+    if (!p.type || p.n < 64 || p.classes < 64 || p.d < 32) return kTile;
+    return (long long)ceil_div(a, 256) * ceil_div(b, 256) * deep >= 192 ? 256 : 128;
+}
+
+XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool grad, bool want_dx, bool want_dw, bool want_db) {
     XentPlan q = {};
     q.esize = p.type ? 2 : 4;
-    // the large tiles where the operands' rows lie on 16 bytes and there are tiles for half the CUs
-    q.big = p.type && aligned && (long long)ceil_div(p.n, kBigTile) * ceil_div(p.classes, kBigTile) >= 128;
-    q.tile = q.big ? kBigTile : kTile;
-    q.tile_shift = q.big ? 8 : 6;
+    q.tile = tile_for(p, p.n, p.classes, 1);
+    q.tile_shift = q.tile == 256 ? 8 : q.tile == 128 ? 7 : 6;
+    // the tile kernels read 16 bytes at a time and whole steps of 64 k: operands that do not allow it are laid out anew
+    q.ld_pack = (p.d + 63LL) / 64 * 64;
+    q.pack_x = q.tile > 64 && !lies_well(x, p.ld_x, p.d);
+    q.pack_w = q.tile > 64 && !lies_well(w, p.ld_w, p.d);
     q.tiles = ceil_div(p.classes, q.tile);
     q.ld_e = (long long)q.tiles * q.tile;
     long long rows = p.n < kPieceRows ? p.n : kPieceRows;
@@ -473,9 +487,14 @@ XentPlan xent_plan(const asl_xent_params& p, bool aligned, bool grad, bool want_
     q.pieces = p.n ? ceil_div(p.n, rows) : 0;
     q.row_groups = ceil_div(rows, kGradRows);
     const int bk = p.type ? Mma<short>::BK : Mma<float>::BK;
-    const int want = q.big ? 256 : 512;   // workgroups: one a CU, or two
-    q.dx_splits = splits_for((long long)ceil_div(rows, q.tile) * ceil_div(p.d, q.tile), p.classes, bk, want);
-    q.dw_splits = splits_for((long long)ceil_div(p.classes, q.tile) * ceil_div(p.d, q.tile), (int)rows, bk, want);
+    q.dx_splits = q.dw_splits = 1;
+    q.dx_tile = q.dw_tile = kTile;
+    if (grad && p.n) {
+        q.dx_tile = tile_for(p, rows, p.d, 2);
+        q.dw_tile = tile_for(p, p.classes, p.d, 2);
+        q.dx_splits = splits_for((long long)ceil_div(rows, q.dx_tile) * ceil_div(p.d, q.dx_tile), p.classes, bk, q.dx_tile == 256 ? 256 : 512);
+        q.dw_splits = splits_for((long long)ceil_div(p.classes, q.dw_tile) * ceil_div(p.d, q.dw_tile), (int)rows, bk, q.dw_tile == 256 ? 256 : 512);
+    }
     q.dx_splits = ceil_div(p.classes, k_per_split(p.classes, q.dx_splits, bk));
     q.dw_splits = rows ? ceil_div(rows, k_per_split((int)rows, q.dw_splits, bk)) : 1;
     q.dw_slabs = q.dw_splits > 1 || q.pieces > 1;
@@ -501,6 +520,8 @@ XentPlan xent_plan(const asl_xent_params& p, bool aligned, bool grad, bool want_
         q.dxs = take(want_dx && q.dx_splits > 1 ? 4LL * q.dx_splits * rows * p.d : 0);
         q.dws = take(want_dw && q.dw_slabs ? 4LL * q.dw_splits * p.classes * p.d : 0);
     }
+    q.xp = take(q.pack_x ? 2LL * rows * q.ld_pack : 0);
+    q.wp = take(q.pack_w ? 2LL * p.classes * q.ld_pack : 0);
     q.total = at;
     return q;
 }
@@ -516,6 +537,8 @@ int xent_check(const asl_xent_params* p) {
     return ASL_OK;
 }
 
+__global__ void xent_pack_kernel(const short* src, long long ld, int rows, int d, short* dst, int per_row);
+
 template <typename T>
 int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void* x, const void* w, const void* bias,
              const long long* target, const float* upstream, float* loss, float* lse, void* dx, void* dw, void* db, char* ws,
@@ -527,17 +550,34 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
     float* shared = (float*)(ws + q.shared);
     if (grad && mean && p.n > kCountInPlace)
         hipLaunchKernelGGL(xent_count_kernel, dim3(1), dim3(256), 0, s, target, p.n, (long long)p.ignore_index, count);
+    const void* wk = w;                   // what the products read: the caller's tensors, or their copies
+    long long ld_w = p.ld_w, ld_x = p.ld_x;
+    const auto pack = [&](const void* src, long long ld, int rows, void* dst) {
+        const long long vectors = rows * (q.ld_pack / 8);
+        hipLaunchKernelGGL(xent_pack_kernel, dim3(ceil_div(vectors, 1024) < 8192 ? ceil_div(vectors, 1024) : 8192), dim3(256), 0, s,
+                           (const short*)src, ld, rows, p.d, (short*)dst, (int)(q.ld_pack / 8));
+    };
+    if (q.pieces && q.pack_w) {
+        pack(w, p.ld_w, p.classes, ws + q.wp);
+        wk = ws + q.wp;
+        ld_w = q.ld_pack;
+    }
+    if (q.pack_x) ld_x = q.ld_pack;
     for (int piece = 0; piece < q.pieces; ++piece) {
         const int r0 = piece * q.rows, rows = p.n - r0 < q.rows ? p.n - r0 : q.rows;
         const T* xr = (const T*)x + r0 * p.ld_x;
+        if (q.pack_x) {
+            pack(xr, p.ld_x, rows, ws + q.xp);
+            xr = (const T*)(ws + q.xp);
+        }
         XentGemm g = {};
-        g.p = w; g.ld_p = p.ld_w; g.q = xr; g.ld_q = p.ld_x; g.I = p.classes; g.Jn = rows; g.K = p.d; g.k_per_split = p.d;
+        g.p = wk; g.ld_p = ld_w; g.q = xr; g.ld_q = ld_x; g.I = p.classes; g.Jn = rows; g.K = p.d; g.k_per_split = p.d;
         g.out = ws + q.e; g.ld_out = q.ld_e; g.bias = bias; g.bias_bf16 = p.bias_type; g.smooth = p.label_smoothing != 0.f;
         g.store_e = grad; g.target = target + r0; g.tile_max = (float*)(ws + q.tmax); g.tile_sum = (float*)(ws + q.tsum);
         g.tile_lin = (float*)(ws + q.tlin); g.target_logit = (float*)(ws + q.tlogit); g.tiles = q.tiles;
         g.splits = 1;
-        if (q.big) {
-            const int rc = xent_big_logits(g, s);
+        if (q.tile > kTile) {
+            const int rc = xent_tiles_logits(g, q.tile, s);
             if (rc) return rc;
         } else {
             hipLaunchKernelGGL((xent_gemm_kernel<T, true, true, true>), dim3(q.tiles, ceil_div(rows, kTile)), dim3(256), 0, s, g);
@@ -563,14 +603,14 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         hipLaunchKernelGGL((xent_g_kernel<T>), dim3(ceil_div(q.ld_e, 2048), groups), dim3(256), 0, s, c);
         if (dx) {                          // dx[row][k] = sum over classes G[row][v] W[v][k]
             XentGemm h = {};
-            h.p = w; h.ld_p = p.ld_w; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
+            h.p = wk; h.ld_p = ld_w; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
             h.k_per_split = k_per_split(p.classes, q.dx_splits, bk);
             h.slabs = q.dx_splits > 1; h.factor = shared;
             T* dxr = (T*)dx + (long long)r0 * p.d;
             h.out = h.slabs ? (void*)(ws + q.dxs) : (void*)dxr; h.ld_out = p.d;
             h.splits = q.dx_splits;
-            if (q.big) {
-                const int rc = xent_big_dx(h, s);
+            if (q.dx_tile > kTile) {
+                const int rc = xent_tiles_dx(h, q.dx_tile, s);
                 if (rc) return rc;
             } else {
                 hipLaunchKernelGGL((xent_gemm_kernel<T, false, true, false>),
@@ -583,13 +623,13 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         }
         if (dw) {                          // dW[v][k] = sum over rows G[row][v] x[row][k]
             XentGemm h = {};
-            h.p = xr; h.ld_p = p.ld_x; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
+            h.p = xr; h.ld_p = ld_x; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
             h.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
             h.slabs = q.dw_slabs; h.factor = shared; h.add = piece > 0;
             h.out = h.slabs ? (void*)(ws + q.dws) : dw; h.ld_out = p.d;
             h.splits = q.dw_splits;
-            if (q.big) {
-                const int rc = xent_big_dw(h, s);
+            if (q.dw_tile > kTile) {
+                const int rc = xent_tiles_dw(h, q.dw_tile, s);
                 if (rc) return rc;
             } else {
                 hipLaunchKernelGGL((xent_gemm_kernel<T, false, false, false>),
@@ -615,15 +655,28 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
     return (int)hipGetLastError();
 }
 
+// rows of d bf16 elements at any alignment to rows of `per_row` 16-byte vectors, noughts behind d
+__global__ __launch_bounds__(256) void xent_pack_kernel(const short* src, long long ld, int rows, int d, short* dst, int per_row) {
+    const long long vectors = (long long)rows * per_row;
+    for (long long v = blockIdx.x * 256LL + threadIdx.x; v < vectors; v += gridDim.x * 256LL) {
+        const long long r = v / per_row;
+        const int c = (int)(v - r * per_row) * 8;
+        bf16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
+        const short* p = src + r * ld + c;
+        if (c + 8 <= d) {
+            o = *(const bf16x8u*)p;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < d) o[e] = p[e];
+        }
+        *(bf16x8*)(dst + v * 8) = o;
+    }
+}
+
 // no rows: the weight's and bias's gradients are nought
 __global__ __launch_bounds__(256) void xent_zero_kernel(char* p, long long bytes) {
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < bytes; i += gridDim.x * 256LL) p[i] = 0;
-}
-
-// what the large tiles' 16-byte loads need (eight k lie on either side of d's end, never across it); a tile's rows are then
-// under 2 GiB
-inline bool aligned_rows(const asl_xent_params& p, const void* x, const void* w) {
-    return p.type && !(p.d & 7) && !(((uintptr_t)x | (uintptr_t)w) & 15) && !((p.ld_x | p.ld_w) & 7) && p.ld_x <= (1 << 20) && p.ld_w <= (1 << 20);
 }
 
 inline bool off(const void* p, int type) { return ((uintptr_t)p & (type ? 1 : 3)) != 0; }
@@ -631,12 +684,10 @@ inline bool off(const void* p, int type) { return ((uintptr_t)p & (type ? 1 : 3)
 }  // namespace asl_detail
 using namespace asl_detail;
 
-extern "C" int64_t asl_linear_xent_workspace(const asl_xent_params* p, int grad) {
+extern "C" int64_t asl_linear_xent_workspace(const asl_xent_params* p, const void* x, const void* w, int grad) {
     const int rc = xent_check(p);
     if (rc != ASL_OK) return rc;
-    // whichever kernels the pointers' alignment will allow
-    const long long one = xent_plan(*p, false, grad != 0, true, true, true).total, two = xent_plan(*p, true, grad != 0, true, true, true).total;
-    return one > two ? one : two;
+    return xent_plan(*p, x, w, grad != 0, true, true, true).total;
 }
 
 extern "C" int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, const void* w, const void* bias,
@@ -646,7 +697,7 @@ extern "C" int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, cons
     if (!w || !workspace || ((uintptr_t)workspace & 255) || !loss || ((uintptr_t)loss & 3) || ((uintptr_t)lse & 3)) return ASL_EINVAL;
     if (p->n && (!x || !target)) return ASL_EINVAL;
     if (off(x, p->type) || off(w, p->type) || off(bias, p->bias_type) || ((uintptr_t)target & 7)) return ASL_EINVAL;
-    const XentPlan q = xent_plan(*p, aligned_rows(*p, x, w), false, false, false, false);
+    const XentPlan q = xent_plan(*p, x, w, false, false, false, false);
     const long long* t = (const long long*)target;
     if (p->type) return xent_run<short>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
     return xent_run<float>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
@@ -672,7 +723,7 @@ extern "C" int asl_linear_xent_grad(const asl_xent_params* p, const void* x, con
         zero(dw, (long long)p->classes * p->d * (p->type ? 2 : 4));
         zero(dbias, (long long)p->classes * (p->bias_type ? 2 : 4));
     }
-    const XentPlan q = xent_plan(*p, aligned_rows(*p, x, w), true, dx != nullptr, dw != nullptr, dbias != nullptr);
+    const XentPlan q = xent_plan(*p, x, w, true, dx != nullptr, dw != nullptr, dbias != nullptr);
     const long long* t = (const long long*)target;
     if (p->type) return xent_run<short>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
     return xent_run<float>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);

@@ -1,4 +1,4 @@
-// What the two product kernels of the cross entropy operator share (linear_xent.hip, xent_tile256.hip).
+// What the two product kernels of the cross entropy operator share (linear_xent.hip, xent_tiles.hip).
 #pragma once
 #include "train_common.h"
 
@@ -31,11 +31,10 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 constexpr float kExpScale16 = 32768.f;    // exponentials in (0, 1] held as fp16: times this, so that fp16's range is used
 
-constexpr int kBigTile = 256;             // of either index in the large bf16 kernel
-
-// xent_tile256.hip: bf16, rows of both operands on 16 bytes
-int xent_big_logits(const XentGemm& a, hipStream_t s);
-int xent_big_dx(const XentGemm& a, hipStream_t s);     // P along its own index, Q along k
-int xent_big_dw(const XentGemm& a, hipStream_t s);     // both along their own index
+// xent_tiles.hip, tile 128 or 256: bf16, both operands' rows on 16 bytes and at most 2^21 bytes apart; those contiguous along
+// k hold noughts from K to the next multiple of 64
+int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s);
+int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s);     // P along its own index, Q along k
+int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s);     // both along their own index
 
 }  // namespace asl_detail

@@ -1,0 +1,407 @@
+// The products of the cross entropy operator for bf16 problems on gfx950: tiles of 256 x 256 (or 128 x 128, where those are
+// too few for 256 CUs), 64 deep.
+//
+// Four waves of 128 x 128, one a SIMD: at 64 FLOP per LDS byte a tile of that shape asks the LDS for 3/4 of its rate (reads
+// and the DMA's writes) while the matrix pipe runs at its own; two waves a SIMD on 128 x 64 each ask for all of it.  The 256
+// accumulators leave each wave alone on its SIMD, so it hides its own latencies: while the MFMAs of one 16-deep slice run,
+// the next slice's fragments are read into a second set of registers, and the tile after next is on its way from memory by
+// LDS-DMA.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs still
+// to issue: behind it the other buffer is whole and this one is free for the DMA.
+//
+// Operands contiguous along k are staged as [tile][64] and read as 16-byte fragments.  Operands contiguous along their own
+// index (W for dx, x and G for dW) are staged as they lie, [64][tile], and read with the transposing LDS read, which hands a
+// group of 16 lanes four k of 16 indices; no transposed copy of anything is made.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "asl_hip.h"
+#include "patch_args.h"
+#include "xent_args.h"
+
+namespace asl_detail {
+
+constexpr int kBK = 64;
+
+// LDS of a tile kernel: two stages of both operands, then the output rows over them (padded, so that consecutive rows start
+// in different banks), then what the logits' epilogue exchanges
+template <int TILE>
+struct TileLds {
+    static constexpr int kPanel = TILE * kBK * 2;        // one operand's tile
+    static constexpr int kOutRow = TILE * 2 + 16;
+    static constexpr int kMain = 4 * kPanel > TILE * kOutRow ? 4 * kPanel : TILE * kOutRow;
+    static constexpr int kLogits = kMain + TILE * 4 * 8;
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// 1 KiB (16 bytes a lane) from a buffer into LDS at `lds` (wave-uniform).  Written out because the compiler, which knows
+// only that the builtin writes LDS somewhere, drains the whole queue ahead of the next transposing read; it has no result in
+// registers, and the kernel's own counted waits and barriers are what orders it (LDS addresses go through M0, which wants
+// one instruction between its write and its use;
+// nothing else in these kernels uses it).
+template <int AT>
+__device__ __forceinline__ void dma_1k(i32x4 rsrc, unsigned voff, unsigned lds) {
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "n"(AT) : "scc");
+}
+
+// One operand's way from memory to registers.  Its two stages lie behind one another in LDS, so that a fragment's address is
+// one register and an immediate.
+template <int TILE, bool KC>
+struct Panel {
+    static constexpr int kPanel = TileLds<TILE>::kPanel, ND = TILE / 32, F = TILE / 64;   // DMA instructions and fragments a wave
+    const char* at;          // first byte of the K step to be staged next
+    long long row_bytes;
+    int idx;                 // rows (KC) or columns of the stored matrix that belong to this tile
+    int krem;                // k left from `at` on
+    unsigned lds;            // this wave's part of stage 0
+    unsigned voff[ND];
+    unsigned rd[KC ? 4 : F]; // fragment addresses in stage 0: by slice (KC) or by fragment
+
+    __device__ __forceinline__ void init(const void* base, long long ld, int i0, int n, int kb, int ke, int wave, int lane,
+                                         int w0, unsigned stages) {
+        row_bytes = ld * 2;
+        idx = n - i0 < TILE ? n - i0 : TILE;
+        krem = ke - kb;
+        at = (const char*)base + (KC ? (long long)i0 * row_bytes + kb * 2LL : (long long)kb * row_bytes + i0 * 2LL);
+        lds = stages + wave * (kPanel / 4);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            if constexpr (KC) {                          // eight rows of 128 bytes a DMA instruction
+                const int row = wave * (TILE / 4) + i * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+                voff[i] = (unsigned)(row * row_bytes + c * 16);
+            } else {                                     // two or four k rows; their 32-byte units swapped by k's low bits
+                constexpr int L = TILE / 8;              // lanes a row
+                const int k = wave * 16 + i * (64 / L) + lane / L, u = ((lane % L) >> 1) ^ ((k & 3) << 1);
+                voff[i] = (unsigned)(k * row_bytes + u * 32 + (lane & 1) * 16);
+            }
+        }
+        if constexpr (KC) {
+            const int r = w0 + (lane & 31), sw = (r >> 1) & 7;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) rd[kk] = stages + r * 128 + (((kk * 2 + (lane >> 5)) ^ sw) << 4);
+        } else {
+            const int g = lane >> 4, s = lane & 15, x = (s >> 2) << 1;
+#pragma unroll
+            for (int u = 0; u < F; ++u)
+                rd[u] = stages + ((g >> 1) * 8 + (s >> 2)) * (TILE * 2) + (((w0 >> 4) + u * 2 + (g & 1)) ^ x) * 32 + (s & 3) * 8;
+        }
+    }
+    // The descriptor of the step at `at`: everything past the operand's last element reads as nought, all of it behind the
+    // last step.  Rows that are contiguous along k hold noughts up to a whole step (the caller sees to that).
+    __device__ __forceinline__ i32x4 rsrc() const {
+        // (32 bits: a tile's rows are at most 2^21 bytes apart)
+        const int k = krem < kBK ? krem : kBK;
+        const int n = KC ? (idx - 1) * (int)row_bytes + kBK * 2 : (k - 1) * (int)row_bytes + idx * 2;
+        const unsigned long long p = (unsigned long long)at;
+        return i32x4{__builtin_amdgcn_readfirstlane((int)p), __builtin_amdgcn_readfirstlane((int)(p >> 32) & 0xffff),
+                     __builtin_amdgcn_readfirstlane(krem > 0 ? (n + 3) & ~3 : 0), 0x00020000};
+    }
+    __device__ __forceinline__ void advance() {
+        at += KC ? kBK * 2 : kBK * row_bytes;
+        krem -= kBK;
+    }
+    template <int STAGE, int I>
+    __device__ __forceinline__ void dma(i32x4 r) const {
+        dma_1k<STAGE * kPanel + I * 1024>(r, voff[I], lds);
+    }
+    // fragment u (32 indices) of the 16-deep slice kk
+    __device__ __forceinline__ bf16x8 frag(int stage, int kk, int u) const {
+        typedef __attribute__((address_space(3))) char* P1;
+        if constexpr (KC) {
+            return *(const __attribute__((address_space(3))) bf16x8*)((P1)(unsigned long long)rd[kk] + (stage * kPanel + u * 4096));
+        } else {
+            typedef __attribute__((address_space(3))) bf16x4* P4;
+            const P1 a = (P1)(unsigned long long)rd[u];
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(a + (stage * kPanel + kk * (TILE * 32))));
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(a + (stage * kPanel + kk * (TILE * 32) + TILE * 8)));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+template <int N, typename F>
+__device__ __forceinline__ void unroll(F&& f) {
+    if constexpr (N > 0) {
+        unroll<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+#endif
+
+// tile order: XCD-contiguous ranges (workgroups go to the XCDs in turn), within which tiles run in blocks of 8 j by all i
+// of a strip of 4, so that the tiles an XCD's 32 CUs hold at a time share panels in its L2
+__device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) {
+    const int n = ti * tj, q = n >> 3, r = n & 7, xcd = id & 7;
+    const int l = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
+    constexpr int GJ = 8;
+    const int strip = l / (GJ * ti), first = strip * GJ, w = tj - first < GJ ? tj - first : GJ, in = l - strip * GJ * ti;
+    i = in / w;
+    j = first + in % w;
+}
+
+template <int TILE, bool PKC, bool QKC, bool LOGITS>
+__global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(const XentGemm a, int ti, int tj) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    using Lds = TileLds<TILE>;
+    constexpr int F = TILE / 64, W = TILE / 2;       // fragments of 32 and indices a wave has of either operand
+    float* const bias_row = (float*)(smem + Lds::kMain);
+    int* const target_at = (int*)(smem + Lds::kMain + TILE * 4);             // within the tile, or -1
+    float (*const red)[TILE][3] = (float (*)[TILE][3])(smem + Lds::kMain + TILE * 8);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = (wave >> 1) * W, wj = (wave & 1) * W;
+    int bi, bj;
+    tile_of(blockIdx.x, ti, tj, bi, bj);
+    const int i0 = bi * TILE, j0 = bj * TILE;
+    const int kb = blockIdx.y * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
+    const int steps = ke > kb ? (ke - kb + kBK - 1) / kBK : 0;
+
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
+    Panel<TILE, PKC> P;
+    Panel<TILE, QKC> Q;
+    P.init(a.p, a.ld_p, i0, a.I, kb, ke, wave, lane, wi, lds0);
+    Q.init(a.q, a.ld_q, j0, a.Jn, kb, ke, wave, lane, wj, lds0 + 2 * Lds::kPanel);
+    const auto next = [&]() {
+        P.advance();
+        Q.advance();
+    };
+    const auto dma = [&](i32x4 pr, i32x4 qr, auto stage, auto n) {  // the n-th of a stage's DMA instructions
+        constexpr int N = decltype(n)::value, S = decltype(stage)::value;
+        if constexpr (N & 1) Q.template dma<S, N / 2>(qr);
+        else P.template dma<S, N / 2>(pr);
+    };
+    const auto first = [&](auto stage) {
+        const i32x4 pr = P.rsrc(), qr = Q.rsrc();
+        unroll<4 * F>([&](auto n) { dma(pr, qr, stage, n); });
+        next();
+    };
+    constexpr std::integral_constant<int, 0> s0{};
+    constexpr std::integral_constant<int, 1> s1{};
+    first(s0);
+    first(s1);                                       // past the end: nought, and no memory touched
+
+    if constexpr (LOGITS) {
+        const int at = threadIdx.x % TILE, i = i0 + at, j = j0 + at;
+        float b = -INFINITY;                         // classes behind the last are masked like any other
+        if (i < a.I) b = !a.bias ? 0.f : a.bias_bf16 ? load1((const short*)a.bias + i) : load1((const float*)a.bias + i);
+        bias_row[at] = b;
+        const long long t = j < a.Jn ? a.target[j] : -1;
+        target_at[at] = t >= i0 && t < i0 + TILE && t < a.I ? (int)(t - i0) : -1;
+    }
+
+    f32x16 acc[F][F];
+#pragma unroll
+    for (int u = 0; u < F; ++u)
+#pragma unroll
+        for (int v = 0; v < F; ++v)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
+
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * F) : "memory");
+    bf16x8 pf[2][F], qf[2][F];
+    const auto read = [&](int set, int stage, int kk, int n) {      // the n-th of a slice's fragments
+        if (n & 1) qf[set][n >> 1] = Q.frag(stage, kk, n >> 1);
+        else pf[set][n >> 1] = P.frag(stage, kk, n >> 1);
+    };
+    const auto mma = [&](int set, int n) {                          // the n-th of its products, in the fragments' order
+        constexpr unsigned char U[16] = {0, 1, 0, 1, 2, 2, 0, 1, 2, 3, 3, 3, 0, 1, 2, 3};
+        constexpr unsigned char V[16] = {0, 0, 1, 1, 0, 1, 2, 2, 2, 0, 1, 2, 3, 3, 3, 3};
+        f32x16& c = acc[U[n]][V[n]];
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pf[set][U[n]], qf[set][V[n]], c, 0, 0, 0);
+    };
+#pragma unroll
+    for (int n = 0; n < 2 * F; ++n) read(0, 0, 0, n);
+    const auto step = [&](auto stage) {
+        constexpr int S = decltype(stage)::value, N = F * F;
+        i32x4 pr, qr;
+        // slices 0 .. 2: the next slice's fragments under the first of this one's MFMAs
+#pragma unroll
+        for (int kk = 0; kk < 3; ++kk) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if (n < 2 * F) read((kk + 1) & 1, S, kk + 1, n);
+                if (kk == 1 && n == N / 2 + 1) pr = P.rsrc();
+                if (kk == 1 && n == N - 1) qr = Q.rsrc();
+                if (kk == 2 && n == N / 2) next();
+                mma(kk & 1, n);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // this wave has read all it needs of this stage, and its part of the other one has landed
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        unroll<N>([&](auto n) {
+            constexpr int M = decltype(n)::value, D = 4 * F / N;    // one or two DMA instructions an MFMA
+            if (M < 2 * F) read(0, S ^ 1, 0, M);
+            unroll<D>([&](auto d) { dma(pr, qr, stage, std::integral_constant<int, M * D + decltype(d)::value>{}); });
+            mma(1, M);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+#pragma unroll 1
+    for (int s = 0; s < steps; s += 2) {
+        step(s0);
+        step(s1);                                    // behind the last: noughts
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+    // ---- lane: i = wi + u*32 + 8*(r/4) + 4*(lane/32) + r%4, j = wj + v*32 + lane%32 ------------------------------
+    const int h4 = (lane >> 5) * 4;
+    if constexpr (!LOGITS) {
+        if (a.slabs) {
+#pragma unroll
+            for (int v = 0; v < F; ++v) {
+                const int j = j0 + wj + v * 32 + (lane & 31);
+                if (j >= a.Jn) continue;
+                float* row = (float*)a.out + ((long long)blockIdx.y * a.Jn + j) * a.I;
+#pragma unroll
+                for (int u = 0; u < F; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = i0 + wi + u * 32 + r * 8 + h4;
+                        f32x4 d = {acc[u][v][r * 4], acc[u][v][r * 4 + 1], acc[u][v][r * 4 + 2], acc[u][v][r * 4 + 3]};
+                        if (i + 3 < a.I) {
+                            if (a.add) d += *(const f32x4u*)(row + i);
+                            *(f32x4u*)(row + i) = d;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (i + e < a.I) row[i + e] = a.add ? row[i + e] + d[e] : d[e];
+                        }
+                    }
+            }
+            return;
+        }
+        const float c = *a.factor;
+#pragma unroll
+        for (int v = 0; v < F; ++v)
+#pragma unroll
+            for (int u = 0; u < F; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    bf16x4 o;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(acc[u][v][r * 4 + e] * c);
+                    *(bf16x4*)(smem + (wj + v * 32 + (lane & 31)) * Lds::kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
+                }
+    } else {
+        float m[F];
+#pragma unroll
+        for (int v = 0; v < F; ++v) m[v] = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < F; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f32x4 b = *(const f32x4*)(bias_row + wi + u * 32 + r * 8 + h4);
+#pragma unroll
+                for (int v = 0; v < F; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc[u][v][r * 4 + e] += b[e];
+                        m[v] = fmaxf(m[v], acc[u][v][r * 4 + e]);
+                    }
+            }
+#pragma unroll
+        for (int v = 0; v < F; ++v) {
+            const int jl = wj + v * 32 + (lane & 31), j = j0 + jl;
+            m[v] = fmaxf(m[v], __shfl_xor(m[v], 32, 64));
+            if (lane < 32) red[wave >> 1][jl][0] = m[v];
+            const int t = target_at[jl] - wi;
+            const bool mine = t >= 0 && t < W;
+            if (__any(mine)) {
+                float l = 0.f;
+#pragma unroll
+                for (int u = 0; u < F; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) l = t == u * 32 + (r >> 2) * 8 + h4 + (r & 3) ? acc[u][v][r] : l;
+                if (mine && ((t >> 2) & 1) * 4 == h4) a.target_logit[j] = l;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < F; ++v) {
+            const int jl = wj + v * 32 + (lane & 31);
+            const float mm = fmaxf(red[0][jl][0], red[1][jl][0]);
+            const float ref = mm == -INFINITY ? 0.f : mm;          // a tile whose classes are all masked: sum nought, not NaN
+            float s = 0.f, lin = 0.f;
+#pragma unroll
+            for (int u = 0; u < F; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    half4 o;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __expf(acc[u][v][r * 4 + e] - ref);
+                        s += x;
+                        o[e] = (_Float16)(x * kExpScale16);
+                    }
+                    *(half4*)(smem + jl * Lds::kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
+                }
+            if (a.smooth) {
+#pragma unroll
+                for (int u = 0; u < F; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        lin += i0 + wi + u * 32 + (r >> 2) * 8 + h4 + (r & 3) < a.I ? acc[u][v][r] : 0.f;
+                lin += __shfl_xor(lin, 32, 64);
+            }
+            s += __shfl_xor(s, 32, 64);
+            if (lane < 32) {
+                red[wave >> 1][jl][1] = s;
+                red[wave >> 1][jl][2] = lin;
+            }
+        }
+    }
+    __syncthreads();
+    if constexpr (LOGITS) {
+        const int jl = threadIdx.x, j = j0 + jl;
+        if (jl < TILE && j < a.Jn) {
+            const long long at = (long long)j * a.tiles + bi;
+            a.tile_max[at] = fmaxf(red[0][jl][0], red[1][jl][0]);
+            a.tile_sum[at] = red[0][jl][1] + red[1][jl][1];
+            if (a.smooth) a.tile_lin[at] = red[0][jl][2] + red[1][jl][2];
+        }
+        if (!a.store_e) return;
+    }
+    // rows out of LDS, 16 bytes a lane
+    constexpr int L = TILE / 8;
+#pragma unroll 8
+    for (int n = 0; n < TILE * L / 256; ++n) {
+        const int jl = n * (256 / L) + threadIdx.x / L, c = (threadIdx.x % L) * 8, j = j0 + jl;
+        if (j >= a.Jn) break;
+        const bf16x8 o = *(const bf16x8*)(smem + jl * Lds::kOutRow + c * 2);
+        short* dst = (short*)a.out + j * a.ld_out + i0 + c;
+        if (LOGITS || i0 + c + 8 <= a.I) {           // the exponentials' rows are padded to whole tiles
+            *(bf16x8u*)dst = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i0 + c + e < a.I) dst[e] = o[e];
+        }
+    }
+#endif
+}
+
+template <int TILE, bool PKC, bool QKC, bool LOGITS>
+static int launch_tiles(const XentGemm& a, hipStream_t s) {
+    const int ti = ceil_div(a.I, TILE), tj = ceil_div(a.Jn, TILE);
+    if ((long long)ti * tj > 0x7fffffffLL) return ASL_ETOOBIG;
+    constexpr int lds = LOGITS ? TileLds<TILE>::kLogits : TileLds<TILE>::kMain;
+    static unsigned char lds_done[64];
+    const int rc = ensure_dynamic_lds((const void*)xent_tile_kernel<TILE, PKC, QKC, LOGITS>, lds, lds_done);
+    if (rc != ASL_OK) return rc;
+    hipLaunchKernelGGL((xent_tile_kernel<TILE, PKC, QKC, LOGITS>), dim3((unsigned)(ti * tj), a.splits), dim3(256), lds, s, a, ti, tj);
+    return (int)hipGetLastError();
+}
+
+int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s) {
+    return tile == 256 ? launch_tiles<256, true, true, true>(a, s) : launch_tiles<128, true, true, true>(a, s);
+}
+int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s) {
+    return tile == 256 ? launch_tiles<256, false, true, false>(a, s) : launch_tiles<128, false, true, false>(a, s);
+}
+int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s) {
+    return tile == 256 ? launch_tiles<256, false, false, false>(a, s) : launch_tiles<128, false, false, false>(a, s);
+}
+
+}  // namespace asl_detail

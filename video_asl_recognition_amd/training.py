@@ -189,7 +189,7 @@ def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torc
     dev = x.device
     loss = torch.empty(target.shape if reduction == "none" else (), dtype=torch.float32, device=dev)
     lse = torch.empty(target.shape, dtype=torch.float32, device=dev)
-    ws = torch.empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), 0), "linear_cross_entropy"), dtype=torch.uint8, device=dev)
+    ws = torch.empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), _ptr(x2), _ptr(w2), 0), "linear_cross_entropy"), dtype=torch.uint8, device=dev)
     if loss.numel():
         with _on(dev):
             L.check(L.lib.asl_linear_xent_fwd(C.byref(p), _ptr(x2), _ptr(w2), _ptr(b), _ptr(t), _ptr(loss), _ptr(lse), _ptr(ws),
@@ -204,7 +204,7 @@ def _xent_grad(x, weight, target, bias, upstream, ignore_index, label_smoothing,
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
     dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want[1] else None
     db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if want[2] and bias is not None else None
-    ws = torch.empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), 1), "linear_cross_entropy"), dtype=torch.uint8, device=dev)
+    ws = torch.empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), _ptr(x2), _ptr(w2), 1), "linear_cross_entropy"), dtype=torch.uint8, device=dev)
     # a 0-row "none" loss has no storage: the entry point wants an address all the same and writes nothing there
     with _on(dev):
         L.check(L.lib.asl_linear_xent_grad(C.byref(p), _ptr(x2), _ptr(w2), _ptr(b), _ptr(t), _ptr(upstream),
