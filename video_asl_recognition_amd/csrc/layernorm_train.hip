@@ -44,11 +44,9 @@ __device__ __forceinline__ float not_below_nought(float v) { return v < 0.f ? 0.
 // call to call, so one barrier a call is enough (a slot is written again only behind the next call's barrier).
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* lds, int& slot) {
-    constexpr int W = G < 64 ? G : 64;
+    static_assert(G == 16 || G >= 64, "a quarter wave, or whole waves");
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], o, 64);
+    for (int k = 0; k < N; ++k) v[k] = G == 16 ? row16_sum(v[k]) : wave64_sum(v[k]);
     if constexpr (G > 64) {
         constexpr int NW = G / 64;
         float* s = lds + slot * (NW * N);
@@ -67,15 +65,16 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* lds, int& slot) 
     }
 }
 
+// w and b stay in registers from row to row where a lane has at most two vectors of a row; with more, the registers go to
+// occupancy and both come from the L1 with every row.  The next row is on its way while this one is worked on.
 template <typename XT, typename YT, int G, int J>
 __global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs a) {
     constexpr int BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
+    constexpr bool HOLD = J <= 2;
     __shared__ float lds[2 * 2 * (G > 64 ? G / 64 : 1)];
     int slot = 0;
     const int t = threadIdx.x % G;
     const float inv_d = 1.0f / (float)a.d;
-    // w and b stay in registers from row to row; a workgroup of 1024 has 128 registers a lane and reads them again instead
-    constexpr bool HOLD = G < 1024;
     F8 w[HOLD ? J : 1], b[HOLD ? J : 1];
     if constexpr (HOLD) {
 #pragma unroll
@@ -85,19 +84,29 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs 
             b[j] = load8_or(a.b, a.w_bf16, k < a.d ? k : 0, a.d - k, 0.f);
         }
     }
-    for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB) {
-        const long long row = row0 + threadIdx.x / G;
-        if (G <= 64 && row >= a.rows) return;        // groups within a wave share no barrier
+    typename RawOf<XT>::type next[J];
+    const auto fetch = [&](long long row) {
         const XT* xr = (const XT*)a.x + row * a.ld_x;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            next[j] = load8_raw(xr + (k < a.d ? k : 0), row < a.rows ? a.d - k : 0);
+        }
+    };
+    const long long stride = (long long)gridDim.x * RPB;
+    long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
+    fetch(row < a.rows ? row : 0);
+    // groups wider than a wave are one a workgroup, so all of its threads leave the loop together
+    for (; row < a.rows; row += stride) {
         F8 x[J];
         float s[1] = {0.f};
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8;
-            x[j] = load8(xr + (k < a.d ? k : 0), a.d - k);
+            x[j] = widen(next[j]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[0] += x[j].v[e];
         }
+        if (row + stride < a.rows) fetch(row + stride);
         group_sum<G>(s, lds, slot);
         const float mean = s[0] * inv_d;
         // about the rounded mean; the rest of the mean that its rounding left comes out of the same pass, so a row of
@@ -189,12 +198,12 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
 template <typename XT, typename YT, int G, int J>
 __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs a) {
     constexpr int BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
+    constexpr bool HOLD = J <= 2 && G * J < 2048;
     __shared__ float lds[2 * 2 * (G > 64 ? G / 64 : 1)];
-    __shared__ __attribute__((aligned(16))) float cols[RPB > 1 ? (BLOCK / 64) * 2 * (G < 64 ? G : 64) * J * 8 : 1];
+    __shared__ __attribute__((aligned(16))) float cols[RPB > 1 ? 4 * 2 * (G < 64 ? G : 64) * 8 : 1];
     int slot = 0;
     const int t = threadIdx.x % G;
     const float inv_d = 1.0f / (float)a.d;
-    constexpr bool HOLD = G * J < 2048;
     F8 w[HOLD ? J : 1], dw[J], db[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -203,20 +212,34 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[j].v[e] = db[j].v[e] = 0.f;
     }
-    for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB) {
-        const long long row = row0 + threadIdx.x / G;
-        if (G <= 64 && row >= a.rows) break;         // groups within a wave share no barrier inside the loop
+    typename RawOf<XT>::type next_x[J];
+    typename RawOf<YT>::type next_dy[J];
+    float next_mean, next_rstd;
+    const auto fetch = [&](long long row) {
         const XT* xr = (const XT*)a.x + row * a.ld_x;
         const YT* dyr = (const YT*)a.dy + row * a.ld_dy;
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        next_mean = a.mean[row];
+        next_rstd = a.rstd[row];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8, n = a.d - k;
+            next_x[j] = load8_raw(xr + (k < a.d ? k : 0), n);
+            next_dy[j] = load8_raw(dyr + (k < a.d ? k : 0), n);
+        }
+    };
+    const long long stride = (long long)gridDim.x * RPB;
+    long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
+    if (row < a.rows) fetch(row);
+    for (; row < a.rows; row += stride) {
+        const float mean = next_mean, rstd = next_rstd;
         F8 h[J], g[J];
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8, n = a.d - k;
-            h[j] = load8(xr + (k < a.d ? k : 0), n);
-            g[j] = load8(dyr + (k < a.d ? k : 0), n);
+            h[j] = widen(next_x[j]);
+            g[j] = widen(next_dy[j]);
         }
+        if (row + stride < a.rows) fetch(row + stride);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int k = (t + j * G) * 8, n = a.d - k;
@@ -257,10 +280,11 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
             }
         }
     } else {
-        // several groups a workgroup: within the wave by lane exchange, then the waves' sums through LDS
-        constexpr int COLS = (G < 64 ? G : 64) * J * 8, NW = BLOCK / 64;
+        // several groups a workgroup: within the wave by lane exchange, then the waves' sums through LDS, a vector at a time
+        constexpr int L = G < 64 ? G : 64, COLS = L * 8, NW = BLOCK / 64;
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < J; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -268,22 +292,19 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
                     dw[j].v[e] += __shfl_xor(dw[j].v[e], o, 64);
                     db[j].v[e] += __shfl_xor(db[j].v[e], o, 64);
                 }
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-        if (lane < G) {
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int k = (t + j * G) * 8;
-                store8_full(cols + (wave * 2 + 0) * COLS + k, dw[j]);
-                store8_full(cols + (wave * 2 + 1) * COLS + k, db[j]);
+            if (lane < L) {
+                store8_full(cols + (wave * 2 + 0) * COLS + lane * 8, dw[j]);
+                store8_full(cols + (wave * 2 + 1) * COLS + lane * 8, db[j]);
             }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * COLS; i += BLOCK) {
-            const int which = i / COLS, k = i % COLS;
-            float v = 0.f;
+            __syncthreads();
+            for (int i = threadIdx.x; i < 2 * COLS; i += BLOCK) {
+                const int which = i / COLS, k = i % COLS;
+                float v = 0.f;
 #pragma unroll
-            for (int q = 0; q < NW; ++q) v += cols[(q * 2 + which) * COLS + k];
-            if (k < a.d) part[which * a.d + k] = v;
+                for (int q = 0; q < NW; ++q) v += cols[(q * 2 + which) * COLS + k];
+                if (j * COLS + k < a.d) part[which * a.d + j * COLS + k] = v;
+            }
+            __syncthreads();
         }
     }
 }
@@ -337,18 +358,18 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
     }
 }
 
-// dw and db: the workgroups' partial rows [parts][2][d] added up, 16 columns-of-four by 16 row strides a workgroup
-__global__ __launch_bounds__(256) void ln_cols_kernel(const float* __restrict__ part, int parts, int d, void* dw, void* db,
-                                                      int bf16) {
+// 64 columns a workgroup: 16 lanes of four columns by 16 row strides
+__global__ __launch_bounds__(256) void column_sums_kernel(const float* __restrict__ part, int parts, long long ld, long long cols,
+                                                          long long split, void* out0, void* out1, int bf16, const float* factor) {
     __shared__ float s[16][64 + 1];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-    const long long cols = 2LL * d, c0 = (long long)blockIdx.x * 64 + c * 4;
+    const long long c0 = (long long)blockIdx.x * 64 + c * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c0 < cols) {
         const int n = cols - c0 < 4 ? (int)(cols - c0) : 4;
-#pragma unroll 4
+#pragma unroll 8
         for (int p = r; p < parts; p += 16) {
-            const float* src = part + p * cols + c0;
+            const float* src = part + p * ld + c0;
             if (n == 4) {
                 const f32x4u q = *(const f32x4u*)src;
 #pragma unroll
@@ -369,8 +390,9 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const float* __restrict__ 
             float o = 0.f;
 #pragma unroll
             for (int p = 0; p < 16; ++p) o += s[p][threadIdx.x];
-            void* out = col < d ? dw : db;
-            const long long at = col < d ? col : col - d;
+            if (factor) o *= *factor;
+            void* out = col < split ? out0 : out1;
+            const long long at = col < split ? col : col - split;
             if (out) {
                 if (bf16) store1((short*)out + at, o);
                 else store1((float*)out + at, o);
@@ -379,8 +401,15 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const float* __restrict__ 
     }
 }
 
+int column_sums(const float* part, int parts, long long ld, long long cols, long long split, void* out0, void* out1, int bf16,
+                const float* factor, hipStream_t s) {
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s, part, parts, ld, cols, split, out0, out1,
+                       bf16, factor);
+    return (int)hipGetLastError();
+}
+
 // Lanes a row and vectors a lane, by the row's length.  Forward holds one row (8 J registers), so a wave takes up to 2048
-// elements; backward holds x, dy, w and two column sums (40 J registers), so a wave takes up to 1024.
+// elements; backward holds x, dy and two column sums (32 J registers), so a wave takes up to 2048 as well, at two a SIMD.
 struct LnShape {
     int g, j;
 };
@@ -398,7 +427,7 @@ inline LnShape bwd_shape(int d) {
     if (d <= 128) return {16, 1};
     if (d <= 512) return {64, 1};
     if (d <= 1024) return {64, 2};
-    if (d <= 2048) return {256, 1};
+    if (d <= 2048) return {64, 4};
     if (d <= 4096) return {256, 2};
     if (d <= 8192) return {1024, 1};
     if (d <= 16384) return {1024, 2};
@@ -441,7 +470,7 @@ int launch_bwd(const LnArgs& a, int blocks, hipStream_t s) {
         case 16 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 16, 1>), grid, b256, 0, s, a); break;
         case 64 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
         case 64 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
-        case 256 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 1>), grid, b256, 0, s, a); break;
+        case 64 * 8 + 4: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 4>), grid, b256, 0, s, a); break;
         case 256 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
         case 1024 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 1>), grid, b1024, 0, s, a); break;
         case 1024 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 2>), grid, b1024, 0, s, a); break;
@@ -505,9 +534,7 @@ extern "C" int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, 
         else e = p->y_type ? launch_bwd<float, short>(a, blocks, s) : launch_bwd<float, float>(a, blocks, s);
         if (e) return e;
     }
-    if (dgamma || dbeta) {
-        const unsigned nb = (unsigned)((2LL * p->d + 63) / 64);
-        hipLaunchKernelGGL(ln_cols_kernel, dim3(nb), dim3(256), 0, s, workspace, blocks, p->d, dgamma, dbeta, p->w_type);
-    }
+    if (dgamma || dbeta)
+        return column_sums(workspace, blocks, 2LL * p->d, 2LL * p->d, p->d, dgamma, dbeta, p->w_type, nullptr, s);
     return (int)hipGetLastError();
 }

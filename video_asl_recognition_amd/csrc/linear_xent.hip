@@ -235,29 +235,8 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
     }
 }
 
-// rows that carry a label, among all n of the call
-__device__ __forceinline__ int count_kept(const long long* target, int n, long long ignore, int* lds) {
-    int c = 0;
-    for (int i = threadIdx.x; i < n; i += 256) c += target[i] != ignore;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = c;
-    __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
-}
-
-constexpr int kCountInPlace = 1024;       // up to so many rows every workgroup counts for itself; above, one launch ahead
-
-__global__ __launch_bounds__(256) void xent_count_kernel(const long long* target, int n, long long ignore, int* count) {
-    __shared__ int lds[4];
-    const int c = count_kept(target, n, ignore, lds);
-    if (threadIdx.x == 0) *count = c;
-}
-
 struct XentRows {
     const long long* target;              // of this piece's rows
-    const long long* all_target;
-    const int* count;                     // null: count here (mean)
     const float* upstream;                // null: 1
     float* tile_max;                      // in: maxima; out (factors != 0): g exp(m - lse)
     const float* tile_sum;
@@ -265,25 +244,15 @@ struct XentRows {
     const float* target_logit;
     float* target_g;                      // G at the target
     float* row_g;                         // g (label smoothing's even part)
-    float* shared;                        // c
     float* loss;
     float* lse;
     long long ignore;
     float smoothing, inv_classes, exp_unit;         // exp_unit: one over the scale the exponentials are held at
-    int rows, n, classes, tiles, reduction, upstream_rows, factors;
+    int rows, classes, tiles, factors;
 };
 
 // one wave a row: the tiles' maxima and sums to lse, the loss, and the factors that turn exp(l - m) into G
 __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
-    __shared__ int lds[4];
-    if (a.factors && blockIdx.x == 0) {
-        float c = a.upstream && !a.upstream_rows ? *a.upstream : 1.f;
-        if (a.reduction == ASL_REDUCE_MEAN) {
-            const int kept = a.count ? *a.count : count_kept(a.all_target, a.n, a.ignore, lds);
-            c = kept ? c / (float)kept : 0.f;                // no row with a label: gradients are nought, not 0 / 0
-        }
-        if (threadIdx.x == 0) *a.shared = c;
-    }
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (row >= a.rows) return;
     float* mx = a.tile_max + (long long)row * a.tiles;
@@ -304,7 +273,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
     const long long t = a.target[row];
     const bool kept = t != a.ignore, valid = t >= 0 && t < a.classes;
     float g = 0.f;
-    if (kept) g = a.upstream && a.upstream_rows ? a.upstream[row] : 1.f;
+    if (kept) g = a.upstream ? a.upstream[row] : 1.f;
     const float lt = valid ? a.target_logit[row] : NAN;       // a label outside the vocabulary makes loss and gradients NaN
     if (lane == 0) {
         float l = lse - lt;
@@ -320,31 +289,51 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
         for (int t2 = lane; t2 < a.tiles; t2 += 64) mx[t2] = valid ? g * a.exp_unit * expf(mx[t2] - lse) : NAN;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
-}
+// What concerns all of a call's rows, by one workgroup: the loss (the rows' sum, or their mean over those that carry a label;
+// none of them: 0 / 0), and the factor c of the gradients.
+struct XentAll {
+    const long long* target;
+    const float* loss_rows;               // null: the loss is not this launch's business
+    float* loss;
+    const float* upstream;                // null: 1
+    float* factor;                        // null: not this launch's
+    long long ignore;
+    int n, mean;
+};
 
-// the call's loss from the rows' losses: sum, or mean over the rows that carry a label (none: 0 / 0)
-__device__ __forceinline__ void reduce_loss(const float* rows, const long long* target, int n, long long ignore, int mean,
-                                            float* out) {
+__device__ __forceinline__ void over_all_rows(const XentAll& a) {
     __shared__ float lf[4];
     __shared__ int li[4];
     float v = 0.f;
-    for (int i = threadIdx.x; i < n; i += 256) v += rows[i];
-    v = block_sum(v, lf);
-    if (mean) v /= (float)count_kept(target, n, ignore, li);
-    if (threadIdx.x == 0) *out = v;
+    int kept = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.n; i += 256) {
+        kept += a.target[i] != a.ignore;
+        if (a.loss_rows) v += a.loss_rows[i];
+    }
+    v = wave_sum(v);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) kept += __shfl_xor(kept, o, 64);
+    if ((threadIdx.x & 63) == 0) {
+        lf[threadIdx.x >> 6] = v;
+        li[threadIdx.x >> 6] = kept;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        v = lf[0] + lf[1] + lf[2] + lf[3];
+        kept = li[0] + li[1] + li[2] + li[3];
+        if (a.loss_rows) *a.loss = a.mean ? v / (float)kept : v;
+        if (a.factor) {
+            const float up = a.upstream ? *a.upstream : 1.f;
+            *a.factor = !a.mean ? up : kept ? up / (float)kept : 0.f;      // no row with a label: gradients are nought
+        }
+    }
 }
 
-__global__ __launch_bounds__(256) void xent_loss_kernel(const float* rows, const long long* target, int n, long long ignore,
-                                                        int mean, float* out) {
-    reduce_loss(rows, target, n, ignore, mean, out);
-}
+__global__ __launch_bounds__(256) void xent_loss_kernel(const XentAll a) { over_all_rows(a); }
 
 constexpr int kGradRows = 32;             // rows a workgroup of the G pass takes; it leaves one partial row of db
+constexpr int kGradCols = 256;            // and columns
 
 struct XentG {
     void* e;                              // exp(l - m) in, G out
@@ -353,13 +342,11 @@ struct XentG {
     const float* target_g;
     const float* row_g;
     const long long* target;
-    const float* loss_rows;               // with loss: the whole call's rows
-    const long long* all_target;
-    float* loss;                          // null: not this launch's business
     float* db_part;                       // [row groups][ld], null: no bias gradient
     long long ignore;
     float smoothing, inv_classes;
-    int rows, classes, tiles, tile_shift, n, mean, db_add;
+    int rows, classes, tiles, tile_shift, db_add;
+    XentAll all;
 };
 
 __device__ __forceinline__ F8 load8_exp(const float* p) { return load8_full(p); }
@@ -372,41 +359,58 @@ __device__ __forceinline__ F8 load8_exp(const _Float16* p) {
     return r;
 }
 
+// 256 columns x 32 rows a workgroup: half a wave on each row, four rows a lane, all of them on their way at once
 template <typename T>
 __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
-    const long long col = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
-    const int r0 = blockIdx.y * kGradRows, r1 = r0 + kGradRows < a.rows ? r0 + kGradRows : a.rows;
-    if (col < a.ld) {
-        F8 db;
+    constexpr int R = kGradRows / 8;
+    __shared__ __attribute__((aligned(16))) float cols[8][kGradCols];
+    const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const long long col = (long long)blockIdx.x * kGradCols + lane * 8;
+    const bool in = col < a.ld;
+    const int r0 = blockIdx.y * kGradRows + rl;
+    F8 g[R], db;
+    float f[R], even[R], tg[R];
+    long long t[R];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) db.v[e] = 0.f;
-        for (int r = r0; r < r1; ++r) {
-            const long long t = a.target[r];
-            T* p = (T*)a.e + r * a.ld + col;
-            F8 g = load8_exp((const typename Mma<T>::Exp*)p);
-            const float f = a.factor[(long long)r * a.tiles + (col >> a.tile_shift)];
-            const float even = a.smoothing * a.inv_classes * a.row_g[r];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                g.v[e] = col + e < a.classes ? g.v[e] * f - even : 0.f;
-                if (col + e == t) g.v[e] = a.target_g[r];
-                if (t == a.ignore) g.v[e] = 0.f;             // whatever the row held
-                db.v[e] += g.v[e];
-            }
-            store8_full(p, g);
+    for (int u = 0; u < R; ++u) {
+        const int r = r0 + u * 8 < a.rows ? r0 + u * 8 : a.rows - 1;
+        t[u] = a.target[r];
+        if (in) {
+            g[u] = load8_exp((const typename Mma<T>::Exp*)a.e + r * a.ld + col);
+            f[u] = a.factor[(long long)r * a.tiles + (col >> a.tile_shift)];
         }
-        if (a.db_part) {
-            float* o = a.db_part + blockIdx.y * a.ld + col;
-            if (a.db_add) {                                  // on top of the earlier pieces' rows
-                const F8 q = load8_full(o);
+        even[u] = a.smoothing * a.inv_classes * a.row_g[r];
+        tg[u] = a.target_g[r];
+    }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) db.v[e] += q.v[e];
-            }
-            store8_full(o, db);
+    for (int e = 0; e < 8; ++e) db.v[e] = 0.f;
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int r = r0 + u * 8;
+        if (!in || r >= a.rows) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v = col + e < a.classes ? g[u].v[e] * f[u] - even[u] : 0.f;
+            if (col + e == t[u]) v = tg[u];
+            if (t[u] == a.ignore) v = 0.f;                   // whatever the row held
+            g[u].v[e] = v;
+            db.v[e] += v;
+        }
+        store8_full((T*)a.e + r * a.ld + col, g[u]);
+    }
+    if (a.db_part) {
+        store8_full(&cols[rl][lane * 8], db);
+        __syncthreads();
+        const long long c = (long long)blockIdx.x * kGradCols + threadIdx.x;
+        if (c < a.ld) {
+            float* o = a.db_part + blockIdx.y * a.ld + c;
+            float v = a.db_add ? *o : 0.f;                   // on top of the earlier pieces' rows
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v += cols[q][threadIdx.x];
+            *o = v;
         }
     }
-    if (a.loss && blockIdx.x == 0 && blockIdx.y == 0)
-        reduce_loss(a.loss_rows, a.all_target, a.n, a.ignore, a.mean, a.loss);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && (a.all.factor || a.all.loss_rows)) over_all_rows(a.all);
 }
 
 // out[r][c] = *factor times the sum over s of slab s, in the order of s; a row of `cols` values, slabs `stride` apart
@@ -438,7 +442,7 @@ struct XentPlan {
     long long ld_e, ld_pack;
     bool dw_slabs, pack_x, pack_w;
     // workspace offsets, bytes
-    long long count, shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, total;
+    long long shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, total;
 };
 
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
@@ -504,7 +508,6 @@ XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool 
         at += (bytes + 255) / 256 * 256;
         return r;
     };
-    q.count = take(4);
     q.shared = take(4);
     q.loss = take(4LL * p.n);
     q.lse = take(4LL * p.n);
@@ -546,10 +549,10 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
     constexpr int bk = Mma<T>::BK;
     const bool none = p.reduction == ASL_REDUCE_NONE, mean = p.reduction == ASL_REDUCE_MEAN;
     float* loss_rows = none ? loss : (float*)(ws + q.loss);
-    int* count = (int*)(ws + q.count);
     float* shared = (float*)(ws + q.shared);
-    if (grad && mean && p.n > kCountInPlace)
-        hipLaunchKernelGGL(xent_count_kernel, dim3(1), dim3(256), 0, s, target, p.n, (long long)p.ignore_index, count);
+    XentAll all = {};
+    all.target = target; all.loss = loss; all.upstream = none ? nullptr : upstream; all.ignore = p.ignore_index; all.n = p.n;
+    all.mean = mean;
     const void* wk = w;                   // what the products read: the caller's tensors, or their copies
     long long ld_w = p.ld_w, ld_x = p.ld_x;
     const auto pack = [&](const void* src, long long ld, int rows, void* dst) {
@@ -583,24 +586,23 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             hipLaunchKernelGGL((xent_gemm_kernel<T, true, true, true>), dim3(q.tiles, ceil_div(rows, kTile)), dim3(256), 0, s, g);
         }
         XentRows r = {};
-        r.target = target + r0; r.all_target = target; r.count = p.n > kCountInPlace ? count : nullptr;
-        r.upstream = upstream ? upstream + (none ? r0 : 0) : nullptr; r.upstream_rows = none;
+        r.target = target + r0; r.upstream = upstream && none ? upstream + r0 : nullptr;
         r.tile_max = g.tile_max; r.tile_sum = g.tile_sum; r.tile_lin = g.tile_lin; r.target_logit = g.target_logit;
-        r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg); r.shared = shared;
+        r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
         r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr;
         r.ignore = p.ignore_index; r.smoothing = p.label_smoothing; r.inv_classes = 1.f / (float)p.classes; r.exp_unit = 1.f / Mma<T>::SCALE;
-        r.rows = rows; r.n = p.n; r.classes = p.classes; r.tiles = q.tiles; r.reduction = p.reduction; r.factors = grad;
+        r.rows = rows; r.classes = p.classes; r.tiles = q.tiles; r.factors = grad;
         hipLaunchKernelGGL(xent_rows_kernel, dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
         if (!grad) continue;
         const bool last = piece == q.pieces - 1;
         XentG c = {};
         c.e = ws + q.e; c.ld = q.ld_e; c.factor = g.tile_max; c.target_g = r.target_g; c.row_g = r.row_g; c.target = target + r0;
-        c.loss_rows = loss_rows; c.all_target = target; c.loss = !none && last && loss ? loss : nullptr;
+        c.all = all; c.all.loss_rows = !none && last ? loss_rows : nullptr; c.all.factor = piece == 0 ? shared : nullptr;
         c.db_part = db ? (float*)(ws + q.dbp) : nullptr; c.db_add = piece > 0;
         c.ignore = p.ignore_index; c.smoothing = p.label_smoothing; c.inv_classes = r.inv_classes; c.rows = rows;
-        c.classes = p.classes; c.tiles = q.tiles; c.tile_shift = q.tile_shift; c.n = p.n; c.mean = mean;
+        c.classes = p.classes; c.tiles = q.tiles; c.tile_shift = q.tile_shift;
         const int groups = ceil_div(rows, kGradRows);
-        hipLaunchKernelGGL((xent_g_kernel<T>), dim3(ceil_div(q.ld_e, 2048), groups), dim3(256), 0, s, c);
+        hipLaunchKernelGGL((xent_g_kernel<T>), dim3(ceil_div(q.ld_e, kGradCols), groups), dim3(256), 0, s, c);
         if (dx) {                          // dx[row][k] = sum over classes G[row][v] W[v][k]
             XentGemm h = {};
             h.p = wk; h.ld_p = ld_w; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
@@ -640,18 +642,12 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
                                    (const float*)(ws + q.dws), q.dw_splits, (long long)p.classes * p.d, (long long)p.d, p.classes,
                                    p.d, (T*)dw, (long long)p.d, shared);
         }
-        if (db && last) {
-            const dim3 grid(ceil_div(p.classes, 2048), 1);
-            if (p.bias_type)
-                hipLaunchKernelGGL((xent_slab_kernel<short>), grid, dim3(256), 0, s, (const float*)(ws + q.dbp), q.row_groups, q.ld_e, 0LL, 1,
-                                   p.classes, (short*)db, 0LL, shared);
-            else
-                hipLaunchKernelGGL((xent_slab_kernel<float>), grid, dim3(256), 0, s, (const float*)(ws + q.dbp), q.row_groups, q.ld_e, 0LL, 1,
-                                   p.classes, (float*)db, 0LL, shared);
-        }
+        if (db && last) column_sums((const float*)(ws + q.dbp), q.row_groups, q.ld_e, p.classes, p.classes, db, nullptr, p.bias_type, shared, s);
     }
-    if (!none && loss && (!grad || !q.pieces))
-        hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, s, loss_rows, target, p.n, (long long)p.ignore_index, (int)mean, loss);
+    if (!none && (!grad || !q.pieces)) {
+        all.loss_rows = loss_rows;
+        hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, s, all);
+    }
     return (int)hipGetLastError();
 }
 

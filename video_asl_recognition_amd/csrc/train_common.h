@@ -1,5 +1,7 @@
 // Device helpers shared by the training operators: eight consecutive elements of a fp32 or bf16 row as fp32 registers.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace asl_detail {
@@ -62,9 +64,92 @@ __device__ __forceinline__ void store8(T* p, int n, const F8& r) {
         if (e < n) store1(p + e, r.v[e]);
 }
 
+// The same in two steps, for loads that are issued well ahead of their use: as they lie in memory, then as fp32.
+struct Raw8F {
+    f32x4 a, b;
+};
+__device__ __forceinline__ F8 widen(const Raw8F& r) { return {{r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]}}; }
+__device__ __forceinline__ F8 widen(const bf16x8& r) {
+    F8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.v[e] = bf16_to_f32(r[e]);
+    return o;
+}
+__device__ __forceinline__ Raw8F load8_raw(const float* p, int n) {
+    Raw8F r = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (n >= 8) {
+        r.a = *(const f32x4u*)p;
+        r.b = *(const f32x4u*)(p + 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e < n) r.a[e] = p[e];
+            if (e + 4 < n) r.b[e] = p[e + 4];
+        }
+    }
+    return r;
+}
+__device__ __forceinline__ bf16x8 load8_raw(const short* p, int n) {
+    bf16x8 r = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (n >= 8) {
+        r = *(const bf16x8u*)p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) r[e] = p[e];
+    }
+    return r;
+}
+template <typename T>
+struct RawOf;
+template <>
+struct RawOf<float> {
+    using type = Raw8F;
+};
+template <>
+struct RawOf<short> {
+    using type = bf16x8;
+};
+
+// Sum over each 16 lanes, then over the wave, the same in every lane: lane exchanges within the vector unit (data-parallel
+// primitives and the row swaps of gfx950), where a shuffle goes through the LDS.
+__device__ __forceinline__ float row16_sum(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto with = [](float x, auto ctrl) {
+        return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    v = with(v, std::integral_constant<int, 0xb1>{});        // lane ^ 1
+    v = with(v, std::integral_constant<int, 0x4e>{});        // lane ^ 2
+    v = with(v, std::integral_constant<int, 0x141>{});       // the other four of eight (mirrored)
+    v = with(v, std::integral_constant<int, 0x140>{});       // the other eight of sixteen (mirrored)
+#endif
+    return v;
+}
+__device__ __forceinline__ float wave64_sum(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    v = row16_sum(v);
+    // the swap of a register's rows with its own copy's (elements taken out before the cast: a bit cast of an element reads
+    // the vector's first)
+    int i = __builtin_bit_cast(int, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+    const unsigned a0 = a[0], a1 = a[1];
+    v = __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
+    i = __builtin_bit_cast(int, v);
+    const auto b = __builtin_amdgcn_permlane32_swap(i, i, false, false);
+    const unsigned b0 = b[0], b1 = b[1];
+    v = __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
+#endif
+    return v;
+}
+
 // the same from a tensor whose type is only known at run time (a launch-uniform branch)
 __device__ __forceinline__ F8 load8_any(const void* base, int bf16, long long at, int n) {
     return bf16 ? load8((const short*)base + at, n) : load8((const float*)base + at, n);
 }
+
+// Column sums of partial rows [parts][ld], added up in a fixed order: columns [0, split) to out0, [split, cols) to out1 (null:
+// not wanted), times *factor where that is given (layernorm_train.hip).
+int column_sums(const float* part, int parts, long long ld, long long cols, long long split, void* out0, void* out1, int bf16,
+                const float* factor, hipStream_t s);
 
 }  // namespace asl_detail
