@@ -448,13 +448,20 @@ struct XentPlan {
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
 constexpr int kPieceRows = 1 << 17;               // and rows: what grids and per-tile numbers are sized by
 
-// slices of a contraction so that `tiles` workgroups become `enough` to fill the CUs, none shorter than four steps, and few
-// enough that the slabs stay small
-inline int splits_for(long long tiles, int k, int bk, int enough) {
-    const long long want = tiles > 0 ? enough / tiles : 1;
-    const long long most = ((long long)k + 4 * bk - 1) / (4 * bk);
-    const long long s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
+// Slices of a contraction of `steps` steps for a product of `tiles` tiles and `out` values: what the tiles take one after
+// another on the 256 CUs at `us` a step, against what the slabs of partial sums cost (written and read back at 4 TB/s, and one
+// more launch).
+inline int splits_for(long long tiles, int steps, double us, double out) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 32 && s * 2 <= steps + 1; ++s) {
+        const double t = ceil_div(tiles * s, 256) * (ceil_div(steps, s) * us + 2.0) + (s > 1 ? 3.0 + s * out * 8.0 / 4e6 : 0.0);
+        if (t < least) {
+            least = t;
+            best = s;
+        }
+    }
+    return best;
 }
 inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, splits), bk) * bk; }
 
@@ -496,8 +503,12 @@ XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool 
     if (grad && p.n) {
         q.dx_tile = tile_for(p, rows, p.d, 2);
         q.dw_tile = tile_for(p, p.classes, p.d, 2);
-        q.dx_splits = splits_for((long long)ceil_div(rows, q.dx_tile) * ceil_div(p.d, q.dx_tile), p.classes, bk, q.dx_tile == 256 ? 256 : 512);
-        q.dw_splits = splits_for((long long)ceil_div(p.classes, q.dw_tile) * ceil_div(p.d, q.dw_tile), (int)rows, bk, q.dw_tile == 256 ? 256 : 512);
+        // measured per step of a tile's contraction, one workgroup a CU
+        const auto step_us = [&](int tile) { return !p.type ? 0.3 : tile == 256 ? 1.6 : tile == 128 ? 0.5 : 0.4; };
+        q.dx_splits = splits_for((long long)ceil_div(rows, q.dx_tile) * ceil_div(p.d, q.dx_tile), ceil_div(p.classes, bk),
+                                 step_us(q.dx_tile), (double)rows * p.d);
+        q.dw_splits = splits_for((long long)ceil_div(p.classes, q.dw_tile) * ceil_div(p.d, q.dw_tile), ceil_div(rows, bk),
+                                 step_us(q.dw_tile), (double)p.classes * p.d);
     }
     q.dx_splits = ceil_div(p.classes, k_per_split(p.classes, q.dx_splits, bk));
     q.dw_splits = rows ? ceil_div(rows, k_per_split((int)rows, q.dw_splits, bk)) : 1;

@@ -33,21 +33,29 @@ def _type(t: torch.Tensor, what: str) -> int:
     return c
 
 
-def _on(dev: torch.device):
+_HERE = nullcontext()
+
+
+def _on(index: int):
     """kernels are launched on the device their tensors live on, whichever is current"""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _same_device(dev, **tensors):
-    if dev.type != "cuda":
-        raise ValueError(f"tensors must be on the GPU, got {dev}")
+def _device(x: torch.Tensor, **tensors) -> int:
+    """index of the GPU that all of them are on"""
+    index = x.get_device()
+    if index < 0:
+        raise ValueError(f"tensors must be on the GPU, got {x.device}")
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, expected {x.device}")
+    return index
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., d] -> [rows, d] with unit stride along d and rows that do not overlap; a view where the strides allow it"""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     d = t.shape[-1]
     t = t.reshape(-1, d) if d else t.reshape(0, 0)
     if (d > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < d):
@@ -63,8 +71,9 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+# handle of a device's current stream; the shortcut saves the stream object that torch.cuda.current_stream builds (1.7 us of a
+# small call's 10)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _bytes(n: int, what: str) -> int:
@@ -78,57 +87,52 @@ def _check_norm(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., d] with d >= 1, got {tuple(x.shape)}")
     d = x.shape[-1]
-    _same_device(x.device, weight=weight, bias=bias)
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != (d,):
+        if t is not None and (t.dim() != 1 or t.shape[0] != d):
             raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight is {weight.dtype}, bias {bias.dtype}: one type for both")
     w = weight if weight is not None else bias
-    return _type(x, "x"), (_type(w, "weight") if w is not None else L.F32)
+    return d, _type(x, "x"), (_type(w, "weight") if w is not None else L.F32)
 
 
 def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5,
                    out_dtype: Optional[torch.dtype] = None):
     """x [..., d] -> (y [..., d], mean [...], rstd [...]): LayerNorm over the last dimension, y in `out_dtype` (default: x's),
     and the fp32 statistics that layer_norm_bwd takes."""
-    xt, wt = _check_norm(x, weight, bias)
-    dev, lead, d = x.device, x.shape[:-1], x.shape[-1]
+    d, xt, wt = _check_norm(x, weight, bias)
+    index = _device(x, weight=weight, bias=bias)
     x2 = _rows(x)
-    rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=dev)
-    stats = torch.empty((2,) + tuple(lead), dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
+    y = x.new_empty(x.shape, dtype=out_dtype)
+    mean, rstd = x.new_empty((2,) + x.shape[:-1], dtype=torch.float32).unbind(0)
     w = weight.contiguous() if weight is not None else None
     b = bias.contiguous() if bias is not None else None
-    p = L.LayerNormParams(rows, d, _ld(x2), d, d, xt, wt, _type(y, "out_dtype"), eps)
-    with _on(dev):
-        L.check(L.lib.asl_layernorm_fwd(C.byref(p), _ptr(x2), _ptr(w), _ptr(b), _ptr(y), _ptr(mean), _ptr(rstd), _stream(dev)),
-                "layer_norm_fwd")
+    p = L.LayerNormParams(x2.shape[0], d, _ld(x2), d, d, xt, wt, _type(y, "out_dtype"), eps)
+    with _on(index):
+        L.check(L.lib.asl_layernorm_fwd(C.byref(p), x2.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                        _stream(index)), "layer_norm_fwd")
     return y, mean, rstd
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor):
     """(dx, dweight, dbias) of layer_norm_fwd: dx in x's type, the other two in the weight's (fp32 without one)."""
-    xt, wt = _check_norm(x, weight, None)
-    dev, lead, d = x.device, x.shape[:-1], x.shape[-1]
-    _same_device(dev, dy=dy, mean=mean, rstd=rstd)
+    d, xt, wt = _check_norm(x, weight, None)
+    index = _device(x, weight=weight, dy=dy, mean=mean, rstd=rstd)
     if dy.shape != x.shape:
         raise ValueError(f"dy is {tuple(dy.shape)}, x {tuple(x.shape)}")
     for name, t in (("mean", mean), ("rstd", rstd)):
-        if t.dtype != torch.float32 or t.shape != lead:
-            raise ValueError(f"{name} must be float32 {tuple(lead)}, got {t.dtype} {tuple(t.shape)}")
+        if t.dtype != torch.float32 or t.shape != x.shape[:-1]:
+            raise ValueError(f"{name} must be float32 {tuple(x.shape[:-1])}, got {t.dtype} {tuple(t.shape)}")
     x2, dy2, mean, rstd = _rows(x), _rows(dy), mean.contiguous(), rstd.contiguous()
     w = weight.contiguous() if weight is not None else None
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dwb = torch.empty(2, d, dtype=weight.dtype if weight is not None else torch.float32, device=dev)
+    dx = x.new_empty(x.shape)
+    dw, db = x.new_empty((2, d), dtype=weight.dtype if weight is not None else torch.float32).unbind(0)
     p = L.LayerNormParams(x2.shape[0], d, _ld(x2), _ld(dy2), d, xt, wt, _type(dy, "dy"), 0.0)
-    ws = torch.empty(_bytes(L.lib.asl_layernorm_bwd_workspace(C.byref(p)), "layer_norm_bwd"), dtype=torch.uint8, device=dev)
-    base = dwb.data_ptr()
-    with _on(dev):
-        L.check(L.lib.asl_layernorm_bwd(C.byref(p), _ptr(dy2), _ptr(x2), _ptr(w), _ptr(mean), _ptr(rstd), _ptr(dx), base,
-                                        base + d * dwb.element_size(), _ptr(ws), _stream(dev)), "layer_norm_bwd")
-    return dx, dwb[0], dwb[1]
+    ws = x.new_empty(_bytes(L.lib.asl_layernorm_bwd_workspace(C.byref(p)), "layer_norm_bwd"), dtype=torch.uint8)
+    with _on(index):
+        L.check(L.lib.asl_layernorm_bwd(C.byref(p), dy2.data_ptr(), x2.data_ptr(), _ptr(w), mean.data_ptr(), rstd.data_ptr(),
+                                        dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), _stream(index)), "layer_norm_bwd")
+    return dx, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -158,7 +162,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 def _check_xent(x, weight, target, bias, reduction, label_smoothing):
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
         raise ValueError(f"x must be [..., d] and weight [classes, d], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    _same_device(x.device, weight=weight, target=target, bias=bias)
+    index = _device(x, weight=weight, target=target, bias=bias)
     if x.dtype != weight.dtype:
         raise ValueError(f"x is {x.dtype}, weight {weight.dtype}: one type for both")
     if target.dtype != torch.int64 or target.shape != x.shape[:-1]:
@@ -169,15 +173,16 @@ def _check_xent(x, weight, target, bias, reduction, label_smoothing):
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    return index
 
 
 def _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction):
-    _check_xent(x, weight, target, bias, reduction, label_smoothing)
+    index = _check_xent(x, weight, target, bias, reduction, label_smoothing)
     x2, w2, t = _rows(x), _rows(weight), target.contiguous()
     b = bias.contiguous() if bias is not None else None
     p = L.XentParams(x2.shape[0], w2.shape[0], w2.shape[1], _type(x, "x"), _type(b, "bias") if b is not None else L.F32,
                      _REDUCTIONS[reduction], _ld(x2), _ld(w2), ignore_index, label_smoothing, 0)
-    return x2, w2, t, b, p
+    return index, x2, w2, t, b, p
 
 
 def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -185,31 +190,31 @@ def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torc
     """(loss, lse) of cross_entropy(linear(x, weight, bias), target): x [..., d], weight [classes, d] of the same type, target
     int64 [...].  loss is fp32, 0-d or (reduction "none") of target's shape; lse, fp32 of target's shape, is log sum exp of
     the logits."""
-    x2, w2, t, b, p = _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction)
-    dev = x.device
-    loss = torch.empty(target.shape if reduction == "none" else (), dtype=torch.float32, device=dev)
-    lse = torch.empty(target.shape, dtype=torch.float32, device=dev)
-    ws = torch.empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), _ptr(x2), _ptr(w2), 0), "linear_cross_entropy"), dtype=torch.uint8, device=dev)
+    index, x2, w2, t, b, p = _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction)
+    loss = x.new_empty(target.shape if reduction == "none" else (), dtype=torch.float32)
+    lse = x.new_empty(target.shape, dtype=torch.float32)
+    ws = x.new_empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), x2.data_ptr(), w2.data_ptr(), 0), "linear_cross_entropy"),
+                     dtype=torch.uint8)
     if loss.numel():
-        with _on(dev):
-            L.check(L.lib.asl_linear_xent_fwd(C.byref(p), _ptr(x2), _ptr(w2), _ptr(b), _ptr(t), _ptr(loss), _ptr(lse), _ptr(ws),
-                                              _stream(dev)), "linear_cross_entropy_fwd")
+        with _on(index):
+            L.check(L.lib.asl_linear_xent_fwd(C.byref(p), x2.data_ptr(), w2.data_ptr(), _ptr(b), t.data_ptr(), loss.data_ptr(),
+                                              lse.data_ptr(), ws.data_ptr(), _stream(index)), "linear_cross_entropy_fwd")
     return loss, lse
 
 
 def _xent_grad(x, weight, target, bias, upstream, ignore_index, label_smoothing, reduction, want):
-    x2, w2, t, b, p = _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction)
-    dev = x.device
-    loss = torch.empty(target.shape if reduction == "none" else (), dtype=torch.float32, device=dev)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want[1] else None
-    db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if want[2] and bias is not None else None
-    ws = torch.empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), _ptr(x2), _ptr(w2), 1), "linear_cross_entropy"), dtype=torch.uint8, device=dev)
+    index, x2, w2, t, b, p = _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction)
+    loss = x.new_empty(target.shape if reduction == "none" else (), dtype=torch.float32)
+    dx = x.new_empty(x.shape) if want[0] else None
+    dw = x.new_empty(weight.shape) if want[1] else None
+    db = x.new_empty(bias.shape, dtype=bias.dtype) if want[2] and bias is not None else None
+    ws = x.new_empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), x2.data_ptr(), w2.data_ptr(), 1), "linear_cross_entropy"),
+                     dtype=torch.uint8)
     # a 0-row "none" loss has no storage: the entry point wants an address all the same and writes nothing there
-    with _on(dev):
-        L.check(L.lib.asl_linear_xent_grad(C.byref(p), _ptr(x2), _ptr(w2), _ptr(b), _ptr(t), _ptr(upstream),
-                                           _ptr(loss) or _ptr(ws), None, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), _stream(dev)),
-                "linear_cross_entropy_grad")
+    with _on(index):
+        L.check(L.lib.asl_linear_xent_grad(C.byref(p), x2.data_ptr(), w2.data_ptr(), _ptr(b), t.data_ptr(), _ptr(upstream),
+                                           loss.data_ptr() or ws.data_ptr(), None, _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(),
+                                           _stream(index)), "linear_cross_entropy_grad")
     return loss, dx, dw, db
 
 
@@ -259,67 +264,75 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _clip(grads: Sequence[torch.Tensor], max_norm, norm_type, out: Optional[Sequence[torch.Tensor]], device):
+def _layout(tensors, index, what):
+    """(types, addresses, whether all are contiguous) of tensors that must be dense and on one GPU; a few C-level passes over
+    the list, because a model has hundreds of them"""
+    n = len(tensors)
+    where = list(map(torch.Tensor.get_device, tensors))
+    if where.count(index) != n:
+        i = next(i for i, w in enumerate(where) if w != index)
+        raise ValueError(f"{what} {i} is on {tensors[i].device}, expected cuda:{index}")
+    types = [_TYPES.get(t.dtype, -1) for t in tensors]
+    if -1 in types:
+        i = types.index(-1)
+        raise ValueError(f"{what} {i} must be float32 or bfloat16, got {tensors[i].dtype}")
+    flat = all(map(torch.Tensor.is_contiguous, tensors))
+    if not flat:
+        for i, t in enumerate(tensors):
+            if not _dense(t):
+                raise ValueError(f"{what} {i} is not dense: strides {t.stride()} for {tuple(t.shape)}")
+    return array.array("i", types), array.array("Q", list(map(torch.Tensor.data_ptr, tensors))), flat
+
+
+def _clip(grads: Sequence[torch.Tensor], max_norm, norm_type, out: Optional[Sequence[torch.Tensor]]):
     grads = list(grads)
-    norm_type = float(norm_type)
-    if norm_type not in (2.0, float("inf")):
+    if norm_type not in (2, float("inf")):
         raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
     if max_norm is not None and not max_norm >= 0:
         raise ValueError(f"max_norm must be at least 0, got {max_norm}")
-    if not grads and device is None:
+    if not grads:
         raise ValueError("no gradients")
-    dev = grads[0].device if grads else torch.device(device)
-    if dev.type != "cuda":
-        raise ValueError(f"gradients must be on the GPU, got {dev}")
-    if out is None and max_norm is not None:
-        out = grads
-    elif out is not None:
+    index, n = grads[0].get_device(), len(grads)
+    if index < 0:
+        raise ValueError(f"gradients must be on the GPU, got {grads[0].device}")
+    types, ptrs, flat = _layout(grads, index, "gradient")
+    numel = array.array("q", list(map(torch.Tensor.numel, grads)))
+    otypes = optrs = None
+    if out is not None:
         out = list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"{len(grads)} gradients, {len(out)} outputs")
-    kinds, okinds = array.array("i"), array.array("i")
-    for i, g in enumerate(grads):
-        if g.device != dev:
-            raise ValueError(f"gradient {i} is on {g.device}, expected {dev}")
-        kinds.append(_type(g, "gradients"))
-        if not _dense(g):
-            raise ValueError(f"gradient {i} is not dense: strides {g.stride()} for {tuple(g.shape)}")
-        if out is not None and out is not grads:
-            o = out[i]
-            if o.device != dev or o.shape != g.shape:
-                raise ValueError(f"output {i} is {tuple(o.shape)} on {o.device}, gradient {tuple(g.shape)} on {dev}")
-            if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                raise ValueError(f"output {i} has strides {o.stride()}, gradient {g.stride()}")
-            okinds.append(_type(o, "outputs"))
-    n = len(grads)
-    ptrs = array.array("Q", [g.data_ptr() for g in grads])
-    numel = array.array("q", [g.numel() for g in grads])
-    optrs = ptrs if out is grads else array.array("Q", [o.data_ptr() for o in out]) if out is not None else None
-    if out is grads:
-        okinds = kinds
-    addr = lambda a: a.buffer_info()[0] if a is not None and n else None
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(_bytes(L.lib.asl_grad_clip_workspace(n, addr(numel)), "clip_grads"), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        L.check(L.lib.asl_grad_clip(n, addr(ptrs), addr(numel), addr(kinds), addr(optrs), addr(okinds) if optrs is not None else None,
-                                    0.0 if max_norm is None else float(max_norm), int(norm_type != 2.0), _ptr(norm), _ptr(ws),
-                                    _stream(dev)), "clip_grads")
+        otypes, optrs, oflat = _layout(out, index, "output")
+        if len(out) != n or list(map(torch.Tensor.numel, out)) != numel.tolist():
+            raise ValueError(f"{n} gradients, {len(out)} outputs, or not tensor for tensor the same number of elements")
+        if not (flat and oflat):
+            for i, (g, o) in enumerate(zip(grads, out)):
+                if not (g.is_contiguous() and o.is_contiguous()) and (g.shape != o.shape or g.stride() != o.stride()):
+                    raise ValueError(f"output {i} has strides {o.stride()}, gradient {g.stride()}")
+    elif max_norm is not None:
+        otypes, optrs = types, ptrs
+    addr = lambda a: a.buffer_info()[0] if a is not None else None
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    ws = norm.new_empty(_bytes(L.lib.asl_grad_clip_workspace(n, addr(numel)), "clip_grads"), dtype=torch.uint8)
+    with _on(index):
+        L.check(L.lib.asl_grad_clip(n, addr(ptrs), addr(numel), addr(types), addr(optrs), addr(otypes),
+                                    0.0 if max_norm is None else float(max_norm), int(norm_type != 2), norm.data_ptr(), ws.data_ptr(),
+                                    _stream(index)), "clip_grads")
     return norm
 
 
 @torch.no_grad()
 def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The 2-norm (or, norm_type inf, the largest magnitude) over all elements of all tensors: fp32, 0-d, on the GPU."""
-    return _clip(grads, None, norm_type, None, None)
+    return _clip(grads, None, norm_type, None)
 
 
 @torch.no_grad()
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
-    """Scales the gradients by min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensor for tensor, fp32 or bf16 each:
-    bf16 gradients into an optimizer's fp32 buffers in the same pass), and returns the norm they had.  A tensor may not be
+    """Scales the gradients by min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensor for tensor, fp32 or bf16 each, of
+    the same strides or both contiguous: bf16 gradients into an optimizer's fp32 buffers in the same pass), and returns the
+    norm they had.  A tensor may not be
     listed twice.  NaN in, NaN out."""
-    return _clip(grads, max_norm, norm_type, out, None)
+    return _clip(grads, max_norm, norm_type, out)
 
 
 @torch.no_grad()
@@ -331,4 +344,4 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     grads: List[torch.Tensor] = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=parameters[0].device if parameters else None)
-    return _clip(grads, max_norm, norm_type, None, None)
+    return _clip(grads, max_norm, norm_type, None)
