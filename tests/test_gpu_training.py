@@ -292,6 +292,19 @@ def test_linear_cross_entropy_large_tiles(gpu, n, v, d):
     _xent_check(x, w, b, t, smooth=0.1, reduction="sum", what="large, smoothed")
 
 
+@pytest.mark.parametrize("n,v,d", [(256, 8192, 64), (300, 8211, 72), (1100, 1003, 200), (2100, 6000, 33), (64, 70000, 64)])
+def test_linear_cross_entropy_large_fp32(gpu, n, v, d):
+    """sizes that take fp32 apart into bf16 planes: held to the bounds of fp32 products"""
+    x, w, b, t = _xent_case(n, v, d, F32, F32, 0.1)
+    b[v // 3: v // 2] = float("-inf")
+    t = torch.where((t >= v // 3) & (t < v // 2), 0, t)
+    _xent_check(x, w, b, t, what="large fp32")
+    # wide ranges: rows of very different size, weights that differ by 2^20
+    x *= torch.exp2(torch.randint(-12, 1, (n, 1), generator=_gen(1), device="cuda").float())
+    w *= torch.exp2(torch.randint(-20, 1, (v, 1), generator=_gen(2), device="cuda").float())
+    _xent_check(x, w, b, t, smooth=0.1 if not b.isinf().any() else 0.0, reduction="sum", what="large fp32, wide range")
+
+
 def test_linear_cross_entropy_bias_types_and_strides(gpu):
     g = _gen(9)
     x, w, b, t = _xent_case(70, 150, 96, BF16, F32, 0.2)
@@ -318,8 +331,8 @@ def test_linear_cross_entropy_leading_dimensions(gpu):
 
 def test_linear_cross_entropy_pieces(gpu):
     """more rows than one piece of exponentials holds"""
-    for dt, v, n in ((BF16, 65536, 8192 + 300), (F32, 65530, 4096 + 4100)):
-        x, w, b, t = _xent_case(n, v, 24, dt, F32, 0.1)
+    for dt, v, n, d in ((BF16, 65536, 8192 + 300, 24), (F32, 65530, 4096 + 4100, 24), (BF16, 65600, 8192 + 300, 40), (F32, 70000, 3000, 40)):
+        x, w, b, t = _xent_case(n, v, d, dt, F32, 0.1)
         _xent_check(x, w, b, t, smooth=0.1)
 
 

@@ -346,6 +346,8 @@ struct XentG {
     long long ignore;
     float smoothing, inv_classes;
     int rows, classes, tiles, tile_shift, db_add;
+    short* planes;                        // not null: G goes here, as three bf16 planes
+    long long plane;
     XentAll all;
 };
 
@@ -357,6 +359,27 @@ __device__ __forceinline__ F8 load8_exp(const _Float16* p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) r.v[e] = (float)a[e];
     return r;
+}
+
+// fp32 as the sum of three bf16, each the rest's nearest.  Infinities and NaN lie in the first alone; a value that would round
+// to infinity is cut instead.
+__device__ __forceinline__ void store_planes(short* p, long long plane, const F8& v) {
+    bf16x8 h, m, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float x = v.v[e];
+        short a = f32_to_bf16(x);
+        if (!(fabsf(bf16_to_f32(a)) < INFINITY)) a = fabsf(x) < INFINITY ? (short)(__builtin_bit_cast(unsigned, x) >> 16) : a;
+        float rest = x - bf16_to_f32(a);
+        if (!(fabsf(x) < INFINITY)) rest = 0.f;
+        const short b = f32_to_bf16(rest);
+        h[e] = a;
+        m[e] = b;
+        l[e] = f32_to_bf16(rest - bf16_to_f32(b));
+    }
+    *(bf16x8*)p = h;
+    *(bf16x8*)(p + plane) = m;
+    *(bf16x8*)(p + 2 * plane) = l;
 }
 
 // 256 columns x 32 rows a workgroup: half a wave on each row, four rows a lane, all of them on their way at once
@@ -396,7 +419,8 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
             g[u].v[e] = v;
             db.v[e] += v;
         }
-        store8_full((T*)a.e + r * a.ld + col, g[u]);
+        if (a.planes) store_planes(a.planes + r * a.ld + col, a.plane, g[u]);
+        else store8_full((T*)a.e + r * a.ld + col, g[u]);
     }
     if (a.db_part) {
         store8_full(&cols[rl][lane * 8], db);
@@ -440,9 +464,9 @@ __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int sla
 struct XentPlan {
     int esize, rows, pieces, tiles, tile, tile_shift, dx_tile, dw_tile, dx_splits, dw_splits, row_groups;
     long long ld_e, ld_pack;
-    bool dw_slabs, pack_x, pack_w;
+    bool dw_slabs, pack_x, pack_w, wide;
     // workspace offsets, bytes
-    long long shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, total;
+    long long shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, gp, total;
 };
 
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
@@ -471,10 +495,11 @@ inline bool lies_well(const void* t, long long ld, int d) {
 }
 
 // Tile of a product with `a` x `b` results.  256 x 256 takes the fewest bytes per FLOP but needs tiles for most of the 256
-// CUs (a long contraction makes `deep` of one); 128 x 128 fills them from a quarter of that; fp32, and results too narrow
-// for either, take 64 x 64.
+// CUs (a long contraction makes `deep` of one); 128 x 128 fills them from a quarter of that; products too narrow for either,
+// and fp32 ones too small to be worth taking apart into planes, take 64 x 64.
 inline int tile_for(const asl_xent_params& p, long long a, long long b, int deep) {
-    if (!p.type || p.n < 64 || p.classes < 64 || p.d < 32) return kTile;
+    if (p.n < 64 || p.classes < 64 || p.d < 32) return kTile;
+    if (!p.type && (double)p.n * p.classes * p.d < (double)(1 << 27)) return kTile;
     return (long long)ceil_div(a, 256) * ceil_div(b, 256) * deep >= 192 ? 256 : 128;
 }
 
@@ -485,26 +510,28 @@ XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool 
     q.tile_shift = q.tile == 256 ? 8 : q.tile == 128 ? 7 : 6;
     // the tile kernels read 16 bytes at a time and whole steps of 64 k: operands that do not allow it are laid out anew
     q.ld_pack = (p.d + 63LL) / 64 * 64;
-    q.pack_x = q.tile > 64 && !lies_well(x, p.ld_x, p.d);
-    q.pack_w = q.tile > 64 && !lies_well(w, p.ld_w, p.d);
+    q.wide = q.tile > kTile && !p.type;
+    q.pack_x = q.tile > kTile && (q.wide || !lies_well(x, p.ld_x, p.d));
+    q.pack_w = q.tile > kTile && (q.wide || !lies_well(w, p.ld_w, p.d));
+    const int planes = q.wide ? 3 : 1;
     q.tiles = ceil_div(p.classes, q.tile);
     q.ld_e = (long long)q.tiles * q.tile;
     long long rows = p.n < kPieceRows ? p.n : kPieceRows;
     if (grad) {
-        const long long most = kPieceBytes / (q.ld_e * q.esize) / 256 * 256;
+        const long long most = kPieceBytes / (q.ld_e * (q.wide ? 10 : q.esize)) / 256 * 256;
         if (rows > most) rows = most < 256 ? 256 : most;
     }
     q.rows = (int)rows;
     q.pieces = p.n ? ceil_div(p.n, rows) : 0;
     q.row_groups = ceil_div(rows, kGradRows);
-    const int bk = p.type ? Mma<short>::BK : Mma<float>::BK;
+    const int bk = p.type || q.wide ? Mma<short>::BK : Mma<float>::BK;
     q.dx_splits = q.dw_splits = 1;
     q.dx_tile = q.dw_tile = kTile;
     if (grad && p.n) {
         q.dx_tile = tile_for(p, rows, p.d, 2);
         q.dw_tile = tile_for(p, p.classes, p.d, 2);
         // measured per step of a tile's contraction, one workgroup a CU
-        const auto step_us = [&](int tile) { return !p.type ? 0.3 : tile == 256 ? 1.6 : tile == 128 ? 0.5 : 0.4; };
+        const auto step_us = [&](int tile) { return tile == kTile && !p.type ? 0.3 : (q.wide ? 6 : 1) * ( tile == 256 ? 1.6 : tile == 128 ? 0.5 : 0.4); };
         q.dx_splits = splits_for((long long)ceil_div(rows, q.dx_tile) * ceil_div(p.d, q.dx_tile), ceil_div(p.classes, bk),
                                  step_us(q.dx_tile), (double)rows * p.d);
         q.dw_splits = splits_for((long long)ceil_div(p.classes, q.dw_tile) * ceil_div(p.d, q.dw_tile), ceil_div(rows, bk),
@@ -534,8 +561,9 @@ XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool 
         q.dxs = take(want_dx && q.dx_splits > 1 ? 4LL * q.dx_splits * rows * p.d : 0);
         q.dws = take(want_dw && q.dw_slabs ? 4LL * q.dw_splits * p.classes * p.d : 0);
     }
-    q.xp = take(q.pack_x ? 2LL * rows * q.ld_pack : 0);
-    q.wp = take(q.pack_w ? 2LL * p.classes * q.ld_pack : 0);
+    q.xp = take(q.pack_x ? 2LL * planes * rows * q.ld_pack : 0);
+    q.wp = take(q.pack_w ? 2LL * planes * p.classes * q.ld_pack : 0);
+    q.gp = take(q.wide && grad ? 6LL * rows * q.ld_e : 0);
     q.total = at;
     return q;
 }
@@ -551,13 +579,25 @@ int xent_check(const asl_xent_params* p) {
     return ASL_OK;
 }
 
-__global__ void xent_pack_kernel(const short* src, long long ld, int rows, int d, short* dst, int per_row);
+// Rows of d elements at any alignment to rows of `per_row` 16-byte vectors of bf16, noughts behind d; fp32 to three planes of
+// them.
+template <typename T>
+__global__ __launch_bounds__(256) void xent_pack_kernel(const T* src, long long ld, int rows, int d, short* dst, int per_row) {
+    const long long vectors = (long long)rows * per_row;
+    for (long long v = blockIdx.x * 256LL + threadIdx.x; v < vectors; v += gridDim.x * 256LL) {
+        const long long r = v / per_row;
+        const int c = (int)(v - r * per_row) * 8;
+        const auto raw = load8_raw(src + r * ld + (c < d ? c : 0), d - c);
+        if constexpr (std::is_same<T, short>::value) *(bf16x8*)(dst + v * 8) = raw;
+        else store_planes(dst + v * 8, vectors * 8, widen(raw));
+    }
+}
 
 template <typename T>
 int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void* x, const void* w, const void* bias,
              const long long* target, const float* upstream, float* loss, float* lse, void* dx, void* dw, void* db, char* ws,
              hipStream_t s) {
-    constexpr int bk = Mma<T>::BK;
+    const int bk = q.wide ? Mma<short>::BK : Mma<T>::BK;
     const bool none = p.reduction == ASL_REDUCE_NONE, mean = p.reduction == ASL_REDUCE_MEAN;
     float* loss_rows = none ? loss : (float*)(ws + q.loss);
     float* shared = (float*)(ws + q.shared);
@@ -568,8 +608,8 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
     long long ld_w = p.ld_w, ld_x = p.ld_x;
     const auto pack = [&](const void* src, long long ld, int rows, void* dst) {
         const long long vectors = rows * (q.ld_pack / 8);
-        hipLaunchKernelGGL(xent_pack_kernel, dim3(ceil_div(vectors, 1024) < 8192 ? ceil_div(vectors, 1024) : 8192), dim3(256), 0, s,
-                           (const short*)src, ld, rows, p.d, (short*)dst, (int)(q.ld_pack / 8));
+        hipLaunchKernelGGL((xent_pack_kernel<T>), dim3(ceil_div(vectors, 512) < 8192 ? ceil_div(vectors, 512) : 8192), dim3(256), 0, s,
+                           (const T*)src, ld, rows, p.d, (short*)dst, (int)(q.ld_pack / 8));
     };
     if (q.pieces && q.pack_w) {
         pack(w, p.ld_w, p.classes, ws + q.wp);
@@ -590,6 +630,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         g.store_e = grad; g.target = target + r0; g.tile_max = (float*)(ws + q.tmax); g.tile_sum = (float*)(ws + q.tsum);
         g.tile_lin = (float*)(ws + q.tlin); g.target_logit = (float*)(ws + q.tlogit); g.tiles = q.tiles;
         g.splits = 1;
+        if (q.wide) g.plane_p = p.classes * ld_w, g.plane_q = rows * ld_x;
         if (q.tile > kTile) {
             const int rc = xent_tiles_logits(g, q.tile, s);
             if (rc) return rc;
@@ -607,7 +648,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         if (!grad) continue;
         const bool last = piece == q.pieces - 1;
         XentG c = {};
-        c.e = ws + q.e; c.ld = q.ld_e; c.factor = g.tile_max; c.target_g = r.target_g; c.row_g = r.row_g; c.target = target + r0;
+        c.e = ws + q.e; c.ld = q.ld_e; c.planes = q.wide ? (short*)(ws + q.gp) : nullptr; c.plane = rows * q.ld_e; c.factor = g.tile_max; c.target_g = r.target_g; c.row_g = r.row_g; c.target = target + r0;
         c.all = all; c.all.loss_rows = !none && last ? loss_rows : nullptr; c.all.factor = piece == 0 ? shared : nullptr;
         c.db_part = db ? (float*)(ws + q.dbp) : nullptr; c.db_add = piece > 0;
         c.ignore = p.ignore_index; c.smoothing = p.label_smoothing; c.inv_classes = r.inv_classes; c.rows = rows;
@@ -616,7 +657,8 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         hipLaunchKernelGGL((xent_g_kernel<T>), dim3(ceil_div(q.ld_e, kGradCols), groups), dim3(256), 0, s, c);
         if (dx) {                          // dx[row][k] = sum over classes G[row][v] W[v][k]
             XentGemm h = {};
-            h.p = wk; h.ld_p = ld_w; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
+            h.p = wk; h.ld_p = ld_w; h.q = ws + (q.wide ? q.gp : q.e); h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
+            if (q.wide) h.plane_p = p.classes * ld_w, h.plane_q = rows * q.ld_e;
             h.k_per_split = k_per_split(p.classes, q.dx_splits, bk);
             h.slabs = q.dx_splits > 1; h.factor = shared;
             T* dxr = (T*)dx + (long long)r0 * p.d;
@@ -636,7 +678,8 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         }
         if (dw) {                          // dW[v][k] = sum over rows G[row][v] x[row][k]
             XentGemm h = {};
-            h.p = xr; h.ld_p = ld_x; h.q = ws + q.e; h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
+            h.p = xr; h.ld_p = ld_x; h.q = ws + (q.wide ? q.gp : q.e); h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
+            if (q.wide) h.plane_p = rows * ld_x, h.plane_q = rows * q.ld_e;
             h.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
             h.slabs = q.dw_slabs; h.factor = shared; h.add = piece > 0;
             h.out = h.slabs ? (void*)(ws + q.dws) : dw; h.ld_out = p.d;
@@ -660,25 +703,6 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, s, all);
     }
     return (int)hipGetLastError();
-}
-
-// rows of d bf16 elements at any alignment to rows of `per_row` 16-byte vectors, noughts behind d
-__global__ __launch_bounds__(256) void xent_pack_kernel(const short* src, long long ld, int rows, int d, short* dst, int per_row) {
-    const long long vectors = (long long)rows * per_row;
-    for (long long v = blockIdx.x * 256LL + threadIdx.x; v < vectors; v += gridDim.x * 256LL) {
-        const long long r = v / per_row;
-        const int c = (int)(v - r * per_row) * 8;
-        bf16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
-        const short* p = src + r * ld + c;
-        if (c + 8 <= d) {
-            o = *(const bf16x8u*)p;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c + e < d) o[e] = p[e];
-        }
-        *(bf16x8*)(dst + v * 8) = o;
-    }
 }
 
 // no rows: the weight's and bias's gradients are nought

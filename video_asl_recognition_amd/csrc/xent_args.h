@@ -10,6 +10,7 @@ struct XentGemm {
     const void* p;
     const void* q;
     long long ld_p, ld_q;    // elements from one row of the stored matrix to the next
+    long long plane_p, plane_q;   // fp32 operands as three bf16 planes: elements from one plane to the next (0: one plane)
     int I, Jn, K;
     // plain products
     void* out;               // of the operands' type, or fp32 slabs [splits][Jn][I] when slabs != 0
@@ -31,7 +32,7 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 constexpr float kExpScale16 = 32768.f;    // exponentials in (0, 1] held as fp16: times this, so that fp16's range is used
 
-// xent_tiles.hip, tile 128 or 256: bf16, both operands' rows on 16 bytes and at most 2^21 bytes apart; those contiguous along
+// xent_tiles.hip, tile 128 or 256: bf16 (or fp32 as planes of it), both operands' rows on 16 bytes and at most 2^21 bytes apart; those contiguous along
 // k hold noughts from K to the next multiple of 64
 int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s);
 int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s);     // P along its own index, Q along k

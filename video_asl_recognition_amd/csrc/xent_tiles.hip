@@ -11,6 +11,12 @@
 // Operands contiguous along k are staged as [tile][64] and read as 16-byte fragments.  Operands contiguous along their own
 // index (W for dx, x and G for dW) are staged as they lie, [64][tile], and read with the transposing LDS read, which hands a
 // group of 16 lanes four k of 16 indices; no transposed copy of anything is made.
+//
+// fp32 operands come as three bf16 planes, x = h + m + l to all its 24 bits (rounded to nearest one after the other), and the
+// contraction runs over six pairs of planes, h l + l h + m m + h m + m h + h h, smallest first.  What is left out, m l + l m +
+// l l, is below 2^-23 of the product of the absolute values at worst and 2^-25 of it in the mean: the fp32 sums' own
+// rounding.  Six bf16 products still take less than half the time of one fp32 product on this card's matrix pipe (2048 x 8192
+// x 1024 with gradients: see linear_xent.hip).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -51,6 +57,9 @@ template <int TILE, bool KC>
 struct Panel {
     static constexpr int kPanel = TileLds<TILE>::kPanel, ND = TILE / 32, F = TILE / 64;   // DMA instructions and fragments a wave
     const char* at;          // first byte of the K step to be staged next
+    const char* origin;      // of the first step, and how far apart planes lie
+    long long plane;
+    int kall;
     long long row_bytes;
     int idx;                 // rows (KC) or columns of the stored matrix that belong to this tile
     int krem;                // k left from `at` on
@@ -62,8 +71,8 @@ struct Panel {
                                          int w0, unsigned stages) {
         row_bytes = ld * 2;
         idx = n - i0 < TILE ? n - i0 : TILE;
-        krem = ke - kb;
-        at = (const char*)base + (KC ? (long long)i0 * row_bytes + kb * 2LL : (long long)kb * row_bytes + i0 * 2LL);
+        krem = kall = ke - kb;
+        origin = at = (const char*)base + (KC ? (long long)i0 * row_bytes + kb * 2LL : (long long)kb * row_bytes + i0 * 2LL);
         lds = stages + wave * (kPanel / 4);
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
@@ -100,6 +109,10 @@ struct Panel {
     __device__ __forceinline__ void advance() {
         at += KC ? kBK * 2 : kBK * row_bytes;
         krem -= kBK;
+    }
+    __device__ __forceinline__ void to_plane(int which, bool turn, bool more) {
+        at = turn ? origin + which * plane : at;
+        krem = turn ? (more ? kall : 0) : krem;
     }
     template <int STAGE, int I>
     __device__ __forceinline__ void dma(i32x4 r) const {
@@ -140,7 +153,7 @@ __device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) 
     j = first + in % w;
 }
 
-template <int TILE, bool PKC, bool QKC, bool LOGITS>
+template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
 __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(const XentGemm a, int ti, int tj) {
 #if defined(__HIP_DEVICE_COMPILE__)
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -155,16 +168,29 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
     tile_of(blockIdx.x, ti, tj, bi, bj);
     const int i0 = bi * TILE, j0 = bj * TILE;
     const int kb = blockIdx.y * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
-    const int steps = ke > kb ? (ke - kb + kBK - 1) / kBK : 0;
+    const int steps = ke > kb ? (ke - kb + kBK - 1) / kBK * (WIDE ? 6 : 1) : 0;
 
     const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
     Panel<TILE, PKC> P;
     Panel<TILE, QKC> Q;
     P.init(a.p, a.ld_p, i0, a.I, kb, ke, wave, lane, wi, lds0);
     Q.init(a.q, a.ld_q, j0, a.Jn, kb, ke, wave, lane, wj, lds0 + 2 * Lds::kPanel);
+    int pair = 0;
+    constexpr int kPlaneP = 0 << 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10, kPlaneQ = 2 << 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10;
+    if constexpr (WIDE) {
+        P.plane = a.plane_p * 2;
+        Q.plane = a.plane_q * 2;
+        Q.at += 2 * Q.plane;                         // h l first
+    }
     const auto next = [&]() {
         P.advance();
         Q.advance();
+        if constexpr (WIDE) {
+            const bool turn = P.krem <= 0;
+            pair += turn;
+            P.to_plane(kPlaneP >> (pair * 2) & 3, turn, pair < 6);
+            Q.to_plane(kPlaneQ >> (pair * 2) & 3, turn, pair < 6);
+        }
     };
     const auto dma = [&](i32x4 pr, i32x4 qr, auto stage, auto n) {  // the n-th of a stage's DMA instructions
         constexpr int N = decltype(n)::value, S = decltype(stage)::value;
@@ -248,18 +274,19 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
     // ---- lane: i = wi + u*32 + 8*(r/4) + 4*(lane/32) + r%4, j = wj + v*32 + lane%32 ------------------------------
     const int h4 = (lane >> 5) * 4;
     if constexpr (!LOGITS) {
-        if (a.slabs) {
+        const float c = a.slabs ? 1.f : *a.factor;
+        if (WIDE || a.slabs) {
 #pragma unroll
             for (int v = 0; v < F; ++v) {
                 const int j = j0 + wj + v * 32 + (lane & 31);
                 if (j >= a.Jn) continue;
-                float* row = (float*)a.out + ((long long)blockIdx.y * a.Jn + j) * a.I;
+                float* row = (float*)a.out + (a.slabs ? ((long long)blockIdx.y * a.Jn + j) * a.I : j * a.ld_out);
 #pragma unroll
                 for (int u = 0; u < F; ++u)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int i = i0 + wi + u * 32 + r * 8 + h4;
-                        f32x4 d = {acc[u][v][r * 4], acc[u][v][r * 4 + 1], acc[u][v][r * 4 + 2], acc[u][v][r * 4 + 3]};
+                        f32x4 d = {acc[u][v][r * 4] * c, acc[u][v][r * 4 + 1] * c, acc[u][v][r * 4 + 2] * c, acc[u][v][r * 4 + 3] * c};
                         if (i + 3 < a.I) {
                             if (a.add) d += *(const f32x4u*)(row + i);
                             *(f32x4u*)(row + i) = d;
@@ -272,7 +299,6 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
             }
             return;
         }
-        const float c = *a.factor;
 #pragma unroll
         for (int v = 0; v < F; ++v)
 #pragma unroll
@@ -329,13 +355,16 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     half4 o;
+                    f32x4 o32;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = __expf(acc[u][v][r * 4 + e] - ref);
+                        const float x = WIDE ? expf(acc[u][v][r * 4 + e] - ref) : __expf(acc[u][v][r * 4 + e] - ref);
                         s += x;
                         o[e] = (_Float16)(x * kExpScale16);
+                        o32[e] = x;
                     }
-                    *(half4*)(smem + jl * Lds::kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
+                    if constexpr (!WIDE) *(half4*)(smem + jl * Lds::kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
+                    else if (a.store_e && j0 + jl < a.Jn) *(f32x4*)((float*)a.out + (j0 + jl) * a.ld_out + i0 + wi + u * 32 + r * 8 + h4) = o32;
                 }
             if (a.smooth) {
 #pragma unroll
@@ -361,7 +390,7 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
             a.tile_sum[at] = red[0][jl][1] + red[1][jl][1];
             if (a.smooth) a.tile_lin[at] = red[0][jl][2] + red[1][jl][2];
         }
-        if (!a.store_e) return;
+        if (WIDE || !a.store_e) return;
     }
     // rows out of LDS, 16 bytes a lane
     constexpr int L = TILE / 8;
@@ -382,26 +411,26 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
 #endif
 }
 
-template <int TILE, bool PKC, bool QKC, bool LOGITS>
+template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
 static int launch_tiles(const XentGemm& a, hipStream_t s) {
     const int ti = ceil_div(a.I, TILE), tj = ceil_div(a.Jn, TILE);
     if ((long long)ti * tj > 0x7fffffffLL) return ASL_ETOOBIG;
     constexpr int lds = LOGITS ? TileLds<TILE>::kLogits : TileLds<TILE>::kMain;
     static unsigned char lds_done[64];
-    const int rc = ensure_dynamic_lds((const void*)xent_tile_kernel<TILE, PKC, QKC, LOGITS>, lds, lds_done);
+    const int rc = ensure_dynamic_lds((const void*)xent_tile_kernel<TILE, PKC, QKC, LOGITS, WIDE>, lds, lds_done);
     if (rc != ASL_OK) return rc;
-    hipLaunchKernelGGL((xent_tile_kernel<TILE, PKC, QKC, LOGITS>), dim3((unsigned)(ti * tj), a.splits), dim3(256), lds, s, a, ti, tj);
+    hipLaunchKernelGGL((xent_tile_kernel<TILE, PKC, QKC, LOGITS, WIDE>), dim3((unsigned)(ti * tj), a.splits), dim3(256), lds, s, a, ti, tj);
     return (int)hipGetLastError();
 }
+template <bool PKC, bool QKC, bool LOGITS>
+static int launch_any(const XentGemm& a, int tile, hipStream_t s) {
+    if (a.plane_p)
+        return tile == 256 ? launch_tiles<256, PKC, QKC, LOGITS, true>(a, s) : launch_tiles<128, PKC, QKC, LOGITS, true>(a, s);
+    return tile == 256 ? launch_tiles<256, PKC, QKC, LOGITS, false>(a, s) : launch_tiles<128, PKC, QKC, LOGITS, false>(a, s);
+}
 
-int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s) {
-    return tile == 256 ? launch_tiles<256, true, true, true>(a, s) : launch_tiles<128, true, true, true>(a, s);
-}
-int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s) {
-    return tile == 256 ? launch_tiles<256, false, true, false>(a, s) : launch_tiles<128, false, true, false>(a, s);
-}
-int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s) {
-    return tile == 256 ? launch_tiles<256, false, false, false>(a, s) : launch_tiles<128, false, false, false>(a, s);
-}
+int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s) { return launch_any<true, true, true>(a, tile, s); }
+int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s) { return launch_any<false, true, false>(a, tile, s); }
+int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s) { return launch_any<false, false, false>(a, tile, s); }
 
 }  // namespace asl_detail
