@@ -186,7 +186,8 @@ def test_layer_norm_autograd_and_differences(gpu):
 
 
 # ------------------------------------------------------------------------------------------------ Linear + cross entropy
-XENT_SIZES = [(1, 1, 1), (1, 2, 3), (8, 2000, 512), (5, 100, 64), (65, 63, 33), (64, 64, 64), (130, 257, 100), (300, 1000, 70),
+XENT_SIZES = [(1, 1, 1), (1, 2, 3), (2, 31, 5), (16, 2000, 512), (17, 33, 65), (32, 1000, 130), (33, 1000, 130), (3, 16384, 70), (3, 16385, 20),
+              (20, 4500, 300), (8, 2000, 512), (5, 100, 64), (65, 63, 33), (64, 64, 64), (130, 257, 100), (300, 1000, 70),
               (257, 129, 513), (16, 5003, 129)]
 
 
@@ -225,9 +226,10 @@ def xent_reference(x, w, b, t, up, ignore, smooth, reduction, bf16):
     G = gr * (p - (1 - smooth) * hot - smooth / v)
     G = torch.where(keep[:, None], G, 0.0)
     # a logit's bound and lse's move p by as much of itself; rounded on the way for bf16: the exponential to fp16 of 2^15 its
-    # ratio to the tile's largest (2^-12 of it, or 2^-40 of the largest), then G to bf16
+    # ratio to the tile's largest (fp16 has 11 significant bits, half a step is 2^-11 of the value; below 2^-14 its steps are
+    # 2^-24, half of one 2^-25, which over 2^15 is 2^-40 of the largest), then G to bf16
     tG = gr.abs() * p * (bound + trow[:, None] + rel + 4 * U32) + 4 * U32 * (gr.abs() * (p + hot + smooth / v))
-    tG32 = tG + (gr.abs() * (1 - hot) * (2.0 ** -12 * p + 2.0 ** -40 * p.max(1, keepdim=True).values) if bf16 else 0.0)
+    tG32 = tG + (gr.abs() * (1 - hot) * (2.0 ** -11 * p + 2.0 ** -40 * p.max(1, keepdim=True).values) if bf16 else 0.0)
     tG = tG32 + (2.0 ** -8 * G.abs() * (1 + 2.0 ** -8) if bf16 else 0.0)
     tG, tG32 = (torch.where(keep[:, None], q, 0.0) for q in (tG, tG32))
     dx, tdx = G @ w, tG @ w.abs() + (v + 40) * U32 * (G.abs() @ w.abs())

@@ -447,6 +447,7 @@ __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int sla
     const int n = (int)(cols - c < 8 ? cols - c : 8);
     for (int r = blockIdx.y; r < rows; r += gridDim.y) {
         F8 v = load8(in + r * ld_in + c, n);
+#pragma unroll 4
         for (int s = 1; s < slabs; ++s) {
             const F8 q = load8(in + s * stride + r * ld_in + c, n);
 #pragma unroll
@@ -464,7 +465,7 @@ __global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int sla
 struct XentPlan {
     int esize, rows, pieces, tiles, tile, tile_shift, dx_tile, dw_tile, dx_splits, dw_splits, row_groups;
     long long ld_e, ld_pack;
-    bool dw_slabs, pack_x, pack_w, wide;
+    bool dw_slabs, pack_x, pack_w, wide, few;
     // workspace offsets, bytes
     long long shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, gp, total;
 };
@@ -472,21 +473,6 @@ struct XentPlan {
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
 constexpr int kPieceRows = 1 << 17;               // and rows: what grids and per-tile numbers are sized by
 
-// Slices of a contraction of `steps` steps for a product of `tiles` tiles and `out` values: what the tiles take one after
-// another on the 256 CUs at `us` a step, against what the slabs of partial sums cost (written and read back at 4 TB/s, and one
-// more launch).
-inline int splits_for(long long tiles, int steps, double us, double out) {
-    int best = 1;
-    double least = 1e30;
-    for (int s = 1; s <= 32 && s * 2 <= steps + 1; ++s) {
-        const double t = ceil_div(tiles * s, 256) * (ceil_div(steps, s) * us + 2.0) + (s > 1 ? 3.0 + s * out * 8.0 / 4e6 : 0.0);
-        if (t < least) {
-            least = t;
-            best = s;
-        }
-    }
-    return best;
-}
 inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, splits), bk) * bk; }
 
 // rows on 16 bytes, whole steps of 64 k, a tile's rows within 32-bit offsets
@@ -494,25 +480,46 @@ inline bool lies_well(const void* t, long long ld, int d) {
     return !((uintptr_t)t & 15) && !(ld & 7) && !(d & 63) && ld <= (1 << 20);
 }
 
-// Tile of a product with `a` x `b` results.  256 x 256 takes the fewest bytes per FLOP but needs tiles for most of the 256
-// CUs (a long contraction makes `deep` of one); 128 x 128 fills them from a quarter of that; products too narrow for either,
-// and fp32 ones too small to be worth taking apart into planes, take 64 x 64.
-inline int tile_for(const asl_xent_params& p, long long a, long long b, int deep) {
-    if (p.n < 64 || p.classes < 64 || p.d < 32) return kTile;
-    if (!p.type && (double)p.n * p.classes * p.d < (double)(1 << 27)) return kTile;
-    return (long long)ceil_div(a, 256) * ceil_div(b, 256) * deep >= 192 ? 256 : 128;
+// Tile and slices of a product with `a` x `b` results over `k`: what its tiles take one after another on the 256 CUs, against
+// what slabs of partial sums cost (written and read back at 4 TB/s, and one more launch).  Measured with one workgroup a CU:
+// 1.65 us per 64 of k for 256 x 256, 0.65 for 128 x 128, 0.4 for 64 x 64 (fp32: 0.6), and about 8, 5 and 3 us around that a
+// tile.  Products too narrow for the larger tiles, and fp32 ones too small to be worth taking apart into planes (128 M
+// multiplications: 512 x 512 x 512), take 64 x 64.
+struct TilePlan {
+    int tile, splits;
+};
+inline TilePlan tiles_for(const asl_xent_params& p, long long a, long long b, int k, bool may_split) {
+    const bool narrow = p.n < 64 || p.classes < 64 || p.d < 32 || (!p.type && (double)p.n * p.classes * p.d < (double)(1 << 27));
+    TilePlan best = {kTile, 1};
+    double least = 1e30;
+    const int steps = ceil_div(k, 64);
+    for (const int tile : {64, 128, 256}) {
+        if (narrow != (tile == 64)) continue;
+        const long long tiles = (long long)ceil_div(a, tile) * ceil_div(b, tile);
+        const double us = tile == 256 ? 1.65 : tile == 128 ? 0.65 : p.type ? 0.4 : 0.6, around = tile == 256 ? 8.0 : tile == 128 ? 5.0 : 3.0;
+        for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || s * 2 <= steps); ++s) {
+            const double t = ceil_div(tiles * s, 256) * (ceil_div(steps, s) * us * (p.type || tile == 64 ? 1 : 6) + around) +
+                             (s > 1 ? 3.0 + s * (double)a * b * 8.0 / 4e6 : 0.0);
+            if (t < least) {
+                least = t;
+                best = {tile, s};
+            }
+        }
+    }
+    return best;
 }
 
-XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool grad, bool want_dx, bool want_dw, bool want_db) {
+XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, bool grad, bool want_dx, bool want_dw, bool want_db) {
     XentPlan q = {};
     q.esize = p.type ? 2 : 4;
-    q.tile = tile_for(p, p.n, p.classes, 1);
-    q.tile_shift = q.tile == 256 ? 8 : q.tile == 128 ? 7 : 6;
+    q.few = p.n && p.n <= kFewRows && p.classes <= kFewClasses;
+    q.tile = q.few ? kFewTile : tiles_for(p, p.n, p.classes, p.d, false).tile;
+    q.tile_shift = q.tile == 256 ? 8 : q.tile == 128 ? 7 : 6;       // (few rows: not used)
     // the tile kernels read 16 bytes at a time and whole steps of 64 k: operands that do not allow it are laid out anew
     q.ld_pack = (p.d + 63LL) / 64 * 64;
     q.wide = q.tile > kTile && !p.type;
-    q.pack_x = q.tile > kTile && (q.wide || !lies_well(x, p.ld_x, p.d));
-    q.pack_w = q.tile > kTile && (q.wide || !lies_well(w, p.ld_w, p.d));
+    q.pack_x = q.tile > kTile && (q.wide || !lies_well(xp, p.ld_x, p.d));
+    q.pack_w = q.tile > kTile && (q.wide || !lies_well(wp, p.ld_w, p.d));
     const int planes = q.wide ? 3 : 1;
     q.tiles = ceil_div(p.classes, q.tile);
     q.ld_e = (long long)q.tiles * q.tile;
@@ -528,18 +535,19 @@ XentPlan xent_plan(const asl_xent_params& p, const void* x, const void* w, bool 
     q.dx_splits = q.dw_splits = 1;
     q.dx_tile = q.dw_tile = kTile;
     if (grad && p.n) {
-        q.dx_tile = tile_for(p, rows, p.d, 2);
-        q.dw_tile = tile_for(p, p.classes, p.d, 2);
-        // measured per step of a tile's contraction, one workgroup a CU
-        const auto step_us = [&](int tile) { return tile == kTile && !p.type ? 0.3 : (q.wide ? 6 : 1) * ( tile == 256 ? 1.6 : tile == 128 ? 0.5 : 0.4); };
-        q.dx_splits = splits_for((long long)ceil_div(rows, q.dx_tile) * ceil_div(p.d, q.dx_tile), ceil_div(p.classes, bk),
-                                 step_us(q.dx_tile), (double)rows * p.d);
-        q.dw_splits = splits_for((long long)ceil_div(p.classes, q.dw_tile) * ceil_div(p.d, q.dw_tile), ceil_div(rows, bk),
-                                 step_us(q.dw_tile), (double)p.classes * p.d);
+        const TilePlan x = tiles_for(p, rows, p.d, p.classes, true), w = tiles_for(p, p.classes, p.d, (int)rows, true);
+        q.dx_tile = x.tile; q.dx_splits = x.splits;
+        q.dw_tile = w.tile; q.dw_splits = w.splits;
     }
     q.dx_splits = ceil_div(p.classes, k_per_split(p.classes, q.dx_splits, bk));
     q.dw_splits = rows ? ceil_div(rows, k_per_split((int)rows, q.dw_splits, bk)) : 1;
     q.dw_slabs = q.dw_splits > 1 || q.pieces > 1;
+    if (q.few) {                          // exponentials and G in fp32 whatever the operands
+        q.esize = 4;
+        q.dx_splits = xent_few_slabs(p.classes) + 1;
+        q.dw_slabs = false;
+        want_db = false;
+    }
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long r = at;
@@ -591,6 +599,19 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const T* src, long long 
         if constexpr (std::is_same<T, short>::value) *(bf16x8*)(dst + v * 8) = raw;
         else store_planes(dst + v * 8, vectors * 8, widen(raw));
     }
+}
+
+int xent_run_few(const asl_xent_params& p, const XentPlan& q, bool grad, const void* x, const void* w, const void* bias,
+                 const long long* target, const float* upstream, float* loss, float* lse, void* dx, void* dw, void* db, char* ws,
+                 hipStream_t s) {
+    XentFew a = {};
+    a.x = x; a.w = w; a.bias = bias; a.target = target; a.upstream = upstream; a.loss = loss; a.lse = lse; a.dx = dx; a.dw = dw; a.db = db;
+    a.e = grad ? (float*)(ws + q.e) : nullptr; a.tile_max = (float*)(ws + q.tmax); a.tile_sum = (float*)(ws + q.tsum);
+    a.tile_lin = (float*)(ws + q.tlin); a.target_logit = (float*)(ws + q.tlogit); a.factor = grad ? (float*)(ws + q.shared) : nullptr;
+    a.slabs = (float*)(ws + q.dxs); a.ld_x = p.ld_x; a.ld_w = p.ld_w; a.ld_e = q.ld_e; a.ignore = p.ignore_index;
+    a.smoothing = p.label_smoothing; a.inv_classes = 1.f / (float)p.classes; a.n = p.n; a.classes = p.classes; a.d = p.d;
+    a.tiles = q.tiles; a.bias_bf16 = p.bias_type; a.none = p.reduction == ASL_REDUCE_NONE; a.mean = p.reduction == ASL_REDUCE_MEAN;
+    return xent_few(a, p.type, s);
 }
 
 template <typename T>
@@ -730,6 +751,7 @@ extern "C" int asl_linear_xent_fwd(const asl_xent_params* p, const void* x, cons
     if (off(x, p->type) || off(w, p->type) || off(bias, p->bias_type) || ((uintptr_t)target & 7)) return ASL_EINVAL;
     const XentPlan q = xent_plan(*p, x, w, false, false, false, false);
     const long long* t = (const long long*)target;
+    if (q.few) return xent_run_few(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
     if (p->type) return xent_run<short>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
     return xent_run<float>(*p, q, false, x, w, bias, t, nullptr, loss, lse, nullptr, nullptr, nullptr, (char*)workspace, (hipStream_t)stream);
 }
@@ -756,6 +778,7 @@ extern "C" int asl_linear_xent_grad(const asl_xent_params* p, const void* x, con
     }
     const XentPlan q = xent_plan(*p, x, w, true, dx != nullptr, dw != nullptr, dbias != nullptr);
     const long long* t = (const long long*)target;
+    if (q.few) return xent_run_few(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
     if (p->type) return xent_run<short>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
     return xent_run<float>(*p, q, true, x, w, bias, t, upstream, loss, lse, dx, dw, dbias, (char*)workspace, s);
 }

@@ -38,4 +38,32 @@ int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s);
 int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s);     // P along its own index, Q along k
 int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s);     // both along their own index
 
+// xent_few.hip: up to 32 rows
+constexpr int kFewRows = 32, kFewTile = 32, kFewClasses = 16384;
+struct XentFew {
+    const void* x;
+    const void* w;
+    const void* bias;
+    const long long* target;
+    const float* upstream;   // null: 1; one value a row with `none`
+    float* loss;
+    float* lse;              // null: not wanted
+    void* dx;                // each null: not wanted
+    void* dw;
+    void* db;
+    float* e;                // [n][ld_e]: exponentials, then G; null: no gradients
+    float* tile_max;         // [n][tiles]
+    float* tile_sum;
+    float* tile_lin;
+    float* target_logit;
+    float* factor;           // with gradients
+    float* slabs;            // [xent_few_slabs][n][d]
+    long long ld_x, ld_w, ld_e, ignore;
+    float smoothing, inv_classes;
+    int n, classes, d, tiles, bias_bf16, none, mean;
+};
+// slices of the classes for dx: 128 classes a workgroup, at most 32 slices
+inline int xent_few_slabs(int classes) { return classes < 128 * 32 ? ceil_div(classes, 128) : 32; }
+int xent_few(const XentFew& a, int type, hipStream_t s);
+
 }  // namespace asl_detail
