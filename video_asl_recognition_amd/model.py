@@ -559,6 +559,16 @@ class AslClipModel:
 
     # ------------------------------------------------------------------ I3D
     def _run_i3d(self, B: int, T: int, fill_frames, fill_chunk=None):
+        """logits of B clips through the 3-D backbone (see _i3d_pooled)"""
+        spec = self.spec
+        pooled = self._i3d_pooled(B, T, fill_frames, fill_chunk)
+        stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        logits = torch.empty(B, spec.num_classes, dtype=torch.float32, device=self.device)
+        L.check(L.lib.asl_head_f32(_ptr(pooled), B, pooled.shape[1], _ptr(self._fc_w), _ptr(self._fc_b), spec.num_classes,
+                                   _ptr(logits), stream), "head")
+        return logits
+
+    def _i3d_pooled(self, B: int, T: int, fill_frames, fill_chunk=None):
         """fill_frames(f0, n, dst_ptr, stream) writes frames [f0, f0+n) (flattened over B*T) as packed
         [n][S+6][S+6][4] at dst_ptr; fill_chunk(b0, n, x0_ptr, stream), when given, packs clips [b0, b0+n) into a plan's
         whole input tensor with one launch instead.  Clips run through the 3-D backbone a chunk (16 clips of 64 frames) at a time, the
@@ -630,10 +640,56 @@ class AslClipModel:
         stream = C.c_void_p(main.cuda_stream)
         pooled = torch.empty(B, last.c, dtype=torch.float32, device=dev)
         L.check(L.lib.asl_window_mean_t_f32(_ptr(frame_feats), B, D, last.c, min(2, D), _ptr(pooled), stream), "window_mean")
-        logits = torch.empty(B, spec.num_classes, dtype=torch.float32, device=dev)
-        L.check(L.lib.asl_head_f32(_ptr(pooled), B, last.c, _ptr(self._fc_w), _ptr(self._fc_b), spec.num_classes,
-                                   _ptr(logits), stream), "head")
-        return logits
+        return pooled
+
+    def _i3d_clip_fill(self, clips: torch.Tensor, T: int):
+        """the two packing callbacks of _i3d_pooled for checked clips"""
+        S, esz, in_f32, base = self.spec.size, clips.element_size(), int(clips.dtype == torch.float32), clips.data_ptr()
+
+        def fill(f0, n, dst, stream):
+            L.check(L.lib.asl_pack_clips(C.c_void_p(base + f0 * 3 * S * S * esz), in_f32, n, S, 3, dst, stream),
+                    "pack_clips")
+
+        def fill_chunk(b0, n, dst, stream):
+            L.check(L.lib.asl_pack_clips_3d(C.c_void_p(base + b0 * T * 3 * S * S * esz), in_f32, n, T, S, 3, 3, dst, stream),
+                    "pack_clips_3d")
+        return fill, fill_chunk
+
+    # ------------------------------------------------------------------ classifier end
+    @torch.no_grad()
+    def head_input(self, clips: torch.Tensor, keypoints: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """What the classifier end reads, fp32: per clip [B, F] the features of the Linear (mean, BiLSTM, I3D), or, for the
+        transformer, per frame [B*T, d_model] the input of the encoder's last LayerNorm."""
+        if not self._w:
+            raise RuntimeError("load_state_dict() first (or construct with seed=...)")
+        B, T = clips.shape[:2]
+        if self.spec.backbone == "i3d":
+            clips = self._check_clips(clips)
+            return self._i3d_pooled(B, T, *self._i3d_clip_fill(clips, T))
+        if self.spec.keypoints and keypoints is None:
+            raise ValueError(f"spec {self.spec.name} needs keypoints [B,T,21,2]")
+        feats, feats_b = self.frame_features(clips, want_bf16=self.spec.temporal != "mean")
+        stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        if self.spec.temporal != "mean":
+            return self._temporal.encode(feats, feats_b, feats_b.shape[1], B, T, keypoints, stream)
+        pooled = torch.empty(B, self.spec.feat_dim, dtype=torch.float32, device=self.device)
+        L.check(L.lib.asl_mean_t_f32(_ptr(feats), B, T, self.spec.feat_dim, _ptr(pooled), stream), "mean_t")
+        return pooled
+
+    def head_parameters(self) -> Dict[str, torch.Tensor]:
+        """The classifier end's weights by their state-dict names: the fp32 tensors on the GPU that forward() reads, so what is
+        written into them is what the next forward computes with."""
+        if not self._w:
+            raise RuntimeError("load_state_dict() first (or construct with seed=...)")
+        if self.spec.backbone == "i3d":
+            return {"backbone.logits.weight": self._fc_w, "backbone.logits.bias": self._fc_b}
+        if self.spec.temporal == "mean":
+            return {"fc.weight": self._fc_w, "fc.bias": self._fc_b}
+        out = {"fc.weight": self._temporal.fc_w, "fc.bias": self._temporal.fc_b}
+        if self.spec.temporal == "transformer":
+            p = f"encoder.layers.{self.spec.n_layers - 1}.norm2"
+            out[p + ".weight"], out[p + ".bias"] = self._temporal.layers[-1]["n2"]
+        return out
 
     @torch.no_grad()
     def forward(self, clips: torch.Tensor, keypoints: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -642,15 +698,7 @@ class AslClipModel:
         B, T = clips.shape[:2]
         if self.spec.backbone == "i3d":
             clips = self._check_clips(clips)
-            S, esz, in_f32, base = self.spec.size, clips.element_size(), int(clips.dtype == torch.float32), clips.data_ptr()
-
-            def fill(f0, n, dst, stream):
-                L.check(L.lib.asl_pack_clips(C.c_void_p(base + f0 * 3 * S * S * esz), in_f32, n, S, 3, dst, stream),
-                        "pack_clips")
-            def fill_chunk(b0, n, dst, stream):
-                L.check(L.lib.asl_pack_clips_3d(C.c_void_p(base + b0 * T * 3 * S * S * esz), in_f32, n, T, S, 3, 3, dst, stream),
-                        "pack_clips_3d")
-            return self._run_i3d(B, T, fill, fill_chunk)
+            return self._run_i3d(B, T, *self._i3d_clip_fill(clips, T))
         if self.spec.keypoints and keypoints is None:
             raise ValueError(f"spec {self.spec.name} needs keypoints [B,T,21,2]")
         if self._heads_per_chunk():

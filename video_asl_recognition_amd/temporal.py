@@ -45,8 +45,9 @@ class BiLstmHead:
         self.fc_w = sd["fc.weight"].float().contiguous().to(dev)
         self.fc_b = sd["fc.bias"].float().contiguous().to(dev)
 
-    def __call__(self, feats, feats_b, ld_b, B, T, keypoints, stream):
-        spec, dev, H = self.spec, self.dev, self.spec.lstm_hidden
+    def encode(self, feats, feats_b, ld_b, B, T, keypoints, stream):
+        """what the classifier Linear reads: the mean over T of the last layer's outputs, fp32 [B, 2H]"""
+        dev, H = self.dev, self.spec.lstm_hidden
         x, ldx = _ptr(feats_b), ld_b
         keep = []
         ysum = torch.empty(B, 2 * H, dtype=torch.float32, device=dev)
@@ -61,10 +62,16 @@ class BiLstmHead:
                                                _ptr(state), stream), "lstm")
             keep += [gx, y]
             x, ldx = _ptr(y), 4 * H
-        logits = torch.empty(B, spec.num_classes, dtype=torch.float32, device=dev)
-        L.check(L.lib.asl_head_f32(_ptr(ysum), B, 2 * H, _ptr(self.fc_w), _ptr(self.fc_b), spec.num_classes,
+        self._keep = keep + [state]     # the launches above are asynchronous: keep their buffers until the next call
+        return ysum
+
+    def __call__(self, feats, feats_b, ld_b, B, T, keypoints, stream):
+        spec = self.spec
+        ysum = self.encode(feats, feats_b, ld_b, B, T, keypoints, stream)
+        logits = torch.empty(B, spec.num_classes, dtype=torch.float32, device=self.dev)
+        L.check(L.lib.asl_head_f32(_ptr(ysum), B, 2 * spec.lstm_hidden, _ptr(self.fc_w), _ptr(self.fc_b), spec.num_classes,
                                    _ptr(logits), stream), "head")
-        self._keep = keep       # the launches above are asynchronous: keep their buffers until the next call
+        self._keep.append(ysum)
         return logits
 
 
@@ -102,7 +109,8 @@ class TwoStreamTransformerHead:
         self.fc_b = f("fc.bias").contiguous().to(dev)
         self._pe = {}
 
-    def __call__(self, feats, feats_b, ld_b, B, T, keypoints, stream):
+    def encode(self, feats, feats_b, ld_b, B, T, keypoints, stream):
+        """the encoder up to its last LayerNorm: that norm's input, fp32 [B*T, d_model]"""
         spec, dev = self.spec, self.dev
         d, M = spec.d_model, B * T
         if keypoints is None or tuple(keypoints.shape[:2]) != (B, T):
@@ -129,7 +137,7 @@ class TwoStreamTransformerHead:
         L.check(L.lib.asl_add_rows_f32(_ptr(x0), M, d, _ptr(pe), T, _ptr(xf), _ptr(xb), d, stream), "posenc")
         qkv, att, r, hbuf = new(M, 3 * d), new(M, d), new(M, d, dt=f32), new(M, spec.ffn_dim)
         ap = L.AttnParams(batch=B, t=T, heads=spec.n_heads, head_dim=d // spec.n_heads, ld_qkv=3 * d, ld_out=d)
-        for lw in self.layers:
+        for li, lw in enumerate(self.layers):
             _linear(_ptr(xb), d, lw["qkv"], M, _ptr(qkv), 3 * d, stream)
             L.check(L.lib.asl_attention_fwd(C.byref(ap), _ptr(qkv), _ptr(att), stream), "attention")
             _linear(_ptr(att), d, lw["out"], M, _ptr(r), d, stream, out_f32=True, res=_ptr(xf), ldres=d, res_f32=True)
@@ -138,14 +146,24 @@ class TwoStreamTransformerHead:
             _linear(_ptr(xb), d, lw["l1"], M, _ptr(hbuf), spec.ffn_dim, stream, relu=True)
             _linear(_ptr(hbuf), spec.ffn_dim, lw["l2"], M, _ptr(r), d, stream, out_f32=True, res=_ptr(xf), ldres=d,
                     res_f32=True)
-            L.check(L.lib.asl_layernorm_f32(_ptr(r), M, d, _ptr(lw["n2"][0]), _ptr(lw["n2"][1]), 1e-5, _ptr(xb), d,
-                                            _ptr(xf), stream), "layernorm")
-        pooled = new(B, d, dt=f32)
+            if li < len(self.layers) - 1:
+                L.check(L.lib.asl_layernorm_f32(_ptr(r), M, d, _ptr(lw["n2"][0]), _ptr(lw["n2"][1]), 1e-5, _ptr(xb), d,
+                                                _ptr(xf), stream), "layernorm")
+        self._keep = [kp, kp_b, k1, x0, xf, xb, qkv, att, hbuf]
+        return r
+
+    def __call__(self, feats, feats_b, ld_b, B, T, keypoints, stream):
+        spec, d = self.spec, self.spec.d_model
+        r = self.encode(feats, feats_b, ld_b, B, T, keypoints, stream)
+        xf = torch.empty_like(r)
+        gamma, beta = self.layers[-1]["n2"]
+        L.check(L.lib.asl_layernorm_f32(_ptr(r), B * T, d, _ptr(gamma), _ptr(beta), 1e-5, None, 0, _ptr(xf), stream), "layernorm")
+        pooled = torch.empty(B, d, dtype=torch.float32, device=self.dev)
         L.check(L.lib.asl_mean_t_f32(_ptr(xf), B, T, d, _ptr(pooled), stream), "mean_t")
-        logits = new(B, spec.num_classes, dt=f32)
+        logits = torch.empty(B, spec.num_classes, dtype=torch.float32, device=self.dev)
         L.check(L.lib.asl_head_f32(_ptr(pooled), B, d, _ptr(self.fc_w), _ptr(self.fc_b), spec.num_classes,
                                    _ptr(logits), stream), "head")
-        self._keep = [kp, kp_b, k1, x0, xf, xb, qkv, att, r, hbuf, pooled]
+        self._keep += [r, xf, pooled]
         return logits
 
 
