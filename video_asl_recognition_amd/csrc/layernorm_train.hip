@@ -358,52 +358,45 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
     }
 }
 
-// 64 columns a workgroup: 16 lanes of four columns by 16 row strides
-__global__ __launch_bounds__(256) void column_sums_kernel(const float* __restrict__ part, int parts, long long ld, long long cols,
-                                                          long long split, void* out0, void* out1, int bf16, const float* factor) {
-    __shared__ float s[16][64 + 1];
+// 64 columns a workgroup of 1024: 16 lanes of four columns by 64 row strides, so that the up to 512 partial rows, which other
+// XCDs have just written and which come from memory, are all on their way at once
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ part, int parts, long long ld, long long cols,
+                                                           long long split, void* out0, void* out1, int bf16, const float* factor) {
+    __shared__ float s[64][64 + 1];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
     const long long c0 = (long long)blockIdx.x * 64 + c * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c0 < cols) {
-        const int n = cols - c0 < 4 ? (int)(cols - c0) : 4;
+    const int n = cols - c0 >= 4 ? 4 : cols > c0 ? (int)(cols - c0) : 0;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n == 4) {
 #pragma unroll 8
-        for (int p = r; p < parts; p += 16) {
-            const float* src = part + p * ld + c0;
-            if (n == 4) {
-                const f32x4u q = *(const f32x4u*)src;
+        for (int p = r; p < parts; p += 64) v += *(const f32x4u*)(part + p * ld + c0);
+    } else if (n) {
+        for (int p = r; p < parts; p += 64)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += q[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < n) v[e] += src[e];
-            }
-        }
+            for (int e = 0; e < 3; ++e)
+                if (e < n) v[e] += part[p * ld + c0 + e];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[r][c * 4 + e] = v[e];
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const long long col = (long long)blockIdx.x * 64 + threadIdx.x;
-        if (col < cols) {
-            float o = 0.f;
-#pragma unroll
-            for (int p = 0; p < 16; ++p) o += s[p][threadIdx.x];
-            if (factor) o *= *factor;
-            void* out = col < split ? out0 : out1;
-            const long long at = col < split ? col : col - split;
-            if (out) {
-                if (bf16) store1((short*)out + at, o);
-                else store1((float*)out + at, o);
-            }
+    // sixteen lanes a column, four rows each, then across the lanes
+    const int k = threadIdx.x >> 4, q = threadIdx.x & 15;
+    const float o = row16_sum((s[q][k] + s[q + 16][k]) + (s[q + 32][k] + s[q + 48][k]));
+    const long long col = (long long)blockIdx.x * 64 + k;
+    if (q == 0 && col < cols) {
+        void* out = col < split ? out0 : out1;
+        const long long at = col < split ? col : col - split;
+        const float f = factor ? o * *factor : o;
+        if (out) {
+            if (bf16) store1((short*)out + at, f);
+            else store1((float*)out + at, f);
         }
     }
 }
 
 int column_sums(const float* part, int parts, long long ld, long long cols, long long split, void* out0, void* out1, int bf16,
                 const float* factor, hipStream_t s) {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s, part, parts, ld, cols, split, out0, out1,
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, s, part, parts, ld, cols, split, out0, out1,
                        bf16, factor);
     return (int)hipGetLastError();
 }

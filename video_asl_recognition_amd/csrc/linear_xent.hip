@@ -90,16 +90,16 @@ struct Stage {
     }
 };
 
-// Any sizes, strides and alignment.  Four waves, 32 x 32 of the tile each.
+// Any sizes, strides and alignment.  Four waves, 32 x 32 of the tile each.  Workgroup `id` of ti * tj * splits.
 template <typename T, bool PKC, bool QKC, bool LOGITS>
-__global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
+__device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int tj) {
     constexpr int BK = Mma<T>::BK, LD = BK + Mma<T>::PAD, KSTEP = Mma<T>::KSTEP;
     __shared__ __attribute__((aligned(16))) T lp[kTile * LD];
     __shared__ __attribute__((aligned(16))) T lq[kTile * LD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-    const int i0 = blockIdx.x * kTile, j0 = blockIdx.y * kTile;
-    const int kb = blockIdx.z * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
+    const int bi = id % ti, bj = id / ti % tj, slice = id / (ti * tj), i0 = bi * kTile, j0 = bj * kTile;
+    const int kb = slice * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
     f32x4 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -135,6 +135,7 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
     // lane: i = i0 + wi + u*16 + fq*4 + e, j = j0 + wj + v*16 + fr
     if constexpr (!LOGITS) {
         const float c = a.slabs ? 1.f : *a.factor;
+        const long long ld = (long long)ti * kTile;        // of a slab
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const int j = j0 + wj + v * 16 + fr;
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
                 for (int e = 0; e < 4; ++e) {
                     if (i + e >= a.I) continue;
                     if (a.slabs) {
-                        float* o = (float*)a.out + ((long long)blockIdx.z * a.Jn + j) * a.I + i + e;
+                        float* o = (float*)a.out + ((long long)slice * a.Jn + j) * ld + i + e;
                         *o = a.add ? *o + acc[u][v][e] : acc[u][v][e];
                     } else {
                         store1((T*)a.out + j * a.ld_out + i + e, acc[u][v][e] * c);
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
         }
     } else {
         __shared__ float red[2][kTile][3];
-        const int tile = blockIdx.x;
+        const int tile = bi;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const int j = j0 + wj + v * 16 + fr;
@@ -235,58 +236,48 @@ __global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a) {
     }
 }
 
+template <typename T, bool LOGITS>
+__global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a, int ti, int tj) {
+    static_assert(LOGITS, "the gradient products go in pairs");
+    gemm_body<T, true, true, true>(a, blockIdx.x, ti, tj);
+}
+
+// dx and dW in one launch, dx's workgroups first
+template <typename T>
+__global__ __launch_bounds__(256) void xent_gemm_pair_kernel(const XentGemm dx, const XentGemm dw, int dx_ti, int dx_tj, int dw_ti, int dw_tj,
+                                                             int dx_blocks) {
+    if ((int)blockIdx.x < dx_blocks) gemm_body<T, false, true, false>(dx, blockIdx.x, dx_ti, dx_tj);
+    else gemm_body<T, false, false, false>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
+}
+
 struct XentRows {
-    const long long* target;              // of this piece's rows
-    const float* upstream;                // null: 1
-    float* tile_max;                      // in: maxima; out (factors != 0): g exp(m - lse)
-    const float* tile_sum;
-    const float* tile_lin;
-    const float* target_logit;
+    XentStats st;
+    float* factor;                        // with gradients: [rows][tiles] g exp(m - lse); may be the maxima themselves
     float* target_g;                      // G at the target
     float* row_g;                         // g (label smoothing's even part)
     float* loss;
     float* lse;
-    long long ignore;
-    float smoothing, inv_classes, exp_unit;         // exp_unit: one over the scale the exponentials are held at
-    int rows, classes, tiles, factors;
+    float exp_unit;                       // one over the scale the exponentials are held at
 };
 
-// one wave a row: the tiles' maxima and sums to lse, the loss, and the factors that turn exp(l - m) into G
+// one wave a row: statistics, loss, and the factors that turn exp(l - m) into G
 __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= a.rows) return;
-    float* mx = a.tile_max + (long long)row * a.tiles;
-    const float* sm = a.tile_sum + (long long)row * a.tiles;
-    float m = -INFINITY, lin = 0.f;
-    for (int t = lane; t < a.tiles; t += 64) m = fmaxf(m, mx[t]);
-    m = wave_max(m);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    for (int t = lane; t < a.tiles; t += 64) s += sm[t] * expf(mx[t] - ref);
-    if (a.smoothing != 0.f) {
-        const float* ln = a.tile_lin + (long long)row * a.tiles;
-        for (int t = lane; t < a.tiles; t += 64) lin += ln[t];
-        lin = wave_sum(lin);
-    }
-    s = wave_sum(s);
-    const float lse = ref + logf(s);
-    const long long t = a.target[row];
-    const bool kept = t != a.ignore, valid = t >= 0 && t < a.classes;
-    float g = 0.f;
-    if (kept) g = a.upstream ? a.upstream[row] : 1.f;
-    const float lt = valid ? a.target_logit[row] : NAN;       // a label outside the vocabulary makes loss and gradients NaN
+    if (row >= a.st.rows) return;
+    const XentRow r = row_stats<64>(a.st, row, lane);
     if (lane == 0) {
-        float l = lse - lt;
-        if (a.smoothing != 0.f) l = lse - (1.f - a.smoothing) * lt - a.smoothing * a.inv_classes * lin;
-        a.loss[row] = kept ? l : 0.f;
-        if (a.lse) a.lse[row] = lse;
-        if (a.factors) {
-            a.target_g[row] = g * (expm1f(lt - lse) + a.smoothing - a.smoothing * a.inv_classes);
-            a.row_g[row] = g;
+        a.loss[row] = r.loss;
+        if (a.lse) a.lse[row] = r.lse;
+        if (a.factor) {
+            a.target_g[row] = r.target_g;
+            a.row_g[row] = r.g;
         }
     }
-    if (a.factors)
-        for (int t2 = lane; t2 < a.tiles; t2 += 64) mx[t2] = valid ? g * a.exp_unit * expf(mx[t2] - lse) : NAN;
+    if (a.factor)
+        for (int t = lane; t < a.st.tiles; t += 64) {
+            const long long at = (long long)row * a.st.tiles + t;
+            a.factor[at] = r.valid ? r.g * a.exp_unit * expf(a.st.tile_max[at] - r.lse) : NAN;
+        }
 }
 
 // What concerns all of a call's rows, by one workgroup: the loss (the rows' sum, or their mean over those that carry a label;
@@ -335,17 +326,14 @@ __global__ __launch_bounds__(256) void xent_loss_kernel(const XentAll a) { over_
 constexpr int kGradRows = 32;             // rows a workgroup of the G pass takes; it leaves one partial row of db
 constexpr int kGradCols = 256;            // and columns
 
+constexpr int kOwnStats = 64;             // tiles a row up to which the G pass takes the statistics for itself
+
 struct XentG {
+    XentRows rows;                        // `factor`, `target_g`, `row_g`: taken from there (or, with own statistics, not used)
     void* e;                              // exp(l - m) in, G out
     long long ld;
-    const float* factor;                  // [rows][tiles]
-    const float* target_g;
-    const float* row_g;
-    const long long* target;
     float* db_part;                       // [row groups][ld], null: no bias gradient
-    long long ignore;
-    float smoothing, inv_classes;
-    int rows, classes, tiles, tile_shift, db_add;
+    int tile_shift, db_add;
     short* planes;                        // not null: G goes here, as three bf16 planes
     long long plane;
     XentAll all;
@@ -353,7 +341,6 @@ struct XentG {
 
 __device__ __forceinline__ F8 load8_exp(const float* p) { return load8_full(p); }
 __device__ __forceinline__ F8 load8_exp(const _Float16* p) {
-    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
     const half8 a = *(const half8*)p;
     F8 r;
 #pragma unroll
@@ -382,40 +369,73 @@ __device__ __forceinline__ void store_planes(short* p, long long plane, const F8
     *(bf16x8*)(p + 2 * plane) = l;
 }
 
-// 256 columns x 32 rows a workgroup: half a wave on each row, four rows a lane, all of them on their way at once
-template <typename T>
+// 256 columns x 32 rows a workgroup: half a wave on each row, four rows a lane, all of them on their way at once.  OWN: the
+// rows' statistics are taken here, by every column's workgroup anew, instead of in a launch ahead.
+template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
-    constexpr int R = kGradRows / 8;
+    constexpr int R = kGradRows / 8, TPB = kGradCols / kTile;
     __shared__ __attribute__((aligned(16))) float cols[8][kGradCols];
+    __shared__ float own_f[OWN ? kGradRows : 1][TPB], own_tg[OWN ? kGradRows : 1], own_g[OWN ? kGradRows : 1];
+    const XentStats& st = a.rows.st;
     const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = (long long)blockIdx.x * kGradCols + lane * 8;
     const bool in = col < a.ld;
-    const int r0 = blockIdx.y * kGradRows + rl;
+    const int b0 = blockIdx.y * kGradRows, r0 = b0 + rl;
     F8 g[R], db;
     float f[R], even[R], tg[R];
     long long t[R];
 #pragma unroll
     for (int u = 0; u < R; ++u) {
-        const int r = r0 + u * 8 < a.rows ? r0 + u * 8 : a.rows - 1;
-        t[u] = a.target[r];
+        const int r = r0 + u * 8 < st.rows ? r0 + u * 8 : st.rows - 1;
+        t[u] = st.target[r];
         if (in) {
             g[u] = load8_exp((const typename Mma<T>::Exp*)a.e + r * a.ld + col);
-            f[u] = a.factor[(long long)r * a.tiles + (col >> a.tile_shift)];
+            // (columns of a last, half empty 256 x 256 tile lie behind the last block of maxima)
+            const int tile = (int)(col >> a.tile_shift);
+            if (!OWN) f[u] = tile < st.tiles ? a.rows.factor[(long long)r * st.tiles + tile] : 0.f;
         }
-        even[u] = a.smoothing * a.inv_classes * a.row_g[r];
-        tg[u] = a.target_g[r];
+        if (!OWN) {
+            even[u] = st.smoothing * st.inv_classes * a.rows.row_g[r];
+            tg[u] = a.rows.target_g[r];
+        }
+    }
+    if constexpr (OWN) {
+        const int l16 = threadIdx.x & 15, blocks = kGradCols >> a.tile_shift;
+#pragma unroll
+        for (int k = threadIdx.x >> 4; k < kGradRows; k += 16) {               // sixteen rows at once
+            if (b0 + k >= st.rows) continue;
+            const XentRow q = row_stats<16>(st, b0 + k, l16);
+            if (l16 == 0) {
+                own_tg[k] = q.target_g;
+                own_g[k] = q.g;
+                if (blockIdx.x == 0) {
+                    a.rows.loss[b0 + k] = q.loss;
+                    if (a.rows.lse) a.rows.lse[b0 + k] = q.lse;
+                }
+            }
+            const int tile = blockIdx.x * blocks + l16;
+            if (l16 < blocks)
+                own_f[k][l16] = tile >= st.tiles ? 0.f : q.valid ? q.g * a.rows.exp_unit * expf(st.tile_max[(long long)(b0 + k) * st.tiles + tile] - q.lse) : NAN;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            f[u] = own_f[rl + u * 8][(lane * 8) >> a.tile_shift];
+            even[u] = st.smoothing * st.inv_classes * own_g[rl + u * 8];
+            tg[u] = own_tg[rl + u * 8];
+        }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) db.v[e] = 0.f;
 #pragma unroll
     for (int u = 0; u < R; ++u) {
         const int r = r0 + u * 8;
-        if (!in || r >= a.rows) continue;
+        if (!in || r >= st.rows) continue;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v = col + e < a.classes ? g[u].v[e] * f[u] - even[u] : 0.f;
+            float v = col + e < st.classes ? g[u].v[e] * f[u] - even[u] : 0.f;
             if (col + e == t[u]) v = tg[u];
-            if (t[u] == a.ignore) v = 0.f;                   // whatever the row held
+            if (t[u] == st.ignore) v = 0.f;                  // whatever the row held
             g[u].v[e] = v;
             db.v[e] += v;
         }
@@ -437,26 +457,83 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && (a.all.factor || a.all.loss_rows)) over_all_rows(a.all);
 }
 
-// out[r][c] = *factor times the sum over s of slab s, in the order of s; a row of `cols` values, slabs `stride` apart
-template <typename U>
-__global__ __launch_bounds__(256) void xent_slab_kernel(const float* in, int slabs, long long stride, long long ld_in, int rows,
-                                                        int cols, U* out, long long ld_out, const float* factor) {
-    const float f = *factor;
-    const long long c = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (c >= cols) return;
-    const int n = (int)(cols - c < 8 ? cols - c : 8);
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-        F8 v = load8(in + r * ld_in + c, n);
+// What is left when the products are done, in one launch: slabs of partial sums added up in their order, partial rows of db,
+// the loss.
+struct XentSlabs {
+    const float* in;                      // [slabs][rows][ld]
+    void* out;                            // [rows][cols], dense
+    long long ld;
+    int slabs, rows, cols, blocks;        // blocks: 0 for nothing to do
+};
+struct XentFinish {
+    XentSlabs dx, dw;
+    const float* db_part;                 // [groups][ld_db]
+    void* db;
+    long long ld_db;
+    int groups, classes, db_bf16, db_blocks;
+    const float* factor;
+    XentAll all;                          // with loss_rows: by the last workgroup
+};
+constexpr int kSlabPerBlock = 256 * 8 * 2;       // results a workgroup
+
+template <typename T>
+__device__ __forceinline__ void add_slabs(const XentSlabs& a, int block, float f) {
+    const int per_row = (a.cols + 7) / 8;
+    const long long vectors = (long long)a.rows * per_row, stride = a.rows * a.ld;
+#pragma unroll 1
+    for (int n = 0; n < 2; ++n) {
+        const long long v = ((long long)block * 2 + n) * 256 + threadIdx.x;
+        if (v >= vectors) return;
+        const long long r = v / per_row;
+        const int c = (int)(v - r * per_row) * 8;
+        const float* src = a.in + r * a.ld + c;                // (slab rows are padded to whole tiles)
+        F8 o = load8_full(src);
 #pragma unroll 4
-        for (int s = 1; s < slabs; ++s) {
-            const F8 q = load8(in + s * stride + r * ld_in + c, n);
+        for (int s = 1; s < a.slabs; ++s) {
+            const F8 q = load8_full(src + s * stride);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v.v[e] += q.v[e];
+            for (int e = 0; e < 8; ++e) o.v[e] += q.v[e];
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v.v[e] *= f;
-        store8(out + r * ld_out + c, n, v);
+        for (int e = 0; e < 8; ++e) o.v[e] *= f;
+        store8((T*)a.out + r * a.cols + c, a.cols - c, o);
     }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void xent_finish_kernel(const XentFinish a) {
+    int b = blockIdx.x;
+    if (b < a.dx.blocks) {
+        add_slabs<T>(a.dx, b, *a.factor);
+        return;
+    }
+    b -= a.dx.blocks;
+    if (b < a.dw.blocks) {
+        add_slabs<T>(a.dw, b, *a.factor);
+        return;
+    }
+    b -= a.dw.blocks;
+    if (b < a.db_blocks) {                // 64 columns: 16 lanes of four by 16 row strides
+        __shared__ float s[16][64 + 1];
+        const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int p = r; p < a.groups; p += 16) v += *(const f32x4*)(a.db_part + p * a.ld_db + b * 64 + c * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][c * 4 + e] = v[e];
+        __syncthreads();
+        const int col = b * 64 + threadIdx.x;
+        if (threadIdx.x < 64 && col < a.classes) {
+            float o = 0.f;
+#pragma unroll
+            for (int p = 0; p < 16; ++p) o += s[p][threadIdx.x];
+            o *= *a.factor;
+            if (a.db_bf16) store1((short*)a.db + col, o);
+            else store1((float*)a.db + col, o);
+        }
+        return;
+    }
+    over_all_rows(a.all);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -479,6 +556,8 @@ inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, 
 inline bool lies_well(const void* t, long long ld, int d) {
     return !((uintptr_t)t & 15) && !(ld & 7) && !(d & 63) && ld <= (1 << 20);
 }
+
+inline long long slab_ld(int d, int tile) { return (long long)ceil_div(d, tile) * tile; }
 
 // Tile and slices of a product with `a` x `b` results over `k`: what its tiles take one after another on the 256 CUs, against
 // what slabs of partial sums cost (written and read back at 4 TB/s, and one more launch).  Measured with one workgroup a CU:
@@ -514,15 +593,15 @@ XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, boo
     q.esize = p.type ? 2 : 4;
     q.few = p.n && p.n <= kFewRows && p.classes <= kFewClasses;
     q.tile = q.few ? kFewTile : tiles_for(p, p.n, p.classes, p.d, false).tile;
-    q.tile_shift = q.tile == 256 ? 8 : q.tile == 128 ? 7 : 6;       // (few rows: not used)
+    q.tile_shift = q.tile == 256 ? 7 : 6;                // maxima and sums are kept per 128 classes, or 64
     // the tile kernels read 16 bytes at a time and whole steps of 64 k: operands that do not allow it are laid out anew
     q.ld_pack = (p.d + 63LL) / 64 * 64;
     q.wide = q.tile > kTile && !p.type;
     q.pack_x = q.tile > kTile && (q.wide || !lies_well(xp, p.ld_x, p.d));
     q.pack_w = q.tile > kTile && (q.wide || !lies_well(wp, p.ld_w, p.d));
     const int planes = q.wide ? 3 : 1;
-    q.tiles = ceil_div(p.classes, q.tile);
-    q.ld_e = (long long)q.tiles * q.tile;
+    q.tiles = ceil_div(p.classes, q.few ? kFewTile : 1 << q.tile_shift);
+    q.ld_e = (long long)ceil_div(p.classes, q.tile) * q.tile;
     long long rows = p.n < kPieceRows ? p.n : kPieceRows;
     if (grad) {
         const long long most = kPieceBytes / (q.ld_e * (q.wide ? 10 : q.esize)) / 256 * 256;
@@ -566,8 +645,8 @@ XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, boo
         q.rg = take(4LL * rows);
         q.e = take(q.esize * rows * q.ld_e);
         q.dbp = take(want_db ? 4LL * q.row_groups * q.ld_e : 0);
-        q.dxs = take(want_dx && q.dx_splits > 1 ? 4LL * q.dx_splits * rows * p.d : 0);
-        q.dws = take(want_dw && q.dw_slabs ? 4LL * q.dw_splits * p.classes * p.d : 0);
+        q.dxs = take(want_dx && q.dx_splits > 1 ? 4LL * q.dx_splits * rows * slab_ld(p.d, q.dx_tile) : 0);
+        q.dws = take(want_dw && q.dw_slabs ? 4LL * q.dw_splits * p.classes * slab_ld(p.d, q.dw_tile) : 0);
     }
     q.xp = take(q.pack_x ? 2LL * planes * rows * q.ld_pack : 0);
     q.wp = take(q.pack_w ? 2LL * planes * p.classes * q.ld_pack : 0);
@@ -656,68 +735,73 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             const int rc = xent_tiles_logits(g, q.tile, s);
             if (rc) return rc;
         } else {
-            hipLaunchKernelGGL((xent_gemm_kernel<T, true, true, true>), dim3(q.tiles, ceil_div(rows, kTile)), dim3(256), 0, s, g);
+            const int tj = ceil_div(rows, kTile);
+            hipLaunchKernelGGL((xent_gemm_kernel<T, true>), dim3((unsigned)(q.tiles * tj)), dim3(256), 0, s, g, q.tiles, tj);
         }
         XentRows r = {};
-        r.target = target + r0; r.upstream = upstream && none ? upstream + r0 : nullptr;
-        r.tile_max = g.tile_max; r.tile_sum = g.tile_sum; r.tile_lin = g.tile_lin; r.target_logit = g.target_logit;
-        r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
-        r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr;
-        r.ignore = p.ignore_index; r.smoothing = p.label_smoothing; r.inv_classes = 1.f / (float)p.classes; r.exp_unit = 1.f / Mma<T>::SCALE;
-        r.rows = rows; r.classes = p.classes; r.tiles = q.tiles; r.factors = grad;
-        hipLaunchKernelGGL(xent_rows_kernel, dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
+        r.st.target = target + r0; r.st.upstream = upstream && none ? upstream + r0 : nullptr;
+        r.st.tile_max = g.tile_max; r.st.tile_sum = g.tile_sum; r.st.tile_lin = g.tile_lin; r.st.target_logit = g.target_logit;
+        r.st.ignore = p.ignore_index; r.st.smoothing = p.label_smoothing; r.st.inv_classes = 1.f / (float)p.classes;
+        r.st.rows = rows; r.st.classes = p.classes; r.st.tiles = q.tiles;
+        r.factor = grad ? g.tile_max : nullptr; r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
+        r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr; r.exp_unit = 1.f / Mma<T>::SCALE;
+        const bool own = grad && q.tiles <= kOwnStats, last = piece == q.pieces - 1;
+        if (!own) hipLaunchKernelGGL(xent_rows_kernel, dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
         if (!grad) continue;
-        const bool last = piece == q.pieces - 1;
         XentG c = {};
-        c.e = ws + q.e; c.ld = q.ld_e; c.planes = q.wide ? (short*)(ws + q.gp) : nullptr; c.plane = rows * q.ld_e; c.factor = g.tile_max; c.target_g = r.target_g; c.row_g = r.row_g; c.target = target + r0;
-        c.all = all; c.all.loss_rows = !none && last ? loss_rows : nullptr; c.all.factor = piece == 0 ? shared : nullptr;
-        c.db_part = db ? (float*)(ws + q.dbp) : nullptr; c.db_add = piece > 0;
-        c.ignore = p.ignore_index; c.smoothing = p.label_smoothing; c.inv_classes = r.inv_classes; c.rows = rows;
-        c.classes = p.classes; c.tiles = q.tiles; c.tile_shift = q.tile_shift;
+        c.rows = r; c.e = ws + q.e; c.ld = q.ld_e; c.planes = q.wide ? (short*)(ws + q.gp) : nullptr; c.plane = rows * q.ld_e;
+        c.db_part = db ? (float*)(ws + q.dbp) : nullptr; c.db_add = piece > 0; c.tile_shift = q.tile_shift;
+        c.all = all; c.all.loss_rows = !none && last && !own ? loss_rows : nullptr; c.all.factor = piece == 0 ? shared : nullptr;
         const int groups = ceil_div(rows, kGradRows);
-        hipLaunchKernelGGL((xent_g_kernel<T>), dim3(ceil_div(q.ld_e, kGradCols), groups), dim3(256), 0, s, c);
-        if (dx) {                          // dx[row][k] = sum over classes G[row][v] W[v][k]
-            XentGemm h = {};
-            h.p = wk; h.ld_p = ld_w; h.q = ws + (q.wide ? q.gp : q.e); h.ld_q = q.ld_e; h.I = p.d; h.Jn = rows; h.K = p.classes;
-            if (q.wide) h.plane_p = p.classes * ld_w, h.plane_q = rows * q.ld_e;
-            h.k_per_split = k_per_split(p.classes, q.dx_splits, bk);
-            h.slabs = q.dx_splits > 1; h.factor = shared;
-            T* dxr = (T*)dx + (long long)r0 * p.d;
-            h.out = h.slabs ? (void*)(ws + q.dxs) : (void*)dxr; h.ld_out = p.d;
-            h.splits = q.dx_splits;
-            if (q.dx_tile > kTile) {
-                const int rc = xent_tiles_dx(h, q.dx_tile, s);
-                if (rc) return rc;
-            } else {
-                hipLaunchKernelGGL((xent_gemm_kernel<T, false, true, false>),
-                                   dim3(ceil_div(p.d, kTile), ceil_div(rows, kTile), q.dx_splits), dim3(256), 0, s, h);
-            }
-            if (h.slabs)
-                hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), rows < 4096 ? rows : 4096), dim3(256), 0, s,
-                                   (const float*)(ws + q.dxs), q.dx_splits, (long long)rows * p.d, (long long)p.d, rows, p.d, dxr,
-                                   (long long)p.d, shared);
+        const dim3 g_grid(ceil_div(q.ld_e, kGradCols), groups);
+        if (own) hipLaunchKernelGGL((xent_g_kernel<T, true>), g_grid, dim3(256), 0, s, c);
+        else hipLaunchKernelGGL((xent_g_kernel<T, false>), g_grid, dim3(256), 0, s, c);
+
+        XentGemm hx = {}, hw = {};
+        const void* G = ws + (q.wide ? q.gp : q.e);
+        // dx[row][k] = sum over classes G[row][v] W[v][k]
+        hx.p = wk; hx.ld_p = ld_w; hx.q = G; hx.ld_q = q.ld_e; hx.I = p.d; hx.Jn = rows; hx.K = p.classes;
+        if (q.wide) hx.plane_p = p.classes * ld_w, hx.plane_q = rows * q.ld_e;
+        hx.k_per_split = k_per_split(p.classes, q.dx_splits, bk);
+        hx.slabs = q.dx_splits > 1; hx.factor = shared;
+        T* dxr = (T*)dx + (long long)r0 * p.d;
+        hx.out = hx.slabs ? (void*)(ws + q.dxs) : (void*)dxr; hx.ld_out = p.d; hx.splits = q.dx_splits;
+        // dW[v][k] = sum over rows G[row][v] x[row][k]
+        hw.p = xr; hw.ld_p = ld_x; hw.q = G; hw.ld_q = q.ld_e; hw.I = p.d; hw.Jn = p.classes; hw.K = rows;
+        if (q.wide) hw.plane_p = rows * ld_x, hw.plane_q = rows * q.ld_e;
+        hw.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
+        hw.slabs = q.dw_slabs; hw.factor = shared; hw.add = piece > 0;
+        hw.out = hw.slabs ? (void*)(ws + q.dws) : dw; hw.ld_out = p.d; hw.splits = q.dw_splits;
+        int rc = 0;
+        if (q.dx_tile == kTile) {                    // (then dW's is as well)
+            const int xi = ceil_div(p.d, kTile), xj = dx ? ceil_div(rows, kTile) : 0, wj = dw ? ceil_div(p.classes, kTile) : 0;
+            const int nx = xi * xj * q.dx_splits, nw = xi * wj * q.dw_splits;
+            if (nx + nw)
+                hipLaunchKernelGGL((xent_gemm_pair_kernel<T>), dim3((unsigned)(nx + nw)), dim3(256), 0, s, hx, hw, xi, xj, xi, wj, nx);
+        } else if (dx && dw && q.dx_tile == 128 && q.dw_tile == 128) {
+            rc = xent_tiles_pair(hx, hw, s);
+        } else {
+            if (dx) rc = xent_tiles_dx(hx, q.dx_tile, s);
+            if (dw && !rc) rc = xent_tiles_dw(hw, q.dw_tile, s);
         }
-        if (dw) {                          // dW[v][k] = sum over rows G[row][v] x[row][k]
-            XentGemm h = {};
-            h.p = xr; h.ld_p = ld_x; h.q = ws + (q.wide ? q.gp : q.e); h.ld_q = q.ld_e; h.I = p.d; h.Jn = p.classes; h.K = rows;
-            if (q.wide) h.plane_p = rows * ld_x, h.plane_q = rows * q.ld_e;
-            h.k_per_split = k_per_split(q.rows, q.dw_splits, bk);
-            h.slabs = q.dw_slabs; h.factor = shared; h.add = piece > 0;
-            h.out = h.slabs ? (void*)(ws + q.dws) : dw; h.ld_out = p.d;
-            h.splits = q.dw_splits;
-            if (q.dw_tile > kTile) {
-                const int rc = xent_tiles_dw(h, q.dw_tile, s);
-                if (rc) return rc;
-            } else {
-                hipLaunchKernelGGL((xent_gemm_kernel<T, false, false, false>),
-                                   dim3(ceil_div(p.d, kTile), ceil_div(p.classes, kTile), q.dw_splits), dim3(256), 0, s, h);
-            }
-            if (h.slabs && last)
-                hipLaunchKernelGGL((xent_slab_kernel<T>), dim3(ceil_div(p.d, 2048), p.classes < 4096 ? p.classes : 4096), dim3(256), 0, s,
-                                   (const float*)(ws + q.dws), q.dw_splits, (long long)p.classes * p.d, (long long)p.d, p.classes,
-                                   p.d, (T*)dw, (long long)p.d, shared);
+        if (rc) return rc;
+
+        XentFinish f = {};
+        const auto slabs = [&](XentSlabs& o, const void* in, void* out, int n, int rows_, int tile) {
+            o.in = (const float*)in; o.out = out; o.slabs = n; o.rows = rows_; o.cols = p.d; o.ld = slab_ld(p.d, tile);
+            o.blocks = ceil_div((long long)rows_ * ceil_div(p.d, 8), kSlabPerBlock / 8);
+        };
+        if (dx && hx.slabs) slabs(f.dx, ws + q.dxs, dxr, q.dx_splits, rows, q.dx_tile);
+        if (dw && hw.slabs && last) slabs(f.dw, ws + q.dws, dw, q.dw_splits, p.classes, q.dw_tile);
+        if (db && last) {
+            f.db_part = c.db_part; f.db = db; f.ld_db = q.ld_e; f.groups = q.row_groups; f.classes = p.classes; f.db_bf16 = p.bias_type;
+            f.db_blocks = ceil_div(p.classes, 64);
         }
-        if (db && last) column_sums((const float*)(ws + q.dbp), q.row_groups, q.ld_e, p.classes, p.classes, db, nullptr, p.bias_type, shared, s);
+        f.factor = shared;
+        f.all = all; f.all.loss_rows = !none && last && own ? loss_rows : nullptr;
+        const long long blocks = (long long)f.dx.blocks + f.dw.blocks + f.db_blocks + (f.all.loss_rows ? 1 : 0);
+        if (blocks > 0x7fffffffLL) return ASL_ETOOBIG;
+        if (blocks) hipLaunchKernelGGL((xent_finish_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, f);
     }
     if (!none && (!grad || !q.pieces)) {
         all.loss_rows = loss_rows;

@@ -10,6 +10,7 @@ namespace asl_detail {
 // the compiler still issues 16-byte accesses, which gfx950 executes at any alignment.
 typedef short bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct F8 {
@@ -122,6 +123,19 @@ __device__ __forceinline__ float row16_sum(float v) {
     v = with(v, std::integral_constant<int, 0x4e>{});        // lane ^ 2
     v = with(v, std::integral_constant<int, 0x141>{});       // the other four of eight (mirrored)
     v = with(v, std::integral_constant<int, 0x140>{});       // the other eight of sixteen (mirrored)
+#endif
+    return v;
+}
+__device__ __forceinline__ float row16_max(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto with = [](float x, auto ctrl) {
+        const int i = __builtin_bit_cast(int, x);
+        return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, decltype(ctrl)::value, 0xf, 0xf, true)));
+    };
+    v = with(v, std::integral_constant<int, 0xb1>{});
+    v = with(v, std::integral_constant<int, 0x4e>{});
+    v = with(v, std::integral_constant<int, 0x141>{});
+    v = with(v, std::integral_constant<int, 0x140>{});
 #endif
     return v;
 }

@@ -13,7 +13,7 @@ struct XentGemm {
     long long plane_p, plane_q;   // fp32 operands as three bf16 planes: elements from one plane to the next (0: one plane)
     int I, Jn, K;
     // plain products
-    void* out;               // of the operands' type, or fp32 slabs [splits][Jn][I] when slabs != 0
+    void* out;               // of the operands' type, or fp32 slabs [splits][Jn][I up to whole tiles] when slabs != 0
     long long ld_out;
     const float* factor;     // on the device; multiplies the sums on their way out (slabs: not yet)
     int slabs, add, k_per_split, splits;
@@ -37,6 +37,59 @@ constexpr float kExpScale16 = 32768.f;    // exponentials in (0, 1] held as fp16
 int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s);
 int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s);     // P along its own index, Q along k
 int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s);     // both along their own index
+int xent_tiles_pair(const XentGemm& dx, const XentGemm& dw, hipStream_t s);     // both, on 128 x 128 tiles
+
+// What the products leave of a piece of rows, and what becomes of it.
+struct XentStats {
+    const long long* target; // of the piece's rows
+    const float* upstream;   // null: 1
+    const float* tile_max;   // [rows][tiles]
+    const float* tile_sum;
+    const float* tile_lin;
+    const float* target_logit;
+    long long ignore;
+    float smoothing, inv_classes;
+    int rows, classes, tiles;
+};
+struct XentRow {
+    float lse, loss, g, target_g;            // g: the row's own weight, nought for an ignored row; target_g: G at the target
+    bool valid;                              // a label outside the vocabulary makes loss and gradients NaN
+};
+
+// LANES lanes (a wave, or a quarter of one) on a row: its tile maxima and sums to its statistics, in one pass, the running sum
+// rescaled where the maximum moves.
+template <int LANES>
+__device__ __forceinline__ XentRow row_stats(const XentStats& a, int row, int lane) {
+    const float* mx = a.tile_max + (long long)row * a.tiles;
+    const float* sm = a.tile_sum + (long long)row * a.tiles;
+    const long long t = a.target[row];
+    XentRow o;
+    o.valid = t >= 0 && t < a.classes;
+    const bool kept = t != a.ignore;
+    o.g = !kept ? 0.f : a.upstream ? a.upstream[row] : 1.f;
+    const float lt = o.valid ? a.target_logit[row] : NAN;
+    float m = -INFINITY, s = 0.f, lin = 0.f;
+#pragma unroll 4
+    for (int k = lane; k < a.tiles; k += LANES) {
+        const float v = mx[k], q = sm[k];
+        if (v > m) {
+            s = s * expf(m - v) + q;
+            m = v;
+        } else {
+            s += q * expf(v - (m == -INFINITY ? 0.f : m));
+        }
+        if (a.smoothing != 0.f) lin += a.tile_lin[(long long)row * a.tiles + k];
+    }
+    const auto sum = [](float v) { return LANES == 16 ? row16_sum(v) : wave64_sum(v); };
+    const float top = LANES == 16 ? row16_max(m) : wave_max(m);
+    const float ref = top == -INFINITY ? 0.f : top;
+    o.lse = ref + logf(sum(s * expf(m - ref)));
+    o.loss = o.lse - lt;
+    if (a.smoothing != 0.f) o.loss = o.lse - (1.f - a.smoothing) * lt - a.smoothing * a.inv_classes * sum(lin);
+    if (!kept) o.loss = 0.f;
+    o.target_g = o.g * (expm1f(lt - o.lse) + a.smoothing - a.smoothing * a.inv_classes);
+    return o;
+}
 
 // xent_few.hip: up to 32 rows
 constexpr int kFewRows = 32, kFewTile = 32, kFewClasses = 16384;

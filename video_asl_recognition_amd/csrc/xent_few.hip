@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
     constexpr int R = kFewRows / 8, TPB = 256 / kFewTile;
     __shared__ float fac[kFewRows][TPB], target_g[kFewRows], row_g[kFewRows], loss_row[kFewRows];
     __shared__ __attribute__((aligned(16))) float cols[8][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 63, cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = (long long)blockIdx.x * 256 + cl * 8;
     const bool in = a.e && col < a.ld_e;
     F8 g[R];
@@ -174,45 +174,25 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
     for (int u = 0; u < R; ++u)
         if (in && rl + u * 8 < a.n) g[u] = load8_full(a.e + (rl + u * 8) * a.ld_e + col);
     const int kept_all = __popcll(__ballot(lane < a.n && a.target[lane < a.n ? lane : 0] != a.ignore));
-    for (int row = wave; row < a.n; row += 4) {
-        const float* mx = a.tile_max + (long long)row * a.tiles;
-        const float* sm = a.tile_sum + (long long)row * a.tiles;
-        float m = -INFINITY, s = 0.f, lin = 0.f;
-        // one pass, the running sum rescaled where the maximum moves
-        for (int t = lane; t < a.tiles; t += 64) {
-            const float v = mx[t], q = sm[t];
-            if (v > m) {
-                s = s * expf(m - v) + q;
-                m = v;
-            } else {
-                s += q * expf(v - (m == -INFINITY ? 0.f : m));
-            }
-            if (a.smoothing != 0.f) lin += a.tile_lin[(long long)row * a.tiles + t];
-        }
-        const float top = wave_max(m);
-        const float ref = top == -INFINITY ? 0.f : top;
-        s = wave64_sum(s * expf(m - ref));
-        lin = wave64_sum(lin);
-        const float lse = ref + logf(s);
-        const long long t = a.target[row];
-        const bool kept = t != a.ignore, valid = t >= 0 && t < a.classes;
-        const float gr = !kept ? 0.f : a.upstream && a.none ? a.upstream[row] : 1.f;
-        const float lt = valid ? a.target_logit[row] : NAN;   // a label outside the vocabulary makes loss and gradients NaN
-        if (lane == 0) {
-            float l = lse - lt;
-            if (a.smoothing != 0.f) l = lse - (1.f - a.smoothing) * lt - a.smoothing * a.inv_classes * lin;
-            l = kept ? l : 0.f;
-            loss_row[row] = l;
-            target_g[row] = gr * (expm1f(lt - lse) + a.smoothing - a.smoothing * a.inv_classes);
-            row_g[row] = gr;
+    XentStats st = {};
+    st.target = a.target; st.upstream = a.none ? a.upstream : nullptr; st.tile_max = a.tile_max; st.tile_sum = a.tile_sum;
+    st.tile_lin = a.tile_lin; st.target_logit = a.target_logit; st.ignore = a.ignore; st.smoothing = a.smoothing;
+    st.inv_classes = a.inv_classes; st.rows = a.n; st.classes = a.classes; st.tiles = a.tiles;
+    const int l16 = threadIdx.x & 15;                        // sixteen rows at once
+    for (int row = threadIdx.x >> 4; row < a.n; row += 16) {
+        const XentRow r = row_stats<16>(st, row, l16);
+        if (l16 == 0) {
+            loss_row[row] = r.loss;
+            target_g[row] = r.target_g;
+            row_g[row] = r.g;
             if (blockIdx.x == 0) {
-                if (a.none) a.loss[row] = l;
-                if (a.lse) a.lse[row] = lse;
+                if (a.none) a.loss[row] = r.loss;
+                if (a.lse) a.lse[row] = r.lse;
             }
         }
-        if (a.e && lane < TPB) {
-            const int tile = blockIdx.x * TPB + lane;
-            if (tile < a.tiles) fac[row][lane] = valid ? gr * expf(mx[tile] - lse) : NAN;
+        if (a.e && l16 < TPB) {
+            const int tile = blockIdx.x * TPB + l16;
+            if (tile < a.tiles) fac[row][l16] = r.valid ? r.g * expf(a.tile_max[(long long)row * a.tiles + tile] - r.lse) : NAN;
         }
     }
     __syncthreads();

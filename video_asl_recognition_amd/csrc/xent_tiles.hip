@@ -5,7 +5,7 @@
 // and the DMA's writes) while the matrix pipe runs at its own; two waves a SIMD on 128 x 64 each ask for all of it.  The 256
 // accumulators leave each wave alone on its SIMD, so it hides its own latencies: while the MFMAs of one 16-deep slice run,
 // the next slice's fragments are read into a second set of registers, and the tile after next is on its way from memory by
-// LDS-DMA.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs still
+// LDS-DMA.  Of the 128 x 128 form two workgroups fit a CU.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs still
 // to issue: behind it the other buffer is whole and this one is free for the DMA.
 //
 // Operands contiguous along k are staged as [tile][64] and read as 16-byte fragments.  Operands contiguous along their own
@@ -30,14 +30,18 @@ namespace asl_detail {
 
 constexpr int kBK = 64;
 
-// LDS of a tile kernel: two stages of both operands, then the output rows over them (padded, so that consecutive rows start
-// in different banks), then what the logits' epilogue exchanges
+// LDS of a tile kernel: two stages of both operands; over them, behind the K loop, the results on their way out: all rows in
+// 16 bits, or 128 of them in 32 (padded, so that consecutive rows start in different banks); then a tile's bias and targets
 template <int TILE>
 struct TileLds {
+    static constexpr int kStages = 2;
     static constexpr int kPanel = TILE * kBK * 2;        // one operand's tile
-    static constexpr int kOutRow = TILE * 2 + 16;
-    static constexpr int kMain = 4 * kPanel > TILE * kOutRow ? 4 * kPanel : TILE * kOutRow;
-    static constexpr int kLogits = kMain + TILE * 4 * 8;
+    static constexpr int kStaged = 2 * kStages * kPanel;
+    static constexpr int kRow16 = TILE * 2 + 16;         // bytes
+    static constexpr int kRow32 = TILE * 4 + 16;
+    static constexpr int kOut = TILE * kRow16 > 128 * kRow32 ? TILE * kRow16 : 128 * kRow32;
+    static constexpr int kMain = kStaged > kOut ? kStaged : kOut;
+    static constexpr int kLogits = kMain + TILE * 8;
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -153,28 +157,29 @@ __device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) 
     j = first + in % w;
 }
 
-template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
-__global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(const XentGemm a, int ti, int tj) {
 #if defined(__HIP_DEVICE_COMPILE__)
+// One tile of a product: workgroup `id` of ti * tj * splits.
+template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
+__device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int tj) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     using Lds = TileLds<TILE>;
     constexpr int F = TILE / 64, W = TILE / 2;       // fragments of 32 and indices a wave has of either operand
     float* const bias_row = (float*)(smem + Lds::kMain);
     int* const target_at = (int*)(smem + Lds::kMain + TILE * 4);             // within the tile, or -1
-    float (*const red)[TILE][3] = (float (*)[TILE][3])(smem + Lds::kMain + TILE * 8);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave >> 1) * W, wj = (wave & 1) * W;
     int bi, bj;
-    tile_of(blockIdx.x, ti, tj, bi, bj);
+    const int slice = id / (ti * tj);
+    tile_of(id % (ti * tj), ti, tj, bi, bj);
     const int i0 = bi * TILE, j0 = bj * TILE;
-    const int kb = blockIdx.y * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
+    const int kb = slice * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
     const int steps = ke > kb ? (ke - kb + kBK - 1) / kBK * (WIDE ? 6 : 1) : 0;
 
     const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
     Panel<TILE, PKC> P;
     Panel<TILE, QKC> Q;
     P.init(a.p, a.ld_p, i0, a.I, kb, ke, wave, lane, wi, lds0);
-    Q.init(a.q, a.ld_q, j0, a.Jn, kb, ke, wave, lane, wj, lds0 + 2 * Lds::kPanel);
+    Q.init(a.q, a.ld_q, j0, a.Jn, kb, ke, wave, lane, wj, lds0 + Lds::kStaged / 2);
     int pair = 0;
     constexpr int kPlaneP = 0 << 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10, kPlaneQ = 2 << 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10;
     if constexpr (WIDE) {
@@ -202,10 +207,7 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
         unroll<4 * F>([&](auto n) { dma(pr, qr, stage, n); });
         next();
     };
-    constexpr std::integral_constant<int, 0> s0{};
-    constexpr std::integral_constant<int, 1> s1{};
-    first(s0);
-    first(s1);                                       // past the end: nought, and no memory touched
+    unroll<Lds::kStages>(first);                     // past the end: nought, and no memory touched
 
     if constexpr (LOGITS) {
         const int at = threadIdx.x % TILE, i = i0 + at, j = j0 + at;
@@ -217,14 +219,29 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
     }
 
     f32x16 acc[F][F];
+    if constexpr (LOGITS) {
+        // the sums start from the bias, while the first stages are on their way
+        __syncthreads();
 #pragma unroll
-    for (int u = 0; u < F; ++u)
+        for (int u = 0; u < F; ++u)
 #pragma unroll
-        for (int v = 0; v < F; ++v)
+            for (int r = 0; r < 4; ++r) {
+                const f32x4 b = *(const f32x4*)(bias_row + wi + u * 32 + r * 8 + (lane >> 5) * 4);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
+                for (int v = 0; v < F; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[u][v][r * 4 + e] = b[e];
+            }
+    } else {
+#pragma unroll
+        for (int u = 0; u < F; ++u)
+#pragma unroll
+            for (int v = 0; v < F; ++v)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
+    }
 
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * F) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((Lds::kStages - 1) * 4 * F) : "memory");
     bf16x8 pf[2][F], qf[2][F];
     const auto read = [&](int set, int stage, int kk, int n) {      // the n-th of a slice's fragments
         if (n & 1) qf[set][n >> 1] = Q.frag(stage, kk, n >> 1);
@@ -254,48 +271,146 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // this wave has read all it needs of this stage, and its part of the other one has landed
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // this wave has read all it needs of this stage, and its part of the next one has landed
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((Lds::kStages - 2) * 4 * F) : "memory");
         unroll<N>([&](auto n) {
             constexpr int M = decltype(n)::value, D = 4 * F / N;    // one or two DMA instructions an MFMA
-            if (M < 2 * F) read(0, S ^ 1, 0, M);
+            if (M < 2 * F) read(0, (S + 1) % Lds::kStages, 0, M);
             unroll<D>([&](auto d) { dma(pr, qr, stage, std::integral_constant<int, M * D + decltype(d)::value>{}); });
             mma(1, M);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
 #pragma unroll 1
-    for (int s = 0; s < steps; s += 2) {
-        step(s0);
-        step(s1);                                    // behind the last: noughts
-    }
+    for (int s = 0; s < steps; s += Lds::kStages) unroll<Lds::kStages>(step);      // behind the last step: noughts
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-    // ---- lane: i = wi + u*32 + 8*(r/4) + 4*(lane/32) + r%4, j = wj + v*32 + lane%32 ------------------------------
+    // ---- results.  Lane: i = wi + u*32 + 8*(r/4) + 4*(lane/32) + r%4, j = wj + v*32 + lane%32 -------------------------
     const int h4 = (lane >> 5) * 4;
-    if constexpr (!LOGITS) {
-        const float c = a.slabs ? 1.f : *a.factor;
-        if (WIDE || a.slabs) {
+    if constexpr (LOGITS) {
+        // Maxima and sums are kept per W classes, a wave's own: nothing is exchanged but between a row's two lanes.  The
+        // exponential is the hardware's power of two of a fused multiply-add, which makes it 2^15 times as large for the 16-bit
+        // form on the way.
+        constexpr float kLog2e = 1.44269504088896341f;
+        const int block = bi * 2 + (wi ? 1 : 0);
 #pragma unroll
-            for (int v = 0; v < F; ++v) {
-                const int j = j0 + wj + v * 32 + (lane & 31);
-                if (j >= a.Jn) continue;
-                float* row = (float*)a.out + (a.slabs ? ((long long)blockIdx.y * a.Jn + j) * a.I : j * a.ld_out);
+        for (int v = 0; v < F; ++v) {
+            const int jl = wj + v * 32 + (lane & 31), j = j0 + jl;
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < F; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[u][v][r]);
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const float ref = m == -INFINITY ? 0.f : m;            // classes that are all masked: sum nought, not NaN
+            float s = 0.f, lin = 0.f;
+#pragma unroll
+            for (int u = 0; u < F; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float l = acc[u][v][r * 4 + e];
+                        x[e] = WIDE ? expf(l - ref) : __builtin_amdgcn_exp2f(fmaf(l - ref, kLog2e, 15.f));
+                        s += x[e];
+                    }
+                    const int at = wi + u * 32 + r * 8 + h4;
+                    if constexpr (WIDE) {
+                        if (a.store_e && j < a.Jn) *(f32x4*)((float*)a.out + j * a.ld_out + i0 + at) = x;
+                    } else {
+                        half4 o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = (_Float16)x[e];
+                        *(half4*)(smem + jl * Lds::kRow16 + at * 2) = o;
+                    }
+                }
+            s += __shfl_xor(s, 32, 64);
+            if (!WIDE) s *= 1.f / kExpScale16;
+            if (a.smooth) {
 #pragma unroll
                 for (int u = 0; u < F; ++u)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = i0 + wi + u * 32 + r * 8 + h4;
-                        f32x4 d = {acc[u][v][r * 4] * c, acc[u][v][r * 4 + 1] * c, acc[u][v][r * 4 + 2] * c, acc[u][v][r * 4 + 3] * c};
-                        if (i + 3 < a.I) {
-                            if (a.add) d += *(const f32x4u*)(row + i);
-                            *(f32x4u*)(row + i) = d;
-                        } else {
+                    for (int r = 0; r < 16; ++r) lin += i0 + wi + u * 32 + (r >> 2) * 8 + h4 + (r & 3) < a.I ? acc[u][v][r] : 0.f;
+                lin += __shfl_xor(lin, 32, 64);
+            }
+            if (lane < 32 && j < a.Jn && block < a.tiles) {
+                const long long o = (long long)j * a.tiles + block;
+                a.tile_max[o] = m;
+                a.tile_sum[o] = s;
+                if (a.smooth) a.tile_lin[o] = lin;
+            }
+            const int t = target_at[jl] - wi;
+            const bool mine = t >= 0 && t < W && ((t >> 2) & 1) * 4 == h4;
+            if (__any(mine)) {
+                float l = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (i + e < a.I) row[i + e] = a.add ? row[i + e] + d[e] : d[e];
+                for (int u = 0; u < F; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) l = (t & ~4) == u * 32 + (r >> 2) * 8 + (r & 3) ? acc[u][v][r] : l;
+                if (mine) a.target_logit[j] = l;
+            }
+        }
+        if (WIDE || !a.store_e) return;
+        __syncthreads();
+    } else if (a.slabs) {                              // rows padded to whole tiles: nothing to cut
+        const long long ld = (long long)ti * TILE;
+#pragma unroll
+        for (int v = 0; v < F; ++v) {
+            const int j = j0 + wj + v * 32 + (lane & 31);
+            float* row = (float*)a.out + ((long long)slice * a.Jn + j) * ld + i0 + wi + h4;
+            if (j < a.Jn) {
+                if (a.add) {
+#pragma unroll
+                    for (int u = 0; u < F; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const f32x4 q = *(const f32x4*)(row + u * 32 + r * 8);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[u][v][r * 4 + e] += q[e];
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < F; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        *(f32x4*)(row + u * 32 + r * 8) = f32x4{acc[u][v][r * 4], acc[u][v][r * 4 + 1], acc[u][v][r * 4 + 2], acc[u][v][r * 4 + 3]};
+            }
+        }
+        return;
+    } else {
+        const float c = *a.factor;
+        if constexpr (WIDE) {                          // fp32 rows through LDS, 128 at a time
+#pragma unroll 1
+            for (int half = 0; half < TILE / 128; ++half) {
+                if (half) __syncthreads();
+                if (TILE == 128 || wj == half * 128) {
+#pragma unroll
+                    for (int v = 0; v < F; ++v)
+#pragma unroll
+                        for (int u = 0; u < F; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                *(f32x4*)(smem + (wj % 128 + v * 32 + (lane & 31)) * Lds::kRow32 + (wi + u * 32 + r * 8 + h4) * 4) =
+                                    f32x4{acc[u][v][r * 4] * c, acc[u][v][r * 4 + 1] * c, acc[u][v][r * 4 + 2] * c, acc[u][v][r * 4 + 3] * c};
+                }
+                __syncthreads();
+                constexpr int L = TILE / 4;            // four results a lane
+#pragma unroll 4
+                for (int n = 0; n < 128 * L / 256; ++n) {
+                    const int row = n * (256 / L) + threadIdx.x / L, at = (threadIdx.x % L) * 4, j = j0 + half * 128 + row;
+                    const f32x4 x = *(const f32x4*)(smem + row * Lds::kRow32 + at * 4);
+                    float* dst = (float*)a.out + j * a.ld_out + i0 + at;
+                    if (j < a.Jn && i0 + at < a.I) {
+                        if (i0 + at + 4 <= a.I) {
+                            *(f32x4u*)dst = x;
+                        } else {
+                            dst[0] = x[0];
+                            if (i0 + at + 1 < a.I) dst[1] = x[1];
+                            if (i0 + at + 2 < a.I) dst[2] = x[2];
                         }
                     }
+                }
             }
             return;
         }
@@ -308,118 +423,73 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
                     bf16x4 o;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(acc[u][v][r * 4 + e] * c);
-                    *(bf16x4*)(smem + (wj + v * 32 + (lane & 31)) * Lds::kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
+                    *(bf16x4*)(smem + (wj + v * 32 + (lane & 31)) * Lds::kRow16 + (wi + u * 32 + r * 8 + h4) * 2) = o;
                 }
-    } else {
-        float m[F];
-#pragma unroll
-        for (int v = 0; v < F; ++v) m[v] = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < F; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x4 b = *(const f32x4*)(bias_row + wi + u * 32 + r * 8 + h4);
-#pragma unroll
-                for (int v = 0; v < F; ++v)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        acc[u][v][r * 4 + e] += b[e];
-                        m[v] = fmaxf(m[v], acc[u][v][r * 4 + e]);
-                    }
-            }
-#pragma unroll
-        for (int v = 0; v < F; ++v) {
-            const int jl = wj + v * 32 + (lane & 31), j = j0 + jl;
-            m[v] = fmaxf(m[v], __shfl_xor(m[v], 32, 64));
-            if (lane < 32) red[wave >> 1][jl][0] = m[v];
-            const int t = target_at[jl] - wi;
-            const bool mine = t >= 0 && t < W;
-            if (__any(mine)) {
-                float l = 0.f;
-#pragma unroll
-                for (int u = 0; u < F; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) l = t == u * 32 + (r >> 2) * 8 + h4 + (r & 3) ? acc[u][v][r] : l;
-                if (mine && ((t >> 2) & 1) * 4 == h4) a.target_logit[j] = l;
-            }
-        }
         __syncthreads();
-#pragma unroll
-        for (int v = 0; v < F; ++v) {
-            const int jl = wj + v * 32 + (lane & 31);
-            const float mm = fmaxf(red[0][jl][0], red[1][jl][0]);
-            const float ref = mm == -INFINITY ? 0.f : mm;          // a tile whose classes are all masked: sum nought, not NaN
-            float s = 0.f, lin = 0.f;
-#pragma unroll
-            for (int u = 0; u < F; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    half4 o;
-                    f32x4 o32;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = WIDE ? expf(acc[u][v][r * 4 + e] - ref) : __expf(acc[u][v][r * 4 + e] - ref);
-                        s += x;
-                        o[e] = (_Float16)(x * kExpScale16);
-                        o32[e] = x;
-                    }
-                    if constexpr (!WIDE) *(half4*)(smem + jl * Lds::kOutRow + (wi + u * 32 + r * 8 + h4) * 2) = o;
-                    else if (a.store_e && j0 + jl < a.Jn) *(f32x4*)((float*)a.out + (j0 + jl) * a.ld_out + i0 + wi + u * 32 + r * 8 + h4) = o32;
-                }
-            if (a.smooth) {
-#pragma unroll
-                for (int u = 0; u < F; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        lin += i0 + wi + u * 32 + (r >> 2) * 8 + h4 + (r & 3) < a.I ? acc[u][v][r] : 0.f;
-                lin += __shfl_xor(lin, 32, 64);
-            }
-            s += __shfl_xor(s, 32, 64);
-            if (lane < 32) {
-                red[wave >> 1][jl][1] = s;
-                red[wave >> 1][jl][2] = lin;
-            }
-        }
     }
-    __syncthreads();
-    if constexpr (LOGITS) {
-        const int jl = threadIdx.x, j = j0 + jl;
-        if (jl < TILE && j < a.Jn) {
-            const long long at = (long long)j * a.tiles + bi;
-            a.tile_max[at] = fmaxf(red[0][jl][0], red[1][jl][0]);
-            a.tile_sum[at] = red[0][jl][1] + red[1][jl][1];
-            if (a.smooth) a.tile_lin[at] = red[0][jl][2] + red[1][jl][2];
-        }
-        if (WIDE || !a.store_e) return;
-    }
-    // rows out of LDS, 16 bytes a lane
+    // 16-bit rows out of LDS, 16 bytes a lane
     constexpr int L = TILE / 8;
-#pragma unroll 8
-    for (int n = 0; n < TILE * L / 256; ++n) {
-        const int jl = n * (256 / L) + threadIdx.x / L, c = (threadIdx.x % L) * 8, j = j0 + jl;
-        if (j >= a.Jn) break;
-        const bf16x8 o = *(const bf16x8*)(smem + jl * Lds::kOutRow + c * 2);
-        short* dst = (short*)a.out + j * a.ld_out + i0 + c;
-        if (LOGITS || i0 + c + 8 <= a.I) {           // the exponentials' rows are padded to whole tiles
-            *(bf16x8u*)dst = o;
-        } else {
+    const int at = (threadIdx.x % L) * 8, left = LOGITS ? 8 : a.I - i0 - at;   // (the exponentials' rows are padded to whole tiles)
+    short* out = (short*)a.out + (j0 + threadIdx.x / L) * a.ld_out + i0 + at;
+    const char* src = smem + threadIdx.x / L * Lds::kRow16 + at * 2;
+    const int rows = a.Jn - j0 - (int)threadIdx.x / L;             // this lane's first row is there if positive
+    if (left >= 8) {
+#pragma unroll 4
+        for (int n = 0; n < TILE * L / 256; ++n)
+            if (n * (256 / L) < rows) *(bf16x8u*)(out + (long long)n * (256 / L) * a.ld_out) = *(const bf16x8*)(src + n * (256 / L) * Lds::kRow16);
+    } else if (left > 0) {
+#pragma unroll 1
+        for (int n = 0; n < TILE * L / 256; ++n)
+            if (n * (256 / L) < rows) {
+                const bf16x8 x = *(const bf16x8*)(src + n * (256 / L) * Lds::kRow16);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (i0 + c + e < a.I) dst[e] = o[e];
-        }
+                for (int e = 0; e < 7; ++e)
+                    if (e < left) out[(long long)n * (256 / L) * a.ld_out + e] = x[e];
+            }
     }
+}
+#endif
+
+template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
+__global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(const XentGemm a, int ti, int tj) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    tile_body<TILE, PKC, QKC, LOGITS, WIDE>(a, blockIdx.x, ti, tj);
+#endif
+}
+
+// Both gradient products in one launch, dx's workgroups first: they do not depend on one another, and where neither fills
+// the CUs they fill them together.  (128 x 128 only: two bodies of the large tile in one kernel leave the compiler no way to
+// keep 256 accumulators where they are, and products that take it fill the CUs alone.)
+template <int TILE, bool WIDE>
+__global__ __launch_bounds__(256, 2) void xent_tile_pair_kernel(const XentGemm dx, const XentGemm dw, int dx_ti, int dx_tj,
+                                                                                  int dw_ti, int dw_tj, int dx_blocks) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if ((int)blockIdx.x < dx_blocks) tile_body<TILE, false, true, false, WIDE>(dx, blockIdx.x, dx_ti, dx_tj);
+    else tile_body<TILE, false, false, false, WIDE>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
 #endif
 }
 
 template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
 static int launch_tiles(const XentGemm& a, hipStream_t s) {
     const int ti = ceil_div(a.I, TILE), tj = ceil_div(a.Jn, TILE);
-    if ((long long)ti * tj > 0x7fffffffLL) return ASL_ETOOBIG;
+    if ((long long)ti * tj * a.splits > 0x7fffffffLL) return ASL_ETOOBIG;
     constexpr int lds = LOGITS ? TileLds<TILE>::kLogits : TileLds<TILE>::kMain;
     static unsigned char lds_done[64];
     const int rc = ensure_dynamic_lds((const void*)xent_tile_kernel<TILE, PKC, QKC, LOGITS, WIDE>, lds, lds_done);
     if (rc != ASL_OK) return rc;
-    hipLaunchKernelGGL((xent_tile_kernel<TILE, PKC, QKC, LOGITS, WIDE>), dim3((unsigned)(ti * tj), a.splits), dim3(256), lds, s, a, ti, tj);
+    hipLaunchKernelGGL((xent_tile_kernel<TILE, PKC, QKC, LOGITS, WIDE>), dim3((unsigned)(ti * tj * a.splits)), dim3(256), lds, s, a, ti, tj);
+    return (int)hipGetLastError();
+}
+template <int TILE, bool WIDE>
+static int launch_pair(const XentGemm& dx, const XentGemm& dw, hipStream_t s) {
+    const int xi = ceil_div(dx.I, TILE), xj = ceil_div(dx.Jn, TILE), wi = ceil_div(dw.I, TILE), wj = ceil_div(dw.Jn, TILE);
+    const long long nx = (long long)xi * xj * dx.splits, nw = (long long)wi * wj * dw.splits;
+    if (nx + nw > 0x7fffffffLL) return ASL_ETOOBIG;
+    constexpr int lds = TileLds<TILE>::kMain;
+    static unsigned char lds_done[64];
+    const int rc = ensure_dynamic_lds((const void*)xent_tile_pair_kernel<TILE, WIDE>, lds, lds_done);
+    if (rc != ASL_OK) return rc;
+    hipLaunchKernelGGL((xent_tile_pair_kernel<TILE, WIDE>), dim3((unsigned)(nx + nw)), dim3(256), lds, s, dx, dw, xi, xj, wi, wj, (int)nx);
     return (int)hipGetLastError();
 }
 template <bool PKC, bool QKC, bool LOGITS>
@@ -429,6 +499,9 @@ static int launch_any(const XentGemm& a, int tile, hipStream_t s) {
     return tile == 256 ? launch_tiles<256, PKC, QKC, LOGITS, false>(a, s) : launch_tiles<128, PKC, QKC, LOGITS, false>(a, s);
 }
 
+int xent_tiles_pair(const XentGemm& dx, const XentGemm& dw, hipStream_t s) {
+    return dx.plane_p ? launch_pair<128, true>(dx, dw, s) : launch_pair<128, false>(dx, dw, s);
+}
 int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s) { return launch_any<true, true, true>(a, tile, s); }
 int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s) { return launch_any<false, true, false>(a, tile, s); }
 int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s) { return launch_any<false, false, false>(a, tile, s); }
