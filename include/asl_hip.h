@@ -523,7 +523,8 @@ int asl_linear_xent_grad(const asl_xent_params* p, const void* x, const void* w,
  * grads, numel, in_type (ASL_F32 / ASL_BF16 each), out and out_type are HOST arrays, read during the call; grads[i] and
  * out[i] are device pointers.  out == NULL computes the norm alone; out[i] == grads[i] clips in place (same type); any other
  * overlap of an output with another tensor returns ASL_EINVAL.  norm: fp32, one value, on the device; nothing is waited for.
- * A NaN among the gradients makes norm and every output NaN.  workspace: 8-byte aligned, asl_grad_clip_workspace bytes. */
+ * A NaN among the gradients makes norm and every output NaN.  workspace: 8-byte aligned, asl_grad_clip_workspace bytes.
+ * A tensor of more than 2^36 elements returns ASL_ETOOBIG. */
 int64_t asl_grad_clip_workspace(int count, const int64_t* numel);
 int asl_grad_clip(int count, const void* const* grads, const int64_t* numel, const int32_t* in_type, void* const* out,
                   const int32_t* out_type, float max_norm, int inf_norm, float* norm, double* workspace, asl_stream_t stream);

@@ -136,7 +136,8 @@ def test_grad_clip_workspace():
     arr = lambda v: (C.c_int64 * len(v))(*v)
     assert L.lib.asl_grad_clip_workspace(0, None) == 0
     assert L.lib.asl_grad_clip_workspace(2, arr((0, 1))) == 8
-    assert L.lib.asl_grad_clip_workspace(2, arr((1 << 40, 1))) == 2048 * 8
+    assert L.lib.asl_grad_clip_workspace(2, arr((1 << 36, 1))) == 2048 * 8
+    assert L.lib.asl_grad_clip_workspace(2, arr((1, (1 << 36) + 1))) == L.ASL_ETOOBIG
     assert L.lib.asl_grad_clip_workspace(2, arr((5, -1))) == L.ASL_EINVAL
 
 

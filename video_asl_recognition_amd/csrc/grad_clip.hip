@@ -22,20 +22,30 @@
 
 namespace asl_detail {
 
-constexpr int kTensors = 96;              // per launch: 96 * 36 bytes of arguments and a little, under the 4 KiB they may take
+constexpr int kTensors = 140;             // per launch: 28 bytes of arguments each, of the 4 KiB that a launch may take
 constexpr int kChunk = 8192;              // elements: 256 threads x 8 x 4
+constexpr long long kMostElements = 1LL << 36;   // of one tensor: a launch's chunks are counted in 32 bits
 constexpr int kClipBlocks = 2048;         // at most, per launch: 8 workgroups of 256 a CU
 
+// A tensor's address with its type in bit 0 (elements are at least two bytes apart: the bit is free; set: bf16).
+struct Tagged {
+    unsigned long long bits;
+    __device__ __forceinline__ bool bf16() const { return bits & 1; }
+    // (said to be global memory: the compiler cannot know of an address that was a number, and would use flat accesses)
+    template <typename T>
+    __device__ __forceinline__ T* ptr() const {
+        return (T*)(__attribute__((address_space(1))) T*)(bits & ~1ull);
+    }
+};
+
 struct ClipArgs {
-    const void* in[kTensors];
-    void* out[kTensors];
+    Tagged in[kTensors], out[kTensors];
     long long n[kTensors];
-    long long first[kTensors + 1];        // first chunk of each tensor in this launch; the last entry is the chunk count
-    unsigned char in_bf16[kTensors], out_bf16[kTensors];
+    int first[kTensors + 1];              // first chunk of each tensor in this launch; the last entry is the chunk count
+    int tensors, part0, parts, inf_norm, write_norm;
+    float max_norm;
     double* part;
     float* norm;
-    float max_norm;
-    int tensors, part0, parts, inf_norm, write_norm;
 };
 static_assert(sizeof(ClipArgs) <= 4096, "kernel arguments");
 
@@ -53,7 +63,7 @@ __device__ __forceinline__ double block_combine(double v, int inf_norm, double* 
     return combine(combine(lds[0], lds[1], inf_norm), combine(lds[2], lds[3], inf_norm), inf_norm);
 }
 
-__device__ __forceinline__ int tensor_of(const ClipArgs& a, long long chunk) {
+__device__ __forceinline__ int tensor_of(const ClipArgs& a, int chunk) {
     int lo = 0, hi = a.tensors;           // first[lo] <= chunk < first[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -63,31 +73,50 @@ __device__ __forceinline__ int tensor_of(const ClipArgs& a, long long chunk) {
     return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ void accumulate(const T* p, long long left, int inf_norm, double& v) {
-    F8 g[4];
+// A chunk's share of a thread: vectors of V elements, 256 apart, so that a wave's access is one run of lines.
+template <int V>
+__device__ __forceinline__ int vector_len(long long left, int i) {
+    const long long k = left - (i * 256 + (int)threadIdx.x) * V;
+    return k >= V ? V : k > 0 ? (int)k : 0;
+}
+
+__device__ __forceinline__ void add_square(float g, int inf_norm, double& v) {
+    const double x = (double)g;
+    v = inf_norm ? max_nan(fabs(x), v) : v + x * x;
+}
+__device__ __forceinline__ void accumulate(const float* p, long long left, int inf_norm, double& v) {
+    f32x4 g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int n = vector_len<4>(left, i);
+        g[i] = load4(p + (n ? (i * 256 + threadIdx.x) * 4 : 0), n);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) add_square(g[i][e], inf_norm, v);
+}
+__device__ __forceinline__ void accumulate(const short* p, long long left, int inf_norm, double& v) {
+    bf16x8 g[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const long long k = (i * 256 + threadIdx.x) * 8LL;
-        g[i] = load8(p + (k < left ? k : 0), left - k > 8 ? 8 : (int)(left - k < 0 ? 0 : left - k));
+        const int n = vector_len<8>(left, i);
+        g[i] = load8_raw(p + (n ? (i * 256 + threadIdx.x) * 8 : 0), n);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const double x = (double)g[i].v[e];
-            v = inf_norm ? max_nan(fabs(x), v) : v + x * x;
-        }
+        for (int e = 0; e < 8; ++e) add_square(bf16_to_f32(g[i][e]), inf_norm, v);
 }
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const ClipArgs a) {
     __shared__ double lds[4];
     double v = 0.0;
-    for (long long c = blockIdx.x; c < a.first[a.tensors]; c += gridDim.x) {
+    for (int c = blockIdx.x; c < a.first[a.tensors]; c += gridDim.x) {
         const int t = tensor_of(a, c);
-        const long long at = (c - a.first[t]) * kChunk;
-        if (a.in_bf16[t]) accumulate((const short*)a.in[t] + at, a.n[t] - at, a.inf_norm, v);
-        else accumulate((const float*)a.in[t] + at, a.n[t] - at, a.inf_norm, v);
+        const long long at = (long long)(c - a.first[t]) * kChunk;
+        if (a.in[t].bf16()) accumulate(a.in[t].ptr<const short>() + at, a.n[t] - at, a.inf_norm, v);
+        else accumulate(a.in[t].ptr<const float>() + at, a.n[t] - at, a.inf_norm, v);
     }
     v = block_combine(v, a.inf_norm, lds);
     if (threadIdx.x == 0) a.part[a.part0 + blockIdx.x] = v;
@@ -95,21 +124,16 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const ClipArgs a) {
 
 template <typename T, typename U>
 __device__ __forceinline__ void scale_chunk(const T* p, U* q, long long left, float c) {
-    F8 g[4];
-    int n[4];
+    f32x4 g[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long k = (i * 256 + threadIdx.x) * 8LL;
-        n[i] = left - k > 8 ? 8 : (int)(left - k < 0 ? 0 : left - k);
-        g[i] = load8(p + (k < left ? k : 0), n[i]);
+    for (int i = 0; i < 8; ++i) {
+        const int n = vector_len<4>(left, i);
+        g[i] = load4(p + (n ? (i * 256 + threadIdx.x) * 4 : 0), n);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (n[i] > 0) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[i].v[e] *= c;
-            store8(q + (i * 256 + threadIdx.x) * 8LL, n[i], g[i]);
-        }
+    for (int i = 0; i < 8; ++i) {
+        const int n = vector_len<4>(left, i);
+        if (n) store4(q + (i * 256 + threadIdx.x) * 4, n, f32x4{g[i][0] * c, g[i][1] * c, g[i][2] * c, g[i][3] * c});
     }
 }
 
@@ -123,18 +147,18 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const ClipArgs a) {
     // a norm that is not a number makes every gradient one, an infinite norm makes them nought (and NaN where infinite)
     const float r = a.max_norm / (norm + 1e-6f);
     const float c = r > 1.0f ? 1.0f : r;
-    const long long chunks = a.first[a.tensors];
-    for (long long i = blockIdx.x; i < chunks; i += gridDim.x) {
-        const long long k = chunks - 1 - i;
-        const int t = tensor_of(a, k);
-        if (c == 1.0f && a.in[t] == a.out[t]) continue;        // in place and nothing to clip: as it is
-        const long long at = (k - a.first[t]) * kChunk, left = a.n[t] - at;
-        if (a.in_bf16[t]) {
-            if (a.out_bf16[t]) scale_chunk((const short*)a.in[t] + at, (short*)a.out[t] + at, left, c);
-            else scale_chunk((const short*)a.in[t] + at, (float*)a.out[t] + at, left, c);
+    const int chunks = a.first[a.tensors];
+    for (int i = blockIdx.x; i < chunks; i += gridDim.x) {
+        const int k = chunks - 1 - i, t = tensor_of(a, k);
+        const Tagged in = a.in[t], out = a.out[t];
+        if (c == 1.0f && in.bits == out.bits) continue;        // in place and nothing to clip: as it is
+        const long long at = (long long)(k - a.first[t]) * kChunk, left = a.n[t] - at;
+        if (in.bf16()) {
+            if (out.bf16()) scale_chunk(in.ptr<const short>() + at, out.ptr<short>() + at, left, c);
+            else scale_chunk(in.ptr<const short>() + at, out.ptr<float>() + at, left, c);
         } else {
-            if (a.out_bf16[t]) scale_chunk((const float*)a.in[t] + at, (short*)a.out[t] + at, left, c);
-            else scale_chunk((const float*)a.in[t] + at, (float*)a.out[t] + at, left, c);
+            if (out.bf16()) scale_chunk(in.ptr<const float>() + at, out.ptr<short>() + at, left, c);
+            else scale_chunk(in.ptr<const float>() + at, out.ptr<float>() + at, left, c);
         }
     }
 }
@@ -148,6 +172,7 @@ __global__ __launch_bounds__(256) void grad_norm_finish_kernel(const double* par
     if (threadIdx.x == 0) *norm = (float)(inf_norm ? v : sqrt(v));
 }
 
+static_assert(kTensors * (kMostElements / kChunk + 1) < 0x7fffffffLL, "chunks of a launch");
 inline int launch_parts(long long chunks) { return (int)(chunks < kClipBlocks ? chunks : kClipBlocks); }
 
 // an output may be its own input, in place and of the same type; any other overlap of an output would race
@@ -179,6 +204,7 @@ extern "C" int64_t asl_grad_clip_workspace(int count, const int64_t* numel) {
     long long parts = 0, chunks = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] < 0) return ASL_EINVAL;
+        if (numel[i] > kMostElements) return ASL_ETOOBIG;
         chunks += (numel[i] + kChunk - 1) / kChunk;
         if (i % kTensors == kTensors - 1 || i == count - 1) {
             parts += launch_parts(chunks);
@@ -195,7 +221,8 @@ extern "C" int asl_grad_clip(int count, const void* const* grads, const int64_t*
     if (count && (!grads || !numel || !in_type)) return ASL_EINVAL;
     if (out && (!out_type || !(max_norm >= 0.f))) return ASL_EINVAL;
     const int64_t need = asl_grad_clip_workspace(count, numel);
-    if (need < 0 || (need && !workspace)) return ASL_EINVAL;
+    if (need < 0) return (int)need;
+    if (need && !workspace) return ASL_EINVAL;
     for (int i = 0; i < count; ++i) {
         if (in_type[i] < 0 || in_type[i] > 1 || (out && (out_type[i] < 0 || out_type[i] > 1))) return ASL_EINVAL;
         if (!numel[i]) continue;
@@ -215,12 +242,10 @@ extern "C" int asl_grad_clip(int count, const void* const* grads, const int64_t*
         a.tensors = count - t0 < kTensors ? count - t0 : kTensors;
         a.first[0] = 0;
         for (int i = 0; i < a.tensors; ++i) {
-            a.in[i] = grads[t0 + i];
-            a.out[i] = out ? out[t0 + i] : nullptr;
+            a.in[i].bits = (unsigned long long)(uintptr_t)grads[t0 + i] | (unsigned long long)in_type[t0 + i];
+            a.out[i].bits = out ? (unsigned long long)(uintptr_t)out[t0 + i] | (unsigned long long)out_type[t0 + i] : 0;
             a.n[i] = numel[t0 + i];
-            a.in_bf16[i] = (unsigned char)in_type[t0 + i];
-            a.out_bf16[i] = out ? (unsigned char)out_type[t0 + i] : 0;
-            a.first[i + 1] = a.first[i] + (a.n[i] + kChunk - 1) / kChunk;
+            a.first[i + 1] = a.first[i] + (int)((a.n[i] + kChunk - 1) / kChunk);
         }
         return launch_parts(a.first[a.tensors]);
     };

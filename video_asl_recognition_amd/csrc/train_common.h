@@ -9,6 +9,7 @@ namespace asl_detail {
 // Rows of a tensor need only their element's own alignment (odd widths, sliced tensors): the vector types below say so and
 // the compiler still issues 16-byte accesses, which gfx950 executes at any alignment.
 typedef short bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef short bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -156,6 +157,49 @@ __device__ __forceinline__ float wave64_sum(float v) {
     return v;
 }
 
+// four elements, and fewer at a row's end
+__device__ __forceinline__ f32x4 load4(const float* p, int n) {
+    if (n >= 4) return *(const f32x4u*)p;
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) r[e] = p[e];
+    return r;
+}
+__device__ __forceinline__ f32x4 load4(const short* p, int n) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+        const bf16x4u q = *(const bf16x4u*)p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = bf16_to_f32(q[e]);
+        return r;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) r[e] = bf16_to_f32(p[e]);
+    return r;
+}
+__device__ __forceinline__ void store4(float* p, int n, f32x4 v) {
+    if (n >= 4) {
+        *(f32x4u*)p = v;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = v[e];
+}
+__device__ __forceinline__ void store4(short* p, int n, f32x4 v) {
+    bf16x4u o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(v[e]);
+    if (n >= 4) {
+        *(bf16x4u*)p = o;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = o[e];
+}
 // the same from a tensor whose type is only known at run time (a launch-uniform branch)
 __device__ __forceinline__ F8 load8_any(const void* base, int bf16, long long at, int n) {
     return bf16 ? load8((const short*)base + at, n) : load8((const float*)base + at, n);

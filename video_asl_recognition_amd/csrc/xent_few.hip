@@ -16,50 +16,6 @@
 
 namespace asl_detail {
 
-__device__ __forceinline__ f32x4 load4(const float* p, int n) {
-    if (n >= 4) return *(const f32x4u*)p;
-    f32x4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-        if (e < n) r[e] = p[e];
-    return r;
-}
-__device__ __forceinline__ f32x4 load4(const short* p, int n) {
-    typedef short bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
-    f32x4 r = {0.f, 0.f, 0.f, 0.f};
-    if (n >= 4) {
-        const bf16x4u q = *(const bf16x4u*)p;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = bf16_to_f32(q[e]);
-        return r;
-    }
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-        if (e < n) r[e] = bf16_to_f32(p[e]);
-    return r;
-}
-__device__ __forceinline__ void store4(float* p, int n, f32x4 v) {
-    if (n >= 4) {
-        *(f32x4u*)p = v;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-        if (e < n) p[e] = v[e];
-}
-__device__ __forceinline__ void store4(short* p, int n, f32x4 v) {
-    typedef short bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
-    bf16x4u o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(v[e]);
-    if (n >= 4) {
-        *(bf16x4u*)p = o;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-        if (e < n) p[e] = o[e];
-}
 __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
