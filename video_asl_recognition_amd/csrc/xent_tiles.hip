@@ -1,15 +1,16 @@
 // The products of the cross entropy operator for bf16 problems on gfx950: tiles of 256 x 256 (or 128 x 128, where those are
-// too few for 256 CUs), 64 deep.
+// too few for 256 CUs), 32 deep.
 //
 // Four waves of 128 x 128, one a SIMD: at 64 FLOP per LDS byte a tile of that shape asks the LDS for 3/4 of its rate (reads
 // and the DMA's writes) while the matrix pipe runs at its own; two waves a SIMD on 128 x 64 each ask for all of it.  The 256
 // accumulators leave each wave alone on its SIMD, so it hides its own latencies: while the MFMAs of one 16-deep slice run,
-// the next slice's fragments are read into a second set of registers, and the tile after next is on its way from memory by
-// LDS-DMA.  Of the 128 x 128 form two workgroups fit a CU.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs still
-// to issue: behind it the other buffer is whole and this one is free for the DMA.
+// the next slice's fragments are read into a second set of registers, and the next three stages are on their way from memory
+// by LDS-DMA.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs
+// still to issue: behind it the next stage is whole and this one is free for the DMA.  Of the 128 x 128 form two workgroups
+// fit a CU.
 //
-// Operands contiguous along k are staged as [tile][64] and read as 16-byte fragments.  Operands contiguous along their own
-// index (W for dx, x and G for dW) are staged as they lie, [64][tile], and read with the transposing LDS read, which hands a
+// Operands contiguous along k are staged as [tile][32] and read as 16-byte fragments.  Operands contiguous along their own
+// index (W for dx, x and G for dW) are staged as they lie, [32][tile], and read with the transposing LDS read, which hands a
 // group of 16 lanes four k of 16 indices; no transposed copy of anything is made.
 //
 // fp32 operands come as three bf16 planes, x = h + m + l to all its 24 bits (rounded to nearest one after the other), and the
@@ -28,13 +29,13 @@
 
 namespace asl_detail {
 
-constexpr int kBK = 64;
+constexpr int kBK = 32;
 
-// LDS of a tile kernel: two stages of both operands; over them, behind the K loop, the results on their way out: all rows in
+// LDS of a tile kernel: four stages of both operands; over them, behind the K loop, the results on their way out: all rows in
 // 16 bits, or 128 of them in 32 (padded, so that consecutive rows start in different banks); then a tile's bias and targets
 template <int TILE>
 struct TileLds {
-    static constexpr int kStages = 2;
+    static constexpr int kStages = 4;
     static constexpr int kPanel = TILE * kBK * 2;        // one operand's tile
     static constexpr int kStaged = 2 * kStages * kPanel;
     static constexpr int kRow16 = TILE * 2 + 16;         // bytes
@@ -59,7 +60,7 @@ __device__ __forceinline__ void dma_1k(i32x4 rsrc, unsigned voff, unsigned lds) 
 // one register and an immediate.
 template <int TILE, bool KC>
 struct Panel {
-    static constexpr int kPanel = TileLds<TILE>::kPanel, ND = TILE / 32, F = TILE / 64;   // DMA instructions and fragments a wave
+    static constexpr int kPanel = TileLds<TILE>::kPanel, ND = TILE / 64, F = TILE / 64;   // DMA instructions and fragments a wave
     const char* at;          // first byte of the K step to be staged next
     const char* origin;      // of the first step, and how far apart planes lie
     long long plane;
@@ -69,7 +70,7 @@ struct Panel {
     int krem;                // k left from `at` on
     unsigned lds;            // this wave's part of stage 0
     unsigned voff[ND];
-    unsigned rd[KC ? 4 : F]; // fragment addresses in stage 0: by slice (KC) or by fragment
+    unsigned rd[KC ? 2 : F]; // fragment addresses in stage 0: by slice (KC) or by fragment
 
     __device__ __forceinline__ void init(const void* base, long long ld, int i0, int n, int kb, int ke, int wave, int lane,
                                          int w0, unsigned stages) {
@@ -80,19 +81,19 @@ struct Panel {
         lds = stages + wave * (kPanel / 4);
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
-            if constexpr (KC) {                          // eight rows of 128 bytes a DMA instruction
-                const int row = wave * (TILE / 4) + i * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+            if constexpr (KC) {                          // sixteen rows of 64 bytes a DMA instruction
+                const int row = wave * (TILE / 4) + i * 16 + (lane >> 2), c = (lane & 3) ^ ((row >> 2) & 3);
                 voff[i] = (unsigned)(row * row_bytes + c * 16);
             } else {                                     // two or four k rows; their 32-byte units swapped by k's low bits
                 constexpr int L = TILE / 8;              // lanes a row
-                const int k = wave * 16 + i * (64 / L) + lane / L, u = ((lane % L) >> 1) ^ ((k & 3) << 1);
+                const int k = wave * 8 + i * (64 / L) + lane / L, u = ((lane % L) >> 1) ^ ((k & 3) << 1);
                 voff[i] = (unsigned)(k * row_bytes + u * 32 + (lane & 1) * 16);
             }
         }
         if constexpr (KC) {
-            const int r = w0 + (lane & 31), sw = (r >> 1) & 7;
+            const int r = w0 + (lane & 31), sw = (r >> 2) & 3;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) rd[kk] = stages + r * 128 + (((kk * 2 + (lane >> 5)) ^ sw) << 4);
+            for (int kk = 0; kk < 2; ++kk) rd[kk] = stages + r * 64 + (((kk * 2 + (lane >> 5)) ^ sw) << 4);
         } else {
             const int g = lane >> 4, s = lane & 15, x = (s >> 2) << 1;
 #pragma unroll
@@ -126,7 +127,7 @@ struct Panel {
     __device__ __forceinline__ bf16x8 frag(int stage, int kk, int u) const {
         typedef __attribute__((address_space(3))) char* P1;
         if constexpr (KC) {
-            return *(const __attribute__((address_space(3))) bf16x8*)((P1)(unsigned long long)rd[kk] + (stage * kPanel + u * 4096));
+            return *(const __attribute__((address_space(3))) bf16x8*)((P1)(unsigned long long)rd[kk] + (stage * kPanel + u * 2048));
         } else {
             typedef __attribute__((address_space(3))) bf16x4* P4;
             const P1 a = (P1)(unsigned long long)rd[u];
@@ -202,12 +203,15 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
         if constexpr (N & 1) Q.template dma<S, N / 2>(qr);
         else P.template dma<S, N / 2>(pr);
     };
-    const auto first = [&](auto stage) {
-        const i32x4 pr = P.rsrc(), qr = Q.rsrc();
-        unroll<4 * F>([&](auto n) { dma(pr, qr, stage, n); });
+    i32x4 pr, qr;                                    // of the stage that is being filled
+    constexpr int kDma = 2 * F;                      // DMA instructions a stage
+    const auto fill = [&](auto stage) {
+        pr = P.rsrc();
+        qr = Q.rsrc();
+        unroll<decltype(stage)::value == Lds::kStages - 1 ? kDma / 2 : kDma>([&](auto n) { dma(pr, qr, stage, n); });
         next();
     };
-    unroll<Lds::kStages>(first);                     // past the end: nought, and no memory touched
+    unroll<Lds::kStages>(fill);                      // past the end: nought, and no memory touched; the last one half
 
     if constexpr (LOGITS) {
         const int at = threadIdx.x % TILE, i = i0 + at, j = j0 + at;
@@ -241,7 +245,7 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
                 for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
     }
 
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((Lds::kStages - 1) * 4 * F) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((Lds::kStages - 2) * kDma + kDma / 2) : "memory");
     bf16x8 pf[2][F], qf[2][F];
     const auto read = [&](int set, int stage, int kk, int n) {      // the n-th of a slice's fragments
         if (n & 1) qf[set][n >> 1] = Q.frag(stage, kk, n >> 1);
@@ -255,28 +259,37 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
     };
 #pragma unroll
     for (int n = 0; n < 2 * F; ++n) read(0, 0, 0, n);
+    // A step is two slices of 16 k.  The DMA goes out at an even pace, an instruction every few MFMAs: 64 of them a step in one
+    // burst hold the waves up at the address unit, which takes 16 cycles each.
     const auto step = [&](auto stage) {
-        constexpr int S = decltype(stage)::value, N = F * F;
-        i32x4 pr, qr;
-        // slices 0 .. 2: the next slice's fragments under the first of this one's MFMAs
-#pragma unroll
-        for (int kk = 0; kk < 3; ++kk) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                if (n < 2 * F) read((kk + 1) & 1, S, kk + 1, n);
-                if (kk == 1 && n == N / 2 + 1) pr = P.rsrc();
-                if (kk == 1 && n == N - 1) qr = Q.rsrc();
-                if (kk == 2 && n == N / 2) next();
-                mma(kk & 1, n);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        // this wave has read all it needs of this stage, and its part of the next one has landed
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((Lds::kStages - 2) * 4 * F) : "memory");
+        constexpr int S = decltype(stage)::value, N = F * F, kEvery = N / (kDma / 2);
+        constexpr std::integral_constant<int, (S + Lds::kStages - 1) % Lds::kStages> before{};
+        i32x4 next_p, next_q;
+        // slice 0, under it the fragments of slice 1 and the rest of the stage that the last step began to fill
         unroll<N>([&](auto n) {
-            constexpr int M = decltype(n)::value, D = 4 * F / N;    // one or two DMA instructions an MFMA
+            constexpr int M = decltype(n)::value;
+            if (M < 2 * F) read(1, S, 1, M);
+            if constexpr (M % kEvery == 0) dma(pr, qr, before, std::integral_constant<int, kDma / 2 + M / kEvery>{});
+            // the next stage's descriptors between the last MFMAs (the empty asm holds them there: left to itself the
+            // compiler computes them where they are used, in one gap behind the barrier)
+            if constexpr (M == N - 3 && F == 4) next_p = P.rsrc();
+            if constexpr (M == N - 2) next_q = Q.rsrc();
+            if constexpr (M == N - 2 && F == 2) next_p = P.rsrc();
+            if constexpr (M == N - 1) next();
+            mma(0, M);
+            if constexpr (M == N - 3 && F == 4) asm volatile("" : "+s"(next_p));
+            if constexpr (M == N - 2) asm volatile("" : "+s"(next_q));
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        pr = next_p;
+        qr = next_q;
+        // this wave has read all it needs of this stage, and its part of the next one has landed
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((Lds::kStages - 2) * kDma) : "memory");
+        // slice 1, under it the next stage's first fragments and half of this stage's next filling
+        unroll<N>([&](auto n) {
+            constexpr int M = decltype(n)::value;
             if (M < 2 * F) read(0, (S + 1) % Lds::kStages, 0, M);
-            unroll<D>([&](auto d) { dma(pr, qr, stage, std::integral_constant<int, M * D + decltype(d)::value>{}); });
+            if constexpr (M % kEvery == 0) dma(pr, qr, stage, std::integral_constant<int, M / kEvery>{});
             mma(1, M);
             __builtin_amdgcn_sched_barrier(0);
         });
