@@ -1,16 +1,16 @@
 // The products of the cross entropy operator for bf16 problems on gfx950: tiles of 256 x 256 (or 128 x 128, where those are
-// too few for 256 CUs), 32 deep.
+// too few for 256 CUs), 64 or 32 deep.
 //
 // Four waves of 128 x 128, one a SIMD: at 64 FLOP per LDS byte a tile of that shape asks the LDS for 3/4 of its rate (reads
 // and the DMA's writes) while the matrix pipe runs at its own; two waves a SIMD on 128 x 64 each ask for all of it.  The 256
 // accumulators leave each wave alone on its SIMD, so it hides its own latencies: while the MFMAs of one 16-deep slice run,
-// the next slice's fragments are read into a second set of registers, and the next three stages are on their way from memory
-// by LDS-DMA.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs
+// the next slice's fragments are read into a second set of registers, and the stages after this one are on their way from
+// memory by LDS-DMA.  A K step has one barrier, placed where a wave holds the last slice's fragments and has that slice's MFMAs
 // still to issue: behind it the next stage is whole and this one is free for the DMA.  Of the 128 x 128 form two workgroups
 // fit a CU.
 //
-// Operands contiguous along k are staged as [tile][32] and read as 16-byte fragments.  Operands contiguous along their own
-// index (W for dx, x and G for dW) are staged as they lie, [32][tile], and read with the transposing LDS read, which hands a
+// Operands contiguous along k are staged as [tile][step] and read as 16-byte fragments.  Operands contiguous along their own
+// index (W for dx, x and G for dW) are staged as they lie, [step][tile], and read with the transposing LDS read, which hands a
 // group of 16 lanes four k of 16 indices; no transposed copy of anything is made.
 //
 // fp32 operands come as three bf16 planes, x = h + m + l to all its 24 bits (rounded to nearest one after the other), and the
@@ -29,14 +29,17 @@
 
 namespace asl_detail {
 
-constexpr int kBK = 32;
+// k a step, by whether the operands are contiguous along k.  Four stages of 32 hide more of the memory's latency than two of
+// 64 (dW of 8192 x 32768 x 2048: 794 us against 900), but rows contiguous along k are then read 64 bytes at a time, half of
+// each line twice (logits of the same: 1127 us against 1066).
+constexpr int step_depth(bool pkc, bool qkc) { return pkc || qkc ? 64 : 32; }
 
-// LDS of a tile kernel: four stages of both operands; over them, behind the K loop, the results on their way out: all rows in
+// LDS of a tile kernel: the stages of both operands, 128 k in all; over them, behind the K loop, the results on their way out: all rows in
 // 16 bits, or 128 of them in 32 (padded, so that consecutive rows start in different banks); then a tile's bias and targets
-template <int TILE>
+template <int TILE, int BK>
 struct TileLds {
-    static constexpr int kStages = 4;
-    static constexpr int kPanel = TILE * kBK * 2;        // one operand's tile
+    static constexpr int kStages = 128 / BK;
+    static constexpr int kPanel = TILE * BK * 2;         // one operand's tile
     static constexpr int kStaged = 2 * kStages * kPanel;
     static constexpr int kRow16 = TILE * 2 + 16;         // bytes
     static constexpr int kRow32 = TILE * 4 + 16;
@@ -58,9 +61,9 @@ __device__ __forceinline__ void dma_1k(i32x4 rsrc, unsigned voff, unsigned lds) 
 
 // One operand's way from memory to registers.  Its two stages lie behind one another in LDS, so that a fragment's address is
 // one register and an immediate.
-template <int TILE, bool KC>
+template <int TILE, int BK, bool KC>
 struct Panel {
-    static constexpr int kPanel = TileLds<TILE>::kPanel, ND = TILE / 64, F = TILE / 64;   // DMA instructions and fragments a wave
+    static constexpr int kPanel = TileLds<TILE, BK>::kPanel, ND = TILE * BK / 2048, F = TILE / 64;   // DMA instructions and fragments a wave
     const char* at;          // first byte of the K step to be staged next
     const char* origin;      // of the first step, and how far apart planes lie
     long long plane;
@@ -70,7 +73,11 @@ struct Panel {
     int krem;                // k left from `at` on
     unsigned lds;            // this wave's part of stage 0
     unsigned voff[ND];
-    unsigned rd[KC ? 2 : F]; // fragment addresses in stage 0: by slice (KC) or by fragment
+    unsigned rd[KC ? BK / 16 : F]; // fragment addresses in stage 0: by slice (KC) or by fragment
+
+    // 16-byte chunks of rows contiguous along k change places with the row, so that eight consecutive rows' same chunk lies in
+    // different banks
+    static __device__ __forceinline__ int swizzle(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
     __device__ __forceinline__ void init(const void* base, long long ld, int i0, int n, int kb, int ke, int wave, int lane,
                                          int w0, unsigned stages) {
@@ -81,19 +88,20 @@ struct Panel {
         lds = stages + wave * (kPanel / 4);
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
-            if constexpr (KC) {                          // sixteen rows of 64 bytes a DMA instruction
-                const int row = wave * (TILE / 4) + i * 16 + (lane >> 2), c = (lane & 3) ^ ((row >> 2) & 3);
+            if constexpr (KC) {                          // eight rows of 128 bytes a DMA instruction, or sixteen of 64
+                constexpr int L = BK / 8;                // lanes a row
+                const int row = wave * (TILE / 4) + i * (64 / L) + lane / L, c = (lane % L) ^ swizzle(row);
                 voff[i] = (unsigned)(row * row_bytes + c * 16);
             } else {                                     // two or four k rows; their 32-byte units swapped by k's low bits
                 constexpr int L = TILE / 8;              // lanes a row
-                const int k = wave * 8 + i * (64 / L) + lane / L, u = ((lane % L) >> 1) ^ ((k & 3) << 1);
+                const int k = wave * (BK / 4) + i * (64 / L) + lane / L, u = ((lane % L) >> 1) ^ ((k & 3) << 1);
                 voff[i] = (unsigned)(k * row_bytes + u * 32 + (lane & 1) * 16);
             }
         }
         if constexpr (KC) {
-            const int r = w0 + (lane & 31), sw = (r >> 2) & 3;
+            const int r = w0 + (lane & 31);
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) rd[kk] = stages + r * 64 + (((kk * 2 + (lane >> 5)) ^ sw) << 4);
+            for (int kk = 0; kk < BK / 16; ++kk) rd[kk] = stages + r * (BK * 2) + (((kk * 2 + (lane >> 5)) ^ swizzle(r)) << 4);
         } else {
             const int g = lane >> 4, s = lane & 15, x = (s >> 2) << 1;
 #pragma unroll
@@ -105,15 +113,15 @@ struct Panel {
     // last step.  Rows that are contiguous along k hold noughts up to a whole step (the caller sees to that).
     __device__ __forceinline__ i32x4 rsrc() const {
         // (32 bits: a tile's rows are at most 2^21 bytes apart)
-        const int k = krem < kBK ? krem : kBK;
-        const int n = KC ? (idx - 1) * (int)row_bytes + kBK * 2 : (k - 1) * (int)row_bytes + idx * 2;
+        const int k = krem < BK ? krem : BK;
+        const int n = KC ? (idx - 1) * (int)row_bytes + BK * 2 : (k - 1) * (int)row_bytes + idx * 2;
         const unsigned long long p = (unsigned long long)at;
         return i32x4{__builtin_amdgcn_readfirstlane((int)p), __builtin_amdgcn_readfirstlane((int)(p >> 32) & 0xffff),
                      __builtin_amdgcn_readfirstlane(krem > 0 ? (n + 3) & ~3 : 0), 0x00020000};
     }
     __device__ __forceinline__ void advance() {
-        at += KC ? kBK * 2 : kBK * row_bytes;
-        krem -= kBK;
+        at += KC ? BK * 2 : BK * row_bytes;
+        krem -= BK;
     }
     __device__ __forceinline__ void to_plane(int which, bool turn, bool more) {
         at = turn ? origin + which * plane : at;
@@ -127,7 +135,7 @@ struct Panel {
     __device__ __forceinline__ bf16x8 frag(int stage, int kk, int u) const {
         typedef __attribute__((address_space(3))) char* P1;
         if constexpr (KC) {
-            return *(const __attribute__((address_space(3))) bf16x8*)((P1)(unsigned long long)rd[kk] + (stage * kPanel + u * 2048));
+            return *(const __attribute__((address_space(3))) bf16x8*)((P1)(unsigned long long)rd[kk] + (stage * kPanel + u * (BK * 64)));
         } else {
             typedef __attribute__((address_space(3))) bf16x4* P4;
             const P1 a = (P1)(unsigned long long)rd[u];
@@ -137,6 +145,15 @@ struct Panel {
         }
     }
 };
+
+// those of TOTAL things that fall to place I of N when they are spread evenly over the places
+template <int TOTAL, int N, int I, typename F>
+__device__ __forceinline__ void paced(F&& f) {
+    constexpr int first = (I * TOTAL + N - 1) / N, last = ((I + 1) * TOTAL + N - 1) / N;
+    if constexpr (last > first) f(std::integral_constant<int, first>{});
+    if constexpr (last > first + 1) f(std::integral_constant<int, first + 1>{});
+    static_assert(last <= first + 2, "at most two a place");
+}
 
 template <int N, typename F>
 __device__ __forceinline__ void unroll(F&& f) {
@@ -160,10 +177,10 @@ __device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) 
 
 #if defined(__HIP_DEVICE_COMPILE__)
 // One tile of a product: workgroup `id` of ti * tj * splits.
-template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
+template <int TILE, int BK, bool PKC, bool QKC, bool LOGITS, bool WIDE>
 __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int tj) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    using Lds = TileLds<TILE>;
+    using Lds = TileLds<TILE, BK>;
     constexpr int F = TILE / 64, W = TILE / 2;       // fragments of 32 and indices a wave has of either operand
     float* const bias_row = (float*)(smem + Lds::kMain);
     int* const target_at = (int*)(smem + Lds::kMain + TILE * 4);             // within the tile, or -1
@@ -174,11 +191,11 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
     tile_of(id % (ti * tj), ti, tj, bi, bj);
     const int i0 = bi * TILE, j0 = bj * TILE;
     const int kb = slice * a.k_per_split, ke = kb + a.k_per_split < a.K ? kb + a.k_per_split : a.K;
-    const int steps = ke > kb ? (ke - kb + kBK - 1) / kBK * (WIDE ? 6 : 1) : 0;
+    const int steps = ke > kb ? (ke - kb + BK - 1) / BK * (WIDE ? 6 : 1) : 0;
 
     const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
-    Panel<TILE, PKC> P;
-    Panel<TILE, QKC> Q;
+    Panel<TILE, BK, PKC> P;
+    Panel<TILE, BK, QKC> Q;
     P.init(a.p, a.ld_p, i0, a.I, kb, ke, wave, lane, wi, lds0);
     Q.init(a.q, a.ld_q, j0, a.Jn, kb, ke, wave, lane, wj, lds0 + Lds::kStaged / 2);
     int pair = 0;
@@ -204,7 +221,7 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
         else P.template dma<S, N / 2>(pr);
     };
     i32x4 pr, qr;                                    // of the stage that is being filled
-    constexpr int kDma = 2 * F;                      // DMA instructions a stage
+    constexpr int kDma = 2 * Panel<TILE, BK, PKC>::ND;        // DMA instructions a stage
     const auto fill = [&](auto stage) {
         pr = P.rsrc();
         qr = Q.rsrc();
@@ -259,37 +276,39 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
     };
 #pragma unroll
     for (int n = 0; n < 2 * F; ++n) read(0, 0, 0, n);
-    // A step is two slices of 16 k.  The DMA goes out at an even pace, an instruction every few MFMAs: 64 of them a step in one
-    // burst hold the waves up at the address unit, which takes 16 cycles each.
+    // A step is BK / 16 slices.  The DMA goes out at an even pace over two of them, an instruction every few MFMAs: in one
+    // burst a stage's 64 instructions hold the waves up at the address unit, which takes 16 cycles each.
     const auto step = [&](auto stage) {
-        constexpr int S = decltype(stage)::value, N = F * F, kEvery = N / (kDma / 2);
+        constexpr int S = decltype(stage)::value, N = F * F, kSlices = BK / 16;
         constexpr std::integral_constant<int, (S + Lds::kStages - 1) % Lds::kStages> before{};
         i32x4 next_p, next_q;
-        // slice 0, under it the fragments of slice 1 and the rest of the stage that the last step began to fill
-        unroll<N>([&](auto n) {
-            constexpr int M = decltype(n)::value;
-            if (M < 2 * F) read(1, S, 1, M);
-            if constexpr (M % kEvery == 0) dma(pr, qr, before, std::integral_constant<int, kDma / 2 + M / kEvery>{});
+        // all slices but the last: under each the fragments of the next, and under the first the rest of the stage that the
+        // last step began to fill
+        unroll<(kSlices - 1) * N>([&](auto n) {
+            constexpr int M = decltype(n)::value, K = M / N, R = M % N;
+            if (R < 2 * F) read((K + 1) & 1, S, K + 1, R);
+            if constexpr (K == 0) paced<kDma / 2, N, R>([&](auto d) { dma(pr, qr, before, std::integral_constant<int, kDma / 2 + decltype(d)::value>{}); });
             // the next stage's descriptors between the last MFMAs (the empty asm holds them there: left to itself the
             // compiler computes them where they are used, in one gap behind the barrier)
-            if constexpr (M == N - 3 && F == 4) next_p = P.rsrc();
-            if constexpr (M == N - 2) next_q = Q.rsrc();
-            if constexpr (M == N - 2 && F == 2) next_p = P.rsrc();
-            if constexpr (M == N - 1) next();
-            mma(0, M);
-            if constexpr (M == N - 3 && F == 4) asm volatile("" : "+s"(next_p));
-            if constexpr (M == N - 2) asm volatile("" : "+s"(next_q));
+            constexpr bool kEnd = K == kSlices - 2;
+            if constexpr (kEnd && R == N - 3 && F == 4) next_p = P.rsrc();
+            if constexpr (kEnd && R == N - 2) next_q = Q.rsrc();
+            if constexpr (kEnd && R == N - 2 && F == 2) next_p = P.rsrc();
+            if constexpr (kEnd && R == N - 1) next();
+            mma(K & 1, R);
+            if constexpr (kEnd && R == N - 3 && F == 4) asm volatile("" : "+s"(next_p));
+            if constexpr (kEnd && R == N - 2) asm volatile("" : "+s"(next_q));
             __builtin_amdgcn_sched_barrier(0);
         });
         pr = next_p;
         qr = next_q;
         // this wave has read all it needs of this stage, and its part of the next one has landed
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((Lds::kStages - 2) * kDma) : "memory");
-        // slice 1, under it the next stage's first fragments and half of this stage's next filling
+        // the last slice, under it the next stage's first fragments and half of this stage's next filling
         unroll<N>([&](auto n) {
             constexpr int M = decltype(n)::value;
             if (M < 2 * F) read(0, (S + 1) % Lds::kStages, 0, M);
-            if constexpr (M % kEvery == 0) dma(pr, qr, stage, std::integral_constant<int, M / kEvery>{});
+            paced<kDma / 2, N, M>([&](auto d) { dma(pr, qr, stage, d); });
             mma(1, M);
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -466,7 +485,7 @@ __device__ __forceinline__ void tile_body(const XentGemm& a, int id, int ti, int
 template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
 __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(const XentGemm a, int ti, int tj) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    tile_body<TILE, PKC, QKC, LOGITS, WIDE>(a, blockIdx.x, ti, tj);
+    tile_body<TILE, step_depth(PKC, QKC), PKC, QKC, LOGITS, WIDE>(a, blockIdx.x, ti, tj);
 #endif
 }
 
@@ -477,8 +496,8 @@ template <int TILE, bool WIDE>
 __global__ __launch_bounds__(256, 2) void xent_tile_pair_kernel(const XentGemm dx, const XentGemm dw, int dx_ti, int dx_tj,
                                                                                   int dw_ti, int dw_tj, int dx_blocks) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    if ((int)blockIdx.x < dx_blocks) tile_body<TILE, false, true, false, WIDE>(dx, blockIdx.x, dx_ti, dx_tj);
-    else tile_body<TILE, false, false, false, WIDE>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
+    if ((int)blockIdx.x < dx_blocks) tile_body<TILE, step_depth(false, true), false, true, false, WIDE>(dx, blockIdx.x, dx_ti, dx_tj);
+    else tile_body<TILE, step_depth(false, false), false, false, false, WIDE>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
 #endif
 }
 
@@ -486,7 +505,7 @@ template <int TILE, bool PKC, bool QKC, bool LOGITS, bool WIDE>
 static int launch_tiles(const XentGemm& a, hipStream_t s) {
     const int ti = ceil_div(a.I, TILE), tj = ceil_div(a.Jn, TILE);
     if ((long long)ti * tj * a.splits > 0x7fffffffLL) return ASL_ETOOBIG;
-    constexpr int lds = LOGITS ? TileLds<TILE>::kLogits : TileLds<TILE>::kMain;
+    constexpr int lds = LOGITS ? TileLds<TILE, step_depth(PKC, QKC)>::kLogits : TileLds<TILE, step_depth(PKC, QKC)>::kMain;
     static unsigned char lds_done[64];
     const int rc = ensure_dynamic_lds((const void*)xent_tile_kernel<TILE, PKC, QKC, LOGITS, WIDE>, lds, lds_done);
     if (rc != ASL_OK) return rc;
@@ -498,7 +517,8 @@ static int launch_pair(const XentGemm& dx, const XentGemm& dw, hipStream_t s) {
     const int xi = ceil_div(dx.I, TILE), xj = ceil_div(dx.Jn, TILE), wi = ceil_div(dw.I, TILE), wj = ceil_div(dw.Jn, TILE);
     const long long nx = (long long)xi * xj * dx.splits, nw = (long long)wi * wj * dw.splits;
     if (nx + nw > 0x7fffffffLL) return ASL_ETOOBIG;
-    constexpr int lds = TileLds<TILE>::kMain;
+    constexpr int lds = TileLds<TILE, 32>::kMain;
+    static_assert(TileLds<TILE, 32>::kMain == TileLds<TILE, 64>::kMain, "both bodies' LDS");
     static unsigned char lds_done[64];
     const int rc = ensure_dynamic_lds((const void*)xent_tile_pair_kernel<TILE, WIDE>, lds, lds_done);
     if (rc != ASL_OK) return rc;
