@@ -378,6 +378,111 @@ def test_linear_cross_entropy_masks_and_labels(gpu):
             assert dw.isnan().all()
 
 
+# one size for each way the products are computed: few rows, 64 x 64 tiles, 128 x 128, 256 x 256, fp32 as planes of bf16
+PATHS = [(20, 300, 40, BF16), (20, 300, 40, F32), (80, 300, 64, BF16), (80, 300, 64, F32), (400, 1000, 128, BF16), (400, 1003, 77, BF16),
+         (1000, 8200, 256, BF16), (520, 9001, 136, BF16), (600, 1100, 260, F32), (1100, 8200, 65, F32)]
+PATH_IDS = [f"{n}x{v}x{d}-{'f32' if dt == F32 else 'bf16'}" for n, v, d, dt in PATHS]
+
+
+@pytest.mark.parametrize("n,v,d,dt", PATHS, ids=PATH_IDS)
+def test_linear_cross_entropy_every_path_hard_cases(gpu, n, v, d, dt):
+    from video_asl_recognition_amd import training as T
+    x, w, b, t = _xent_case(n, v, d, dt, F32, 0.0)
+    lo, hi = v // 4, v - 5                                        # most classes masked, whole tiles and the last one's all but five
+    b[lo:hi] = float("-inf")
+    t = torch.where((t >= lo) & (t < hi), t % lo, t)
+    t[n // 2:] = -100
+    _xent_check(x, w, b, t, what="masked")
+    clean = T.linear_cross_entropy_grad(x, w, t, b)
+    assert not clean[2][lo:hi].any() and not clean[3][lo:hi].any()
+    # what ignored rows hold stays out of every other row
+    xn = x.clone()
+    xn[n // 2:n // 2 + 3], xn[n // 2 + 3:] = float("nan"), float("inf")
+    dirty = T.linear_cross_entropy_grad(xn, w, t, b)
+    assert torch.equal(dirty[0], clean[0]) and torch.equal(dirty[1], clean[1]) and torch.equal(dirty[3], clean[3])
+    # masked by the type's lowest value
+    b[lo:hi] = torch.finfo(dt).min
+    low = T.linear_cross_entropy_grad(x, w, t, b)
+    assert low[0].isfinite() and not low[3][lo:hi].any()
+    # a label outside the vocabulary
+    for wrong in (-1, v, 1 << 40):
+        tw = t.clone()
+        tw[1] = wrong
+        loss, dx, dw, db = T.linear_cross_entropy_grad(x, w, tw, b, reduction="none")
+        assert loss[1].isnan() and loss[2:].isfinite().all() and dx[1].isnan().all() and dx[2:].isfinite().all() and dw.isnan().all()
+    # every row ignored; labels all smoothing
+    x, w, b, t = _xent_case(n, v, d, dt, dt, 0.1)
+    _xent_check(x, w, b, t, smooth=1.0, what="smoothed away")
+    t[:] = -100
+    loss, dx, dw, db = T.linear_cross_entropy_grad(x, w, t, b)
+    assert loss.isnan() and not dx.any() and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("n,v,d,dt", PATHS, ids=PATH_IDS)
+def test_linear_cross_entropy_every_path_upstream_and_slices(gpu, n, v, d, dt):
+    """a gradient for every row, through autograd; x and w as slices of larger tensors off any alignment; memory that held
+    NaN before"""
+    from video_asl_recognition_amd import training as T
+    x, w, b, t = _xent_case(n, v, d, dt, dt, 0.1)
+    up = torch.rand(n, generator=_gen(3), device="cuda") * 2 - 0.5
+    xb, wb = torch.zeros(n, d + 9, dtype=dt, device="cuda"), torch.zeros(2 * v, d + 5, dtype=dt, device="cuda")
+    xs, ws = xb[:, 3:d + 3], wb[::2, 1:d + 1]
+    xs.copy_(x), ws.copy_(w)
+    del wb, xb
+    junk = torch.full((1 << 28,), float("nan"), device="cuda")    # 1 GiB for the outputs and workspaces to come from
+    del junk
+    grads = []
+    for a, c in ((x, w), (xs, ws)):
+        leaves = [q.detach().requires_grad_() for q in (a, c, b)]
+        loss = T.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+        grads.append([loss] + list(torch.autograd.grad((loss * up).sum(), leaves)))
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+    ref = xent_reference(x, w, b, t, up.double(), -100, 0.0, "none", dt == BF16)
+    for got, r, tol in zip(grads[0][1:], (ref[3], ref[5], ref[7]), (ref[4], ref[6], ref[8])):
+        _ok(got, r, tol + _u(dt) * (r.abs() + tol) + 1e-38, "gradient")
+
+
+@pytest.mark.parametrize("n,v,d,dt", PATHS, ids=PATH_IDS)
+def test_linear_cross_entropy_writes_no_further_than_its_outputs(gpu, n, v, d, dt):
+    """the C entry point with outputs at their types' own alignment inside larger buffers, and with each of them left out"""
+    from video_asl_recognition_amd import _lib as L, training as T
+    x, w, b, t = _xent_case(n, v, d, dt, dt, 0.1)
+    want = T.linear_cross_entropy_grad(x, w, t, b)
+    code = T._TYPES[dt]
+    p = L.XentParams(n, v, d, code, code, L.REDUCE_MEAN, d, d, -100, 0.0, 0)
+    room = L.lib.asl_linear_xent_workspace(C.byref(p), x.data_ptr(), w.data_ptr(), 1)
+    s = torch.cuda.current_stream().cuda_stream
+    for left_out in (None, 0, 1, 2):
+        ws = torch.full((room + 512,), 0x5a, dtype=torch.uint8, device="cuda")
+        at = -ws.data_ptr() % 256
+        outs = [torch.full((q.numel() + 6,), 7.0, dtype=dt, device="cuda") for q in want[1:]]
+        loss, lse = torch.full((3,), 7.0, device="cuda"), torch.full((n + 2,), 7.0, device="cuda")
+        size = outs[0].element_size()
+        ptr = [None if i == left_out else o.data_ptr() + 3 * size for i, o in enumerate(outs)]
+        L.check(L.lib.asl_linear_xent_grad(C.byref(p), x.data_ptr(), w.data_ptr(), b.data_ptr(), t.data_ptr(), None, loss.data_ptr() + 4,
+                                           lse.data_ptr() + 4, *ptr, ws.data_ptr() + at, s), "grad")
+        assert loss[1] == want[0] and (loss[::2] == 7).all() and (lse[0] == 7) and (lse[-1] == 7) and lse[1:-1].isfinite().all()
+        for i, (o, q) in enumerate(zip(outs, want[1:])):
+            assert (o[:3] == 7).all() and (o[-3:] == 7).all()
+            assert (o == 7).all() if i == left_out else torch.equal(o[3:-3], q.flatten())
+        assert (ws[:at] == 0x5a).all() and (ws[at + room:] == 0x5a).all()
+
+
+def test_linear_cross_entropy_pieces_without_gradients(gpu):
+    """so many classes that the rows' maxima and sums are taken in pieces: the rows' results are those of calls of their own"""
+    from video_asl_recognition_amd import training as T
+    v, n, d = 1 << 21, 2500, 8
+    x, w, b, t = _xent_case(n, v, d, BF16, BF16, 0.1)
+    loss, lse = T.linear_cross_entropy_fwd(x, w, t, b, reduction="none")
+    for part in (slice(0, 500), slice(1900, 2500)):
+        l, e = T.linear_cross_entropy_fwd(x[part], w, t[part], b, reduction="none")
+        assert torch.equal(l, loss[part]) and torch.equal(e, lse[part])
+    rows = slice(2040, 2060)
+    ref = xent_reference(x[rows], w, b, t[rows], 1.0, -100, 0.0, "none", True)
+    _ok(loss[rows], ref[0], ref[1], "loss")
+    _ok(lse[rows], ref[2], ref[1], "lse")
+
+
 def test_linear_cross_entropy_no_rows(gpu):
     from video_asl_recognition_amd import training as T
     x, w, b, t = (torch.empty(0, 16, device="cuda"), torch.randn(9, 16, device="cuda"), torch.randn(9, device="cuda"),
@@ -593,3 +698,37 @@ def test_steps_on_two_streams(gpu):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_autograd_in_a_graph(gpu, dt):
+    """forward and backward through autograd, captured: gradients are taken as values, so nothing of an eager graph is met"""
+    from video_asl_recognition_amd import training as T
+    states = [_step_state(dt, 300, 500, 96, 60 + i) for i in range(3)]
+    keys = ("x", "g", "b", "w", "c")
+
+    def run(s):
+        leaves = [s[k].detach().requires_grad_() for k in keys]
+        y = T.layer_norm(leaves[0], leaves[1], leaves[2])
+        loss = T.linear_cross_entropy(y, leaves[3], s["t"], leaves[4], label_smoothing=0.1)
+        grads = list(torch.autograd.grad(loss, leaves))
+        return [loss.detach(), T.clip_grads(grads, 0.05)] + grads
+    eager = [[o.clone() for o in run(s)] for s in states]
+    static = {k: q.clone() for k, q in states[0].items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(static)
+    for _ in range(3):
+        for s, want in zip(states, eager):
+            for k in static:
+                static[k].copy_(s[k])
+            graph.replay()
+            again = run(s)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) and torch.equal(r, q) for p, q, r in zip(captured, want, again))

@@ -109,6 +109,18 @@ def test_xent_workspace_is_bounded():
     assert small < 1 << 28
 
 
+def test_xent_launches_stay_launchable():
+    """a grid is fewer than 2^32 threads: rows that would need more are taken in pieces, weights that would are refused"""
+    from video_asl_recognition_amd import _lib as L
+    size = lambda grad=0, **kw: L.lib.asl_linear_xent_workspace(C.byref(_xent(L, **kw)), FAKE, FAKE, grad)
+    big = 1 << 20
+    assert size(classes=1 << 15, d=big, ld_x=big, ld_w=big) == L.ASL_ETOOBIG
+    assert size(classes=1 << 14, d=big, ld_x=big, ld_w=big) > 0
+    # the most rows and classes there are: maxima and sums of a piece of rows, not of all
+    assert 0 < size(n=1 << 28, classes=1 << 21, d=8, ld_x=8, ld_w=8) < 4 << 30
+    assert 0 < size(grad=1, n=1 << 28, classes=1 << 21, d=8, ld_x=8, ld_w=8) < 16 << 30
+
+
 def _clip(L, n=2, numel=(8, 8), ptrs=(0x1000, 0x2000), types=(0, 0), out=(0x3000, 0x4000), otypes=(0, 0), max_norm=1.0, norm=FAKE,
           ws=FAKE):
     arr = lambda t, v: (t * len(v))(*v) if v is not None else None

@@ -548,7 +548,9 @@ struct XentPlan {
 };
 
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
-constexpr int kPieceRows = 1 << 17;               // and rows: what grids and per-tile numbers are sized by
+constexpr int kPieceRows = 1 << 17;               // and rows,
+constexpr long long kPieceSums = 1LL << 26;       // maxima and sums per tile,
+constexpr long long kPieceInputs = 1LL << 34;     // and elements of x: what grids are sized by
 
 inline int k_per_split(int k, int splits, int bk) { return ceil_div(ceil_div(k, splits), bk) * bk; }
 
@@ -604,7 +606,9 @@ XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, boo
     // (128 bytes off a power of two, which would put a tile's rows all in the same few channels: dx of 8192 x 32768 x 2048
     // takes 836 us with them and 906 without)
     q.ld_e = (long long)ceil_div(p.classes, q.tile) * q.tile + (q.tile > kTile ? 64 : 0);
-    long long rows = p.n < kPieceRows ? p.n : kPieceRows;
+    long long rows = p.n;
+    for (const long long most : {(long long)kPieceRows, kPieceSums / q.tiles / 256 * 256, kPieceInputs / p.d / 256 * 256})
+        if (rows > most) rows = most;
     if (grad) {
         const long long most = kPieceBytes / (q.ld_e * (q.wide ? 10 : q.esize)) / 256 * 256;
         if (rows > most) rows = most < 256 ? 256 : most;
@@ -663,22 +667,31 @@ int xent_check(const asl_xent_params* p) {
     if (p->reduction < ASL_REDUCE_NONE || p->reduction > ASL_REDUCE_MEAN) return ASL_EINVAL;
     if (p->ld_x < p->d || p->ld_w < p->d) return ASL_EINVAL;
     if (!(p->label_smoothing >= 0.f && p->label_smoothing <= 1.f)) return ASL_EINVAL;
-    // grids take one of their 65535 rows of workgroups per 64 classes
-    if (p->n > (1 << 28) || p->classes > (1 << 21) || p->d > (1 << 20)) return ASL_ETOOBIG;
+    // a launch is fewer than 2^32 threads: 2^24 workgroups, each with at least 64 x 64 results of a product
+    if (p->n > (1 << 28) || p->classes > (1 << 21) || p->d > (1 << 20) || (long long)p->classes * p->d > (1LL << 34)) return ASL_ETOOBIG;
     return ASL_OK;
 }
 
 // Rows of d elements at any alignment to rows of `per_row` 16-byte vectors of bf16, noughts behind d; fp32 to three planes of
-// them.
+// them.  Two matrices in one launch, or one (rows of the other: 0).
 template <typename T>
-__global__ __launch_bounds__(256) void xent_pack_kernel(const T* src, long long ld, int rows, int d, short* dst, int per_row) {
-    const long long vectors = (long long)rows * per_row;
-    for (long long v = blockIdx.x * 256LL + threadIdx.x; v < vectors; v += gridDim.x * 256LL) {
-        const long long r = v / per_row;
-        const int c = (int)(v - r * per_row) * 8;
-        const auto raw = load8_raw(src + r * ld + (c < d ? c : 0), d - c);
-        if constexpr (std::is_same<T, short>::value) *(bf16x8*)(dst + v * 8) = raw;
-        else store_planes(dst + v * 8, vectors * 8, widen(raw));
+struct XentPack {
+    const T* src[2];
+    short* dst[2];
+    long long ld[2];
+    int rows[2], d, per_row;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void xent_pack_kernel(const XentPack<T> a) {
+    const long long first = (long long)a.rows[0] * a.per_row, both = first + (long long)a.rows[1] * a.per_row;
+    for (long long w = blockIdx.x * 256LL + threadIdx.x; w < both; w += gridDim.x * 256LL) {
+        const bool two = w >= first;
+        const long long v = two ? w - first : w, r = v / a.per_row;
+        const int c = (int)(v - r * a.per_row) * 8;
+        const auto raw = load8_raw((two ? a.src[1] : a.src[0]) + r * (two ? a.ld[1] : a.ld[0]) + (c < a.d ? c : 0), a.d - c);
+        short* dst = (two ? a.dst[1] : a.dst[0]) + v * 8;
+        if constexpr (std::is_same<T, short>::value) *(bf16x8*)dst = raw;
+        else store_planes(dst, (two ? both - first : first) * 8, widen(raw));
     }
 }
 
@@ -708,24 +721,20 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
     all.mean = mean;
     const void* wk = w;                   // what the products read: the caller's tensors, or their copies
     long long ld_w = p.ld_w, ld_x = p.ld_x;
-    const auto pack = [&](const void* src, long long ld, int rows, void* dst) {
-        const long long vectors = rows * (q.ld_pack / 8);
-        hipLaunchKernelGGL((xent_pack_kernel<T>), dim3(ceil_div(vectors, 512) < 8192 ? ceil_div(vectors, 512) : 8192), dim3(256), 0, s,
-                           (const T*)src, ld, rows, p.d, (short*)dst, (int)(q.ld_pack / 8));
-    };
-    if (q.pieces && q.pack_w) {
-        pack(w, p.ld_w, p.classes, ws + q.wp);
-        wk = ws + q.wp;
-        ld_w = q.ld_pack;
-    }
+    if (q.pack_w) wk = ws + q.wp, ld_w = q.ld_pack;
     if (q.pack_x) ld_x = q.ld_pack;
     for (int piece = 0; piece < q.pieces; ++piece) {
         const int r0 = piece * q.rows, rows = p.n - r0 < q.rows ? p.n - r0 : q.rows;
         const T* xr = (const T*)x + r0 * p.ld_x;
-        if (q.pack_x) {
-            pack(xr, p.ld_x, rows, ws + q.xp);
-            xr = (const T*)(ws + q.xp);
+        if (q.pack_x || (q.pack_w && piece == 0)) {
+            XentPack<T> c = {};
+            if (q.pack_x) c.src[0] = xr, c.dst[0] = (short*)(ws + q.xp), c.ld[0] = p.ld_x, c.rows[0] = rows;
+            if (q.pack_w && piece == 0) c.src[1] = (const T*)w, c.dst[1] = (short*)(ws + q.wp), c.ld[1] = p.ld_w, c.rows[1] = p.classes;
+            c.d = p.d; c.per_row = (int)(q.ld_pack / 8);
+            const int blocks = ceil_div(((long long)c.rows[0] + c.rows[1]) * c.per_row, 512);
+            hipLaunchKernelGGL((xent_pack_kernel<T>), dim3(blocks < 8192 ? blocks : 8192), dim3(256), 0, s, c);
         }
+        if (q.pack_x) xr = (const T*)(ws + q.xp);
         XentGemm g = {};
         g.p = wk; g.ld_p = ld_w; g.q = xr; g.ld_q = ld_x; g.I = p.classes; g.Jn = rows; g.K = p.d; g.k_per_split = p.d;
         g.out = ws + q.e; g.ld_out = q.ld_e; g.bias = bias; g.bias_bf16 = p.bias_type; g.smooth = p.label_smoothing != 0.f;

@@ -34,8 +34,9 @@ namespace asl_detail {
 // each line twice (logits of the same: 1127 us against 1066).
 constexpr int step_depth(bool pkc, bool qkc) { return pkc || qkc ? 64 : 32; }
 
-// LDS of a tile kernel: the stages of both operands, 128 k in all; over them, behind the K loop, the results on their way out: all rows in
-// 16 bits, or 128 of them in 32 (padded, so that consecutive rows start in different banks); then a tile's bias and targets
+// LDS of a tile kernel: the stages of both operands, 128 k in all; over them, behind the K loop, the results on their way out:
+// all rows in 16 bits, or 128 of them in 32 (padded, so that consecutive rows start in different banks); then a tile's bias
+// and targets
 template <int TILE, int BK>
 struct TileLds {
     static constexpr int kStages = 128 / BK;
@@ -52,14 +53,13 @@ struct TileLds {
 // 1 KiB (16 bytes a lane) from a buffer into LDS at `lds` (wave-uniform).  Written out because the compiler, which knows
 // only that the builtin writes LDS somewhere, drains the whole queue ahead of the next transposing read; it has no result in
 // registers, and the kernel's own counted waits and barriers are what orders it (LDS addresses go through M0, which wants
-// one instruction between its write and its use;
-// nothing else in these kernels uses it).
+// one instruction between its write and its use; nothing else in these kernels uses it).
 template <int AT>
 __device__ __forceinline__ void dma_1k(i32x4 rsrc, unsigned voff, unsigned lds) {
     asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "n"(AT) : "scc");
 }
 
-// One operand's way from memory to registers.  Its two stages lie behind one another in LDS, so that a fragment's address is
+// One operand's way from memory to registers.  Its stages lie behind one another in LDS, so that a fragment's address is
 // one register and an immediate.
 template <int TILE, int BK, bool KC>
 struct Panel {
@@ -493,8 +493,8 @@ __global__ __launch_bounds__(256, TILE == 256 ? 1 : 2) void xent_tile_kernel(con
 // the CUs they fill them together.  (128 x 128 only: two bodies of the large tile in one kernel leave the compiler no way to
 // keep 256 accumulators where they are, and products that take it fill the CUs alone.)
 template <int TILE, bool WIDE>
-__global__ __launch_bounds__(256, 2) void xent_tile_pair_kernel(const XentGemm dx, const XentGemm dw, int dx_ti, int dx_tj,
-                                                                                  int dw_ti, int dw_tj, int dx_blocks) {
+__global__ __launch_bounds__(256, 2) void xent_tile_pair_kernel(const XentGemm dx, const XentGemm dw, int dx_ti, int dx_tj, int dw_ti, int dw_tj,
+                                                                int dx_blocks) {
 #if defined(__HIP_DEVICE_COMPILE__)
     if ((int)blockIdx.x < dx_blocks) tile_body<TILE, step_depth(false, true), false, true, false, WIDE>(dx, blockIdx.x, dx_ti, dx_tj);
     else tile_body<TILE, step_depth(false, false), false, false, false, WIDE>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
