@@ -9,6 +9,10 @@
 // the mean that was just found.  Backward keeps each lane's columns fixed while its group walks over rows, so the column
 // sums dw and db also stay in registers; a workgroup leaves one partial row of each in the workspace and a second launch
 // adds those up in a fixed order (no atomics: results do not vary from run to run).
+//
+// What bounds them is memory: 2^26 elements take, in bf16, 41 us forward and 76 us backward with rows of 1024 (x and y, or x,
+// dy and dx, at 6.5 and 5.3 TB/s, part of it from the 256 MB cache; a copy of 2 GiB reaches 4.95) and 46 and 79 us with rows
+// of 128 and 512, in fp32 102 to 112 us and 148 to 163 us with rows of 64 to 8192.  Small calls are two and three launches.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -159,6 +163,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const XT* xr = (const XT*)a.x + row * a.ld_x;
         float s[1] = {0.f};
+#pragma unroll 4
         for (int k = t * 8; k < a.d; k += G * 8) {
             const F8 x = load8(xr + k, a.d - k);
 #pragma unroll
@@ -167,6 +172,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
         group_sum<G>(s, lds, slot);
         const float mean = s[0] * inv_d;
         float q[2] = {0.f, 0.f};
+#pragma unroll 4
         for (int k = t * 8; k < a.d; k += G * 8) {
             const F8 x = load8(xr + k, a.d - k);
 #pragma unroll
@@ -180,6 +186,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
         const float rest = q[0] * inv_d;
         const float rstd = 1.0f / sqrtf(not_below_nought(q[1] * inv_d - rest * rest) + a.eps);
         YT* yr = (YT*)a.y + row * a.ld_y;
+#pragma unroll 4
         for (int k = t * 8; k < a.d; k += G * 8) {
             const F8 x = load8(xr + k, a.d - k);
             const F8 w = load8_or(a.w, a.w_bf16, k, a.d - k, 1.f), b = load8_or(a.b, a.w_bf16, k, a.d - k, 0.f);
@@ -195,22 +202,25 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
     }
 }
 
-template <typename XT, typename YT, int G, int J>
+// SUMS: with the column sums.  Rows too long for that (a lane's vectors, their sums and the next row's) leave them to
+// ln_cols_kernel.
+template <typename XT, typename YT, int G, int J, bool SUMS>
 __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs a) {
     constexpr int BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
-    constexpr bool HOLD = J <= 2 && G * J < 2048;
+    constexpr bool HOLD = J <= 2 && G * J < 2048, AHEAD = G * J < 4096;
     __shared__ float lds[2 * 2 * (G > 64 ? G / 64 : 1)];
     __shared__ __attribute__((aligned(16))) float cols[RPB > 1 ? 4 * 2 * (G < 64 ? G : 64) * 8 : 1];
     int slot = 0;
     const int t = threadIdx.x % G;
     const float inv_d = 1.0f / (float)a.d;
-    F8 w[HOLD ? J : 1], dw[J], db[J];
+    F8 w[HOLD ? J : 1], dw[SUMS ? J : 1], db[SUMS ? J : 1];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int k = (t + j * G) * 8;
         if constexpr (HOLD) w[j] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, a.d - k, 1.f);
+        if constexpr (SUMS)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dw[j].v[e] = db[j].v[e] = 0.f;
+            for (int e = 0; e < 8; ++e) dw[j].v[e] = db[j].v[e] = 0.f;
     }
     typename RawOf<XT>::type next_x[J];
     typename RawOf<YT>::type next_dy[J];
@@ -229,8 +239,9 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
     };
     const long long stride = (long long)gridDim.x * RPB;
     long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
-    if (row < a.rows) fetch(row);
+    if (AHEAD && row < a.rows) fetch(row);
     for (; row < a.rows; row += stride) {
+        if (!AHEAD) fetch(row);
         const float mean = next_mean, rstd = next_rstd;
         F8 h[J], g[J];
         float s[2] = {0.f, 0.f};
@@ -239,7 +250,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
             h[j] = widen(next_x[j]);
             g[j] = widen(next_dy[j]);
         }
-        if (row + stride < a.rows) fetch(row + stride);
+        if (AHEAD && row + stride < a.rows) fetch(row + stride);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int k = (t + j * G) * 8, n = a.d - k;
@@ -248,8 +259,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 h[j].v[e] = e < n ? (h[j].v[e] - mean) * rstd : 0.f;
-                dw[j].v[e] += g[j].v[e] * h[j].v[e];
-                db[j].v[e] += g[j].v[e];
+                if constexpr (SUMS) {
+                    dw[j].v[e] += g[j].v[e] * h[j].v[e];
+                    db[j].v[e] += g[j].v[e];
+                }
                 g[j].v[e] *= wj.v[e];
                 s[0] += g[j].v[e];
                 s[1] += g[j].v[e] * h[j].v[e];
@@ -270,7 +283,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
         }
     }
     float* part = a.part + (long long)blockIdx.x * 2 * a.d;
-    if constexpr (RPB == 1) {
+    if constexpr (!SUMS) {
+    } else if constexpr (RPB == 1) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int k = (t + j * G) * 8;
@@ -309,8 +323,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
     }
 }
 
-// rows longer than the registers of a workgroup: sums, then dx, from re-read rows; the column sums live in the workgroup's
-// partial row in memory, each element read and written by the one thread that owns it
+// rows longer than the registers of a workgroup: sums, then dx, from re-read rows
 template <typename XT, typename YT>
 __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
     constexpr int G = 1024;
@@ -318,35 +331,26 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
     int slot = 0;
     const int t = threadIdx.x;
     const float inv_d = 1.0f / (float)a.d;
-    float* part = a.part + (long long)blockIdx.x * 2 * a.d;
-    const F8 zero = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
-    for (int k = t * 8; k < a.d; k += G * 8) {
-        store8(part + k, a.d - k, zero);
-        store8(part + a.d + k, a.d - k, zero);
-    }
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const XT* xr = (const XT*)a.x + row * a.ld_x;
         const YT* dyr = (const YT*)a.dy + row * a.ld_dy;
         const float mean = a.mean[row], rstd = a.rstd[row];
         float s[2] = {0.f, 0.f};
+#pragma unroll 4
         for (int k = t * 8; k < a.d; k += G * 8) {
             const int n = a.d - k;
             const F8 x = load8(xr + k, n), dy = load8(dyr + k, n), w = load8_or(a.w, a.w_bf16, k, n, 1.f);
-            F8 pw = load8(part + k, n), pb = load8(part + a.d + k, n);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float h = (x.v[e] - mean) * rstd, g = dy.v[e] * w.v[e];     // dy is nought behind the row's end
-                pw.v[e] += dy.v[e] * h;
-                pb.v[e] += dy.v[e];
+                const float g = dy.v[e] * w.v[e];                // dy is nought behind the row's end
                 s[0] += g;
-                s[1] += g * h;
+                s[1] += g * ((x.v[e] - mean) * rstd);
             }
-            store8(part + k, n, pw);
-            store8(part + a.d + k, n, pb);
         }
         group_sum<G>(s, lds, slot);
         const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
         XT* dxr = (XT*)a.y + row * a.ld_y;
+#pragma unroll 4
         for (int k = t * 8; k < a.d; k += G * 8) {
             const int n = a.d - k;
             const F8 x = load8(xr + k, n), dy = load8(dyr + k, n), w = load8_or(a.w, a.w_bf16, k, n, 1.f);
@@ -355,6 +359,53 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
             for (int e = 0; e < 8; ++e) o.v[e] = (dy.v[e] * w.v[e] - m0 - (x.v[e] - mean) * rstd * m1) * rstd;
             store8(dxr + k, n, o);
         }
+    }
+}
+
+// The column sums of long rows from a second reading: 512 columns a workgroup, its four waves on rows in turn, four rows at a
+// time on their way; blockIdx.y-th of the partial rows.
+template <typename XT, typename YT>
+__global__ __launch_bounds__(256) void ln_cols_kernel(const LnArgs a) {
+    constexpr int U = 4;
+    __shared__ __attribute__((aligned(16))) float cols[2][4][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int k = (blockIdx.x * 64 + lane) * 8, n = a.d - k;
+    F8 dw, db;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw.v[e] = db.v[e] = 0.f;
+    const long long stride = gridDim.y * 4LL;
+    for (long long row = blockIdx.y * 4LL + wave; row < a.rows; row += stride * U) {
+        typename RawOf<XT>::type x[U];
+        typename RawOf<YT>::type dy[U];
+        float mean[U], rstd[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool there = row + u * stride < a.rows;
+            const long long r = there ? row + u * stride : row;
+            x[u] = load8_raw((const XT*)a.x + r * a.ld_x + (n > 0 ? k : 0), n);
+            dy[u] = load8_raw((const YT*)a.dy + r * a.ld_dy + (n > 0 ? k : 0), there ? n : 0);
+            mean[u] = a.mean[r];
+            rstd[u] = a.rstd[r];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool there = row + u * stride < a.rows;
+            const F8 h = widen(x[u]), g = widen(dy[u]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (there) dw.v[e] += g.v[e] * ((h.v[e] - mean[u]) * rstd[u]);
+                if (there) db.v[e] += g.v[e];
+            }
+        }
+    }
+    store8_full(&cols[0][wave][lane * 8], dw);
+    store8_full(&cols[1][wave][lane * 8], db);
+    __syncthreads();
+    float* part = a.part + (long long)blockIdx.y * 2 * a.d;
+    for (int i = threadIdx.x; i < 1024; i += 256) {
+        const int which = i >> 9, c = i & 511;
+        if (blockIdx.x * 512 + c < a.d)
+            part[which * (long long)a.d + blockIdx.x * 512 + c] = (cols[which][0][c] + cols[which][1][c]) + (cols[which][2][c] + cols[which][3][c]);
     }
 }
 
@@ -401,23 +452,30 @@ int column_sums(const float* part, int parts, long long ld, long long cols, long
     return (int)hipGetLastError();
 }
 
-// Lanes a row and vectors a lane, by the row's length.  Forward holds one row (8 J registers), so a wave takes up to 2048
-// elements; backward holds x, dy and two column sums (32 J registers), so a wave takes up to 2048 as well, at two a SIMD.
+// Lanes a row and vectors a lane, by the row's length.  Forward holds one row and the next (16 J registers), so a wave takes
+// up to 2048 elements; backward holds x, dy, two column sums and the next row's (48 J registers), so a wave takes up to 2048 as
+// well, at two a SIMD.  2^26 elements in bf16: rows of 200 on 16 lanes 48 and 83 us, on a wave that they leave more than half
+// idle 95 and 165.  Rows above 8192: forward holds them with 256 threads up to 16384 (68 us, with 1024 threads 110), and reads
+// longer ones three times, twice from the L2 (79 us; from the registers of 1024 threads, whose rows do not overlap, the same).
+// Backward has no registers left for the column sums: from a second reading of x and dy, rows of 12288 take 131 us, with sums
+// that spill 232; rows of 32768 162 us, with sums kept in memory 350.
 struct LnShape {
     int g, j;
 };
 inline LnShape fwd_shape(int d) {
     if (d <= 128) return {16, 1};
+    if (d <= 256) return {16, 2};
     if (d <= 512) return {64, 1};
     if (d <= 1024) return {64, 2};
     if (d <= 2048) return {64, 4};
     if (d <= 4096) return {256, 2};
     if (d <= 8192) return {256, 4};
-    if (d <= 32768) return {1024, 4};
+    if (d <= 16384) return {256, 8};
     return {0, 0};
 }
 inline LnShape bwd_shape(int d) {
     if (d <= 128) return {16, 1};
+    if (d <= 256) return {16, 2};
     if (d <= 512) return {64, 1};
     if (d <= 1024) return {64, 2};
     if (d <= 2048) return {64, 4};
@@ -426,11 +484,16 @@ inline LnShape bwd_shape(int d) {
     if (d <= 16384) return {1024, 2};
     return {0, 0};
 }
+constexpr int kColsWith = 8192;           // longest row whose column sums go along
 inline int rows_per_block(int g) { return g == 0 || g > 256 ? 1 : 256 / g; }
 
 // workgroups of a backward call = partial rows of its column sums: a few a CU, so that the partial rows stay small
 // against the tensors
 inline int bwd_blocks(int rows, int d) {
+    if (d > kColsWith) {                  // ln_cols_kernel: eight workgroups a CU, each of at least 16 rows
+        const int strips = (d + 511) / 512, most = strips < 2048 ? 2048 / strips : 1, need = (int)(((long long)rows + 15) / 16);
+        return need < most ? need : most;
+    }
     const int rpb = rows_per_block(bwd_shape(d).g);
     const long long need = ((long long)rows + rpb - 1) / rpb;
     return (int)(need < 512 ? need : 512);
@@ -442,33 +505,38 @@ int launch_fwd(const LnArgs& a, hipStream_t s) {
     const int rpb = rows_per_block(sh.g);
     const long long need = ((long long)a.rows + rpb - 1) / rpb;
     const dim3 grid((unsigned)(need < 4096 ? need : 4096)), b256(256), b1024(1024);
-    switch (sh.g * 8 + sh.j) {
-        case 16 * 8 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 16, 1>), grid, b256, 0, s, a); break;
-        case 64 * 8 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
-        case 64 * 8 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
-        case 64 * 8 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 4>), grid, b256, 0, s, a); break;
-        case 256 * 8 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
-        case 256 * 8 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 4>), grid, b256, 0, s, a); break;
-        case 1024 * 8 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 1024, 4>), grid, b1024, 0, s, a); break;
+    switch (sh.g * 16 + sh.j) {
+        case 16 * 16 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 16, 1>), grid, b256, 0, s, a); break;
+        case 16 * 16 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 16, 2>), grid, b256, 0, s, a); break;
+        case 64 * 16 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
+        case 64 * 16 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
+        case 64 * 16 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 4>), grid, b256, 0, s, a); break;
+        case 256 * 16 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
+        case 256 * 16 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 4>), grid, b256, 0, s, a); break;
+        case 256 * 16 + 8: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 8>), grid, b256, 0, s, a); break;
         default: hipLaunchKernelGGL((ln_fwd_long_kernel<XT, YT>), grid, b1024, 0, s, a); break;
     }
     return (int)hipGetLastError();
 }
 
 template <typename XT, typename YT>
-int launch_bwd(const LnArgs& a, int blocks, hipStream_t s) {
+int launch_bwd(const LnArgs& a, int blocks, bool want_cols, hipStream_t s) {
     const LnShape sh = bwd_shape(a.d);
-    const dim3 grid((unsigned)blocks), b256(256), b1024(1024);
-    switch (sh.g * 8 + sh.j) {
-        case 16 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 16, 1>), grid, b256, 0, s, a); break;
-        case 64 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
-        case 64 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
-        case 64 * 8 + 4: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 4>), grid, b256, 0, s, a); break;
-        case 256 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
-        case 1024 * 8 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 1>), grid, b1024, 0, s, a); break;
-        case 1024 * 8 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 2>), grid, b1024, 0, s, a); break;
+    const bool apart = a.d > kColsWith;
+    const dim3 grid((unsigned)(!apart ? blocks : a.rows < 4096 ? a.rows : 4096)), b256(256), b1024(1024);
+    switch (sh.g * 16 + sh.j) {
+        case 16 * 16 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 16, 1, true>), grid, b256, 0, s, a); break;
+        case 16 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 16, 2, true>), grid, b256, 0, s, a); break;
+        case 64 * 16 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 1, true>), grid, b256, 0, s, a); break;
+        case 64 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 2, true>), grid, b256, 0, s, a); break;
+        case 64 * 16 + 4: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 4, true>), grid, b256, 0, s, a); break;
+        case 256 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 2, true>), grid, b256, 0, s, a); break;
+        case 1024 * 16 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 1, true>), grid, b1024, 0, s, a); break;
+        case 1024 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 2, false>), grid, b1024, 0, s, a); break;
         default: hipLaunchKernelGGL((ln_bwd_long_kernel<XT, YT>), grid, b1024, 0, s, a); break;
     }
+    if (apart && want_cols)
+        hipLaunchKernelGGL((ln_cols_kernel<XT, YT>), dim3((unsigned)((a.d + 511) / 512), (unsigned)blocks), b256, 0, s, a);
     return (int)hipGetLastError();
 }
 
@@ -523,8 +591,9 @@ extern "C" int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, 
         a.x = x; a.dy = dy; a.w = gamma; a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.part = workspace;
         a.ld_x = p->ld_x; a.ld_y = p->ld_dx; a.ld_dy = p->ld_y; a.rows = p->rows; a.d = p->d; a.w_bf16 = p->w_type;
         int e;
-        if (p->x_type) e = p->y_type ? launch_bwd<short, short>(a, blocks, s) : launch_bwd<short, float>(a, blocks, s);
-        else e = p->y_type ? launch_bwd<float, short>(a, blocks, s) : launch_bwd<float, float>(a, blocks, s);
+        const bool cols = dgamma || dbeta;
+        if (p->x_type) e = p->y_type ? launch_bwd<short, short>(a, blocks, cols, s) : launch_bwd<short, float>(a, blocks, cols, s);
+        else e = p->y_type ? launch_bwd<float, short>(a, blocks, cols, s) : launch_bwd<float, float>(a, blocks, cols, s);
         if (e) return e;
     }
     if (dgamma || dbeta)
