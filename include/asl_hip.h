@@ -475,8 +475,9 @@ enum { ASL_F32 = 0, ASL_BF16 = 1 };
  *   dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy      (NULL: not wanted; written as w_type)
  * x [rows][ld_x] and dx [rows][ld_dx] are of x_type, y and dy [rows][ld_y] of y_type, gamma and beta of w_type.  mean and
  * rstd are fp32 [rows]; forward takes NULL for either.  The places between d and a row's stride are left alone.  rows == 0
- * is a call like any other (dgamma and dbeta are nought).  Backward needs `workspace`, 16-byte aligned, of
- * asl_layernorm_bwd_workspace(p) bytes (a negative return is an ASL_E* code). */
+ * is a call like any other (dgamma and dbeta are nought); d above 2^26 returns ASL_ETOOBIG.  Outputs overlap neither each
+ * other nor an input.  Backward needs `workspace`, 16-byte aligned, of asl_layernorm_bwd_workspace(p) bytes (a negative return
+ * is an ASL_E* code). */
 typedef struct asl_layernorm_params {
     int32_t rows, d;
     int64_t ld_x, ld_y, ld_dx;

@@ -38,6 +38,15 @@ def test_layernorm_refuses(kw):
     assert L.lib.asl_layernorm_bwd_workspace(C.byref(p)) == L.ASL_EINVAL
 
 
+def test_layernorm_refuses_what_no_grid_holds():
+    from video_asl_recognition_amd import _lib as L
+    p = _norm(L, d=(1 << 26) + 1, ld_x=1 << 27, ld_y=1 << 27, ld_dx=1 << 27)
+    assert L.lib.asl_layernorm_fwd(C.byref(p), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == L.ASL_ETOOBIG
+    assert L.lib.asl_layernorm_bwd_workspace(C.byref(p)) == L.ASL_ETOOBIG
+    p = _norm(L, rows=(1 << 31) - 1, d=1 << 26, ld_x=1 << 27, ld_y=1 << 27, ld_dx=1 << 27)
+    assert 0 < L.lib.asl_layernorm_bwd_workspace(C.byref(p)) <= 1 << 30
+
+
 def test_layernorm_refuses_pointers():
     from video_asl_recognition_amd import _lib as L
     p = _norm(L)

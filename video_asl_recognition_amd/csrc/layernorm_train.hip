@@ -411,21 +411,20 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const LnArgs a) {
 
 // 64 columns a workgroup of 1024: 16 lanes of four columns by 64 row strides, so that the up to 512 partial rows, which other
 // XCDs have just written and which come from memory, are all on their way at once
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ part, int parts, long long ld, long long cols,
-                                                           long long split, void* out0, void* out1, int bf16, const float* factor) {
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ part, int parts, int d, void* dw, void* db, int bf16) {
     __shared__ float s[64][64 + 1];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-    const long long c0 = (long long)blockIdx.x * 64 + c * 4;
+    const long long cols = 2LL * d, c0 = (long long)blockIdx.x * 64 + c * 4;
     const int n = cols - c0 >= 4 ? 4 : cols > c0 ? (int)(cols - c0) : 0;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (n == 4) {
 #pragma unroll 8
-        for (int p = r; p < parts; p += 64) v += *(const f32x4u*)(part + p * ld + c0);
+        for (int p = r; p < parts; p += 64) v += *(const f32x4u*)(part + p * cols + c0);
     } else if (n) {
         for (int p = r; p < parts; p += 64)
 #pragma unroll
             for (int e = 0; e < 3; ++e)
-                if (e < n) v[e] += part[p * ld + c0 + e];
+                if (e < n) v[e] += part[p * cols + c0 + e];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[r][c * 4 + e] = v[e];
@@ -435,21 +434,13 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restri
     const float o = row16_sum((s[q][k] + s[q + 16][k]) + (s[q + 32][k] + s[q + 48][k]));
     const long long col = (long long)blockIdx.x * 64 + k;
     if (q == 0 && col < cols) {
-        void* out = col < split ? out0 : out1;
-        const long long at = col < split ? col : col - split;
-        const float f = factor ? o * *factor : o;
+        void* out = col < d ? dw : db;
+        const long long at = col < d ? col : col - d;
         if (out) {
-            if (bf16) store1((short*)out + at, f);
-            else store1((float*)out + at, f);
+            if (bf16) store1((short*)out + at, o);
+            else store1((float*)out + at, o);
         }
     }
-}
-
-int column_sums(const float* part, int parts, long long ld, long long cols, long long split, void* out0, void* out1, int bf16,
-                const float* factor, hipStream_t s) {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, s, part, parts, ld, cols, split, out0, out1,
-                       bf16, factor);
-    return (int)hipGetLastError();
 }
 
 // Lanes a row and vectors a lane, by the row's length.  Forward holds one row and the next (16 J registers), so a wave takes
@@ -541,10 +532,10 @@ int launch_bwd(const LnArgs& a, int blocks, bool want_cols, hipStream_t s) {
 }
 
 int ln_check(const asl_layernorm_params* p) {
-    if (!p || p->rows < 0 || p->d <= 0 || p->d > (1 << 30)) return ASL_EINVAL;
+    if (!p || p->rows < 0 || p->d <= 0) return ASL_EINVAL;
     if (p->x_type < 0 || p->x_type > 1 || p->w_type < 0 || p->w_type > 1 || p->y_type < 0 || p->y_type > 1) return ASL_EINVAL;
     if (p->ld_x < p->d || p->ld_y < p->d || p->ld_dx < p->d) return ASL_EINVAL;
-    return ASL_OK;
+    return p->d > (1 << 26) ? ASL_ETOOBIG : ASL_OK;       // a launch is fewer than 2^32 threads: 1024 per 64 column sums
 }
 inline bool misaligned(const void* p, int type) { return ((uintptr_t)p & (type ? 1 : 3)) != 0; }
 
@@ -569,7 +560,8 @@ extern "C" int asl_layernorm_fwd(const asl_layernorm_params* p, const void* x, c
 }
 
 extern "C" int64_t asl_layernorm_bwd_workspace(const asl_layernorm_params* p) {
-    if (ln_check(p) != ASL_OK) return ASL_EINVAL;
+    const int rc = ln_check(p);
+    if (rc != ASL_OK) return rc;
     return (int64_t)bwd_blocks(p->rows, p->d) * 2 * p->d * (int64_t)sizeof(float);
 }
 
@@ -597,6 +589,7 @@ extern "C" int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, 
         if (e) return e;
     }
     if (dgamma || dbeta)
-        return column_sums(workspace, blocks, 2LL * p->d, 2LL * p->d, p->d, dgamma, dbeta, p->w_type, nullptr, s);
+        hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((2LL * p->d + 63) / 64)), dim3(1024), 0, s, workspace, blocks, p->d, dgamma, dbeta,
+                           p->w_type);
     return (int)hipGetLastError();
 }

@@ -236,9 +236,8 @@ __device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int
     }
 }
 
-template <typename T, bool LOGITS>
-__global__ __launch_bounds__(256) void xent_gemm_kernel(const XentGemm a, int ti, int tj) {
-    static_assert(LOGITS, "the gradient products go in pairs");
+template <typename T>
+__global__ __launch_bounds__(256) void xent_gemm_logits_kernel(const XentGemm a, int ti, int tj) {
     gemm_body<T, true, true, true>(a, blockIdx.x, ti, tj);
 }
 
@@ -747,7 +746,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             if (rc) return rc;
         } else {
             const int tj = ceil_div(rows, kTile);
-            hipLaunchKernelGGL((xent_gemm_kernel<T, true>), dim3((unsigned)(q.tiles * tj)), dim3(256), 0, s, g, q.tiles, tj);
+            hipLaunchKernelGGL((xent_gemm_logits_kernel<T>), dim3((unsigned)(q.tiles * tj)), dim3(256), 0, s, g, q.tiles, tj);
         }
         XentRows r = {};
         r.st.target = target + r0; r.st.upstream = upstream && none ? upstream + r0 : nullptr;

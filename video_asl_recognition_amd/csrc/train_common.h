@@ -205,9 +205,4 @@ __device__ __forceinline__ F8 load8_any(const void* base, int bf16, long long at
     return bf16 ? load8((const short*)base + at, n) : load8((const float*)base + at, n);
 }
 
-// Column sums of partial rows [parts][ld], added up in a fixed order: columns [0, split) to out0, [split, cols) to out1 (null:
-// not wanted), times *factor where that is given (layernorm_train.hip).
-int column_sums(const float* part, int parts, long long ld, long long cols, long long split, void* out0, void* out1, int bf16,
-                const float* factor, hipStream_t s);
-
 }  // namespace asl_detail
