@@ -295,7 +295,8 @@ def test_linear_cross_entropy_large_tiles(gpu, n, v, d):
     _xent_check(x, w, b, t, smooth=0.1, reduction="sum", what="large, smoothed")
 
 
-@pytest.mark.parametrize("n,v,d", [(256, 8192, 64), (300, 8211, 72), (1100, 1003, 200), (2100, 6000, 33), (64, 70000, 64)])
+@pytest.mark.parametrize("n,v,d", [(256, 8192, 64), (300, 8211, 72), (1100, 1003, 200), (2100, 6000, 33), (64, 70000, 64), (256, 33000, 72),
+                                   (1100, 1003, 520), (2100, 6000, 63), (300, 8211, 264)])
 def test_linear_cross_entropy_large_fp32(gpu, n, v, d):
     """sizes that take fp32 apart into bf16 planes: held to the bounds of fp32 products"""
     x, w, b, t = _xent_case(n, v, d, F32, F32, 0.1)
@@ -380,8 +381,9 @@ def test_linear_cross_entropy_masks_and_labels(gpu):
 
 
 # one size for each way the products are computed: few rows, 64 x 64 tiles, 128 x 128, 256 x 256, fp32 as planes of bf16
-PATHS = [(20, 300, 40, BF16), (20, 300, 40, F32), (80, 300, 64, BF16), (80, 300, 64, F32), (400, 1000, 128, BF16), (400, 1003, 77, BF16),
-         (1000, 8200, 256, BF16), (520, 9001, 136, BF16), (600, 1100, 260, F32), (1100, 8200, 65, F32)]
+PATHS = [(12, 300, 40, BF16), (20, 300, 40, F32), (80, 60, 64, BF16), (80, 300, 20, BF16), (80, 300, 64, F32), (600, 1100, 260, F32),
+         (20, 300, 40, BF16), (80, 300, 64, BF16), (400, 1000, 128, BF16), (400, 1003, 77, BF16), (1000, 8200, 256, BF16),
+         (520, 9001, 136, BF16), (600, 4100, 260, F32), (1100, 8200, 65, F32), (9000, 250, 64, BF16)]
 PATH_IDS = [f"{n}x{v}x{d}-{'f32' if dt == F32 else 'bf16'}" for n, v, d, dt in PATHS]
 
 

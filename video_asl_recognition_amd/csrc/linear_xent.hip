@@ -8,8 +8,8 @@
 //
 // The logits are never held.  Rows are taken in pieces; the product x W^T leaves, for every row and every tile of classes, the
 // tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself (fp32, or for bf16 operands
-// fp16 of 2^15 times it: 11 bits of the value down to 2^-29 of the tile's largest, and 2^-40 of that below).  One pass over the per-tile numbers gives lse, the loss and
-// the factors g exp(m - lse); one pass over the exponentials turns them into G in place, the target's entry from its own
+// fp16 of 2^15 times it: 11 bits of the value down to 2^-29 of the tile's largest, and 2^-40 of that below).  One pass over the
+// per-tile numbers gives lse, the loss and the factors g exp(m - lse); one pass over the exponentials turns them into G in place, the target's entry from its own
 // 32-bit logit (g expm1(l_t - lse), where p - 1 of a rounded p would cancel), and adds up db in 32 bits.  Then two products.
 //
 // Both gradient products have operands whose contraction index is not the contiguous one; see the tile kernels.
@@ -254,73 +254,131 @@ struct XentRows {
     float* factor;                        // with gradients: [rows][tiles] g exp(m - lse); may be the maxima themselves
     float* target_g;                      // G at the target
     float* row_g;                         // g (label smoothing's even part)
-    float* loss;
+    float* loss;                          // each null: not wanted
     float* lse;
+    float* loss_part;                     // a workgroup's rows' losses and
+    int* kept_part;                       // those that carry a label
     float exp_unit;                       // one over the scale the exponentials are held at
 };
 
-// one wave a row: statistics, loss, and the factors that turn exp(l - m) into G
-__global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= a.st.rows) return;
-    const XentRow r = row_stats<64>(a.st, row, lane);
-    if (lane == 0) {
-        a.loss[row] = r.loss;
-        if (a.lse) a.lse[row] = r.lse;
-        if (a.factor) {
-            a.target_g[row] = r.target_g;
-            a.row_g[row] = r.g;
-        }
+// the losses of a workgroup's N rows, one a thread `at` of them, to one partial sum
+template <int N>
+__device__ __forceinline__ void leave_part(const XentRows& a, long long part, float (&loss)[N], int (&kept)[N]) {
+    __syncthreads();
+    if (threadIdx.x == 0 && a.loss_part) {
+        float v = 0.f;
+        int k = 0;
+#pragma unroll
+        for (int r = 0; r < N; ++r) v += loss[r], k += kept[r];
+        a.loss_part[part] = v;
+        a.kept_part[part] = k;
     }
-    if (a.factor)
-        for (int t = lane; t < a.st.tiles; t += 64) {
-            const long long at = (long long)row * a.st.tiles + t;
-            a.factor[at] = r.valid ? r.g * a.exp_unit * expf(a.st.tile_max[at] - r.lse) : NAN;
-        }
 }
 
-// What concerns all of a call's rows, by one workgroup: the loss (the rows' sum, or their mean over those that carry a label;
-// none of them: 0 / 0), and the factor c of the gradients.
-struct XentAll {
-    const long long* target;
-    const float* loss_rows;               // null: the loss is not this launch's business
+// A wave a row, or a quarter of one: statistics, loss, and the factors that turn exp(l - m) into G.
+template <int LANES>
+__global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
+    constexpr int N = 256 / LANES;
+    __shared__ float loss[N];
+    __shared__ int kept[N];
+    const int at = threadIdx.x / LANES, row = blockIdx.x * N + at, lane = threadIdx.x % LANES;
+    if (row < a.st.rows) {
+        const XentRow r = row_stats<LANES>(a.st, row, lane);
+        if (lane == 0) {
+            loss[at] = r.loss;
+            kept[at] = a.st.target[row] != a.st.ignore;
+            if (a.loss) a.loss[row] = r.loss;
+            if (a.lse) a.lse[row] = r.lse;
+            if (a.factor) {
+                a.target_g[row] = r.target_g;
+                a.row_g[row] = r.g;
+            }
+        }
+        if (a.factor)
+            for (int t = lane; t < a.st.tiles; t += LANES) {
+                const long long k = (long long)row * a.st.tiles + t;
+                a.factor[k] = r.valid ? r.g * a.exp_unit * expf(a.st.tile_max[k] - r.lse) : NAN;
+            }
+    } else if (lane == 0) {
+        loss[at] = 0.f;
+        kept[at] = 0;
+    }
+    leave_part(a, blockIdx.x, loss, kept);
+}
+
+// What concerns all of a call's rows, each by one workgroup: the loss from the partial sums, and the factor c of the gradients
+// from the targets, or from counts of them where there are many.
+struct XentLoss {
+    const float* loss_part;               // null: not this launch's business
+    const int* kept_part;
     float* loss;
+    int parts, mean;
+};
+struct XentFactor {
+    const long long* target;
+    const int* counts;                    // of kCountRows rows each; null: none were taken
     const float* upstream;                // null: 1
-    float* factor;                        // null: not this launch's
+    float* factor;                        // null: not this launch's business
     long long ignore;
     int n, mean;
 };
+constexpr int kCountRows = 8192;          // rows up to which one workgroup counts them on its way (65536 rows of 100 classes and 512
+                                          // features with gradients: 102 us with a launch that counts them, 172 without)
 
-__device__ __forceinline__ void over_all_rows(const XentAll& a) {
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+__device__ __forceinline__ int block_sum(int v, int* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+__device__ __forceinline__ int count_kept(const long long* target, int n, long long ignore, int* lds) {
+    int kept = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += 256) kept += target[i] != ignore;
+    return block_sum(kept, lds);
+}
+
+// the rows' sum, or their mean over those that carry a label (none of them: 0 / 0)
+__device__ __forceinline__ void finish_loss(const XentLoss& a) {
     __shared__ float lf[4];
     __shared__ int li[4];
     float v = 0.f;
     int kept = 0;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < a.n; i += 256) {
-        kept += a.target[i] != a.ignore;
-        if (a.loss_rows) v += a.loss_rows[i];
+    for (int i = threadIdx.x; i < a.parts; i += 256) v += a.loss_part[i], kept += a.kept_part[i];
+    v = block_sum(v, lf);
+    kept = block_sum(kept, li);
+    if (threadIdx.x == 0) *a.loss = a.mean ? v / (float)kept : v;
+}
+__device__ __forceinline__ void set_factor(const XentFactor& a) {
+    __shared__ int li[4];
+    int kept = 0;
+    if (a.mean && a.counts) {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < (a.n + kCountRows - 1) / kCountRows; i += 256) kept += a.counts[i];
+        kept = block_sum(kept, li);
+    } else if (a.mean) {
+        kept = count_kept(a.target, a.n, a.ignore, li);
     }
-    v = wave_sum(v);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) kept += __shfl_xor(kept, o, 64);
-    if ((threadIdx.x & 63) == 0) {
-        lf[threadIdx.x >> 6] = v;
-        li[threadIdx.x >> 6] = kept;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        v = lf[0] + lf[1] + lf[2] + lf[3];
-        kept = li[0] + li[1] + li[2] + li[3];
-        if (a.loss_rows) *a.loss = a.mean ? v / (float)kept : v;
-        if (a.factor) {
-            const float up = a.upstream ? *a.upstream : 1.f;
-            *a.factor = !a.mean ? up : kept ? up / (float)kept : 0.f;      // no row with a label: gradients are nought
-        }
-    }
+    const float up = a.upstream ? *a.upstream : 1.f;
+    if (threadIdx.x == 0) *a.factor = !a.mean ? up : kept ? up / (float)kept : 0.f;      // no row with a label: gradients are nought
 }
 
-__global__ __launch_bounds__(256) void xent_loss_kernel(const XentAll a) { over_all_rows(a); }
+__global__ __launch_bounds__(256) void xent_loss_kernel(const XentLoss a) { finish_loss(a); }
+
+__global__ __launch_bounds__(256) void xent_count_kernel(const long long* target, int n, long long ignore, int* counts) {
+    __shared__ int li[4];
+    const int first = blockIdx.x * kCountRows, left = n - first < kCountRows ? n - first : kCountRows;
+    const int kept = count_kept(target + first, left, ignore, li);
+    if (threadIdx.x == 0) counts[blockIdx.x] = kept;
+}
 
 constexpr int kGradRows = 32;             // rows a workgroup of the G pass takes; it leaves one partial row of db
 constexpr int kGradCols = 256;            // and columns
@@ -335,7 +393,8 @@ struct XentG {
     int tile_shift, db_add;
     short* planes;                        // not null: G goes here, as three bf16 planes
     long long plane;
-    XentAll all;
+    XentLoss loss;
+    XentFactor factor;
 };
 
 __device__ __forceinline__ F8 load8_exp(const float* p) { return load8_full(p); }
@@ -374,7 +433,8 @@ template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
     constexpr int R = kGradRows / 8, TPB = kGradCols / kTile;
     __shared__ __attribute__((aligned(16))) float cols[8][kGradCols];
-    __shared__ float own_f[OWN ? kGradRows : 1][TPB], own_tg[OWN ? kGradRows : 1], own_g[OWN ? kGradRows : 1];
+    __shared__ float own_f[OWN ? kGradRows : 1][TPB], own_tg[OWN ? kGradRows : 1], own_g[OWN ? kGradRows : 1], own_loss[kGradRows];
+    __shared__ int own_kept[kGradRows];
     const XentStats& st = a.rows.st;
     const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = (long long)blockIdx.x * kGradCols + lane * 8;
@@ -402,21 +462,29 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
         const int l16 = threadIdx.x & 15, blocks = kGradCols >> a.tile_shift;
 #pragma unroll
         for (int k = threadIdx.x >> 4; k < kGradRows; k += 16) {               // sixteen rows at once
-            if (b0 + k >= st.rows) continue;
+            if (b0 + k >= st.rows) {
+                if (l16 == 0) own_loss[k] = 0.f, own_kept[k] = 0;
+                continue;
+            }
             const XentRow q = row_stats<16>(st, b0 + k, l16);
             if (l16 == 0) {
                 own_tg[k] = q.target_g;
                 own_g[k] = q.g;
+                own_loss[k] = q.loss;
+                own_kept[k] = st.target[b0 + k] != st.ignore;
                 if (blockIdx.x == 0) {
-                    a.rows.loss[b0 + k] = q.loss;
+                    if (a.rows.loss) a.rows.loss[b0 + k] = q.loss;
                     if (a.rows.lse) a.rows.lse[b0 + k] = q.lse;
                 }
             }
             const int tile = blockIdx.x * blocks + l16;
             if (l16 < blocks)
-                own_f[k][l16] = tile >= st.tiles ? 0.f : q.valid ? q.g * a.rows.exp_unit * expf(st.tile_max[(long long)(b0 + k) * st.tiles + tile] - q.lse) : NAN;
+                own_f[k][l16] = tile >= st.tiles ? 0.f
+                                : q.valid        ? q.g * a.rows.exp_unit * expf(st.tile_max[(long long)(b0 + k) * st.tiles + tile] - q.lse)
+                                                 : NAN;
         }
-        __syncthreads();
+        if (blockIdx.x == 0) leave_part(a.rows, blockIdx.y, own_loss, own_kept);
+        else __syncthreads();
 #pragma unroll
         for (int u = 0; u < R; ++u) {
             f[u] = own_f[rl + u * 8][(lane * 8) >> a.tile_shift];
@@ -453,7 +521,10 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
             *o = v;
         }
     }
-    if (blockIdx.x == 0 && blockIdx.y == 0 && (a.all.factor || a.all.loss_rows)) over_all_rows(a.all);
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        if (a.factor.factor) set_factor(a.factor);
+        if (a.loss.loss_part) finish_loss(a.loss);
+    }
 }
 
 // What is left when the products are done, in one launch: slabs of partial sums added up in their order, partial rows of db,
@@ -471,7 +542,7 @@ struct XentFinish {
     long long ld_db;
     int groups, classes, db_bf16, db_blocks;
     const float* factor;
-    XentAll all;                          // with loss_rows: by the last workgroup
+    XentLoss loss;                        // by the last workgroup
 };
 constexpr int kSlabPerBlock = 256 * 8 * 2;       // results a workgroup
 
@@ -532,7 +603,7 @@ __global__ __launch_bounds__(256) void xent_finish_kernel(const XentFinish a) {
         }
         return;
     }
-    over_all_rows(a.all);
+    finish_loss(a.loss);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -543,7 +614,7 @@ struct XentPlan {
     long long ld_e, ld_pack;
     bool dw_slabs, pack_x, pack_w, wide, few;
     // workspace offsets, bytes
-    long long shared, loss, lse, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, gp, total;
+    long long shared, loss, kept, counts, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, gp, total;
 };
 
 constexpr long long kPieceBytes = 1LL << 30;      // of exponentials held at a time
@@ -560,16 +631,25 @@ inline bool lies_well(const void* t, long long ld, int d) {
 
 inline long long slab_ld(int d, int tile) { return (long long)ceil_div(d, tile) * tile; }
 
+// Up to 32 rows of fp32 the products run as in xent_few.hip (32 x 2000 x 512 with gradients 28 us, on 64 x 64 tiles 46), of
+// bf16 up to 16 and with a small weight (8 x 2000 x 512 22 us, on 128 x 128 tiles 24; 8 x 8000 x 2048 84, 64; 32 x 2000 x 512
+// 31, 27).
+inline bool takes_few(const asl_xent_params& p) {
+    if (!p.n || p.classes > kFewClasses) return false;
+    return p.type ? p.n <= 16 && (double)p.classes * p.d <= (double)(1 << 20) : p.n <= kFewRows;
+}
+
 // Tile and slices of a product with `a` x `b` results over `k`: what its tiles take one after another on the 256 CUs, against
 // what slabs of partial sums cost (written and read back at 4 TB/s, and one more launch).  Measured with one workgroup a CU:
 // 1.65 us per 64 of k for 256 x 256, 0.65 for 128 x 128, 0.4 for 64 x 64 (fp32: 0.6), and about 8, 5 and 3 us around that a
-// tile.  Products too narrow for the larger tiles, and fp32 ones too small to be worth taking apart into planes (128 M
-// multiplications: 512 x 512 x 512), take 64 x 64.
+// tile.  Products too narrow for the larger tiles take 64 x 64, and so do fp32 ones not worth being taken apart into planes:
+// of few rows, where W's planes cost most (128 x 32768 x 1024 with gradients 315 us, in planes 378; 256 rows 577 and 505), or
+// small (512 x 2000 x 512 70 us, 74; 1024 rows 104, 93).
 struct TilePlan {
     int tile, splits;
 };
 inline TilePlan tiles_for(const asl_xent_params& p, long long a, long long b, int k, bool may_split) {
-    const bool narrow = p.n < 64 || p.classes < 64 || p.d < 32 || (!p.type && (double)p.n * p.classes * p.d < (double)(1 << 27));
+    const bool narrow = p.classes < 64 || p.d < 32 || (!p.type && (p.n < 256 || (double)p.n * p.classes * p.d < (double)(1 << 29)));
     TilePlan best = {kTile, 1};
     double least = 1e30;
     const int steps = ceil_div(k, 64);
@@ -592,7 +672,7 @@ inline TilePlan tiles_for(const asl_xent_params& p, long long a, long long b, in
 XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, bool grad, bool want_dx, bool want_dw, bool want_db) {
     XentPlan q = {};
     q.esize = p.type ? 2 : 4;
-    q.few = p.n && p.n <= kFewRows && p.classes <= kFewClasses;
+    q.few = takes_few(p);
     q.tile = q.few ? kFewTile : tiles_for(p, p.n, p.classes, p.d, false).tile;
     q.tile_shift = q.tile == 256 ? 7 : 6;                // maxima and sums are kept per 128 classes, or 64
     // the tile kernels read 16 bytes at a time and whole steps of 64 k: operands that do not allow it are laid out anew
@@ -639,8 +719,9 @@ XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, boo
         return r;
     };
     q.shared = take(4);
-    q.loss = take(4LL * p.n);
-    q.lse = take(4LL * p.n);
+    q.loss = take(4LL * ceil_div(p.n, 4));               // (partial sums of 4, 16 or 32 rows)
+    q.kept = take(4LL * ceil_div(p.n, 4));
+    q.counts = take(p.n > kCountRows ? 4LL * ceil_div(p.n, kCountRows) : 0);
     q.tmax = take(4LL * rows * q.tiles);
     q.tsum = take(4LL * rows * q.tiles);
     q.tlin = take(p.label_smoothing != 0.f ? 4LL * rows * q.tiles : 0);
@@ -713,11 +794,15 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
              hipStream_t s) {
     const int bk = q.wide ? Mma<short>::BK : Mma<T>::BK;
     const bool none = p.reduction == ASL_REDUCE_NONE, mean = p.reduction == ASL_REDUCE_MEAN;
-    float* loss_rows = none ? loss : (float*)(ws + q.loss);
     float* shared = (float*)(ws + q.shared);
-    XentAll all = {};
-    all.target = target; all.loss = loss; all.upstream = none ? nullptr : upstream; all.ignore = p.ignore_index; all.n = p.n;
-    all.mean = mean;
+    // the rows' statistics by the G pass, or by a launch of their own, a wave or a quarter of one each
+    const bool own = grad && q.tiles <= kOwnStats;
+    const int per_part = own ? kGradRows : q.tiles <= kOwnStats ? 16 : 4;
+    XentLoss all = {(const float*)(ws + q.loss), (const int*)(ws + q.kept), loss, ceil_div(p.n, per_part), mean};
+    int* counts = p.n > kCountRows ? (int*)(ws + q.counts) : nullptr;
+    XentFactor factor = {target, counts, none ? nullptr : upstream, shared, p.ignore_index, p.n, mean};
+    if (grad && mean && counts)
+        hipLaunchKernelGGL(xent_count_kernel, dim3((unsigned)ceil_div(p.n, kCountRows)), dim3(256), 0, s, target, p.n, factor.ignore, counts);
     const void* wk = w;                   // what the products read: the caller's tensors, or their copies
     long long ld_w = p.ld_w, ld_x = p.ld_x;
     if (q.pack_w) wk = ws + q.wp, ld_w = q.ld_pack;
@@ -754,14 +839,17 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         r.st.ignore = p.ignore_index; r.st.smoothing = p.label_smoothing; r.st.inv_classes = 1.f / (float)p.classes;
         r.st.rows = rows; r.st.classes = p.classes; r.st.tiles = q.tiles;
         r.factor = grad ? g.tile_max : nullptr; r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
-        r.loss = loss_rows + r0; r.lse = lse ? lse + r0 : nullptr; r.exp_unit = 1.f / Mma<T>::SCALE;
-        const bool own = grad && q.tiles <= kOwnStats, last = piece == q.pieces - 1;
-        if (!own) hipLaunchKernelGGL(xent_rows_kernel, dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
+        r.loss = none ? loss + r0 : nullptr; r.lse = lse ? lse + r0 : nullptr; r.exp_unit = 1.f / Mma<T>::SCALE;
+        if (!none) r.loss_part = (float*)(ws + q.loss) + r0 / per_part, r.kept_part = (int*)(ws + q.kept) + r0 / per_part;
+        const bool last = piece == q.pieces - 1;
+        if (!own && per_part == 16) hipLaunchKernelGGL((xent_rows_kernel<16>), dim3(ceil_div(rows, 16)), dim3(256), 0, s, r);
+        else if (!own) hipLaunchKernelGGL((xent_rows_kernel<64>), dim3(ceil_div(rows, 4)), dim3(256), 0, s, r);
         if (!grad) continue;
         XentG c = {};
         c.rows = r; c.e = ws + q.e; c.ld = q.ld_e; c.planes = q.wide ? (short*)(ws + q.gp) : nullptr; c.plane = rows * q.ld_e;
         c.db_part = db ? (float*)(ws + q.dbp) : nullptr; c.db_add = piece > 0; c.tile_shift = q.tile_shift;
-        c.all = all; c.all.loss_rows = !none && last && !own ? loss_rows : nullptr; c.all.factor = piece == 0 ? shared : nullptr;
+        if (!none && last && !own) c.loss = all;
+        if (piece == 0) c.factor = factor;
         const int groups = ceil_div(rows, kGradRows);
         const dim3 g_grid(ceil_div(q.ld_e, kGradCols), groups);
         if (own) hipLaunchKernelGGL((xent_g_kernel<T, true>), g_grid, dim3(256), 0, s, c);
@@ -808,15 +896,12 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             f.db_blocks = ceil_div(p.classes, 64);
         }
         f.factor = shared;
-        f.all = all; f.all.loss_rows = !none && last && own ? loss_rows : nullptr;
-        const long long blocks = (long long)f.dx.blocks + f.dw.blocks + f.db_blocks + (f.all.loss_rows ? 1 : 0);
+        if (!none && last && own) f.loss = all;
+        const long long blocks = (long long)f.dx.blocks + f.dw.blocks + f.db_blocks + (f.loss.loss_part ? 1 : 0);
         if (blocks > 0x7fffffffLL) return ASL_ETOOBIG;
         if (blocks) hipLaunchKernelGGL((xent_finish_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, f);
     }
-    if (!none && (!grad || !q.pieces)) {
-        all.loss_rows = loss_rows;
-        hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, s, all);
-    }
+    if (!none && (!grad || !q.pieces)) hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, s, all);
     return (int)hipGetLastError();
 }
 
