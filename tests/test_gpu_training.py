@@ -189,7 +189,8 @@ def test_layer_norm_autograd_and_differences(gpu):
 # ------------------------------------------------------------------------------------------------ Linear + cross entropy
 XENT_SIZES = [(1, 1, 1), (1, 2, 3), (2, 31, 5), (16, 2000, 512), (17, 33, 65), (32, 1000, 130), (33, 1000, 130), (3, 16384, 70), (3, 16385, 20),
               (20, 4500, 300), (8, 2000, 512), (5, 100, 64), (65, 63, 33), (64, 64, 64), (130, 257, 100), (300, 1000, 70),
-              (257, 129, 513), (16, 5003, 129)]
+              (257, 129, 513), (16, 5003, 129),
+              (40, 1, 1), (40, 3, 2), (5000, 2, 3), (300, 130, 9), (12000, 70, 31)]
 
 
 def xent_reference(x, w, b, t, up, ignore, smooth, reduction, bf16):
@@ -380,7 +381,7 @@ def test_linear_cross_entropy_masks_and_labels(gpu):
             assert dw.isnan().all()
 
 
-# one size for each way the products are computed: few rows, 64 x 64 tiles, 128 x 128, 256 x 256, fp32 as planes of bf16
+# sizes for each way the products are computed: few rows, fp32 on 64 x 64 tiles, 128 x 128 and 256 x 256, fp32 as bf16 planes
 PATHS = [(12, 300, 40, BF16), (20, 300, 40, F32), (80, 60, 64, BF16), (80, 300, 20, BF16), (80, 300, 64, F32), (600, 1100, 260, F32),
          (20, 300, 40, BF16), (80, 300, 64, BF16), (400, 1000, 128, BF16), (400, 1003, 77, BF16), (1000, 8200, 256, BF16),
          (520, 9001, 136, BF16), (600, 4100, 260, F32), (1100, 8200, 65, F32), (9000, 250, 64, BF16)]

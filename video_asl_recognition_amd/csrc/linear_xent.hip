@@ -21,49 +21,32 @@
 
 namespace asl_detail {
 
+// how exp(l - m) is held, times SCALE
 template <typename T>
-struct Mma;
+struct Held;
 template <>
-struct Mma<short> {
-    static constexpr int BK = 64, PAD = 8, KSTEP = 32;
-    using Frag = bf16x8;
-    static __device__ __forceinline__ Frag frag(const short* row, int k0, int q) { return *(const bf16x8*)(row + k0 + q * 8); }
-    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-#else
-        return c;
-#endif
-    }
-    static __device__ __forceinline__ float exp_(float v) { return __expf(v); }
-    using Exp = _Float16;                 // how exp(l - m) is held, times SCALE
+struct Held<short> {
+    using Exp = _Float16;
     static constexpr float SCALE = kExpScale16;
 };
 template <>
-struct Mma<float> {
-    static constexpr int BK = 32, PAD = 4, KSTEP = 4;
-    using Frag = float;
-    static __device__ __forceinline__ Frag frag(const float* row, int k0, int q) { return row[k0 + q]; }
-    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-        return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-#else
-        return c;
-#endif
-    }
-    static __device__ __forceinline__ float exp_(float v) { return expf(v); }
+struct Held<float> {
     using Exp = float;
     static constexpr float SCALE = 1.f;
 };
 
-constexpr int kTile = 64;                 // of either index in the general kernel
+// fp32 products that are not worth being taken apart into bf16 planes: 64 x 64 tiles on the fp32 MFMA (16 x 16 x 4), any sizes,
+// strides and alignment.  The matrix pipe's fp32 rate (133 TF/s as a library product reaches it) bounds large ones, a step's
+// round trip to memory the small ones that come here: 300 x 300 x 300 with gradients 42 us, 512 x 2000 x 512 70 us.  Steps of
+// 32 k and of 64 take the same time (500 x 300 x 200: 13.6 and 14.1 us for the logits).
+constexpr int kTile = 64, kStep = 32;     // of either index, and of k
 
-// one thread's share of a 64 x BK operand tile: held in registers while the previous tile is multiplied
-template <typename T, bool KC>
+// one thread's share of a 64 x 32 operand tile: held in registers while the previous tile is multiplied
+template <bool KC>
 struct Stage {
-    static constexpr int BK = Mma<T>::BK, LD = BK + Mma<T>::PAD, N = kTile * BK / 8 / 256;
+    static constexpr int BK = kStep, LD = BK + 4, N = kTile * BK / 8 / 256;
     F8 r[N];
-    __device__ __forceinline__ void load(const T* base, long long ld, int row0, int rows, int k0, int k1) {
+    __device__ __forceinline__ void load(const float* base, long long ld, int row0, int rows, int k0, int k1) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int v = u * 256 + threadIdx.x;
@@ -75,7 +58,7 @@ struct Stage {
             r[u] = load8(base + (n > 0 ? srow * ld + scol : 0), n);
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void store(float* lds) const {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int v = u * 256 + threadIdx.x;
@@ -84,18 +67,18 @@ struct Stage {
             } else {
                 const int k = v / (kTile / 8), i = (v % (kTile / 8)) * 8;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) store1(lds + (i + e) * LD + k, r[u].v[e]);
+                for (int e = 0; e < 8; ++e) lds[(i + e) * LD + k] = r[u].v[e];
             }
         }
     }
 };
 
-// Any sizes, strides and alignment.  Four waves, 32 x 32 of the tile each.  Workgroup `id` of ti * tj * splits.
-template <typename T, bool PKC, bool QKC, bool LOGITS>
+// Four waves, 32 x 32 of the tile each.  Workgroup `id` of ti * tj * splits.
+template <bool PKC, bool QKC, bool LOGITS>
 __device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int tj) {
-    constexpr int BK = Mma<T>::BK, LD = BK + Mma<T>::PAD, KSTEP = Mma<T>::KSTEP;
-    __shared__ __attribute__((aligned(16))) T lp[kTile * LD];
-    __shared__ __attribute__((aligned(16))) T lq[kTile * LD];
+    constexpr int BK = kStep, LD = BK + 4;
+    __shared__ __attribute__((aligned(16))) float lp[kTile * LD];
+    __shared__ __attribute__((aligned(16))) float lq[kTile * LD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
     const int bi = id % ti, bj = id / ti % tj, slice = id / (ti * tj), i0 = bi * kTile, j0 = bj * kTile;
@@ -105,30 +88,30 @@ __device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Stage<T, PKC> sp;
-    Stage<T, QKC> sq;
-    sp.load((const T*)a.p, a.ld_p, i0, a.I, kb, ke);
-    sq.load((const T*)a.q, a.ld_q, j0, a.Jn, kb, ke);
+    Stage<PKC> sp;
+    Stage<QKC> sq;
+    sp.load((const float*)a.p, a.ld_p, i0, a.I, kb, ke);
+    sq.load((const float*)a.q, a.ld_q, j0, a.Jn, kb, ke);
     for (int k = kb; k < ke; k += BK) {
         sp.store(lp);
         sq.store(lq);
         __syncthreads();
         if (k + BK < ke) {
-            sp.load((const T*)a.p, a.ld_p, i0, a.I, k + BK, ke);
-            sq.load((const T*)a.q, a.ld_q, j0, a.Jn, k + BK, ke);
+            sp.load((const float*)a.p, a.ld_p, i0, a.I, k + BK, ke);
+            sq.load((const float*)a.q, a.ld_q, j0, a.Jn, k + BK, ke);
         }
 #pragma unroll
-        for (int ks = 0; ks < BK; ks += KSTEP) {
-            typename Mma<T>::Frag fp[2], fqv[2];
+        for (int ks = 0; ks < BK; ks += 4) {
+            float fp[2], fqv[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                fp[u] = Mma<T>::frag(lp + (wi + u * 16 + fr) * LD, ks, fq);
-                fqv[u] = Mma<T>::frag(lq + (wj + u * 16 + fr) * LD, ks, fq);
+                fp[u] = lp[(wi + u * 16 + fr) * LD + ks + fq];
+                fqv[u] = lq[(wj + u * 16 + fr) * LD + ks + fq];
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = Mma<T>::mma(fp[i], fqv[j], acc[i][j]);
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma4(fp[i], fqv[j], acc[i][j]);
         }
         __syncthreads();
     }
@@ -150,7 +133,7 @@ __device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int
                         float* o = (float*)a.out + ((long long)slice * a.Jn + j) * ld + i + e;
                         *o = a.add ? *o + acc[u][v][e] : acc[u][v][e];
                     } else {
-                        store1((T*)a.out + j * a.ld_out + i + e, acc[u][v][e] * c);
+                        ((float*)a.out)[j * a.ld_out + i + e] = acc[u][v][e] * c;
                     }
                 }
             }
@@ -200,19 +183,16 @@ __device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int i = i0 + wi + u * 16 + fq * 4;
-                F8 o;
+                f32x4 x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float l = acc[u][v][e], x = Mma<T>::exp_(l - ref);
+                    const float l = acc[u][v][e];
+                    x[e] = expf(l - ref);
                     if (a.smooth && i + e < a.I) lin += l;
-                    s += x;
-                    o.v[e] = x;
+                    s += x[e];
                 }
-                if (a.store_e && j < a.Jn) {                 // the exponentials' rows are padded to whole tiles
-                    typename Mma<T>::Exp* er = (typename Mma<T>::Exp*)a.out + j * a.ld_out + i;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) er[e] = (typename Mma<T>::Exp)(o.v[e] * Mma<T>::SCALE);
-                }
+                // the exponentials' rows are padded to whole tiles
+                if (a.store_e && j < a.Jn) *(f32x4*)((float*)a.out + j * a.ld_out + i) = x;
             }
             s += __shfl_xor(s, 16, 64);
             s += __shfl_xor(s, 32, 64);
@@ -236,17 +216,15 @@ __device__ __forceinline__ void gemm_body(const XentGemm& a, int id, int ti, int
     }
 }
 
-template <typename T>
 __global__ __launch_bounds__(256) void xent_gemm_logits_kernel(const XentGemm a, int ti, int tj) {
-    gemm_body<T, true, true, true>(a, blockIdx.x, ti, tj);
+    gemm_body<true, true, true>(a, blockIdx.x, ti, tj);
 }
 
 // dx and dW in one launch, dx's workgroups first
-template <typename T>
 __global__ __launch_bounds__(256) void xent_gemm_pair_kernel(const XentGemm dx, const XentGemm dw, int dx_ti, int dx_tj, int dw_ti, int dw_tj,
                                                              int dx_blocks) {
-    if ((int)blockIdx.x < dx_blocks) gemm_body<T, false, true, false>(dx, blockIdx.x, dx_ti, dx_tj);
-    else gemm_body<T, false, false, false>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
+    if ((int)blockIdx.x < dx_blocks) gemm_body<false, true, false>(dx, blockIdx.x, dx_ti, dx_tj);
+    else gemm_body<false, false, false>(dw, blockIdx.x - dx_blocks, dw_ti, dw_tj);
 }
 
 struct XentRows {
@@ -448,7 +426,7 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
         const int r = r0 + u * 8 < st.rows ? r0 + u * 8 : st.rows - 1;
         t[u] = st.target[r];
         if (in) {
-            g[u] = load8_exp((const typename Mma<T>::Exp*)a.e + r * a.ld + col);
+            g[u] = load8_exp((const typename Held<T>::Exp*)a.e + r * a.ld + col);
             // (columns of a last, half empty 256 x 256 tile lie behind the last block of maxima)
             const int tile = (int)(col >> a.tile_shift);
             if (!OWN) f[u] = tile < st.tiles ? a.rows.factor[(long long)r * st.tiles + tile] : 0.f;
@@ -641,22 +619,24 @@ inline bool takes_few(const asl_xent_params& p) {
 
 // Tile and slices of a product with `a` x `b` results over `k`: what its tiles take one after another on the 256 CUs, against
 // what slabs of partial sums cost (written and read back at 4 TB/s, and one more launch).  Measured with one workgroup a CU:
-// 1.65 us per 64 of k for 256 x 256, 0.65 for 128 x 128, 0.4 for 64 x 64 (fp32: 0.6), and about 8, 5 and 3 us around that a
-// tile.  Products too narrow for the larger tiles take 64 x 64, and so do fp32 ones not worth being taken apart into planes:
-// of few rows, where W's planes cost most (128 x 32768 x 1024 with gradients 315 us, in planes 378; 256 rows 577 and 505), or
-// small (512 x 2000 x 512 70 us, 74; 1024 rows 104, 93).
+// 1.65 us per 64 of k for 256 x 256, 0.65 for 128 x 128 (fp32 in planes: six times that), 0.6 for 64 x 64, and about 8, 5 and 3
+// us around that a tile.  bf16 takes the larger two, however narrow (2000 x 50 x 64 with gradients 25 us, on 64 x 64 tiles of
+// bf16 29; 100000 x 30 x 128 145 and 262).  fp32 takes 64 x 64 where taking it apart into planes does not pay: narrow products
+// (100000 x 30 x 512 504 us, in planes 578; 100000 x 1000 x 16 985, 1123), few rows, for which W's planes cost most (128 x
+// 32768 x 1024 315, 378; 256 rows 577, 505), and small ones (512 x 2000 x 512 70, 74; 1024 rows 104, 93).
 struct TilePlan {
     int tile, splits;
 };
 inline TilePlan tiles_for(const asl_xent_params& p, long long a, long long b, int k, bool may_split) {
-    const bool narrow = p.classes < 64 || p.d < 32 || (!p.type && (p.n < 256 || (double)p.n * p.classes * p.d < (double)(1 << 29)));
+    const bool whole = !p.type && (p.classes < 64 || p.d < 32 || p.n < 256 || (double)p.n * p.classes * p.d < (double)(1 << 29));
     TilePlan best = {kTile, 1};
     double least = 1e30;
     const int steps = ceil_div(k, 64);
     for (const int tile : {64, 128, 256}) {
-        if (narrow != (tile == 64)) continue;
+        if (whole != (tile == 64)) continue;
         const long long tiles = (long long)ceil_div(a, tile) * ceil_div(b, tile);
-        const double us = tile == 256 ? 1.65 : tile == 128 ? 0.65 : p.type ? 0.4 : 0.6, around = tile == 256 ? 8.0 : tile == 128 ? 5.0 : 3.0;
+        const double us = tile == 256 ? 1.65 : tile == 128 ? 0.65 : 0.6;
+        const double around = tile == 256 ? 8.0 : tile == 128 ? 5.0 : 3.0;
         for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || s * 2 <= steps); ++s) {
             const double t = ceil_div(tiles * s, 256) * (ceil_div(steps, s) * us * (p.type || tile == 64 ? 1 : 6) + around) +
                              (s > 1 ? 3.0 + s * (double)a * b * 8.0 / 4e6 : 0.0);
@@ -695,7 +675,7 @@ XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, boo
     q.rows = (int)rows;
     q.pieces = p.n ? ceil_div(p.n, rows) : 0;
     q.row_groups = ceil_div(rows, kGradRows);
-    const int bk = p.type || q.wide ? Mma<short>::BK : Mma<float>::BK;
+    const int bk = q.tile > kTile ? 64 : kStep;
     q.dx_splits = q.dw_splits = 1;
     q.dx_tile = q.dw_tile = kTile;
     if (grad && p.n) {
@@ -792,7 +772,7 @@ template <typename T>
 int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void* x, const void* w, const void* bias,
              const long long* target, const float* upstream, float* loss, float* lse, void* dx, void* dw, void* db, char* ws,
              hipStream_t s) {
-    const int bk = q.wide ? Mma<short>::BK : Mma<T>::BK;
+    const int bk = q.tile > kTile ? 64 : kStep;
     const bool none = p.reduction == ASL_REDUCE_NONE, mean = p.reduction == ASL_REDUCE_MEAN;
     float* shared = (float*)(ws + q.shared);
     // the rows' statistics by the G pass, or by a launch of their own, a wave or a quarter of one each
@@ -831,7 +811,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             if (rc) return rc;
         } else {
             const int tj = ceil_div(rows, kTile);
-            hipLaunchKernelGGL((xent_gemm_logits_kernel<T>), dim3((unsigned)(q.tiles * tj)), dim3(256), 0, s, g, q.tiles, tj);
+            hipLaunchKernelGGL(xent_gemm_logits_kernel, dim3((unsigned)(q.tiles * tj)), dim3(256), 0, s, g, q.tiles, tj);
         }
         XentRows r = {};
         r.st.target = target + r0; r.st.upstream = upstream && none ? upstream + r0 : nullptr;
@@ -839,7 +819,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         r.st.ignore = p.ignore_index; r.st.smoothing = p.label_smoothing; r.st.inv_classes = 1.f / (float)p.classes;
         r.st.rows = rows; r.st.classes = p.classes; r.st.tiles = q.tiles;
         r.factor = grad ? g.tile_max : nullptr; r.target_g = (float*)(ws + q.tg); r.row_g = (float*)(ws + q.rg);
-        r.loss = none ? loss + r0 : nullptr; r.lse = lse ? lse + r0 : nullptr; r.exp_unit = 1.f / Mma<T>::SCALE;
+        r.loss = none ? loss + r0 : nullptr; r.lse = lse ? lse + r0 : nullptr; r.exp_unit = 1.f / Held<T>::SCALE;
         if (!none) r.loss_part = (float*)(ws + q.loss) + r0 / per_part, r.kept_part = (int*)(ws + q.kept) + r0 / per_part;
         const bool last = piece == q.pieces - 1;
         if (!own && per_part == 16) hipLaunchKernelGGL((xent_rows_kernel<16>), dim3(ceil_div(rows, 16)), dim3(256), 0, s, r);
@@ -875,7 +855,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
             const int xi = ceil_div(p.d, kTile), xj = dx ? ceil_div(rows, kTile) : 0, wj = dw ? ceil_div(p.classes, kTile) : 0;
             const int nx = xi * xj * q.dx_splits, nw = xi * wj * q.dw_splits;
             if (nx + nw)
-                hipLaunchKernelGGL((xent_gemm_pair_kernel<T>), dim3((unsigned)(nx + nw)), dim3(256), 0, s, hx, hw, xi, xj, xi, wj, nx);
+                hipLaunchKernelGGL(xent_gemm_pair_kernel, dim3((unsigned)(nx + nw)), dim3(256), 0, s, hx, hw, xi, xj, xi, wj, nx);
         } else if (dx && dw && q.dx_tile == 128 && q.dw_tile == 128) {
             rc = xent_tiles_pair(hx, hw, s);
         } else {

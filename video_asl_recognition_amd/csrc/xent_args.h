@@ -1,4 +1,4 @@
-// What the two product kernels of the cross entropy operator share (linear_xent.hip, xent_tiles.hip).
+// What the cross entropy operator's files share (linear_xent.hip, xent_tiles.hip, xent_few.hip).
 #pragma once
 #include "train_common.h"
 
@@ -32,12 +32,21 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 constexpr float kExpScale16 = 32768.f;    // exponentials in (0, 1] held as fp16: times this, so that fp16's range is used
 
-// xent_tiles.hip, tile 128 or 256: bf16 (or fp32 as planes of it), both operands' rows on 16 bytes and at most 2^21 bytes apart; those contiguous along
-// k hold noughts from K to the next multiple of 64
+// xent_tiles.hip, tile 128 or 256: bf16 (or fp32 as planes of it), both operands' rows on 16 bytes and at most 2^21 bytes
+// apart; those contiguous along k hold noughts from K to the next multiple of 64
 int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s);
 int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s);     // P along its own index, Q along k
 int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s);     // both along their own index
 int xent_tiles_pair(const XentGemm& dx, const XentGemm& dw, hipStream_t s);     // both, on 128 x 128 tiles
+
+// 16 x 16 x 4 in fp32
+__device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+#else
+    return c;
+#endif
+}
 
 // What the products leave of a piece of rows, and what becomes of it.
 struct XentStats {

@@ -16,14 +16,6 @@
 
 namespace asl_detail {
 
-__device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-#else
-    return c;
-#endif
-}
-
 // A workgroup takes 32 classes; its four waves take every fourth 16 k and meet in LDS.  NB: 16-row halves of the batch.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void xent_few_logits_kernel(const XentFew a) {
