@@ -16,8 +16,13 @@
 // fp32 operands come as three bf16 planes, x = h + m + l to all its 24 bits (rounded to nearest one after the other), and the
 // contraction runs over six pairs of planes, h l + l h + m m + h m + m h + h h, smallest first.  What is left out, m l + l m +
 // l l, is below 2^-23 of the product of the absolute values at worst and 2^-25 of it in the mean: the fp32 sums' own
-// rounding.  Six bf16 products still take less than half the time of one fp32 product on this card's matrix pipe (2048 x 8192
-// x 1024 with gradients: see linear_xent.hip).
+// rounding.  Six bf16 products still take less time than one fp32 product on this card's matrix pipe (2048 x 8192 x 1024: 170 us
+// each, 203 TFLOP/s; a library's fp32 product 134 TFLOP/s).
+//
+// Measured, 8192 x 32768 x 2048 (1.10 PFLOP a product): logits 1016 to 1067 us (1.03 to 1.08 PFLOP/s), dx 826 to 847 (1.30 to
+// 1.33), dW 794 to 826 (1.33 to 1.38); a library's plain products of the same shapes 1.20, 1.12 and 0.99 PFLOP/s.  The gradient
+// products keep the matrix pipe 87 % busy at the clock that its power leaves it; a logits tile adds 8 us of exponentials and
+// 6 us of first loads to 32 steps of 1.6 us, alone on its CU.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -76,6 +76,11 @@ def _ptr(t: Optional[torch.Tensor]):
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _like(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """contiguous, of t's shape; empty_like, where it keeps the strides anyway, is the cheaper call"""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def _bytes(n: int, what: str) -> int:
     if n < 0:
         L.check(int(n), what)
@@ -103,7 +108,7 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Option
     d, xt, wt = _check_norm(x, weight, bias)
     index = _device(x, weight=weight, bias=bias)
     x2 = _rows(x)
-    y = x.new_empty(x.shape, dtype=out_dtype)
+    y = _like(x, out_dtype)
     mean, rstd = x.new_empty((2,) + x.shape[:-1], dtype=torch.float32).unbind(0)
     w = weight.contiguous() if weight is not None else None
     b = bias.contiguous() if bias is not None else None
@@ -125,7 +130,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
             raise ValueError(f"{name} must be float32 {tuple(x.shape[:-1])}, got {t.dtype} {tuple(t.shape)}")
     x2, dy2, mean, rstd = _rows(x), _rows(dy), mean.contiguous(), rstd.contiguous()
     w = weight.contiguous() if weight is not None else None
-    dx = x.new_empty(x.shape)
+    dx = _like(x)
     dw, db = x.new_empty((2, d), dtype=weight.dtype if weight is not None else torch.float32).unbind(0)
     p = L.LayerNormParams(x2.shape[0], d, _ld(x2), _ld(dy2), d, xt, wt, _type(dy, "dy"), 0.0)
     ws = x.new_empty(_bytes(L.lib.asl_layernorm_bwd_workspace(C.byref(p)), "layer_norm_bwd"), dtype=torch.uint8)
@@ -205,9 +210,9 @@ def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torc
 def _xent_grad(x, weight, target, bias, upstream, ignore_index, label_smoothing, reduction, want):
     index, x2, w2, t, b, p = _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction)
     loss = x.new_empty(target.shape if reduction == "none" else (), dtype=torch.float32)
-    dx = x.new_empty(x.shape) if want[0] else None
-    dw = x.new_empty(weight.shape) if want[1] else None
-    db = x.new_empty(bias.shape, dtype=bias.dtype) if want[2] and bias is not None else None
+    dx = _like(x) if want[0] else None
+    dw = _like(weight) if want[1] else None
+    db = _like(bias) if want[2] and bias is not None else None
     ws = x.new_empty(_bytes(L.lib.asl_linear_xent_workspace(C.byref(p), x2.data_ptr(), w2.data_ptr(), 1), "linear_cross_entropy"),
                      dtype=torch.uint8)
     # a 0-row "none" loss has no storage: the entry point wants an address all the same and writes nothing there
@@ -330,8 +335,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
                out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensor for tensor, fp32 or bf16 each, of
     the same strides or both contiguous: bf16 gradients into an optimizer's fp32 buffers in the same pass), and returns the
-    norm they had.  A tensor may not be
-    listed twice.  NaN in, NaN out."""
+    norm they had.  Tensors that are written may not overlap, each other or a gradient that is not their own.  NaN in, NaN out."""
     return _clip(grads, max_norm, norm_type, out)
 
 
