@@ -443,10 +443,10 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restri
     }
 }
 
-// Lanes a row and vectors a lane, by the row's length.  Forward holds one row and the next (16 J registers), so a wave takes
-// up to 2048 elements; backward holds x, dy, two column sums and the next row's (48 J registers), so a wave takes up to 2048 as
-// well, at two a SIMD.  2^26 elements in bf16: rows of 200 on 16 lanes 48 and 83 us, on a wave that they leave more than half
-// idle 95 and 165.  Rows above 8192: forward holds them with 256 threads up to 16384 (68 us, with 1024 threads 110), and reads
+// Lanes a row and vectors a lane, by the row's length.  Forward holds one row and the next (16 J registers), backward x, dy, two
+// column sums and the next row's (48 J).  2^26 elements in bf16, forward and backward: rows of 200 on 16 lanes 48 and 83 us, on
+// a wave that they leave more than half idle 95 and 165; rows of 2048 on four waves 45 and 79 us, on one wave, which then has
+// a SIMD to itself but for one other, 50 and 90.  Rows above 8192: forward holds them with 256 threads up to 16384 (68 us, with 1024 threads 110), and reads
 // longer ones three times, twice from the L2 (79 us; from the registers of 1024 threads, whose rows do not overlap, the same).
 // Backward has no registers left for the column sums: from a second reading of x and dy, rows of 12288 take 131 us, with sums
 // that spill 232; rows of 32768 162 us, with sums kept in memory 350.
@@ -458,7 +458,7 @@ inline LnShape fwd_shape(int d) {
     if (d <= 256) return {16, 2};
     if (d <= 512) return {64, 1};
     if (d <= 1024) return {64, 2};
-    if (d <= 2048) return {64, 4};
+    if (d <= 2048) return {256, 1};
     if (d <= 4096) return {256, 2};
     if (d <= 8192) return {256, 4};
     if (d <= 16384) return {256, 8};
@@ -469,7 +469,7 @@ inline LnShape bwd_shape(int d) {
     if (d <= 256) return {16, 2};
     if (d <= 512) return {64, 1};
     if (d <= 1024) return {64, 2};
-    if (d <= 2048) return {64, 4};
+    if (d <= 2048) return {256, 1};
     if (d <= 4096) return {256, 2};
     if (d <= 8192) return {1024, 1};
     if (d <= 16384) return {1024, 2};
@@ -478,16 +478,19 @@ inline LnShape bwd_shape(int d) {
 constexpr int kColsWith = 8192;           // longest row whose column sums go along
 inline int rows_per_block(int g) { return g == 0 || g > 256 ? 1 : 256 / g; }
 
-// workgroups of a backward call = partial rows of its column sums: a few a CU, so that the partial rows stay small
-// against the tensors
-inline int bwd_blocks(int rows, int d) {
+// workgroups of a backward call = partial rows of its column sums: two a CU, so that the partial rows stay small against the
+// tensors, or four where a workgroup has but one row under way, of less than 8 KB of x and dy (2^26 elements, bf16 rows of
+// 1280: 85 us, with two 116; fp32 143 with two, 157 with four)
+inline int bwd_blocks(const asl_layernorm_params& p) {
+    const int rows = p.rows, d = p.d;
     if (d > kColsWith) {                  // ln_cols_kernel: eight workgroups a CU, each of at least 16 rows
         const int strips = (d + 511) / 512, most = strips < 2048 ? 2048 / strips : 1, need = (int)(((long long)rows + 15) / 16);
         return need < most ? need : most;
     }
-    const int rpb = rows_per_block(bwd_shape(d).g);
+    const LnShape sh = bwd_shape(d);
+    const int rpb = rows_per_block(sh.g), most = sh.g == 256 && sh.j == 1 && d * ((p.x_type ? 2 : 4) + (p.y_type ? 2 : 4)) < 8192 ? 1024 : 512;
     const long long need = ((long long)rows + rpb - 1) / rpb;
-    return (int)(need < 512 ? need : 512);
+    return (int)(need < most ? need : most);
 }
 
 template <typename XT, typename YT>
@@ -501,7 +504,7 @@ int launch_fwd(const LnArgs& a, hipStream_t s) {
         case 16 * 16 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 16, 2>), grid, b256, 0, s, a); break;
         case 64 * 16 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 1>), grid, b256, 0, s, a); break;
         case 64 * 16 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 2>), grid, b256, 0, s, a); break;
-        case 64 * 16 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 64, 4>), grid, b256, 0, s, a); break;
+        case 256 * 16 + 1: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 1>), grid, b256, 0, s, a); break;
         case 256 * 16 + 2: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 2>), grid, b256, 0, s, a); break;
         case 256 * 16 + 4: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 4>), grid, b256, 0, s, a); break;
         case 256 * 16 + 8: hipLaunchKernelGGL((ln_fwd_kernel<XT, YT, 256, 8>), grid, b256, 0, s, a); break;
@@ -520,7 +523,7 @@ int launch_bwd(const LnArgs& a, int blocks, bool want_cols, hipStream_t s) {
         case 16 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 16, 2, true>), grid, b256, 0, s, a); break;
         case 64 * 16 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 1, true>), grid, b256, 0, s, a); break;
         case 64 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 2, true>), grid, b256, 0, s, a); break;
-        case 64 * 16 + 4: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 64, 4, true>), grid, b256, 0, s, a); break;
+        case 256 * 16 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 1, true>), grid, b256, 0, s, a); break;
         case 256 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 256, 2, true>), grid, b256, 0, s, a); break;
         case 1024 * 16 + 1: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 1, true>), grid, b1024, 0, s, a); break;
         case 1024 * 16 + 2: hipLaunchKernelGGL((ln_bwd_kernel<XT, YT, 1024, 2, false>), grid, b1024, 0, s, a); break;
@@ -562,7 +565,7 @@ extern "C" int asl_layernorm_fwd(const asl_layernorm_params* p, const void* x, c
 extern "C" int64_t asl_layernorm_bwd_workspace(const asl_layernorm_params* p) {
     const int rc = ln_check(p);
     if (rc != ASL_OK) return rc;
-    return (int64_t)bwd_blocks(p->rows, p->d) * 2 * p->d * (int64_t)sizeof(float);
+    return (int64_t)bwd_blocks(*p) * 2 * p->d * (int64_t)sizeof(float);
 }
 
 extern "C" int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void* x, const void* gamma,
@@ -577,7 +580,7 @@ extern "C" int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, 
         ((uintptr_t)workspace & 15))
         return ASL_EINVAL;
     hipStream_t s = (hipStream_t)stream;
-    const int blocks = bwd_blocks(p->rows, p->d);
+    const int blocks = bwd_blocks(*p);
     if (blocks) {
         LnArgs a = {};
         a.x = x; a.dy = dy; a.w = gamma; a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.part = workspace;
