@@ -34,7 +34,8 @@ def _gen(seed):
 NORM_SIZES = [(1, 1), (3, 7), (2, 16), (5, 100), (130, 128), (9, 129), (33, 512), (17, 777), (6, 1024), (3, 1025), (3, 2047),
               (5, 2048), (2, 4096), (2, 5000), (3, 8192), (2, 8200), (2, 16384), (2, 20000), (2, 32769), (3, 40001), (2000, 64),
               (4100, 256),
-              (3, 200), (301, 250), (70, 12300), (601, 10001), (40, 16384), (65, 16385), (2, 1000003)]
+              (3, 200), (301, 250), (70, 12300), (601, 10001), (40, 16384), (65, 16385), (2, 1000003),
+              (5, 8), (5, 9), (40, 20), (33, 500), (700, 1501), (2500, 1290)]
 
 
 def norm_reference(x, w, b, dy, eps=1e-5):

@@ -69,6 +69,25 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* lds, int& slot) 
     }
 }
 
+// Vector j of lane t begins at column (t + j G) 8, but the one that would reach over the row's end ends with it: it shares its
+// first `lead` columns with its neighbour, which takes them for the sums, and both write them, the same.  So every access is a
+// whole vector, in rows of at least eight elements, and none branches by lane (2^26 bf16 elements, backward: rows of 500 80 us,
+// with a last vector loaded by element 214; rows of 2047 105 and 190).
+template <int G, int J>
+struct Columns {
+    int at[J], lead[J];
+    __device__ __forceinline__ Columns(int t, int d) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int k = (t + j * G) * 8;
+            at[j] = k + 8 <= d ? k : d >= 8 ? d - 8 : 0;
+            lead[j] = k - at[j];
+        }
+    }
+    __device__ __forceinline__ bool any(int j) const { return lead[j] < 8; }
+    __device__ __forceinline__ bool mine(int j, int e, int d) const { return e >= lead[j] && at[j] + e < d; }
+};
+
 // w and b stay in registers from row to row where a lane has at most two vectors of a row; with more, the registers go to
 // occupancy and both come from the L1 with every row.  The next row is on its way while this one is worked on.
 template <typename XT, typename YT, int G, int J>
@@ -78,24 +97,21 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs 
     __shared__ float lds[2 * 2 * (G > 64 ? G / 64 : 1)];
     int slot = 0;
     const int t = threadIdx.x % G;
+    const Columns<G, J> c(t, a.d);
     const float inv_d = 1.0f / (float)a.d;
     F8 w[HOLD ? J : 1], b[HOLD ? J : 1];
     if constexpr (HOLD) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8;
-            w[j] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, a.d - k, 1.f);
-            b[j] = load8_or(a.b, a.w_bf16, k < a.d ? k : 0, a.d - k, 0.f);
+            w[j] = load8_or(a.w, a.w_bf16, c.at[j], a.d, 1.f);
+            b[j] = load8_or(a.b, a.w_bf16, c.at[j], a.d, 0.f);
         }
     }
     typename RawOf<XT>::type next[J];
     const auto fetch = [&](long long row) {
         const XT* xr = (const XT*)a.x + row * a.ld_x;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8;
-            next[j] = load8_raw(xr + (k < a.d ? k : 0), row < a.rows ? a.d - k : 0);
-        }
+        for (int j = 0; j < J; ++j) next[j] = load8_raw(xr + c.at[j], a.d);
     };
     const long long stride = (long long)gridDim.x * RPB;
     long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
@@ -108,7 +124,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs 
         for (int j = 0; j < J; ++j) {
             x[j] = widen(next[j]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[0] += x[j].v[e];
+            for (int e = 0; e < 8; ++e) s[0] += c.mine(j, e, a.d) ? x[j].v[e] : 0.f;
         }
         if (row + stride < a.rows) fetch(row + stride);
         group_sum<G>(s, lds, slot);
@@ -118,12 +134,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs 
         float q[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int n = a.d - (t + j * G) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[j].v[e] = e < n ? x[j].v[e] - mean : 0.f;
-                q[0] += x[j].v[e];
-                q[1] += x[j].v[e] * x[j].v[e];
+                x[j].v[e] -= mean;
+                const float m = c.mine(j, e, a.d) ? x[j].v[e] : 0.f;
+                q[0] += m;
+                q[1] += m * m;
             }
         }
         group_sum<G>(q, lds, slot);
@@ -132,17 +148,16 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const LnArgs 
         YT* yr = (YT*)a.y + row * a.ld_y;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8;
-            if (k < a.d) {
+            if (c.any(j)) {
                 if constexpr (!HOLD) {
-                    w[0] = load8_or(a.w, a.w_bf16, k, a.d - k, 1.f);
-                    b[0] = load8_or(a.b, a.w_bf16, k, a.d - k, 0.f);
+                    w[0] = load8_or(a.w, a.w_bf16, c.at[j], a.d, 1.f);
+                    b[0] = load8_or(a.b, a.w_bf16, c.at[j], a.d, 0.f);
                 }
                 const F8 &wj = w[HOLD ? j : 0], &bj = b[HOLD ? j : 0];
                 F8 o;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o.v[e] = (x[j].v[e] - rest) * rstd * wj.v[e] + bj.v[e];
-                store8(yr + k, a.d - k, o);
+                store8(yr + c.at[j], a.d, o);
             }
         }
         if (t == 0) {
@@ -212,12 +227,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
     __shared__ __attribute__((aligned(16))) float cols[RPB > 1 ? 4 * 2 * (G < 64 ? G : 64) * 8 : 1];
     int slot = 0;
     const int t = threadIdx.x % G;
+    const Columns<G, J> c(t, a.d);
     const float inv_d = 1.0f / (float)a.d;
     F8 w[HOLD ? J : 1], dw[SUMS ? J : 1], db[SUMS ? J : 1];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        const int k = (t + j * G) * 8;
-        if constexpr (HOLD) w[j] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, a.d - k, 1.f);
+        if constexpr (HOLD) w[j] = load8_or(a.w, a.w_bf16, c.at[j], a.d, 1.f);
         if constexpr (SUMS)
 #pragma unroll
             for (int e = 0; e < 8; ++e) dw[j].v[e] = db[j].v[e] = 0.f;
@@ -232,9 +247,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
         next_rstd = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8, n = a.d - k;
-            next_x[j] = load8_raw(xr + (k < a.d ? k : 0), n);
-            next_dy[j] = load8_raw(dyr + (k < a.d ? k : 0), n);
+            next_x[j] = load8_raw(xr + c.at[j], a.d);
+            next_dy[j] = load8_raw(dyr + c.at[j], a.d);
         }
     };
     const long long stride = (long long)gridDim.x * RPB;
@@ -253,19 +267,18 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
         if (AHEAD && row + stride < a.rows) fetch(row + stride);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8, n = a.d - k;
-            if constexpr (!HOLD) w[0] = load8_or(a.w, a.w_bf16, k < a.d ? k : 0, n, 1.f);
+            if constexpr (!HOLD) w[0] = load8_or(a.w, a.w_bf16, c.at[j], a.d, 1.f);
             const F8& wj = w[HOLD ? j : 0];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                h[j].v[e] = e < n ? (h[j].v[e] - mean) * rstd : 0.f;
+                h[j].v[e] = (h[j].v[e] - mean) * rstd;
                 if constexpr (SUMS) {
                     dw[j].v[e] += g[j].v[e] * h[j].v[e];
                     db[j].v[e] += g[j].v[e];
                 }
                 g[j].v[e] *= wj.v[e];
-                s[0] += g[j].v[e];
-                s[1] += g[j].v[e] * h[j].v[e];
+                s[0] += c.mine(j, e, a.d) ? g[j].v[e] : 0.f;
+                s[1] += c.mine(j, e, a.d) ? g[j].v[e] * h[j].v[e] : 0.f;
             }
         }
         group_sum<G>(s, lds, slot);
@@ -273,25 +286,30 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
         XT* dxr = (XT*)a.y + row * a.ld_y;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8;
-            if (k < a.d) {
+            if (c.any(j)) {
                 F8 o;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o.v[e] = (g[j].v[e] - m0 - h[j].v[e] * m1) * rstd;
-                store8(dxr + k, a.d - k, o);
+                store8(dxr + c.at[j], a.d, o);
             }
         }
     }
     float* part = a.part + (long long)blockIdx.x * 2 * a.d;
+    const auto leave = [&](float* row, int j, const F8& v) {      // a vector's own columns of a row that begins at `row`
+        if (c.lead[j] == 0 && a.d >= 8) {
+            store8_full(row + c.at[j], v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c.mine(j, e, a.d)) row[c.at[j] + e] = v.v[e];
+        }
+    };
     if constexpr (!SUMS) {
     } else if constexpr (RPB == 1) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int k = (t + j * G) * 8;
-            if (k < a.d) {
-                store8(part + k, a.d - k, dw[j]);
-                store8(part + a.d + k, a.d - k, db[j]);
-            }
+            leave(part, j, dw[j]);
+            leave(part + a.d, j, db[j]);
         }
     } else {
         // several groups a workgroup: within the wave by lane exchange, then the waves' sums through LDS, a vector at a time
@@ -307,8 +325,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void ln_bwd_kernel(const LnArgs 
                     db[j].v[e] += __shfl_xor(db[j].v[e], o, 64);
                 }
             if (lane < L) {
-                store8_full(cols + (wave * 2 + 0) * COLS + lane * 8, dw[j]);
-                store8_full(cols + (wave * 2 + 1) * COLS + lane * 8, db[j]);
+                leave(cols + (wave * 2 + 0) * COLS - j * COLS, j, dw[j]);
+                leave(cols + (wave * 2 + 1) * COLS - j * COLS, j, db[j]);
             }
             __syncthreads();
             for (int i = threadIdx.x; i < 2 * COLS; i += BLOCK) {
