@@ -337,7 +337,8 @@ def test_linear_cross_entropy_leading_dimensions(gpu):
 
 def test_linear_cross_entropy_pieces(gpu):
     """more rows than one piece of exponentials holds"""
-    for dt, v, n, d in ((BF16, 65536, 8192 + 300, 24), (F32, 65530, 4096 + 4100, 24), (BF16, 65600, 8192 + 300, 40), (F32, 70000, 3000, 40)):
+    for dt, v, n, d in ((BF16, 65536, 8192 + 300, 24), (F32, 65530, 4096 + 4100, 24), (BF16, 65600, 8192 + 300, 40), (F32, 70000, 3000, 40),
+                        (BF16, 70, 140000, 40), (F32, 70, 140000, 40)):
         x, w, b, t = _xent_case(n, v, d, dt, F32, 0.1)
         _xent_check(x, w, b, t, smooth=0.1)
 
@@ -471,6 +472,59 @@ def test_linear_cross_entropy_writes_no_further_than_its_outputs(gpu, n, v, d, d
             assert (o[:3] == 7).all() and (o[-3:] == 7).all()
             assert (o == 7).all() if i == left_out else torch.equal(o[3:-3], q.flatten())
         assert (ws[:at] == 0x5a).all() and (ws[at + room:] == 0x5a).all()
+
+
+def test_linear_cross_entropy_one_row_without_dimensions(gpu):
+    from video_asl_recognition_amd import training as T
+    x, w, b, t = _xent_case(1, 30, 20, F32, F32, 0.0)
+    for red in ("mean", "none"):
+        want = T.linear_cross_entropy_grad(x, w, t, b, reduction=red)
+        got = T.linear_cross_entropy_grad(x[0], w, t[0], b, reduction=red)
+        assert got[0].shape == () and got[1].shape == (20,)
+        assert all(torch.equal(p.flatten(), q.flatten()) for p, q in zip(got, want))
+    y, mean, rstd = T.layer_norm_fwd(x[0], None, None)
+    assert y.shape == (20,) and mean.shape == () and torch.equal(y, T.layer_norm_fwd(x, None, None)[0][0])
+
+
+def test_rows_far_apart(gpu):
+    """rows of larger tensors, 2^20 elements and more from one to the next: the places pass 2^32 bytes and 2^31 elements"""
+    from video_asl_recognition_amd import training as T
+    for dt, ld in ((BF16, 1 << 20), (BF16, (1 << 20) + 8), (F32, 1 << 20)):
+        n, v, d = 2200, 2600, 64
+        x, w, b, t = _xent_case(n, v, d, dt, F32, 0.1)
+        xs, ws = torch.empty(n, ld, dtype=dt, device="cuda")[:, 8:d + 8], torch.empty(v, ld, dtype=dt, device="cuda")[:, -d:]
+        xs.copy_(x), ws.copy_(w)
+        for p, q in zip(T.linear_cross_entropy_grad(xs, ws, t, b), T.linear_cross_entropy_grad(x, w, t, b)):
+            assert torch.equal(p, q)
+        far, near = T.layer_norm_fwd(xs, b[:d], None), T.layer_norm_fwd(x, b[:d], None)
+        assert all(torch.equal(p, q) for p, q in zip(far, near))
+        dy = far[0]
+        assert all(torch.equal(p, q) for p, q in zip(T.layer_norm_bwd(xs, xs, b[:d], *far[1:]), T.layer_norm_bwd(x, x, b[:d], *near[1:])))
+        del xs, ws
+
+
+def test_linear_cross_entropy_weight_of_more_than_32_bits(gpu):
+    from video_asl_recognition_amd import training as T
+    n, v, d = 40, (1 << 21) - 3, 1032
+    g = _gen(5)
+    w = torch.empty(v, d, dtype=BF16, device="cuda").normal_(std=2 / d ** 0.5, generator=g)
+    x = torch.randn(n, d, generator=g, device="cuda").to(BF16)
+    t = torch.randint(0, v, (n,), generator=g, device="cuda")
+    t[:4] = torch.arange(v - 4, v, device="cuda")
+    loss, dx, dw, _ = T.linear_cross_entropy_grad(x, w, t, reduction="sum")
+    l = torch.cat([x.double() @ w[i:i + (1 << 18)].double().t() for i in range(0, v, 1 << 18)], 1)
+    lse = torch.logsumexp(l, 1, keepdim=True)
+    G = torch.exp(l - lse)
+    G.scatter_add_(1, t[:, None], torch.full((n, 1), -1.0, dtype=torch.float64, device="cuda"))
+    rows = (lse - l.gather(1, t[:, None]))[:, 0]
+    # a logit: d additions of products below |x| |w|, some 60 in all, to 32 bits; lse and the loss by as much
+    tol = 2 * (d + 2) * U32 * float((x.double().abs() @ w[:1000].double().abs().t()).max()) * 1.5 + 100 * U32
+    _ok(loss, rows.sum(), torch.tensor(n * tol, device="cuda"), "loss")
+    for part in (slice(0, 100), slice(v - 100, v)):
+        ref = G[:, part].t() @ x.double()
+        # G to bf16, the exponential under it to fp16, the sum to bf16
+        bound = (tol + 2 * 2.0 ** -8 + 2.0 ** -11) * (G[:, part].abs().t() @ x.double().abs()) + 2.0 ** -8 * ref.abs() + 1e-12
+        _ok(dw[part], ref, bound, "dw")
 
 
 def test_linear_cross_entropy_pieces_without_gradients(gpu):

@@ -81,3 +81,32 @@ def test_ignored_clip_and_no_clipping(gpu):
         assert float((grads[n].double() - wg[n]).norm() / wg[n].norm()) < 4096 * 2.0 ** -24
     tuner.step(clips, target)
     assert tuner.grad_norm is None
+
+
+def test_weights_loaded_anew(gpu):
+    """a tuner does not go on with weights that its model no longer computes with"""
+    from video_asl_recognition_amd import HeadTuner, init_state_dict
+    model, clips, kp, target = _setup("tiny", 2, 8)
+    tuner = HeadTuner(model, lambda ps: torch.optim.SGD(ps, lr=0.1))
+    tuner.step(clips, target)
+    model.load_state_dict(init_state_dict(model.spec, 4))
+    for call in (tuner.step, tuner.loss, tuner.gradients):
+        with pytest.raises(RuntimeError, match="loaded anew"):
+            call(clips, target)
+    HeadTuner(model, lambda ps: torch.optim.SGD(ps, lr=0.1)).step(clips, target)
+
+
+def test_steps_on_a_side_stream(gpu):
+    """the same steps on another stream than the model was built on, against the same on the current one"""
+    from video_asl_recognition_amd import HeadTuner
+    runs = []
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        model, clips, kp, target = _setup("twostream_transformer", 2, 16)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            tuner = HeadTuner(model, lambda ps: torch.optim.SGD(ps, lr=0.1), max_norm=0.5)
+            losses = [tuner.step(clips, target, kp) for _ in range(3)]
+        torch.cuda.synchronize()
+        runs.append([float(v) for v in losses] + [p.clone() for p in tuner.params.values()])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b

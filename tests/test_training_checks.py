@@ -162,6 +162,21 @@ def test_grad_clip_workspace():
     assert L.lib.asl_grad_clip_workspace(2, arr((5, -1))) == L.ASL_EINVAL
 
 
+def test_python_refuses_what_32_bits_do_not_count():
+    from video_asl_recognition_amd import training as T
+    one = torch.zeros(1)
+    t = torch.zeros(1, dtype=torch.int64)
+    for shape in (((1 << 32) + 3, 2), (1 << 16, 1 << 16, 2)):
+        with pytest.raises(ValueError, match="2.31"):
+            T.layer_norm_fwd(one.expand(*shape), None, None)
+        with pytest.raises(ValueError, match="2.31"):
+            T.linear_cross_entropy_fwd(one.expand(*shape), torch.zeros(5, 2), t.expand(*shape[:-1]))
+    with pytest.raises(ValueError, match="2.31"):
+        T.layer_norm_fwd(one.expand(2, (1 << 32) + 3), None, None)
+    with pytest.raises(ValueError, match="2.31"):
+        T.linear_cross_entropy_fwd(torch.zeros(3, 2), one.expand((1 << 32) + 3, 2), t.expand(3))
+
+
 def test_python_refuses():
     from video_asl_recognition_amd import training as T
     x, w, b = torch.zeros(3, 8), torch.ones(8), torch.zeros(8)

@@ -32,8 +32,8 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 constexpr float kExpScale16 = 32768.f;    // exponentials in (0, 1] held as fp16: times this, so that fp16's range is used
 
-// xent_tiles.hip, tile 128 or 256: bf16 (or fp32 as planes of it), both operands' rows on 16 bytes and at most 2^21 bytes
-// apart; those contiguous along k hold noughts from K to the next multiple of 64
+// xent_tiles.hip, tile 128 or 256: bf16 (or fp32 as planes of it), both operands' rows on 16 bytes and at most 2^22 + 128
+// bytes apart; those contiguous along k hold noughts from K to the next multiple of 64
 int xent_tiles_logits(const XentGemm& a, int tile, hipStream_t s);
 int xent_tiles_dx(const XentGemm& a, int tile, hipStream_t s);     // P along its own index, Q along k
 int xent_tiles_dw(const XentGemm& a, int tile, hipStream_t s);     // both along their own index

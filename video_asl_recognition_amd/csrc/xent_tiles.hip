@@ -117,7 +117,7 @@ struct Panel {
     // The descriptor of the step at `at`: everything past the operand's last element reads as nought, all of it behind the
     // last step.  Rows that are contiguous along k hold noughts up to a whole step (the caller sees to that).
     __device__ __forceinline__ i32x4 rsrc() const {
-        // (32 bits: a tile's rows are at most 2^21 bytes apart)
+        // (32 bits: a tile's rows are at most 2^22 bytes and some apart, G's of 2^21 classes)
         const int k = krem < BK ? krem : BK;
         const int n = KC ? (idx - 1) * (int)row_bytes + BK * 2 : (k - 1) * (int)row_bytes + idx * 2;
         const unsigned long long p = (unsigned long long)at;

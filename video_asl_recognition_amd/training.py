@@ -52,6 +52,12 @@ def _device(x: torch.Tensor, **tensors) -> int:
     return index
 
 
+def _countable(t: torch.Tensor, what: str):
+    """the C parameters count rows and columns in 32 bits, and ctypes would cut a larger number without a word"""
+    if t.shape[-1] >> 31 or t.numel() // (t.shape[-1] or 1) >> 31:
+        raise ValueError(f"{what} must be of fewer than 2^31 rows and columns, got {tuple(t.shape)}")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., d] -> [rows, d] with unit stride along d and rows that do not overlap; a view where the strides allow it"""
     if t.dim() == 2 and t.is_contiguous():
@@ -91,6 +97,7 @@ def _bytes(n: int, what: str) -> int:
 def _check_norm(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., d] with d >= 1, got {tuple(x.shape)}")
+    _countable(x, "x")
     d = x.shape[-1]
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.dim() != 1 or t.shape[0] != d):
@@ -167,6 +174,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 def _check_xent(x, weight, target, bias, reduction, label_smoothing):
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
         raise ValueError(f"x must be [..., d] and weight [classes, d], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _countable(x, "x")
+    _countable(weight, "weight")
     index = _device(x, weight=weight, target=target, bias=bias)
     if x.dtype != weight.dtype:
         raise ValueError(f"x is {x.dtype}, weight {weight.dtype}: one type for both")
@@ -341,7 +350,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
 
 @torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
-    """torch.nn.utils.clip_grad_norm_ for norm_type 2 and inf: clips the parameters' .grad in place, returns their norm."""
+    """torch.nn.utils.clip_grad_norm_ for norm_type 2 and inf and parameters on one GPU: clips their .grad in place, returns the
+    norm."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     parameters = list(parameters)

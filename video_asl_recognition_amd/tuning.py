@@ -37,6 +37,8 @@ class HeadTuner:
 
     def _features(self, clips, keypoints):
         """(features of the Linear [B, F], and for the transformer what the norm's backward needs)"""
+        if any(p is not self.params.get(n) for n, p in self.model.head_parameters().items()):
+            raise RuntimeError("the model's weights were loaded anew: build another HeadTuner for them")
         x = self.model.head_input(clips, keypoints)
         if not self._norm:
             return x, None
