@@ -598,7 +598,8 @@ def _tensors(sizes, types, seed=0):
 
 
 CLIP_SETS = {"one": [(1,)], "scalars": [()] * 3, "odd": [(3,), (0,), (8191,), (8192,), (8193,), (77, 5), (1, 1)],
-             "many": [((i * 37) % 501,) for i in range(250)], "large": [(3000, 4001), (5,), (1 << 24,)]}
+             "many": [((i * 37) % 501,) for i in range(250)], "one launch": [(51200,), (100,), (513,), (7, 73)], "just": [(65536,)],
+             "just not": [(65536,), (1,)], "slots": [(i % 3 + 1,) for i in range(64)], "slots and more": [(i % 3 + 1,) for i in range(65)], "large": [(3000, 4001), (5,), (1 << 24,)]}
 
 
 @pytest.mark.parametrize("kinds", [(F32,), (BF16,), (F32, BF16)], ids=["f32", "bf16", "mixed"])

@@ -424,6 +424,11 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
     const long long col = (long long)blockIdx.x * kGradCols + lane * 8;
     const bool in = col < a.ld;
     const int b0 = blockIdx.y * kGradRows, r0 = b0 + rl;
+    if (b0 >= st.rows) {                                     // the workgroups behind the last row: what concerns all of them
+        if (blockIdx.x == 0 && a.factor.factor) set_factor(a.factor);
+        if (blockIdx.x == 0 && a.loss.loss_part) finish_loss(a.loss);
+        return;
+    }
     F8 g[R], db;
     float f[R], even[R], tg[R];
     long long t[R];
@@ -504,10 +509,6 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
             for (int q = 0; q < 8; ++q) v += cols[q][threadIdx.x];
             *o = v;
         }
-    }
-    if (blockIdx.x == 0 && blockIdx.y == 0) {
-        if (a.factor.factor) set_factor(a.factor);
-        if (a.loss.loss_part) finish_loss(a.loss);
     }
 }
 
@@ -837,7 +838,7 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         if (!none && last && !own) c.loss = all;
         if (piece == 0) c.factor = factor;
         const int groups = ceil_div(rows, kGradRows);
-        const dim3 g_grid(ceil_div(q.ld_e, kGradCols), groups);
+        const dim3 g_grid(ceil_div(q.ld_e, kGradCols), groups + (c.factor.factor || c.loss.loss_part ? 1 : 0));
         if (own) hipLaunchKernelGGL((xent_g_kernel<T, true>), g_grid, dim3(256), 0, s, c);
         else hipLaunchKernelGGL((xent_g_kernel<T, false>), g_grid, dim3(256), 0, s, c);
 
