@@ -366,7 +366,9 @@ __global__ __launch_bounds__(256) void xent_count_kernel(const long long* target
 constexpr int kGradRows = 32;             // rows a workgroup of the G pass takes; it leaves one partial row of db
 constexpr int kGradCols = 256;            // and columns
 
-constexpr int kOwnStats = 64;             // tiles a row up to which the G pass takes the statistics for itself
+// tiles a row up to which the G pass takes the statistics for itself (1024 x 2000 x 512 bf16, 32 of them, with gradients 38.0 us and
+// 38.8; 1024 x 4000, 63, 48.2 and 46.1)
+constexpr int kOwnStats = 32;
 
 struct XentG {
     XentRows rows;                        // `factor`, `target_g`, `row_g`: taken from there (or, with own statistics, not used)
