@@ -619,7 +619,7 @@ inline bool lies_well(const void* t, long long ld, int d) {
 inline long long slab_ld(int d, int tile) { return (long long)ceil_div(d, tile) * tile; }
 
 // Up to 32 rows of fp32 the products run as in xent_few.hip (32 x 2000 x 512 with gradients 28 us, on 64 x 64 tiles 46), of
-// bf16 up to 16 and with a small weight (8 x 2000 x 512 22 us, on 128 x 128 tiles 24; 8 x 8000 x 2048 84, 64; 32 x 2000 x 512
+// bf16 up to 16 and with a small weight (8 x 2000 x 512 20 us, on 128 x 128 tiles 24; 8 x 8000 x 2048 84, 64; 32 x 2000 x 512
 // 31, 27).
 inline bool takes_few(const asl_xent_params& p) {
     if (!p.n || p.classes > kFewClasses) return false;

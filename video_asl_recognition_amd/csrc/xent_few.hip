@@ -1,11 +1,12 @@
 // Linear + softmax cross entropy for a handful of rows (up to 32: clips of one small batch), with gradients, for gfx950.
 //
 // Such a call is a chain of dependent launches over a weight matrix of a few megabytes, bound by latency: what counts is how
-// few launches there are and that each has all its loads in flight at once.  Four launches: logits with per-tile maxima and
-// sums; statistics, loss, G and the bias's gradient together (every workgroup takes all rows' statistics for itself: 32 rows
-// of at most 512 tiles); both gradient products side by side; the sum of dx's slices.  All products run on fp32 MFMAs, bf16
+// few launches there are and that each has all its loads in flight at once.  Two launches for small weights: logits with
+// per-tile maxima and sums, and the rest.  Four for larger: logits; statistics, loss, G and the bias's gradient together (every
+// workgroup takes all rows' statistics for itself: 32 rows of at most 512 tiles); both gradient products side by side; the sum
+// of dx's slices.  All products run on fp32 MFMAs, bf16
 // operands widened on load, because nothing here is bound by the matrix pipe; G stays fp32.  8 x 2000 x 512 fp32 with gradients
-// takes 20 us as a graph (its launches 6.8, 4.8, 4.6 and 2.9 us): 8 MB, 2 us of this card's memory rate.
+// takes 19 us as a graph (its launches 6.7 and 11.3): 8 MB, 2 us of this card's memory rate.
 //
 // The MFMA (16 x 16 x 4) wants one k of one index a lane.  A lane loads four consecutive elements and deals them to four
 // MFMAs, with the same assignment of k (or of the index) on both sides, so every load is 16 bytes (8 for bf16).
@@ -110,14 +111,14 @@ __global__ __launch_bounds__(256) void xent_few_logits_kernel(const XentFew a) {
     }
 }
 
-// Statistics, loss, G and db: 256 columns and all rows a workgroup.
+// Statistics, loss, G and db: 256 columns and all rows a workgroup (32 x 16384: 22 us, its statistics' chain of loads).
 __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
     constexpr int R = kFewRows / 8, TPB = 256 / kFewTile;
     __shared__ float fac[kFewRows][TPB], target_g[kFewRows], row_g[kFewRows], loss_row[kFewRows];
     __shared__ __attribute__((aligned(16))) float cols[8][256];
     const int lane = threadIdx.x & 63, cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = (long long)blockIdx.x * 256 + cl * 8;
-    const bool in = a.e && col < a.ld_e;
+    const bool in = col < a.ld_e;
     F8 g[R];
 #pragma unroll
     for (int u = 0; u < R; ++u)
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
                 if (a.lse) a.lse[row] = r.lse;
             }
         }
-        if (a.e && l16 < TPB) {
+        if (l16 < TPB) {
             const int tile = blockIdx.x * TPB + l16;
             if (tile < a.tiles) fac[row][l16] = r.valid ? r.g * expf(a.tile_max[(long long)row * a.tiles + tile] - r.lse) : NAN;
         }
@@ -151,9 +152,8 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
         float v = 0.f;
         for (int r = 0; r < a.n; ++r) v += loss_row[r];
         if (!a.none) *a.loss = a.mean ? v / (float)kept_all : v;
-        if (a.factor) *a.factor = c;
+        *a.factor = c;
     }
-    if (!a.e) return;
     F8 db;
 #pragma unroll
     for (int e = 0; e < 8; ++e) db.v[e] = 0.f;
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
     }
 }
 
-// Both gradient products.  Workgroups below `dw_blocks`: dW of 64 classes x 64 features; the others: dx of 64 features from
+// Both gradient products (32 x 16384 x 2048: 91 us, 2.9 TB/s).  Workgroups below `dw_blocks`: dW of 64 classes x 64 features; the others: dx of 64 features from
 // one slice of the classes, into a slab.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void xent_few_grad_kernel(const XentFew a, int dw_blocks, int d_tiles, int slice) {
@@ -288,10 +288,165 @@ __global__ __launch_bounds__(64) void xent_few_dx_kernel(const XentFew a, int sl
     store4((T*)a.dx + (long long)row * a.d + at, a.d - at, o);
 }
 
+// Everything behind the logits in one launch, for small weights: every workgroup takes the rows' statistics for itself, and G as
+// it goes.  Workgroups below `dx_blocks`: dx of 16 features from all classes, a tile of 32 a wave at a time; the others: dW of
+// 64 classes x 256 features, 16 x 64 a wave, and (those of the first features) db.
+template <typename T, int NB>
+__global__ __launch_bounds__(1024) void xent_few_rest_kernel(const XentFew a, int dx_blocks, int d_tiles) {
+    __shared__ float lse[kFewRows], target_g[kFewRows], row_g[kFewRows], loss_row[kFewRows];
+    __shared__ int label[kFewRows];                          // the target's class; -1: outside the vocabulary, -2: ignored
+    __shared__ __attribute__((aligned(16))) float part[16][16 * NB][16 + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+    const int kept_all = __popcll(__ballot(lane < a.n && a.target[lane < a.n ? lane : 0] != a.ignore));
+    XentStats st = {};
+    st.target = a.target; st.upstream = a.none ? a.upstream : nullptr; st.tile_max = a.tile_max; st.tile_sum = a.tile_sum;
+    st.tile_lin = a.tile_lin; st.target_logit = a.target_logit; st.ignore = a.ignore; st.smoothing = a.smoothing;
+    st.inv_classes = a.inv_classes; st.rows = a.n; st.classes = a.classes; st.tiles = a.tiles;
+    const int mine = threadIdx.x >> 4;                       // sixteen lanes a row, all rows at once
+    if (mine < kFewRows) {
+        XentRow r = {0.f, 0.f, 0.f, 0.f, true};
+        if (mine < a.n) r = row_stats<16>(st, mine, fr);
+        if (fr == 0) {
+            lse[mine] = r.lse;
+            target_g[mine] = r.target_g;
+            row_g[mine] = r.valid ? r.g : NAN;
+            loss_row[mine] = r.loss;
+            label[mine] = mine >= a.n || a.target[mine] == a.ignore ? -2 : r.valid ? (int)a.target[mine] : -1;
+            if (blockIdx.x == 0 && mine < a.n) {
+                if (a.none) a.loss[mine] = r.loss;
+                if (a.lse) a.lse[mine] = r.lse;
+            }
+        }
+    }
+    __syncthreads();
+    const float up = a.upstream && !a.none ? *a.upstream : 1.f;
+    const float c = !a.mean ? up : kept_all ? up / (float)kept_all : 0.f;    // no row with a label: gradients are nought
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !a.none) {
+        float v = 0.f;
+        for (int r = 0; r < a.n; ++r) v += loss_row[r];
+        *a.loss = a.mean ? v / (float)kept_all : v;
+    }
+    if (!a.e) return;
+    const float smooth = a.smoothing * a.inv_classes;
+    // G from an exponential and its tile's maximum
+    const auto grad = [&](float e, float f, int row, int col) {
+        float v = col < a.classes ? e * f - smooth * row_g[row] : 0.f;
+        if (col == label[row]) v = target_g[row];
+        return label[row] == -2 ? 0.f : v;                   // whatever the row held
+    };
+    if ((int)blockIdx.x < dx_blocks) {
+        const int i = blockIdx.x * 16 + fr, ic = i < a.d ? i : a.d - 1;      // surplus features repeat one and are dropped
+        f32x4 acc[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // MFMA s takes class 8*fq + s of a tile; two tiles on their way at once
+        constexpr int U = 2;
+        for (int t0 = wave; t0 < a.tiles; t0 += 16 * U) {
+            float wf[U][8], m[U][NB];
+            F8 e[U][NB];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int t = t0 + u * 16 < a.tiles ? t0 + u * 16 : t0, v = t * kFewTile + fq * 8;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) wf[u][s] = load1((const T*)a.w + (v + s < a.classes ? v + s : 0) * a.ld_w + ic);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    const int r = j * 16 + fr < a.n ? j * 16 + fr : 0;
+                    e[u][j] = load8_full(a.e + r * a.ld_e + v);
+                    m[u][j] = a.tile_max[(long long)r * a.tiles + t];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (t0 + u * 16 >= a.tiles) break;
+                const int v = (t0 + u * 16) * kFewTile + fq * 8;
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    const int row = j * 16 + fr;
+                    const float f = row_g[row] * expf(m[u][j] - lse[row]);
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) acc[j] = mma4(v + s < a.classes ? wf[u][s] : 0.f, grad(e[u][j].v[s], f, row, v + s), acc[j]);
+                }
+            }
+        }
+        // lane: feature fq*4 + r, row j*16 + fr
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) part[wave][j * 16 + fr][fq * 4 + r] = acc[j][r];
+        __syncthreads();
+        if (threadIdx.x < 256 * NB) {
+            const int row = threadIdx.x >> 4;
+            float o = 0.f;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) o += part[w][row][fr];
+            if (row < a.n && i < a.d) store1((T*)a.dx + (long long)row * a.d + i, o * c);
+        }
+        return;
+    }
+    const int b = blockIdx.x - dx_blocks, i0 = (b % d_tiles) * 256 + (wave >> 2) * 64, col = (b / d_tiles) * 64 + (wave & 3) * 16 + fr;
+    const int cc = col < a.classes ? col : a.classes - 1, i = i0 + fr * 4;
+    f32x4 xf[4 * NB];
+    float gf[4 * NB], ef[4 * NB], mf[4 * NB];
+#pragma unroll
+    for (int u = 0; u < 4 * NB; ++u) {
+        const int k = u * 4 + fq, r = k < a.n ? k : 0;
+        xf[u] = load4((const T*)a.x + r * a.ld_x + (i < a.d ? i : 0), k < a.n ? a.d - i : 0);
+        ef[u] = a.e[r * a.ld_e + cc];
+        mf[u] = a.tile_max[(long long)r * a.tiles + cc / kFewTile];
+    }
+    float db = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4 * NB; ++u) {
+        const int k = u * 4 + fq;
+        gf[u] = col < a.classes ? grad(ef[u], row_g[k] * expf(mf[u] - lse[k]), k, col) : 0.f;
+        db += gf[u];
+    }
+    if (a.dw) {
+        f32x4 acc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 4 * NB; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[t] = mma4(xf[u][t], gf[u], acc[t]);
+        // tile t, register r: feature i0 + (fq*4 + r)*4 + t -- sixteen consecutive ones a lane
+        if (col < a.classes) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int at = i0 + fq * 16 + r * 4;
+                if (at < a.d)
+                    store4((T*)a.dw + (long long)col * a.d + at, a.d - at, f32x4{acc[0][r] * c, acc[1][r] * c, acc[2][r] * c, acc[3][r] * c});
+            }
+        }
+    }
+    if (a.db && b % d_tiles == 0 && wave < 4) {
+        db += __shfl_xor(db, 16, 64);
+        db += __shfl_xor(db, 32, 64);
+        if (fq == 0 && col < a.classes) {
+            if (a.bias_bf16) store1((short*)a.db + col, db * c);
+            else store1((float*)a.db + col, db * c);
+        }
+    }
+}
+
+// One launch behind the logits for weights up to 2048 x 2048 or as many elements in fewer classes, or for none wanted; three
+// for larger, where what every workgroup would do for itself adds up and strips of 16 features cost W's lines twice.  fp32 with
+// gradients, as graphs: 8 x 100 x 512 13 us against 16, 8 x 2000 x 512 19 against 20 (as calls, which four launches bound, 20
+// and 25), 8 x 2000 x 2048 36 against 39; 32 x 4000 x 512 42 against 36, 8 x 8000 x 1024 57 against 49, 32 x 16384 x 2048 222
+// against 162.
+static bool one_launch(const XentFew& a) { return !a.e || (a.classes <= 2048 && (double)a.classes * a.d <= (double)(1 << 22)); }
+
 template <typename T, int NB>
 static int run_few(const XentFew& a, hipStream_t s) {
     hipLaunchKernelGGL((xent_few_logits_kernel<T, NB>), dim3(a.tiles), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(xent_few_g_kernel, dim3(a.e ? ceil_div(a.ld_e, 256) : 1), dim3(256), 0, s, a);
+    if (one_launch(a)) {
+        const int dx_blocks = a.e && a.dx ? ceil_div(a.d, 16) : 0, d_tiles = a.e && a.dw ? ceil_div(a.d, 256) : 1;
+        const int dw_blocks = a.e && (a.dw || a.db) ? d_tiles * ceil_div(a.classes, 64) : 0, blocks = dx_blocks + dw_blocks;
+        hipLaunchKernelGGL((xent_few_rest_kernel<T, NB>), dim3(blocks ? blocks : 1), dim3(1024), 0, s, a, dx_blocks, d_tiles);
+        return (int)hipGetLastError();
+    }
+    hipLaunchKernelGGL(xent_few_g_kernel, dim3(ceil_div(a.ld_e, 256)), dim3(256), 0, s, a);
     if (a.dx || a.dw) {
         const int d_tiles = ceil_div(a.d, 64), dw_blocks = a.dw ? d_tiles * ceil_div(a.classes, 64) : 0;
         const int slabs = a.dx ? xent_few_slabs(a.classes) : 0, slice = slabs ? ceil_div(ceil_div(a.classes, slabs), 16) * 16 : 1;
