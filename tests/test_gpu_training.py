@@ -384,7 +384,7 @@ def test_linear_cross_entropy_masks_and_labels(gpu):
 
 
 # sizes for each way the products are computed: few rows, fp32 on 64 x 64 tiles, 128 x 128 and 256 x 256, fp32 as bf16 planes
-PATHS = [(12, 300, 40, BF16), (20, 300, 40, F32), (20, 4500, 40, F32), (9, 2100, 30, BF16), (80, 60, 64, BF16), (80, 300, 20, BF16), (80, 300, 64, F32), (600, 1100, 260, F32),
+PATHS = [(12, 300, 40, BF16), (20, 300, 40, F32), (20, 4500, 40, F32), (9, 2100, 30, BF16), (80, 60, 64, BF16), (80, 300, 20, BF16), (80, 300, 64, F32), (70, 4000, 90, F32), (600, 1100, 260, F32),
          (20, 300, 40, BF16), (80, 300, 64, BF16), (400, 1000, 128, BF16), (400, 1003, 77, BF16), (1000, 8200, 256, BF16),
          (520, 9001, 136, BF16), (600, 4100, 260, F32), (1100, 8200, 65, F32), (9000, 250, 64, BF16)]
 PATH_IDS = [f"{n}x{v}x{d}-{'f32' if dt == F32 else 'bf16'}" for n, v, d, dt in PATHS]

@@ -41,7 +41,7 @@ struct Held<float> {
 
 // fp32 products that are not worth being taken apart into bf16 planes: 64 x 64 tiles on the fp32 MFMA (16 x 16 x 4), any sizes,
 // strides and alignment.  The matrix pipe's fp32 rate (133 TF/s as a library product reaches it) bounds large ones, a step's
-// round trip to memory the small ones that come here: 300 x 300 x 300 with gradients 42 us, 512 x 2000 x 512 70 us.  Steps of
+// round trip to memory the small ones that come here: 300 x 300 x 300 with gradients 33 us, 512 x 2000 x 512 70 us.  Steps of
 // 32 k and of 64 take the same time (500 x 300 x 200: 13.6 and 14.1 us for the logits).
 constexpr int kTile = 64, kStep = 32;     // of either index, and of k
 
@@ -417,7 +417,7 @@ __device__ __forceinline__ void store_planes(short* p, long long plane, const F8
 // rows' statistics are taken here, by every column's workgroup anew, instead of in a launch ahead.
 template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
-    constexpr int R = kGradRows / 8, TPB = kGradCols / kTile;
+    constexpr int R = kGradRows / 8, TPB = kGradCols / kFewTile;     // (at least 32 classes a maximum)
     __shared__ __attribute__((aligned(16))) float cols[8][kGradCols];
     __shared__ float own_f[OWN ? kGradRows : 1][TPB], own_tg[OWN ? kGradRows : 1], own_g[OWN ? kGradRows : 1], own_loss[kGradRows];
     __shared__ int own_kept[kGradRows];
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(256) void xent_finish_kernel(const XentFinish a) {
 struct XentPlan {
     int esize, rows, pieces, tiles, tile, tile_shift, dx_tile, dw_tile, dx_splits, dw_splits, row_groups;
     long long ld_e, ld_pack;
-    bool dw_slabs, pack_x, pack_w, wide, few;
+    bool dw_slabs, pack_x, pack_w, wide, few, small;
     // workspace offsets, bytes
     long long shared, loss, kept, counts, tmax, tsum, tlin, tlogit, tg, rg, e, dbp, dxs, dws, xp, wp, gp, total;
 };
@@ -658,19 +658,25 @@ inline TilePlan tiles_for(const asl_xent_params& p, long long a, long long b, in
     return best;
 }
 
+// 64 x 64 tiles up to which the logits are taken on 32 x 32, eight waves sharing the contraction of one: half of the CUs would
+// be idle else, and each of the others wait on a step at a time (fp32 forward: 64 x 2000 x 512, 32 of them, 13.9 us and 24.7;
+// 256 x 2000 x 512, 128 of them, 19.7 and 25.1; 2000 x 300 x 512, 160, 28.0 and 27.9; 512 x 2000 x 512, 256, 30.9 and 25.7)
+constexpr long long kSmallTiles = 128;
+
 XentPlan xent_plan(const asl_xent_params& p, const void* xp, const void* wp, bool grad, bool want_dx, bool want_dw, bool want_db) {
     XentPlan q = {};
     q.esize = p.type ? 2 : 4;
     q.few = takes_few(p);
     q.tile = q.few ? kFewTile : tiles_for(p, p.n, p.classes, p.d, false).tile;
-    q.tile_shift = q.tile == 256 ? 7 : 6;                // maxima and sums are kept per 128 classes, or 64
+    q.small = !q.few && q.tile == kTile && (long long)ceil_div(p.n, kTile) * ceil_div(p.classes, kTile) <= kSmallTiles;
+    q.tile_shift = q.few || q.small ? 5 : q.tile == 256 ? 7 : 6;     // maxima and sums are kept per 32, 128 or 64 classes
     // the tile kernels read 16 bytes at a time and whole steps of 64 k: operands that do not allow it are laid out anew
     q.ld_pack = (p.d + 63LL) / 64 * 64;
     q.wide = q.tile > kTile && !p.type;
     q.pack_x = q.tile > kTile && (q.wide || !lies_well(xp, p.ld_x, p.d));
     q.pack_w = q.tile > kTile && (q.wide || !lies_well(wp, p.ld_w, p.d));
     const int planes = q.wide ? 3 : 1;
-    q.tiles = ceil_div(p.classes, q.few ? kFewTile : 1 << q.tile_shift);
+    q.tiles = ceil_div(p.classes, 1 << q.tile_shift);
     // (128 bytes off a power of two, which would put a tile's rows all in the same few channels: dx of 8192 x 32768 x 2048
     // takes 836 us with them and 906 without)
     q.ld_e = (long long)ceil_div(p.classes, q.tile) * q.tile + (q.tile > kTile ? 64 : 0);
@@ -818,6 +824,13 @@ int xent_run(const asl_xent_params& p, const XentPlan& q, bool grad, const void*
         if (q.tile > kTile) {
             const int rc = xent_tiles_logits(g, q.tile, s);
             if (rc) return rc;
+        } else if (q.small) {
+            XentFew f = {};
+            f.x = xr; f.w = wk; f.bias = bias; f.bias_bf16 = p.bias_type; f.target = g.target; f.e = grad ? (float*)g.out : nullptr;
+            f.tile_max = g.tile_max; f.tile_sum = g.tile_sum; f.tile_lin = g.tile_lin; f.target_logit = g.target_logit;
+            f.ld_x = ld_x; f.ld_w = ld_w; f.ld_e = q.ld_e; f.smoothing = p.label_smoothing; f.n = rows; f.classes = p.classes; f.d = p.d;
+            f.tiles = q.tiles;
+            xent_few_logits(f, s);
         } else {
             const int tj = ceil_div(rows, kTile);
             hipLaunchKernelGGL(xent_gemm_logits_kernel, dim3((unsigned)(q.tiles * tj)), dim3(256), 0, s, g, q.tiles, tj);

@@ -127,5 +127,6 @@ struct XentFew {
 // slices of the classes for dx: 128 classes a workgroup, at most 32 slices
 inline int xent_few_slabs(int classes) { return classes < 128 * 32 ? ceil_div(classes, 128) : 32; }
 int xent_few(const XentFew& a, int type, hipStream_t s);
+void xent_few_logits(const XentFew& a, hipStream_t s);     // the logits of any number of fp32 rows: 32 x 32 tiles
 
 }  // namespace asl_detail

@@ -25,7 +25,7 @@ template <typename T, int NB>
 __global__ __launch_bounds__(64 * kLogitWaves) void xent_few_logits_kernel(const XentFew a) {
     __shared__ __attribute__((aligned(16))) float part[kLogitWaves][32][33]; // [wave][row][class]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-    const int c0 = blockIdx.x * kFewTile;
+    const int c0 = blockIdx.x * kFewTile, row0 = blockIdx.y * kFewRows, n = a.n - row0 < kFewRows ? a.n - row0 : kFewRows;
     f32x4 acc[2][NB];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -41,18 +41,18 @@ __global__ __launch_bounds__(64 * kLogitWaves) void xent_few_logits_kernel(const
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
         const int r = j * 16 + fr;
-        xr[j] = (const T*)a.x + (r < a.n ? r : a.n - 1) * a.ld_x;
+        xr[j] = (const T*)a.x + (row0 + (r < n ? r : n - 1)) * a.ld_x;
     }
     constexpr int U = 4;                                                     // 16-k chunks on their way at once
     for (int k0 = wave * 16; k0 < a.d; k0 += 16 * kLogitWaves * U) {
         f32x4 wf[U][2], xf[U][NB];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = k0 + u * (16 * kLogitWaves) + fq * 4, n = a.d - k;
+            const int k = k0 + u * (16 * kLogitWaves) + fq * 4, left = a.d - k;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) wf[u][i] = load4(wr[i] + (n > 0 ? k : 0), n);
+            for (int i = 0; i < 2; ++i) wf[u][i] = load4(wr[i] + (left > 0 ? k : 0), left);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) xf[u][j] = load4(xr[j] + (n > 0 ? k : 0), n);
+            for (int j = 0; j < NB; ++j) xf[u][j] = load4(xr[j] + (left > 0 ? k : 0), left);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -72,18 +72,19 @@ __global__ __launch_bounds__(64 * kLogitWaves) void xent_few_logits_kernel(const
             for (int r = 0; r < 4; ++r) part[wave][j * 16 + fr][i * 16 + fq * 4 + r] = acc[i][j][r];
     __syncthreads();
     // eight lanes a row, four classes each
-    const int row = threadIdx.x >> 3, cl = (threadIdx.x & 7) * 4;
-    if (row >= a.n) return;                                                  // whole groups of eight leave, and waves behind the rows
+    const int at_row = threadIdx.x >> 3, cl = (threadIdx.x & 7) * 4;
+    if (at_row >= n) return;                                                  // whole groups of eight leave, and waves behind the rows
     float l[4], m = -INFINITY;
+    const int row = row0 + at_row;
     const long long t = a.target[row];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int c = c0 + cl + e;
         float v = -INFINITY;
         if (c < a.classes) {
-            v = part[0][row][cl + e];
+            v = part[0][at_row][cl + e];
 #pragma unroll
-            for (int w = 1; w < kLogitWaves; ++w) v += part[w][row][cl + e];
+            for (int w = 1; w < kLogitWaves; ++w) v += part[w][at_row][cl + e];
             if (a.bias) v += a.bias_bf16 ? load1((const short*)a.bias + c) : load1((const float*)a.bias + c);
             if (c == t) a.target_logit[row] = v;
         }
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(64 * kLogitWaves) void xent_few_logits_kernel(const
         s += __shfl_xor(s, o, 64);
         lin += __shfl_xor(lin, o, 64);
     }
-    if (a.e) *(f32x4*)(a.e + row * a.ld_e + c0 + cl) = x;
+    if (a.e) *(f32x4*)(a.e + (long long)row * a.ld_e + c0 + cl) = x;
     if ((threadIdx.x & 7) == 0) {
         const long long at = (long long)row * a.tiles + blockIdx.x;
         a.tile_max[at] = m;
@@ -458,6 +459,10 @@ static int run_few(const XentFew& a, hipStream_t s) {
         if (a.dx) hipLaunchKernelGGL((xent_few_dx_kernel<T>), dim3(ceil_div(a.d, 256), a.n), dim3(64), 0, s, a, slabs);
     }
     return (int)hipGetLastError();
+}
+
+void xent_few_logits(const XentFew& a, hipStream_t s) {
+    hipLaunchKernelGGL((xent_few_logits_kernel<float, 2>), dim3(a.tiles, ceil_div(a.n, kFewRows)), dim3(64 * kLogitWaves), 0, s, a);
 }
 
 int xent_few(const XentFew& a, int type, hipStream_t s) {
