@@ -192,8 +192,8 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
     }
 }
 
-// Both gradient products (32 x 16384 x 2048: 91 us, 2.9 TB/s).  Workgroups below `dw_blocks`: dW of 64 classes x 64 features; the others: dx of 64 features from
-// one slice of the classes, into a slab.
+// Both gradient products (32 x 16384 x 2048: 91 us, 2.9 TB/s).  Workgroups below `dw_blocks`: dW of 64 classes x 64 features;
+// the others: dx of 64 features from one slice of the classes, into a slab.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void xent_few_grad_kernel(const XentFew a, int dw_blocks, int d_tiles, int slice) {
     __shared__ __attribute__((aligned(16))) float part[4][16 * NB][64 + 4];

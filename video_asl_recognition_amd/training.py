@@ -138,7 +138,8 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
     x2, dy2, mean, rstd = _rows(x), _rows(dy), mean.contiguous(), rstd.contiguous()
     w = weight.contiguous() if weight is not None else None
     dx = _like(x)
-    dw, db = x.new_empty((2, d), dtype=weight.dtype if weight is not None else torch.float32).unbind(0)
+    dw = _like(weight) if weight is not None else x.new_empty(d, dtype=torch.float32)
+    db = torch.empty_like(dw)
     p = L.LayerNormParams(x2.shape[0], d, _ld(x2), _ld(dy2), d, xt, wt, _type(dy, "dy"), 0.0)
     ws = x.new_empty(_bytes(L.lib.asl_layernorm_bwd_workspace(C.byref(p)), "layer_norm_bwd"), dtype=torch.uint8)
     with _on(index):
