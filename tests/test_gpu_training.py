@@ -338,7 +338,7 @@ def test_linear_cross_entropy_leading_dimensions(gpu):
 def test_linear_cross_entropy_pieces(gpu):
     """more rows than one piece of exponentials holds"""
     for dt, v, n, d in ((BF16, 65536, 8192 + 300, 24), (F32, 65530, 4096 + 4100, 24), (BF16, 65600, 8192 + 300, 40), (F32, 70000, 3000, 40),
-                        (BF16, 70, 140000, 40), (F32, 70, 140000, 40)):
+                        (BF16, 70, 140000, 40), (F32, 70, 140000, 40), (BF16, 600, 140000, 64), (F32, 100, 140000, 64)):
         x, w, b, t = _xent_case(n, v, d, dt, F32, 0.1)
         _xent_check(x, w, b, t, smooth=0.1)
 
@@ -472,6 +472,25 @@ def test_linear_cross_entropy_writes_no_further_than_its_outputs(gpu, n, v, d, d
             assert (o[:3] == 7).all() and (o[-3:] == 7).all()
             assert (o == 7).all() if i == left_out else torch.equal(o[3:-3], q.flatten())
         assert (ws[:at] == 0x5a).all() and (ws[at + room:] == 0x5a).all()
+
+
+def test_linear_cross_entropy_pieces_of_a_large_vocabulary(gpu):
+    """more exponentials than a piece holds, against the formula taken a thousand rows at a time"""
+    from video_asl_recognition_amd import training as T
+    n, v, d = 33600, 65530, 32
+    x, w, b, t = _xent_case(n, v, d, BF16, F32, 0.1)
+    loss, dx, dw, db = T.linear_cross_entropy_grad(x, w, t, b, reduction="sum")
+    sums = [0.0] * 6
+    for i in range(0, n, 1000):
+        part = slice(i, i + 1000)
+        rows, trow, _, rdx, tdx, *rest = xent_reference(x[part], w, b, t[part], 1.0, -100, 0.0, "sum", True)[:9]
+        _ok(dx[part], rdx, tdx + 2.0 ** -8 * (rdx.abs() + tdx) + 1e-38, "dx")
+        sums = [p + q for p, q in zip(sums, [rows.sum(), trow.sum() + 30 * U32 * rows.abs().sum()] + rest)]
+    _ok(loss, sums[0], sums[1] + (n / 256 + 16) * U32 * sums[0], "loss")
+    # the bounds of a part's sums, and as many 32-bit additions as there are rows over all of them
+    over = 2 * n * U32
+    _ok(dw, sums[2], sums[3] * (1 + over) + over * sums[2].abs() + 2.0 ** -8 * (sums[2].abs() + sums[3]) + 1e-38, "dw")
+    _ok(db, sums[4], sums[5] * (1 + over) + over * sums[4].abs() + 1e-38, "db")
 
 
 def test_linear_cross_entropy_one_row_without_dimensions(gpu):
