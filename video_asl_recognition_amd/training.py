@@ -54,7 +54,8 @@ def _device(x: torch.Tensor, **tensors) -> int:
 
 def _countable(t: torch.Tensor, what: str):
     """the C parameters count rows and columns in 32 bits, and ctypes would cut a larger number without a word"""
-    if t.shape[-1] >> 31 or t.numel() // (t.shape[-1] or 1) >> 31:
+    d = t.shape[-1]
+    if d >> 31 or (t.numel() >> 31 and t.numel() // d >> 31):
         raise ValueError(f"{what} must be of fewer than 2^31 rows and columns, got {tuple(t.shape)}")
 
 
@@ -95,13 +96,13 @@ def _bytes(n: int, what: str) -> int:
 
 # ---------------------------------------------------------------------------------------------- LayerNorm
 def _check_norm(x, weight, bias):
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must be [..., d] with d >= 1, got {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"x must be [..., d] with d >= 1, got {tuple(shape)}")
     _countable(x, "x")
-    d = x.shape[-1]
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.dim() != 1 or t.shape[0] != d):
-            raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
+    d = shape[-1]
+    if (weight is not None and weight.shape != (d,)) or (bias is not None and bias.shape != (d,)):
+        raise ValueError(f"weight and bias must be [{d}], got {[None if t is None else tuple(t.shape) for t in (weight, bias)]}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight is {weight.dtype}, bias {bias.dtype}: one type for both")
     w = weight if weight is not None else bias
