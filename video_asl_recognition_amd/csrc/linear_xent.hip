@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256) void xent_count_kernel(const long long* target
 constexpr int kGradRows = 32;             // rows a workgroup of the G pass takes; it leaves one partial row of db
 constexpr int kGradCols = 256;            // and columns
 
-// tiles a row up to which the G pass takes the statistics for itself (1024 x 2000 x 512 bf16, 32 of them, with gradients 38.0 us and
+// tiles a row up to which the G pass takes the statistics for itself (1024 x 2000 x 512 bf16, 32 of them, with gradients 36.9 us and
 // 38.8; 1024 x 4000, 63, 48.2 and 46.1)
 constexpr int kOwnStats = 32;
 
@@ -450,15 +450,13 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
         }
     }
     if constexpr (OWN) {
-        const int l16 = threadIdx.x & 15, blocks = kGradCols >> a.tile_shift;
-#pragma unroll
-        for (int k = threadIdx.x >> 4; k < kGradRows; k += 16) {               // sixteen rows at once
-            if (b0 + k >= st.rows) {
-                if (l16 == 0) own_loss[k] = 0.f, own_kept[k] = 0;
-                continue;
-            }
-            const XentRow q = row_stats<16>(st, b0 + k, l16);
-            if (l16 == 0) {
+        const int l8 = threadIdx.x & 7, k = threadIdx.x >> 3, blocks = kGradCols >> a.tile_shift;
+        static_assert(kGradRows * 8 == 256, "eight lanes a row, all rows at once");
+        if (b0 + k >= st.rows) {
+            if (l8 == 0) own_loss[k] = 0.f, own_kept[k] = 0;
+        } else {
+            const XentRow q = row_stats<8>(st, b0 + k, l8);
+            if (l8 == 0) {
                 own_tg[k] = q.target_g;
                 own_g[k] = q.g;
                 own_loss[k] = q.loss;
@@ -468,9 +466,9 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
                     if (a.rows.lse) a.rows.lse[b0 + k] = q.lse;
                 }
             }
-            const int tile = blockIdx.x * blocks + l16;
-            if (l16 < blocks)
-                own_f[k][l16] = tile >= st.tiles ? 0.f
+            const int tile = blockIdx.x * blocks + l8;
+            if (l8 < blocks)
+                own_f[k][l8] = tile >= st.tiles ? 0.f
                                 : q.valid        ? q.g * a.rows.exp_unit * expf(st.tile_max[(long long)(b0 + k) * st.tiles + tile] - q.lse)
                                                  : NAN;
         }

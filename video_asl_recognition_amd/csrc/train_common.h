@@ -113,8 +113,9 @@ struct RawOf<short> {
     using type = bf16x8;
 };
 
-// Sum over each 16 lanes, then over the wave, the same in every lane: lane exchanges within the vector unit (data-parallel
+// Sum over each 16 lanes (or 8), then over the wave, the same in every lane: lane exchanges within the vector unit (data-parallel
 // primitives and the row swaps of gfx950), where a shuffle goes through the LDS.
+template <int LANES = 16>
 __device__ __forceinline__ float row16_sum(float v) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const auto with = [](float x, auto ctrl) {
@@ -123,10 +124,11 @@ __device__ __forceinline__ float row16_sum(float v) {
     v = with(v, std::integral_constant<int, 0xb1>{});        // lane ^ 1
     v = with(v, std::integral_constant<int, 0x4e>{});        // lane ^ 2
     v = with(v, std::integral_constant<int, 0x141>{});       // the other four of eight (mirrored)
-    v = with(v, std::integral_constant<int, 0x140>{});       // the other eight of sixteen (mirrored)
+    if constexpr (LANES == 16) v = with(v, std::integral_constant<int, 0x140>{});       // the other eight of sixteen (mirrored)
 #endif
     return v;
 }
+template <int LANES = 16>
 __device__ __forceinline__ float row16_max(float v) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const auto with = [](float x, auto ctrl) {
@@ -136,7 +138,7 @@ __device__ __forceinline__ float row16_max(float v) {
     v = with(v, std::integral_constant<int, 0xb1>{});
     v = with(v, std::integral_constant<int, 0x4e>{});
     v = with(v, std::integral_constant<int, 0x141>{});
-    v = with(v, std::integral_constant<int, 0x140>{});
+    if constexpr (LANES == 16) v = with(v, std::integral_constant<int, 0x140>{});
 #endif
     return v;
 }

@@ -65,7 +65,7 @@ struct XentRow {
     bool valid;                              // a label outside the vocabulary makes loss and gradients NaN
 };
 
-// LANES lanes (a wave, or a quarter of one) on a row: its tile maxima and sums to its statistics, in one pass, the running sum
+// LANES lanes (a wave, a quarter or an eighth of one) on a row: its tile maxima and sums to its statistics, in one pass, the running sum
 // rescaled where the maximum moves.
 template <int LANES>
 __device__ __forceinline__ XentRow row_stats(const XentStats& a, int row, int lane) {
@@ -89,8 +89,13 @@ __device__ __forceinline__ XentRow row_stats(const XentStats& a, int row, int la
         }
         if (a.smoothing != 0.f) lin += a.tile_lin[(long long)row * a.tiles + k];
     }
-    const auto sum = [](float v) { return LANES == 16 ? row16_sum(v) : wave64_sum(v); };
-    const float top = LANES == 16 ? row16_max(m) : wave_max(m);
+    const auto sum = [](float v) {
+        if constexpr (LANES == 64) return wave64_sum(v);
+        else return row16_sum<LANES>(v);
+    };
+    float top;
+    if constexpr (LANES == 64) top = wave_max(m);
+    else top = row16_max<LANES>(m);
     const float ref = top == -INFINITY ? 0.f : top;
     o.lse = ref + logf(sum(s * expf(m - ref)));
     o.loss = o.lse - lt;
