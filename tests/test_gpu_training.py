@@ -286,7 +286,7 @@ def test_linear_cross_entropy(gpu, n, v, d, dt):
 
 
 @pytest.mark.parametrize("n,v,d", [(256, 32768, 64), (300, 33001, 72), (257, 32769, 8), (513, 22000, 520), (1000, 8200, 256),
-                                   (8200, 1100, 192), (4100, 2049, 1032)])
+                                   (8200, 1100, 192), (4100, 2049, 1032), (2000, 8100, 1032), (1990, 8190, 1024)])
 def test_linear_cross_entropy_large_tiles(gpu, n, v, d):
     """sizes that take the 256 x 256 tiles: whole ones, cut ones, k that ends inside a step"""
     x, w, b, t = _xent_case(n, v, d, BF16, F32, 0.1)
@@ -298,7 +298,7 @@ def test_linear_cross_entropy_large_tiles(gpu, n, v, d):
 
 
 @pytest.mark.parametrize("n,v,d", [(256, 8192, 64), (300, 8211, 72), (1100, 1003, 200), (2100, 6000, 33), (64, 70000, 64), (256, 33000, 72),
-                                   (1100, 1003, 520), (2100, 6000, 63), (300, 8211, 264)])
+                                   (1100, 1003, 520), (2100, 6000, 63), (300, 8211, 264), (2000, 8100, 520)])
 def test_linear_cross_entropy_large_fp32(gpu, n, v, d):
     """sizes that take fp32 apart into bf16 planes: held to the bounds of fp32 products"""
     x, w, b, t = _xent_case(n, v, d, F32, F32, 0.1)
@@ -386,7 +386,7 @@ def test_linear_cross_entropy_masks_and_labels(gpu):
 # sizes for each way the products are computed: few rows, fp32 on 64 x 64 tiles, 128 x 128 and 256 x 256, fp32 as bf16 planes
 PATHS = [(12, 300, 40, BF16), (20, 300, 40, F32), (20, 4500, 40, F32), (9, 2100, 30, BF16), (80, 60, 64, BF16), (80, 300, 20, BF16), (80, 300, 64, F32), (70, 4000, 90, F32), (600, 1100, 260, F32),
          (20, 300, 40, BF16), (80, 300, 64, BF16), (400, 1000, 128, BF16), (400, 1003, 77, BF16), (1000, 8200, 256, BF16),
-         (520, 9001, 136, BF16), (600, 4100, 260, F32), (1100, 8200, 65, F32), (9000, 250, 64, BF16)]
+         (520, 9001, 136, BF16), (600, 4100, 260, F32), (1100, 8200, 65, F32), (9000, 250, 64, BF16), (2000, 8100, 1024, BF16), (2000, 8100, 520, F32)]
 PATH_IDS = [f"{n}x{v}x{d}-{'f32' if dt == F32 else 'bf16'}" for n, v, d, dt in PATHS]
 
 
