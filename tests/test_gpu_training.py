@@ -317,6 +317,10 @@ def test_linear_cross_entropy_bias_types_and_strides(gpu):
     _xent_check(x, w, b, t)
     x, w, b, t = _xent_case(70, 150, 96, F32, BF16, 0.2)
     _xent_check(x, w, b, t)
+    for n, v in ((9, 150), (9, 2500), (30, 400)):
+        for dt, bt in ((BF16, F32), (F32, BF16)):
+            x, w, b, t = _xent_case(n, v, 96, dt, bt, 0.2)
+            _xent_check(x, w, b, t, smooth=0.1)
     for dt in (F32, BF16):
         x, w, b, t = _xent_case(70, 150, 96, dt, dt, 0.2)
         xb, wb = torch.zeros(70, 131, dtype=dt, device="cuda"), torch.zeros(300, 99, dtype=dt, device="cuda")
