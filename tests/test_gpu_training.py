@@ -852,3 +852,44 @@ def test_two_graphs_share_a_workspace(gpu, n, v, d, dt):
         graphs[turn][0].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got[turn], want[turn]))
+
+
+# ------------------------------------------------------------------------------------------------ rows that are nearly certain
+@pytest.mark.parametrize("offset", [0.0, 60.0, -60.0, 4000.0])
+@pytest.mark.parametrize("n,v,d,dt", PATHS, ids=PATH_IDS)
+def test_linear_cross_entropy_of_nearly_certain_rows(gpu, n, v, d, dt, offset):
+    """How unsure a row is (1 - p of some 2^-18) has the error of numbers near 1, however far all its logits lie from nought.
+
+    Every logit is exact: features are rows of the unit matrix, W's entries and the offset are numbers of few bits.  A row has its
+    target at the offset, two classes e^-12.75 and less below it, and the others at -200, whose exponentials are nought.  So the
+    sum, 1 + u, takes two additions that round, each by half a step of a number in [1, 2), u32; the logarithm and the exponential
+    minus one are small numbers with relative errors of a few u32 (a third u32 covers them many times); u itself is a sum of two
+    exponentials, good to 2^-15 of themselves (the fast one: its argument times log2 e, rounded below 32, is off by 2^-20)."""
+    from video_asl_recognition_amd import training as T
+    P = min(d, v // 3, 16)
+    step = v // (3 * P)
+    at = torch.arange(P, device="cuda")
+    gap = 12.75 + 0.25 * (at % 8)
+    w = torch.zeros(v, d, device="cuda")
+    w[:, :P] = -200.0
+    w[3 * at * step, at] = 0.0
+    w[(3 * at + 1) * step, at] = -gap
+    w[(3 * at + 2) * step, at] = -gap - 0.75
+    row = torch.arange(n, device="cuda") % P
+    x = torch.zeros(n, d, device="cuda")
+    x[torch.arange(n, device="cuda"), row] = 1.0
+    t = 3 * row * step
+    x, w, b = x.to(dt), w.to(dt), torch.full((v,), offset, device="cuda")
+    first, second = torch.exp(-gap.double()), torch.exp(-gap.double() - 0.75)
+    u = first + second
+    tol = 3 * U32 + 2.0 ** -15 * u
+    for loss, lse in (T.linear_cross_entropy_fwd(x, w, t, b, reduction="none"), (T.linear_cross_entropy_grad(x, w, t, b, reduction="none")[0], None)):
+        _ok(loss, torch.log1p(u)[row], tol[row], "loss")
+        if lse is not None:
+            _ok(lse, offset + torch.log1p(u)[row], tol[row] + U32 * abs(offset), "lse")
+    db = T.linear_cross_entropy_grad(x, w, t, b, reduction="sum")[3]
+    rows = torch.bincount(row, minlength=P).double()
+    for classes, grad, off in ((3 * at * step, -u / (1 + u), tol), ((3 * at + 1) * step, first / (1 + u), first), ((3 * at + 2) * step, second / (1 + u), second)):
+        if off is not tol:                                        # p: its exponential, and for bf16 operands that held as fp16
+            off = off * (2.0 ** -15 + (2.0 ** -11 if dt == BF16 else 0.0)) + off * tol
+        _ok(db[classes], rows * grad, rows * off + (n + 40) * U32 * rows * grad.abs(), "db")

@@ -10,8 +10,8 @@
 // tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself (fp32, or for bf16 operands
 // fp16 of 2^15 times it: 11 bits of the value down to 2^-29 of the tile's largest, and 2^-40 of that below).  One pass over the
 // per-tile numbers gives lse, the loss and the factors g exp(m - lse); one pass over the exponentials turns them into G in
-// place, the target's entry from its own 32-bit logit (g expm1(l_t - lse), where p - 1 of a rounded p would cancel), and adds
-// up db in 32 bits.  Then two products, whose sums are finished (slabs, db, the loss) by one more launch where there is need.
+// place, the target's entry from its own 32-bit logit (g expm1((l_t - max) - log sum exp(l - max)), where p - 1 of a rounded p,
+// or l_t - lse of a rounded lse, would cancel), and adds up db in 32 bits.  Then two products, whose sums are finished (slabs, db, the loss) by one more launch where there is need.
 //
 // What bounds it is the products where they are large (8192 x 32768 x 2048 bf16: 2.82 ms with gradients, 3.3 PFLOP at 1.17
 // PFLOP/s: the three products 2.63 ms, G 0.19 ms at 5.5 TB/s), the matrix pipe's rate for six bf16 products in the place of one
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
             loss[at] = r.loss;
             kept[at] = a.st.target[row] != a.st.ignore;
             if (a.loss) a.loss[row] = r.loss;
-            if (a.lse) a.lse[row] = r.lse;
+            if (a.lse) a.lse[row] = r.lse();
             if (a.factor) {
                 a.target_g[row] = r.target_g;
                 a.row_g[row] = r.g;
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const XentRows a) {
         if (a.factor)
             for (int t = lane; t < a.st.tiles; t += LANES) {
                 const long long k = (long long)row * a.st.tiles + t;
-                a.factor[k] = r.valid ? r.g * a.exp_unit * expf(a.st.tile_max[k] - r.lse) : NAN;
+                a.factor[k] = r.valid ? r.g * a.exp_unit * r.exp_of(a.st.tile_max[k]) : NAN;
             }
     } else if (lane == 0) {
         loss[at] = 0.f;
@@ -463,13 +463,13 @@ __global__ __launch_bounds__(256) void xent_g_kernel(const XentG a) {
                 own_kept[k] = st.target[b0 + k] != st.ignore;
                 if (blockIdx.x == 0) {
                     if (a.rows.loss) a.rows.loss[b0 + k] = q.loss;
-                    if (a.rows.lse) a.rows.lse[b0 + k] = q.lse;
+                    if (a.rows.lse) a.rows.lse[b0 + k] = q.lse();
                 }
             }
             const int tile = blockIdx.x * blocks + l8;
             if (l8 < blocks)
                 own_f[k][l8] = tile >= st.tiles ? 0.f
-                                : q.valid        ? q.g * a.rows.exp_unit * expf(st.tile_max[(long long)(b0 + k) * st.tiles + tile] - q.lse)
+                                : q.valid        ? q.g * a.rows.exp_unit * q.exp_of(st.tile_max[(long long)(b0 + k) * st.tiles + tile])
                                                  : NAN;
         }
         if (blockIdx.x == 0) leave_part(a.rows, blockIdx.y, own_loss, own_kept);

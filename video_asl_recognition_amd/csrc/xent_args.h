@@ -60,9 +60,15 @@ struct XentStats {
     float smoothing, inv_classes;
     int rows, classes, tiles;
 };
+// log sum exp stays in two parts, the largest logit and the logarithm of the sum relative to it.  Only the lse that a caller
+// reads is their sum: rounded to 32 bits it is off by up to 2^-24 of itself, which is not little beside the 1 - p of a row that is
+// nearly certain (half of it at an lse of 60 and 1 - p = 2^-18), and loss and G taken from it would be off by that.
 struct XentRow {
-    float lse, loss, g, target_g;            // g: the row's own weight, nought for an ignored row; target_g: G at the target
+    float top, rest;                         // lse = top + rest
+    float loss, g, target_g;                 // g: the row's own weight, nought for an ignored row; target_g: G at the target
     bool valid;                              // a label outside the vocabulary makes loss and gradients NaN
+    __device__ __forceinline__ float lse() const { return top + rest; }
+    __device__ __forceinline__ float exp_of(float l) const { return expf((l - top) - rest); }    // exp(l - lse)
 };
 
 // LANES lanes (a wave, a quarter or an eighth of one) on a row: its tile maxima and sums to its statistics, in one pass, the running sum
@@ -96,12 +102,13 @@ __device__ __forceinline__ XentRow row_stats(const XentStats& a, int row, int la
     float top;
     if constexpr (LANES == 64) top = wave_max(m);
     else top = row16_max<LANES>(m);
-    const float ref = top == -INFINITY ? 0.f : top;
-    o.lse = ref + logf(sum(s * expf(m - ref)));
-    o.loss = o.lse - lt;
-    if (a.smoothing != 0.f) o.loss = o.lse - (1.f - a.smoothing) * lt - a.smoothing * a.inv_classes * sum(lin);
+    o.top = top == -INFINITY ? 0.f : top;
+    o.rest = logf(sum(s * expf(m - o.top)));
+    const float above = lt - o.top;
+    o.loss = o.rest - above;
+    if (a.smoothing != 0.f) o.loss = o.rest - (1.f - a.smoothing) * above - a.smoothing * (a.inv_classes * sum(lin) - o.top);
     if (!kept) o.loss = 0.f;
-    o.target_g = o.g * (expm1f(lt - o.lse) + a.smoothing - a.smoothing * a.inv_classes);
+    o.target_g = o.g * (expm1f(above - o.rest) + a.smoothing - a.smoothing * a.inv_classes);
     return o;
 }
 

@@ -142,12 +142,12 @@ __global__ __launch_bounds__(256) void xent_few_g_kernel(const XentFew a) {
             row_g[row] = r.g;
             if (blockIdx.x == 0) {
                 if (a.none) a.loss[row] = r.loss;
-                if (a.lse) a.lse[row] = r.lse;
+                if (a.lse) a.lse[row] = r.lse();
             }
         }
         if (l16 < TPB) {
             const int tile = blockIdx.x * TPB + l16;
-            if (tile < a.tiles) fac[row][l16] = r.valid ? r.g * expf(a.tile_max[(long long)row * a.tiles + tile] - r.lse) : NAN;
+            if (tile < a.tiles) fac[row][l16] = r.valid ? r.g * r.exp_of(a.tile_max[(long long)row * a.tiles + tile]) : NAN;
         }
     }
     __syncthreads();
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64) void xent_few_dx_kernel(const XentFew a, int sl
 // 64 classes x 256 features, 16 x 64 a wave, and (those of the first features) db.
 template <typename T, int NB>
 __global__ __launch_bounds__(1024) void xent_few_rest_kernel(const XentFew a, int dx_blocks, int d_tiles) {
-    __shared__ float lse[kFewRows], target_g[kFewRows], row_g[kFewRows], loss_row[kFewRows];
+    __shared__ float top[kFewRows], rest[kFewRows], target_g[kFewRows], row_g[kFewRows], loss_row[kFewRows];
     __shared__ int label[kFewRows];                          // the target's class; -1: outside the vocabulary, -2: ignored
     __shared__ __attribute__((aligned(16))) float part[16][16 * NB][16 + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
@@ -309,17 +309,18 @@ __global__ __launch_bounds__(1024) void xent_few_rest_kernel(const XentFew a, in
     st.inv_classes = a.inv_classes; st.rows = a.n; st.classes = a.classes; st.tiles = a.tiles;
     const int mine = threadIdx.x >> 4;                       // sixteen lanes a row, all rows at once
     if (mine < kFewRows) {
-        XentRow r = {0.f, 0.f, 0.f, 0.f, true};
+        XentRow r = {0.f, 0.f, 0.f, 0.f, 0.f, true};
         if (mine < a.n) r = row_stats<16>(st, mine, fr);
         if (fr == 0) {
-            lse[mine] = r.lse;
+            top[mine] = r.top;
+            rest[mine] = r.rest;
             target_g[mine] = r.target_g;
             row_g[mine] = r.valid ? r.g : NAN;
             loss_row[mine] = r.loss;
             label[mine] = mine >= a.n || a.target[mine] == a.ignore ? -2 : r.valid ? (int)a.target[mine] : -1;
             if (blockIdx.x == 0 && mine < a.n) {
                 if (a.none) a.loss[mine] = r.loss;
-                if (a.lse) a.lse[mine] = r.lse;
+                if (a.lse) a.lse[mine] = r.lse();
             }
         }
     }
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(1024) void xent_few_rest_kernel(const XentFew a, in
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const int row = j * 16 + fr;
-                    const float f = row_g[row] * expf(m[u][j] - lse[row]);
+                    const float f = row_g[row] * expf((m[u][j] - top[row]) - rest[row]);
 #pragma unroll
                     for (int s = 0; s < 8; ++s) acc[j] = mma4(v + s < a.classes ? wf[u][s] : 0.f, grad(e[u][j].v[s], f, row, v + s), acc[j]);
                 }
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(1024) void xent_few_rest_kernel(const XentFew a, in
 #pragma unroll
     for (int u = 0; u < 4 * NB; ++u) {
         const int k = u * 4 + fq;
-        gf[u] = col < a.classes ? grad(ef[u], row_g[k] * expf(mf[u] - lse[k]), k, col) : 0.f;
+        gf[u] = col < a.classes ? grad(ef[u], row_g[k] * expf((mf[u] - top[k]) - rest[k]), k, col) : 0.f;
         db += gf[u];
     }
     if (a.dw) {
