@@ -893,3 +893,43 @@ def test_linear_cross_entropy_of_nearly_certain_rows(gpu, n, v, d, dt, offset):
         if off is not tol:                                        # p: its exponential, and for bf16 operands that held as fp16
             off = off * (2.0 ** -15 + (2.0 ** -11 if dt == BF16 else 0.0)) + off * tol
         _ok(db[classes], rows * grad, rows * off + (n + 40) * U32 * rows * grad.abs(), "db")
+
+
+# ------------------------------------------------------------------------------------------------ what autograd sees of clipping
+def test_clipping_raises_the_versions_of_what_it_writes(gpu):
+    """a tensor that some backward still needs cannot be clipped unseen, as with torch's own in-place product"""
+    from video_asl_recognition_amd import training as T
+    for sizes in (((40,), (7, 9)), ((3000, 40), (7, 9))):         # one launch, and two
+        leaf = [torch.randn(s, device="cuda", requires_grad=True) for s in sizes]
+        for how in ("grads", "out", "parameters"):
+            saved = [torch.randn(s, device="cuda") for s in sizes]
+            other = [torch.randn(s, device="cuda") for s in sizes]
+            y = sum((a * s).sum() for a, s in zip(leaf, saved))    # its backward needs `saved`
+            before = [t._version for t in saved + other]
+            T.grad_norm(saved)                                    # reads only
+            assert before == [t._version for t in saved + other]
+            if how == "grads":
+                T.clip_grads(saved, 0.01)
+            elif how == "out":
+                T.clip_grads(other, 0.01, out=saved)
+            else:
+                ps = [torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in sizes]
+                for p, s in zip(ps, saved):
+                    p.grad = s
+                T.clip_grad_norm_(ps, 0.01)
+            assert all(t._version > v for t, v in zip(saved, before)) and [t._version for t in other] == before[len(sizes):]
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    # second gradients: the first ones are part of the graph
+    w = torch.randn(50, device="cuda", requires_grad=True)
+    first, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    penalty = first.square().sum()
+    T.clip_grads([first], 0.01)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        penalty.backward()
+    # tensors without a version counter are clipped as before
+    with torch.inference_mode():
+        g = torch.ones(9, device="cuda")
+        T.clip_grads([g], 0.5)
+    T.clip_grads([g], 0.25)
+    assert abs(float(g.norm()) - 0.25) < 1e-6

@@ -332,6 +332,8 @@ def _clip(grads: Sequence[torch.Tensor], max_norm, norm_type, out: Optional[Sequ
         L.check(L.lib.asl_grad_clip(n, addr(ptrs), addr(numel), addr(types), addr(optrs), addr(otypes),
                                     0.0 if max_norm is None else float(max_norm), int(norm_type != 2), norm.data_ptr(), ws.data_ptr(),
                                     _stream(index)), "clip_grads")
+    if otypes is not None:              # written through their addresses: a backward that still needs one of them has to be told
+        torch.autograd.graph.increment_version(grads if out is None else out)
     return norm
 
 
@@ -346,7 +348,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
                out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensor for tensor, fp32 or bf16 each, of
     the same strides or both contiguous: bf16 gradients into an optimizer's fp32 buffers in the same pass), and returns the
-    norm they had.  Tensors that are written may not overlap, each other or a gradient that is not their own.  NaN in, NaN out."""
+    norm they had.  Tensors that are written may not overlap, each other or a gradient that is not their own; autograd sees them as
+    written in place.  NaN in, NaN out."""
     return _clip(grads, max_norm, norm_type, out)
 
 
