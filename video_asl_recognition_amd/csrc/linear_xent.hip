@@ -624,7 +624,7 @@ inline long long slab_ld(int d, int tile) { return (long long)ceil_div(d, tile) 
 // 31, 27).
 inline bool takes_few(const asl_xent_params& p) {
     if (!p.n || p.classes > kFewClasses) return false;
-    return p.type ? p.n <= 16 && (double)p.classes * p.d <= (double)(1 << 20) : p.n <= kFewRows;
+    return p.type ? p.n <= kFewRows16 && (double)p.classes * p.d <= (double)(1 << 20) : p.n <= kFewRows;
 }
 
 // Tile and slices of a product with `a` x `b` results over `k`: what its tiles take one after another on the 256 CUs, against

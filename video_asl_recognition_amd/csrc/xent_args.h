@@ -112,8 +112,8 @@ __device__ __forceinline__ XentRow row_stats(const XentStats& a, int row, int la
     return o;
 }
 
-// xent_few.hip: up to 32 rows
-constexpr int kFewRows = 32, kFewTile = 32, kFewClasses = 16384;
+// xent_few.hip: up to 32 rows, of bf16 up to 16
+constexpr int kFewRows = 32, kFewRows16 = 16, kFewTile = 32, kFewClasses = 16384;      // rows of fp32, and of bf16
 struct XentFew {
     const void* x;
     const void* w;

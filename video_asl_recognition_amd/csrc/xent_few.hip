@@ -467,7 +467,9 @@ void xent_few_logits(const XentFew& a, hipStream_t s) {
 }
 
 int xent_few(const XentFew& a, int type, hipStream_t s) {
-    if (type) return a.n <= 16 ? run_few<short, 1>(a, s) : run_few<short, 2>(a, s);
+    static_assert(kFewRows16 <= 16 && kFewRows <= 32, "halves of 16 rows");
+    if (a.n > (type ? kFewRows16 : kFewRows)) return ASL_EINVAL;
+    if (type) return run_few<short, 1>(a, s);
     return a.n <= 16 ? run_few<float, 1>(a, s) : run_few<float, 2>(a, s);
 }
 
