@@ -35,6 +35,10 @@ class HeadTuner:
         self._norm = [self.params[n] for n in names[2:]]           # the last LayerNorm's weight and bias, if it is trained
         self.grad_norm: Optional[torch.Tensor] = None              # of the last step, before clipping
 
+    def _here(self):
+        """the forward launches on the current device's stream, the training operators on their tensors': one and the same here"""
+        return torch.cuda.device(self._fc_w.device)
+
     def _features(self, clips, keypoints):
         """(features of the Linear [B, F], and for the transformer what the norm's backward needs)"""
         if any(p is not self.params.get(n) for n, p in self.model.head_parameters().items()):
@@ -52,27 +56,30 @@ class HeadTuner:
     @torch.no_grad()
     def gradients(self, clips: torch.Tensor, target: torch.Tensor, keypoints: Optional[torch.Tensor] = None):
         """(loss, {name: gradient}) of the mean cross entropy of clips [B,T,3,S,S] against target int64 [B]"""
-        feats, saved = self._features(clips, keypoints)
-        loss, dfeats, dw, db = training.linear_cross_entropy_grad(feats, self._fc_w, target.to(feats.device), self._fc_b, **self._how)
-        grads = [dw, db]
-        if saved is not None:
-            x, mean, rstd, T = saved
-            dy = (dfeats / T)[:, None].expand(-1, T, -1).reshape(x.shape)      # the mean over T hands every frame its share
-            grads += training.layer_norm_bwd(dy, x, self._norm[0], mean, rstd)[1:]
-        return loss, dict(zip(self.params, grads))
+        with self._here():
+            feats, saved = self._features(clips, keypoints)
+            loss, dfeats, dw, db = training.linear_cross_entropy_grad(feats, self._fc_w, target.to(feats.device), self._fc_b, **self._how)
+            grads = [dw, db]
+            if saved is not None:
+                x, mean, rstd, T = saved
+                dy = (dfeats / T)[:, None].expand(-1, T, -1).reshape(x.shape)      # the mean over T hands every frame its share
+                grads += training.layer_norm_bwd(dy, x, self._norm[0], mean, rstd)[1:]
+            return loss, dict(zip(self.params, grads))
 
     @torch.no_grad()
     def loss(self, clips: torch.Tensor, target: torch.Tensor, keypoints: Optional[torch.Tensor] = None) -> torch.Tensor:
         """the mean loss alone (validation)"""
-        feats, _ = self._features(clips, keypoints)
-        return training.linear_cross_entropy_fwd(feats, self._fc_w, target.to(feats.device), self._fc_b, **self._how)[0]
+        with self._here():
+            feats, _ = self._features(clips, keypoints)
+            return training.linear_cross_entropy_fwd(feats, self._fc_w, target.to(feats.device), self._fc_b, **self._how)[0]
 
     @torch.no_grad()
     def step(self, clips: torch.Tensor, target: torch.Tensor, keypoints: Optional[torch.Tensor] = None) -> torch.Tensor:
         """one update; returns the loss before it"""
         loss, grads = self.gradients(clips, target, keypoints)
         if self.max_norm is not None:
-            self.grad_norm = training.clip_grads(list(grads.values()), self.max_norm)
+            with self._here():
+                self.grad_norm = training.clip_grads(list(grads.values()), self.max_norm)
         for name, p in self.params.items():
             p.grad = grads[name]
         self.optimizer.step()
