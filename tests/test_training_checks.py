@@ -196,3 +196,13 @@ def test_python_refuses():
     with pytest.raises(ValueError, match="weight"):
         T.linear_cross_entropy(x, torch.zeros(5, 7), t)
     assert not T._dense(torch.zeros(4, 4)[:, :2]) and T._dense(torch.zeros(4, 3).t()) and not T._dense(torch.zeros(1).expand(4))
+
+
+def test_python_refuses_an_ignored_label_that_64_bits_do_not_hold():
+    """a C field would take its low 64 bits: 2^64 - 100 would ignore label -100"""
+    from video_asl_recognition_amd import training as T
+    x, w, t = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64)
+    for ignore in ((1 << 64) - 100, 1 << 63, -(1 << 63) - 1):
+        for call in (T.linear_cross_entropy, T.linear_cross_entropy_fwd, T.linear_cross_entropy_grad):
+            with pytest.raises(ValueError, match="ignore_index"):
+                call(x, w, t, ignore_index=ignore)

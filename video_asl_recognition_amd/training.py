@@ -193,6 +193,8 @@ def _check_xent(x, weight, target, bias, reduction, label_smoothing):
 
 
 def _xent(x, weight, target, bias, ignore_index, label_smoothing, reduction):
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"ignore_index must be a 64-bit number, got {ignore_index}")
     index = _check_xent(x, weight, target, bias, reduction, label_smoothing)
     x2, w2, t = _rows(x), _rows(weight), target.contiguous()
     b = bias.contiguous() if bias is not None else None
