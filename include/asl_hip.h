@@ -499,8 +499,8 @@ int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void*
  *   asl_linear_xent_grad also writes dx [n][d], dw [classes][d] (dense, of `type`) and dbias [classes] (of bias_type), each
  *   NULL if not wanted.  upstream is the gradient of the loss: fp32, one value, or [n] for ASL_REDUCE_NONE; NULL stands for 1.
  * A bias of -inf masks a class.  A target outside [0, classes) that is not ignore_index makes the loss, the row's dx and
- * every dw NaN rather than being read.  An ignored row of x still meets its gradient of nought in dw: it has to be finite, as
- * w has to be (0 * inf is NaN).  Outputs overlap neither each other nor an input.  workspace: 256-byte aligned,
+ * every dw NaN rather than being read.  An ignored row of x still meets its gradient of nought in dw: for the gradients it
+ * has to be finite, as w has to be (0 * inf is NaN); the loss alone takes infinite weights, whose logits are infinite.  Outputs overlap neither each other nor an input.  workspace: 256-byte aligned,
  * asl_linear_xent_workspace(p, x, w, grad) bytes -- at most about 4 GiB of exponentials at a time (or 256 rows of them) plus
  * what sums need; x and w are looked at for their alignment only (bf16 operands off 16 bytes, or with d no multiple of 64,
  * are copied there first, fp32 ones of large problems split into bf16 parts).  A negative return is an ASL_E* code; classes

@@ -933,3 +933,34 @@ def test_clipping_raises_the_versions_of_what_it_writes(gpu):
         T.clip_grads([g], 0.5)
     T.clip_grads([g], 0.25)
     assert abs(float(g.norm()) - 0.25) < 1e-6
+
+
+@pytest.mark.parametrize("n,v,d,dt", PATHS, ids=PATH_IDS)
+def test_linear_cross_entropy_infinite_weights(gpu, n, v, d, dt):
+    """a weight of -inf against positive features makes its class's logits -inf, as a bias of -inf does, on every path; NaN
+    weights and +inf are loud; only rows that meet them are touched"""
+    from video_asl_recognition_amd import training as T
+    x, w, b, t = _xent_case(n, v, d, dt, F32, 0.1)
+    k, lo, hi = d - 1, v // 4, v - 5
+    x[:, k] = x[:, k].abs() + 0.25
+    t = torch.where((t >= lo) & (t < hi), t % lo, t)
+    masked = b.clone()
+    masked[lo:hi] = float("-inf")
+    winf = w.clone()
+    winf[lo:hi, k] = float("-inf")
+    for reduction in ("none", "mean"):
+        loss, lse = T.linear_cross_entropy_fwd(x, winf, t, b, reduction=reduction, label_smoothing=0.0)
+        want, want_lse = T.linear_cross_entropy_fwd(x, w, t, masked, reduction=reduction, label_smoothing=0.0)
+        assert want.isfinite().all() and torch.equal(loss, want) and torch.equal(lse, want_lse)
+    for bad in (float("nan"), float("inf")):
+        wb = w.clone()
+        wb[lo, k] = bad
+        loss, lse = T.linear_cross_entropy_fwd(x, wb, t, b, reduction="none")
+        kept = t != -100
+        assert not loss[kept].isfinite().any() and not loss[~kept].any() and not lse.isfinite().any()
+    # an infinite feature concerns its own row
+    xi = x.clone()
+    xi[0, k] = float("inf")
+    loss, lse = T.linear_cross_entropy_fwd(xi, w, t, b, reduction="none")
+    want, want_lse = T.linear_cross_entropy_fwd(x, w, t, b, reduction="none")
+    assert not lse[0].isfinite() and torch.equal(loss[1:], want[1:]) and torch.equal(lse[1:], want_lse[1:])

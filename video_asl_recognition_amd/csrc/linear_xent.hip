@@ -391,21 +391,22 @@ __device__ __forceinline__ F8 load8_exp(const _Float16* p) {
     return r;
 }
 
-// fp32 as the sum of three bf16, each the rest's nearest.  Infinities and NaN lie in the first alone; a value that would round
-// to infinity is cut instead.
+// fp32 as the sum of three bf16, each the rest's nearest.  Infinities and NaN lie in the last alone, which meets the other operand's
+// first and nothing else: in the first they would meet its noughts and differences of either sign, and an infinite product
+// would be NaN.  A value that would round to infinity is cut instead.
 __device__ __forceinline__ void store_planes(short* p, long long plane, const F8& v) {
     bf16x8 h, m, l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float x = v.v[e];
+        const bool finite = fabsf(x) < INFINITY;
         short a = f32_to_bf16(x);
-        if (!(fabsf(bf16_to_f32(a)) < INFINITY)) a = fabsf(x) < INFINITY ? (short)(__builtin_bit_cast(unsigned, x) >> 16) : a;
-        float rest = x - bf16_to_f32(a);
-        if (!(fabsf(x) < INFINITY)) rest = 0.f;
+        if (!(fabsf(bf16_to_f32(a)) < INFINITY)) a = finite ? (short)(__builtin_bit_cast(unsigned, x) >> 16) : 0;
+        const float rest = finite ? x - bf16_to_f32(a) : 0.f;
         const short b = f32_to_bf16(rest);
         h[e] = a;
         m[e] = b;
-        l[e] = f32_to_bf16(rest - bf16_to_f32(b));
+        l[e] = f32_to_bf16(finite ? rest - bf16_to_f32(b) : x);
     }
     *(bf16x8*)p = h;
     *(bf16x8*)(p + plane) = m;
