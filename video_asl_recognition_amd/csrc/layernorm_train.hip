@@ -72,7 +72,7 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* lds, int& slot) 
 // Vector j of lane t begins at column (t + j G) 8, but the one that would reach over the row's end ends with it: it shares its
 // first `lead` columns with its neighbour, which takes them for the sums, and both write them, the same.  So every access is a
 // whole vector, in rows of at least eight elements, and none branches by lane (2^26 bf16 elements, backward: rows of 500 80 us,
-// with a last vector loaded by element 214; rows of 2047 105 and 190).
+// with a last vector loaded by element 214; rows of 2047 109 and 190).
 template <int G, int J>
 struct Columns {
     int at[J], lead[J];
@@ -496,9 +496,11 @@ inline LnShape bwd_shape(int d) {
 constexpr int kColsWith = 8192;           // longest row whose column sums go along
 inline int rows_per_block(int g) { return g == 0 || g > 256 ? 1 : 256 / g; }
 
-// workgroups of a backward call = partial rows of its column sums: two a CU, so that the partial rows stay small against the
-// tensors, or four where a workgroup has but one row under way, of less than 8 KB of x and dy (2^26 elements, bf16 rows of
-// 1280: 85 us, with two 116; fp32 143 with two, 157 with four)
+// Workgroups of a backward call = partial rows of its column sums: two a CU, so that the partial rows stay small against the
+// tensors, or four for bf16 rows of 1025 to 1919, of which a workgroup has but one, and a short one, under way.  Two and four,
+// 2^26 elements: bf16 rows of 1280 115 and 85 us, 1536 99 and 83, 1792 86 and 82, 1920 83 and 81, 2040 81 and 87, 2048 79 and 83;
+// 2^23 elements: 1280 21.3 and 19.5, 1792 18.6 and 18.7, 2040 18.3 and 20.8.  fp32 x and bf16 dy: 1025 154 and 151, 1200 136
+// and 141, 1800 141 and 140; fp32 both: 1280 152 and 160, 2048 149 and 159.
 inline int bwd_blocks(const asl_layernorm_params& p) {
     const int rows = p.rows, d = p.d;
     if (d > kColsWith) {                  // ln_cols_kernel: eight workgroups a CU, each of at least 16 rows
@@ -506,7 +508,7 @@ inline int bwd_blocks(const asl_layernorm_params& p) {
         return need < most ? need : most;
     }
     const LnShape sh = bwd_shape(d);
-    const int rpb = rows_per_block(sh.g), most = sh.g == 256 && sh.j == 1 && d * ((p.x_type ? 2 : 4) + (p.y_type ? 2 : 4)) < 8192 ? 1024 : 512;
+    const int rpb = rows_per_block(sh.g), most = sh.g == 256 && sh.j == 1 && p.x_type && p.y_type && d < 1920 ? 1024 : 512;
     const long long need = ((long long)rows + rpb - 1) / rpb;
     return (int)(need < most ? need : most);
 }
