@@ -491,8 +491,10 @@ int64_t asl_layernorm_bwd_workspace(const asl_layernorm_params* p);
 int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void* x, const void* gamma, const float* mean,
                       const float* rstd, void* dx, void* dgamma, void* dbeta, float* workspace, asl_stream_t stream);
 
-/* F.cross_entropy(F.linear(x, w, bias), target, ignore_index, reduction, label_smoothing), and its gradients, without
- * holding the logits: x [n][ld_x] and w [classes][ld_w] are of `type`, bias (NULL: none) of bias_type, target int64 [n].
+/* F.cross_entropy(F.linear(x, w, bias), target, ignore_index, reduction, label_smoothing), and its gradients.  The loss alone
+ * holds no logits; the gradients are computed from exponentials of as many rows at a time as the workspace holds (bf16: as
+ * fp16, and G, the gradient of the logits, as bf16, but for up to 16 rows and 2^20 weights; fp32: as fp32).
+ *   x [n][ld_x] and w [classes][ld_w] are of `type`, bias (NULL: none) of bias_type, target int64 [n].
  *   loss: fp32, one value, or [n] for ASL_REDUCE_NONE.  ASL_REDUCE_MEAN divides by the rows whose target is not
  *         ignore_index (none of them: NaN, as 0 / 0); ignored rows have loss 0 and gradient 0.
  *   lse:  fp32 [n], log sum exp of each row's logits (NULL: not wanted).
@@ -500,11 +502,12 @@ int asl_layernorm_bwd(const asl_layernorm_params* p, const void* dy, const void*
  *   NULL if not wanted.  upstream is the gradient of the loss: fp32, one value, or [n] for ASL_REDUCE_NONE; NULL stands for 1.
  * A bias of -inf masks a class.  A target outside [0, classes) that is not ignore_index makes the loss, the row's dx and
  * every dw NaN rather than being read.  An ignored row of x still meets its gradient of nought in dw: for the gradients it
- * has to be finite, as w has to be (0 * inf is NaN); the loss alone takes infinite weights, whose logits are infinite.  Outputs overlap neither each other nor an input.  workspace: 256-byte aligned,
- * asl_linear_xent_workspace(p, x, w, grad) bytes -- at most about 4 GiB of exponentials at a time (or 256 rows of them) plus
- * what sums need; x and w are looked at for their alignment only (bf16 operands off 16 bytes, or with d no multiple of 64,
- * are copied there first, fp32 ones of large problems split into bf16 parts).  A negative return is an ASL_E* code; classes
- * above 2^21, d above 2^20, classes * d above 2^34 or n above 2^28 return ASL_ETOOBIG. */
+ * has to be finite, as w has to be (0 * inf is NaN); the loss alone takes infinite weights, whose logits are infinite.
+ * Outputs overlap neither each other nor an input.  workspace: 256-byte aligned, asl_linear_xent_workspace(p, x, w, grad)
+ * bytes -- at most about 4 GiB of exponentials at a time (or 256 rows of them; large fp32 problems' G as three bf16 parts
+ * counted in) plus what sums need; x and w are looked at for their alignment only (bf16 operands off 16 bytes, or with d no
+ * multiple of 64, are copied there first, fp32 ones of large problems split into bf16 parts).  A negative return is an ASL_E*
+ * code; classes above 2^21, d above 2^20, classes * d above 2^34 or n above 2^28 return ASL_ETOOBIG. */
 enum { ASL_REDUCE_NONE = 0, ASL_REDUCE_SUM = 1, ASL_REDUCE_MEAN = 2 };
 typedef struct asl_xent_params {
     int32_t n, classes, d;

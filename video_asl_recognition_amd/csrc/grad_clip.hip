@@ -172,8 +172,8 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const ClipArgs a) {
 }
 
 // A few small tensors in one launch: one workgroup reads them once and holds them in registers, a wave up to four slots of 1024
-// elements, sixteen a lane.  Four tensors of 16 K elements in all take 5.0 us as a graph and 14.0 as a call, of 52 K 7.8 and
-// 13.9; two launches 8.8 and 17.5.  From some 64 K on the one CU is slower than two launches are long (96 K: 12.3 us).
+// elements, sixteen a lane.  Four tensors of 16 K elements in all take 5.0 us as a graph and some 14.5 as a call, of 52 K 7.8 and
+// 14.8; two launches 8.8 and 18.  From some 64 K on the one CU is slower than two launches are long (96 K: 12.3 us).
 constexpr int kWaveSlots = 4, kSlots = 16 * kWaveSlots, kSlot = 1024;
 struct SmallArgs {
     Tagged in[kSlots], out[kSlots];       // a slot's first element

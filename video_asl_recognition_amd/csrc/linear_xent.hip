@@ -6,17 +6,17 @@
 // c is applied to the 32-bit sums: within G it would move every target's entry, -1 for an unsure row, to the same value
 // between two bf16 numbers, and that one rounding would stand in all results.
 //
-// The logits are never held.  Rows are taken in pieces; the product x W^T leaves, for every row and every tile of classes, the
+// The logits themselves are not held.  Rows are taken in pieces; the product x W^T leaves, for every row and every tile of classes, the
 // tile's maximum m, the sum of exp(l - m) and, where gradients are asked for, exp(l - m) itself (fp32, or for bf16 operands
 // fp16 of 2^15 times it: 11 bits of the value down to 2^-29 of the tile's largest, and 2^-40 of that below).  One pass over the
 // per-tile numbers gives lse, the loss and the factors g exp(m - lse); one pass over the exponentials turns them into G in
 // place, the target's entry from its own 32-bit logit (g expm1((l_t - max) - log sum exp(l - max)), where p - 1 of a rounded p,
 // or l_t - lse of a rounded lse, would cancel), and adds up db in 32 bits.  Then two products, whose sums are finished (slabs, db, the loss) by one more launch where there is need.
 //
-// What bounds it is the products where they are large (8192 x 32768 x 2048 bf16: 2.82 ms with gradients, 3.3 PFLOP at 1.17
-// PFLOP/s: the three products 2.63 ms, G 0.19 ms at 5.5 TB/s), the matrix pipe's rate for six bf16 products in the place of one
-// in fp32 (2048 x 8192 x 1024: 588 us with gradients, 175 TFLOP/s; on fp32 MFMAs 1151), and the chain of launches where they
-// are small (2048 x 2000 x 512 bf16: 47 us, of which the products 28).
+// What bounds it is the products where they are large (8192 x 32768 x 2048 bf16: 2.83 to 2.92 ms with gradients from card to card,
+// 3.3 PFLOP at 1.13 to 1.17 PFLOP/s: the three products 2.63 to 2.75 ms, G 0.19 ms at 5.5 TB/s), the matrix pipe's rate for six
+// bf16 products in the place of one in fp32 (2048 x 8192 x 1024: 588 to 611 us with gradients, 169 to 175 TFLOP/s; on fp32 MFMAs
+// 1151), and the chain of launches where they are small (2048 x 2000 x 512 bf16: 47 us, of which the products 28).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -6,7 +6,7 @@
 // workgroup takes all rows' statistics for itself: 32 rows of at most 512 tiles); both gradient products side by side; the sum
 // of dx's slices.  All products run on fp32 MFMAs, bf16
 // operands widened on load, because nothing here is bound by the matrix pipe; G stays fp32.  8 x 2000 x 512 fp32 with gradients
-// takes 19 us as a graph (its launches 6.7 and 11.3): 8 MB, 2 us of this card's memory rate.
+// takes 19 us as a graph (its launches 6.6 and 12): 8 MB, 2 us of this card's memory rate.
 //
 // The MFMA (16 x 16 x 4) wants one k of one index a lane.  A lane loads four consecutive elements and deals them to four
 // MFMAs, with the same assignment of k (or of the index) on both sides, so every load is 16 bytes (8 for bf16).

@@ -20,9 +20,9 @@
 // each, 203 TFLOP/s; a library's fp32 product 134 TFLOP/s).
 //
 // Measured, 8192 x 32768 x 2048 (1.10 PFLOP a product): logits 1016 to 1067 us (1.03 to 1.08 PFLOP/s), dx 826 to 847 (1.30 to
-// 1.33), dW 794 to 826 (1.33 to 1.38); a library's plain products of the same shapes 1.20, 1.12 and 0.99 PFLOP/s.  The gradient
-// products keep the matrix pipe 87 % busy at the clock that its power leaves it; a logits tile adds 8 us of exponentials and
-// 6 us of first loads to 32 steps of 1.6 us, alone on its CU.
+// 1.33), dW 794 to 826 (1.33 to 1.38); a library's plain products of the same shapes 1.20, 1.12 and 0.99 PFLOP/s.  dW keeps the
+// matrix pipe 86 % busy at the clock that its power leaves it, dx 78 to 82 % and the logits 60 %: a logits tile adds 8 us of exponentials
+// and 6 us of first loads to 32 steps of 1.6 us, alone on its CU.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

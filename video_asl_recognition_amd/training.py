@@ -1,5 +1,5 @@
 """Operators for training the classifier end on frozen features: LayerNorm forward and backward, the classifier's Linear and
-softmax cross entropy as one operator that never holds the logits, and the global gradient norm with clipping.
+softmax cross entropy as one operator, and the global gradient norm with clipping.
 
     y = layer_norm(x, weight, bias)                                        # autograd
     loss = linear_cross_entropy(x, weight, target, bias)                   # autograd
@@ -7,9 +7,18 @@ softmax cross entropy as one operator that never holds the logits, and the globa
     norm = clip_grads(grads, max_norm)                                     # or clip_grad_norm_(parameters, max_norm)
 
 Every operator is a launch sequence of libaslhip.so on the current stream; torch allocates outputs and workspaces.  Tensors
-are fp32 or bf16 on one GPU; sums, statistics and softmax are held in fp32 or wider, results are rounded once (the loss's
-gradient with respect to bf16 logits is additionally rounded to bf16, as the operand of the gradient products).  No call
-waits for the GPU.
+are fp32 or bf16 on one GPU; sums, statistics, log sum exp and loss are held in fp32 or wider, and results are rounded once.  No
+call waits for the GPU.
+
+Two values between are held in fewer bits for bf16 features, except for few rows and a small weight (at most 16 rows, 2^20 weights
+and 16384 classes): the softmax's exponentials, as fp16 of 11 significant bits, from which dbias too is added up, and the loss's
+gradient with respect to the logits, as bf16, the type that the matrix instructions of the gradient products take.  The latter
+is what shows: dx and dweight were measured 0.0019 to 0.0024 (relative 2-norm) off the exact gradient, of which their own rounding
+to bf16 is 0.0017.  A caller who wants neither passes fp32 copies of features and weight: everything is then as good as fp32 sums.
+
+The loss alone holds per row and 32 to 128 classes a maximum and a sum, no logits.  With gradients the exponentials are held, for
+as many rows at a time as take 4 GiB (2 bytes an entry for bf16 features, 4 for fp32, 10 for large fp32 problems, whose gradient
+is held as three bf16 parts as well), or 256 rows.
 """
 from __future__ import annotations
 
